@@ -94,6 +94,9 @@ int th_buffer_upload(th_buffer* buf, const void* host, size_t n);
 /* Copy n elements to host memory; synchronises the device stream first. */
 int th_buffer_download(th_buffer* buf, void* host, size_t n);
 int th_buffer_info(const th_buffer* buf, th_dtype* dtype, size_t* n);
+/* Device address of the buffer's memory, for callers with kernels of their own
+ * (their streams are not the device handle's: th_sync between). */
+int th_buffer_ptr(const th_buffer* buf, void** ptr);
 /* ComputeDevice::zero_buffer. */
 int th_buffer_zero(th_buffer* buf);
 /* Device-to-device copy of min(src, dst) bytes on the device stream
@@ -415,6 +418,116 @@ int th_mla_decode(th_device* dev, const th_buffer* q_nope, const th_buffer* q_ro
                   const th_buffer* cache, size_t B, size_t H, size_t L, size_t dn, size_t dr,
                   size_t r, size_t dv, const th_qweight* w_uk, const th_qweight* w_uv,
                   float sm_scale, th_buffer* out);
+
+/* ---- rotary positions: pair layouts, parts of a head, long contexts ----------
+ * No counterpart in the reference beyond th_rope_forward's interleaved pairs.
+ * A pair (x, y) of a row at position p becomes (x c - y s, x s + y c) with c and
+ * s from row p of the tables; dims from rot_dim on pass through. */
+enum {
+    TH_ROPE_INTERLEAVED = 0, /* pairs (2i, 2i + 1) */
+    TH_ROPE_HALF = 1         /* pairs (i, i + rot_dim / 2) */
+};
+/* Frequencies f_i = base^(-2i / rot_dim) scaled for contexts longer than the
+ * trained one; factor >= 1. */
+enum {
+    TH_ROPE_PLAIN = 0,  /* f_i */
+    TH_ROPE_LINEAR = 1, /* f_i / factor */
+    TH_ROPE_BASE = 2,   /* base * factor^(rot_dim / (rot_dim - 2)) in place of base */
+    TH_ROPE_BANDS = 3,  /* by the turns t of a wave over original_len: f_i from `high` turns on,
+                         * f_i / factor up to `low` turns, linear in t between */
+    TH_ROPE_RAMP = 4    /* linear in the pair's index between those that turn `high` times
+                         * (f_i) and `low` times (f_i / factor); tables times warmth (0: 0.1 ln(factor) + 1) */
+};
+typedef struct {
+    int kind; /* TH_ROPE_PLAIN ... */
+    double factor, low, high, warmth;
+    size_t original_len;
+} th_rope_scaling;
+/* Tables cos/sin [max_seq][rot_dim/2] on the host, angles in f64 (s may be NULL). */
+int th_rope_tables_scaled(size_t rot_dim, size_t max_seq, double base, const th_rope_scaling* s, float* cos_table,
+                          float* sin_table);
+/* in, out [n_rows][n_heads][head_dim], each f32, f16 or bf16; computed in f32.  Row i is at position
+ * positions[i] (u32), or at start_pos + i where positions is NULL.  A position
+ * from a buffer that is behind the tables makes its row's pairs NaN.  out may be in. */
+int th_rope_rows(th_device* dev, const th_buffer* in, const th_buffer* cos_buf, const th_buffer* sin_buf,
+                 const th_buffer* positions, size_t start_pos, size_t n_rows, size_t n_heads, size_t head_dim,
+                 size_t rot_dim, int layout, th_buffer* out);
+
+/* ---- paged key/value cache -----------------------------------------------------
+ * For programs that serve several sequences at a time; no counterpart in the
+ * reference, whose caches are one contiguous buffer a sequence (kv_attention,
+ * cpu.rs:257).  A cache has n_pages pages of page_size positions for every
+ * layer; a sequence is a list of pages that grows with it, lowest vacant page first.  Forks share
+ * pages, and a page that is shared is copied when one of its sequences writes
+ * to it.  Bookkeeping is the host's: calls that change sequences cost no
+ * synchronisation, and are made between replays of captured graphs, not recorded.
+ * All calls on a cache are its device handle's: one host thread, one stream. */
+typedef struct th_kv_cache th_kv_cache;
+typedef struct th_kv_batch th_kv_batch;
+typedef struct {
+    th_dtype dtype;    /* TH_F16 or TH_BF16 */
+    size_t n_layers, n_kv_heads;
+    size_t head_dim;   /* a multiple of 8, at most 256 */
+    size_t page_size;  /* positions: a power of two from 8 to 1024 */
+    size_t n_pages, max_seqs;
+    size_t max_len;    /* of a sequence, at most 2^28 */
+} th_kv_cache_config;
+int th_kv_cache_create(th_device* dev, const th_kv_cache_config* cfg, th_kv_cache** out);
+/* Batches of the cache may be destroyed before or after it. */
+int th_kv_cache_destroy(th_kv_cache* c);
+int th_kv_cache_info(const th_kv_cache* c, size_t* pages_vacant, size_t* seqs_vacant);
+/* Device addresses of a layer's K and V pages, [page][kv head][position][dim],
+ * for callers with kernels of their own; layer l's V follows its K, layer l + 1 follows. */
+int th_kv_cache_pages(th_kv_cache* c, size_t layer, void** k, void** v);
+/* Moves pages so that the live ones are the first of the pool (batches that have
+ * begun on a sequence whose pages moved have to begin again). */
+int th_kv_cache_compact(th_kv_cache* c, size_t* n_moved);
+
+/* n empty sequences. */
+int th_kv_seq_create(th_kv_cache* c, size_t n, int32_t* seqs);
+int th_kv_seq_free(th_kv_cache* c, const int32_t* seqs, size_t n);
+int th_kv_seq_len(const th_kv_cache* c, int32_t seq, size_t* len);
+/* Sets the length: pages behind it are freed, or pages for new positions (whose
+ * rows hold what was there before) are taken. */
+int th_kv_seq_resize(th_kv_cache* c, int32_t seq, size_t len);
+/* n new sequences that share the first len positions of seq. */
+int th_kv_seq_fork(th_kv_cache* c, int32_t seq, size_t len, size_t n, int32_t* children);
+/* Keeps the rows at the given positions (host, any order, repeats allowed) as
+ * positions 0..n-1, in pages of the sequence's own, in every layer. */
+int th_kv_seq_select(th_kv_cache* c, int32_t seq, const uint32_t* positions, size_t n);
+/* Rows [from, from + n) of one layer as th_kv_attention takes them,
+ * [n][n_kv_heads * head_dim] of the cache's type. */
+int th_kv_seq_read(th_kv_cache* c, int32_t seq, size_t layer, size_t from, size_t n, th_buffer* k, th_buffer* v);
+
+/* New positions of several sequences, taken through all layers together.
+ * n_heads: query heads.  max_rows: new positions of all its sequences. */
+int th_kv_batch_create(th_kv_cache* c, size_t max_seqs, size_t max_rows, size_t n_heads, th_kv_batch** out);
+int th_kv_batch_destroy(th_kv_batch* b);
+/* Begins a step: sequence seqs[i] (none twice) grows by n_new[i] >= 0 positions.
+ * Rows of the step's buffers are the new positions, sequence by sequence in this
+ * order.  Refused as a whole if pages or lengths do not suffice (TH_ERR_OOM, TH_ERR_INVALID). */
+int th_kv_batch_begin(th_kv_batch* b, const int32_t* seqs, const uint32_t* n_new, size_t n);
+/* Ends it: sequence i keeps its first n_keep[i] new positions (rejected drafts go). */
+int th_kv_batch_trim(th_kv_batch* b, const uint32_t* n_keep, size_t n);
+/* Rotates q [rows][n_heads][head_dim] into q_out and k [rows][n_kv_heads][head_dim]
+ * into the pages, and stores v.  q, k and v of one type, f32, f16 or bf16; q_out of
+ * any of them (it may be q, with q's type).  A row's position is its place in its sequence, or positions[row] where
+ * that is given (as in th_rope_rows).  rot_dim 0 rotates nothing (tables may be NULL);
+ * q and q_out may be NULL together.  Captured: buffers for max_rows rows, and a
+ * replay runs on the batch as it last began. */
+int th_kv_append(th_kv_batch* b, size_t layer, const th_buffer* q, const th_buffer* k, const th_buffer* v,
+                 const th_buffer* cos_buf, const th_buffer* sin_buf, const th_buffer* positions, size_t rot_dim,
+                 int layout, th_buffer* q_out);
+/* Attention of the step's rows over the pages: the row at place p of its sequence
+ * sees keys j <= p with window == 0, j > p - window or j < n_sinks.  q and out
+ * [rows][n_heads][head_dim], each f32, f16 or bf16, query head h reads kv head
+ * h / (n_heads / n_kv_heads); scores times scale (0: 1/sqrt(head_dim)), softmax and sums in f32.  q and out of
+ * the cache's type take probabilities rounded to it; any other mix keeps f32's
+ * precision.  Pages that sequences of the batch share from their start on are read once for all.
+ * Captured (after the same call has been made once): buffers for max_rows rows, and
+ * a replay runs on the batch as it last began. */
+int th_kv_batch_attention(th_kv_batch* b, size_t layer, const th_buffer* q, size_t window, size_t n_sinks, float scale,
+                          th_buffer* out);
 
 /* ---- seeded synthetic data (host) ---------------------------------------
  * xoshiro256** seeded through SplitMix64, as crates/tang-bench/src/lib.rs:7-46.

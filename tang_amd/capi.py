@@ -61,6 +61,7 @@ SIGNATURES = {
     "th_buffer_upload": ([_P, _P, _S], _I),
     "th_buffer_download": ([_P, _P, _S], _I),
     "th_buffer_info": ([_P, _P, _P], _I),
+    "th_buffer_ptr": ([_P, _P], _I),
     "th_buffer_zero": ([_P], _I),
     "th_buffer_copy": ([_P, _P], _I),
     "th_buffer_copy_region": ([_P, _S, _P, _S, _S], _I),
@@ -129,6 +130,26 @@ SIGNATURES = {
     "th_kernel_compile": ([_P, ctypes.c_char_p, ctypes.c_char_p, _P], _I),
     "th_kernel_free": ([_P], _I),
     "th_elementwise": ([_P, _P, _S, _S, _P], _I),
+    "th_rope_tables_scaled": ([_S, _S, _D, _P, _P, _P], _I),
+    "th_rope_rows": ([_P, _P, _P, _P, _P, _S, _S, _S, _S, _S, _I, _P], _I),
+    "th_kv_cache_create": ([_P, _P, _P], _I),
+    "th_kv_cache_destroy": ([_P], _I),
+    "th_kv_cache_info": ([_P, _P, _P], _I),
+    "th_kv_cache_pages": ([_P, _S, _P, _P], _I),
+    "th_kv_cache_compact": ([_P, _P], _I),
+    "th_kv_seq_create": ([_P, _S, _P], _I),
+    "th_kv_seq_free": ([_P, _P, _S], _I),
+    "th_kv_seq_len": ([_P, ctypes.c_int32, _P], _I),
+    "th_kv_seq_resize": ([_P, ctypes.c_int32, _S], _I),
+    "th_kv_seq_fork": ([_P, ctypes.c_int32, _S, _S, _P], _I),
+    "th_kv_seq_select": ([_P, ctypes.c_int32, _P, _S], _I),
+    "th_kv_seq_read": ([_P, ctypes.c_int32, _S, _S, _S, _P, _P], _I),
+    "th_kv_batch_create": ([_P, _S, _S, _S, _P], _I),
+    "th_kv_batch_destroy": ([_P], _I),
+    "th_kv_batch_begin": ([_P, _P, _P, _S], _I),
+    "th_kv_batch_trim": ([_P, _P, _S], _I),
+    "th_kv_append": ([_P, _S, _P, _P, _P, _P, _P, _P, _S, _I, _P], _I),
+    "th_kv_batch_attention": ([_P, _S, _P, _S, _S, _F, _P], _I),
     "th_synth_seed": ([_U64, _U64, _U64], _U64),
     "th_synth_q4": ([_U64, _S, _S, _F, _F, _P, _P], _I),
     "th_synth_q8_rowwise": ([_U64, _S, _S, _F, _F, _P, _P], _I),
@@ -279,6 +300,18 @@ def rope_tables(head_dim, max_seq, base):
     return c, s
 
 
+ROPE_INTERLEAVED, ROPE_HALF = 0, 1
+_ROPE_KINDS = {"plain": 0, "linear": 1, "base": 2, "bands": 3, "ramp": 4}
+
+
+def rope_tables_scaled(rot_dim, max_seq, base, kind="plain", factor=1.0, low=1.0, high=4.0, warmth=0.0, original_len=0):
+    """cos and sin tables [max_seq][rot_dim / 2], frequencies scaled as `kind` says (th_rope_tables_scaled)."""
+    s = RopeScaling(_ROPE_KINDS[kind], factor, low, high, warmth, original_len)
+    c, sn = (np.empty((max_seq, rot_dim // 2), np.float32) for _ in range(2))
+    check(lib().th_rope_tables_scaled(rot_dim, max_seq, base, ctypes.byref(s), ptr(c), ptr(sn)))
+    return c, sn
+
+
 # --------------------------------------------------------------------------
 # device objects
 # --------------------------------------------------------------------------
@@ -305,6 +338,12 @@ class Buffer:
         out = np.empty(n, _NP[self.dtype])
         check(lib().th_buffer_download(self.handle, ptr(out), n))
         return out
+
+    def device_ptr(self):
+        """The device address of the buffer's memory (th_buffer_ptr)."""
+        p = ctypes.c_void_p()
+        check(lib().th_buffer_ptr(self.handle, ctypes.byref(p)))
+        return p.value
 
     def free(self):
         if self.handle:
@@ -470,6 +509,131 @@ class Graph:
             pass
 
 
+class RopeScaling(ctypes.Structure):
+    """th_rope_scaling."""
+    _fields_ = [("kind", ctypes.c_int), ("factor", ctypes.c_double), ("low", ctypes.c_double), ("high", ctypes.c_double),
+                ("warmth", ctypes.c_double), ("original_len", ctypes.c_size_t)]
+
+
+class KvCacheConfig(ctypes.Structure):
+    """th_kv_cache_config."""
+    _fields_ = [("dtype", ctypes.c_int), ("n_layers", ctypes.c_size_t), ("n_kv_heads", ctypes.c_size_t),
+                ("head_dim", ctypes.c_size_t), ("page_size", ctypes.c_size_t), ("n_pages", ctypes.c_size_t),
+                ("max_seqs", ctypes.c_size_t), ("max_len", ctypes.c_size_t)]
+
+
+class KvCache:
+    """A paged key/value cache (th_kv_cache_* and th_kv_seq_*); sequences are numbers."""
+
+    def __init__(self, dev, n_layers, n_kv_heads, head_dim, page_size, n_pages, max_seqs, max_len, dtype=F16):
+        self.dev, self.dtype, self.n_layers, self.n_kv_heads, self.head_dim = dev, dtype, n_layers, n_kv_heads, head_dim
+        cfg = KvCacheConfig(dtype, n_layers, n_kv_heads, head_dim, page_size, n_pages, max_seqs, max_len)
+        h = ctypes.c_void_p()
+        check(lib().th_kv_cache_create(dev.handle, ctypes.byref(cfg), ctypes.byref(h)))
+        self.handle = h
+
+    def info(self):
+        """(vacant pages, vacant sequences)"""
+        p, s = ctypes.c_size_t(), ctypes.c_size_t()
+        check(lib().th_kv_cache_info(self.handle, ctypes.byref(p), ctypes.byref(s)))
+        return p.value, s.value
+
+    def page_pointers(self, layer):
+        """Device addresses of the layer's K and V pages."""
+        k, v = ctypes.c_void_p(), ctypes.c_void_p()
+        check(lib().th_kv_cache_pages(self.handle, layer, ctypes.byref(k), ctypes.byref(v)))
+        return k.value, v.value
+
+    def compact(self):
+        n = ctypes.c_size_t()
+        check(lib().th_kv_cache_compact(self.handle, ctypes.byref(n)))
+        return n.value
+
+    def seq_create(self, n=1):
+        out = (ctypes.c_int32 * max(n, 1))()
+        check(lib().th_kv_seq_create(self.handle, n, out))
+        return list(out[:n])
+
+    def seq_free(self, seqs):
+        check(lib().th_kv_seq_free(self.handle, (ctypes.c_int32 * max(len(seqs), 1))(*seqs), len(seqs)))
+
+    def seq_len(self, seq):
+        n = ctypes.c_size_t()
+        check(lib().th_kv_seq_len(self.handle, seq, ctypes.byref(n)))
+        return n.value
+
+    def seq_resize(self, seq, length):
+        check(lib().th_kv_seq_resize(self.handle, seq, length))
+
+    def seq_fork(self, seq, n=1, length=None):
+        out = (ctypes.c_int32 * max(n, 1))()
+        check(lib().th_kv_seq_fork(self.handle, seq, self.seq_len(seq) if length is None else length, n, out))
+        return list(out[:n])
+
+    def seq_select(self, seq, positions):
+        p = np.ascontiguousarray(positions, np.uint32)
+        check(lib().th_kv_seq_select(self.handle, seq, ptr(p), p.size))
+
+    def seq_read(self, seq, layer, start=0, n=None):
+        """K and V rows [n][n_kv_heads * head_dim] in new buffers."""
+        n = self.seq_len(seq) - start if n is None else n
+        k, v = (self.dev.alloc(n * self.n_kv_heads * self.head_dim, self.dtype) for _ in range(2))
+        check(lib().th_kv_seq_read(self.handle, seq, layer, start, n, k.handle, v.handle))
+        return k, v
+
+    def batch(self, max_seqs, max_rows, n_heads):
+        return KvBatch(self, max_seqs, max_rows, n_heads)
+
+    def free(self):
+        if self.handle:
+            check(lib().th_kv_cache_destroy(self.handle))
+            self.handle = None
+
+    def __del__(self):
+        try:
+            if self.handle and _lib is not None:
+                _lib.th_kv_cache_destroy(self.handle)
+        except Exception:
+            pass
+
+
+class KvBatch:
+    """New positions of several sequences of a cache, step by step (th_kv_batch_*)."""
+
+    def __init__(self, cache, max_seqs, max_rows, n_heads):
+        self.cache = cache
+        h = ctypes.c_void_p()
+        check(lib().th_kv_batch_create(cache.handle, max_seqs, max_rows, n_heads, ctypes.byref(h)))
+        self.handle = h
+
+    def begin(self, seqs, n_new):
+        assert len(seqs) == len(n_new)
+        n = max(len(seqs), 1)
+        check(lib().th_kv_batch_begin(self.handle, (ctypes.c_int32 * n)(*seqs), (ctypes.c_uint32 * n)(*n_new), len(seqs)))
+
+    def trim(self, n_keep):
+        check(lib().th_kv_batch_trim(self.handle, (ctypes.c_uint32 * max(len(n_keep), 1))(*n_keep), len(n_keep)))
+
+    def append(self, layer, q, k, v, q_out, cos_buf=None, sin_buf=None, rot_dim=0, layout=0, positions=None):
+        h = [b.handle if b is not None else None for b in (q, k, v, cos_buf, sin_buf, positions)]
+        check(lib().th_kv_append(self.handle, layer, *h, rot_dim, layout, q_out.handle if q_out is not None else None))
+
+    def attention(self, layer, q, out, window=0, sinks=0, scale=0.0):
+        check(lib().th_kv_batch_attention(self.handle, layer, q.handle, window, sinks, scale, out.handle))
+
+    def free(self):
+        if self.handle:
+            check(lib().th_kv_batch_destroy(self.handle))
+            self.handle = None
+
+    def __del__(self):
+        try:
+            if self.handle and _lib is not None:
+                _lib.th_kv_batch_destroy(self.handle)
+        except Exception:
+            pass
+
+
 class HipComputeDevice:
     """One device handle (one HIP stream), methods named as ComputeDevice's."""
 
@@ -599,6 +763,17 @@ class HipComputeDevice:
         check(lib().th_rope_forward(self.handle, inp.handle, cos_buf.handle, sin_buf.handle, seq_len, n_heads,
                                     head_dim, start_pos, out.handle))
         return out
+
+    def rope_rows(self, x, cos_buf, sin_buf, n_rows, n_heads, head_dim, rot_dim, layout=ROPE_INTERLEAVED, start_pos=0,
+                  positions=None, out=None):
+        """Rotary positions in either pair layout, on the first rot_dim dims of each head."""
+        out = out or self.alloc(n_rows * n_heads * head_dim, x.dtype)
+        h = [b.handle if b is not None else None for b in (x, cos_buf, sin_buf, positions)]
+        check(lib().th_rope_rows(self.handle, *h, start_pos, n_rows, n_heads, head_dim, rot_dim, layout, out.handle))
+        return out
+
+    def kv_cache(self, n_layers, n_kv_heads, head_dim, page_size, n_pages, max_seqs, max_len, dtype=F16):
+        return KvCache(self, n_layers, n_kv_heads, head_dim, page_size, n_pages, max_seqs, max_len, dtype)
 
     def kv_attention(self, q, k_cache, v_cache, cache_start, q_len, n_heads, n_kv_heads, head_dim):
         out = self.alloc(q_len * n_heads * head_dim)

@@ -478,6 +478,13 @@ int th_buffer_info(const th_buffer* b, th_dtype* dt, size_t* n) {
     TH_API_END
 }
 
+int th_buffer_ptr(const th_buffer* b, void** ptr) {
+    TH_API_BEGIN
+    TH_REQUIRE(b && ptr, "null argument");
+    *ptr = b->ptr;
+    TH_API_END
+}
+
 int th_q4_upload_blocks(th_device* d, const th_q4_block* blocks, size_t rows, size_t cols,
                         th_dtype sdt, th_qweight** out) {
     TH_API_BEGIN

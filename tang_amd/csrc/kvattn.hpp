@@ -1,0 +1,157 @@
+// Device code that the two attention kernels over a paged cache share.
+#pragma once
+
+#include "kvcache.hpp"
+#include "ops.hpp"
+#include "qlinear.hpp"
+
+namespace th {
+
+typedef float kv_f32x4_t __attribute__((ext_vector_type(4)));
+typedef float kv_f32x16_t __attribute__((ext_vector_type(16)));
+typedef uint32_t kv_u4_t __attribute__((ext_vector_type(4)));
+typedef short kv_s4_t __attribute__((ext_vector_type(4)));
+typedef __attribute__((address_space(3))) kv_s4_t kv_lds_s4_t;
+
+template <typename E> struct KvVec;
+template <> struct KvVec<_Float16> { typedef _Float16 x8 __attribute__((ext_vector_type(8))); };
+template <> struct KvVec<__bf16> { typedef __bf16 x8 __attribute__((ext_vector_type(8))); };
+
+__device__ __forceinline__ kv_f32x4_t kv_mfma16(KvVec<_Float16>::x8 a, KvVec<_Float16>::x8 b, kv_f32x4_t c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
+}
+__device__ __forceinline__ kv_f32x4_t kv_mfma16(KvVec<__bf16>::x8 a, KvVec<__bf16>::x8 b, kv_f32x4_t c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
+}
+__device__ __forceinline__ kv_f32x16_t kv_mfma32(KvVec<_Float16>::x8 a, KvVec<_Float16>::x8 b, kv_f32x16_t c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);
+}
+__device__ __forceinline__ kv_f32x16_t kv_mfma32(KvVec<__bf16>::x8 a, KvVec<__bf16>::x8 b, kv_f32x16_t c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
+}
+
+// Operands that are wider than the cache's type (f32 queries, the
+// probabilities of f32 results) go in as a sum of NP values of that type: each
+// takes the bits that the ones before left, rounded to nearest.  Two f16 are off by
+// 2^-24 of the value at most (2^-12 is left behind the first, and 2^-12 of that), three
+// bf16 by 2^-27: an f32's own rounding or less.  NP = 1 is for queries and
+// results of the cache's type: the one rounding of a probability (2^-11 f16, 2^-8 bf16
+// at most half a step each) is that of a result.
+template <typename E> constexpr int kv_wide_parts() { return sizeof(E) == 2 && std::is_same<E, __bf16>::value ? 3 : 2; }
+
+template <typename E, int NP>
+__device__ __forceinline__ void kv_split(float x, E (&part)[NP]) {
+#pragma unroll
+    for (int i = 0; i < NP; i++) {
+        part[i] = (E)x;
+        x -= (float)part[i];
+    }
+}
+// f16 parts keep their bits if the largest is near the type's end: queries are brought to
+// [2^14, 2^15) by a power of two for each row, probabilities (at most 1) by 2^14.
+constexpr int KV_Q_TOP = 15;
+constexpr float KV_P_UP = 16384.0f;
+
+__device__ __forceinline__ float kv_exp2(float x) { return __builtin_amdgcn_exp2f(x); }
+
+// Chain of MFMAs before a branch: what follows may read their results.
+__device__ __forceinline__ void kv_mfma_wait() {
+    __builtin_amdgcn_sched_barrier(0);
+    asm volatile("s_nop 15\n\ts_nop 3");
+    __builtin_amdgcn_sched_barrier(0);
+}
+
+__device__ __forceinline__ float kv_load_q(const void* q, th_dtype dt, size_t at) {
+    if (dt == TH_F32) return ((const float*)q)[at];
+    if (dt == TH_F16) return (float)((const _Float16*)q)[at];
+    return (float)((const __bf16*)q)[at];
+}
+
+__device__ __forceinline__ void kv_load_q8(const void* q, th_dtype dt, size_t at, float (&v)[8]) {
+    if (dt == TH_F32) {
+        const kv_f32x4_t a = *(const kv_f32x4_t*)((const float*)q + at), b = *(const kv_f32x4_t*)((const float*)q + at + 4);
+#pragma unroll
+        for (int i = 0; i < 4; i++) { v[i] = a[i]; v[4 + i] = b[i]; }
+    } else if (dt == TH_F16) {
+        const KvVec<_Float16>::x8 a = *(const KvVec<_Float16>::x8*)((const _Float16*)q + at);
+#pragma unroll
+        for (int i = 0; i < 8; i++) v[i] = (float)a[i];
+    } else {
+        const KvVec<__bf16>::x8 a = *(const KvVec<__bf16>::x8*)((const __bf16*)q + at);
+#pragma unroll
+        for (int i = 0; i < 8; i++) v[i] = (float)a[i];
+    }
+}
+
+__device__ __forceinline__ void kv_store_out(void* out, th_dtype dt, size_t at, float v) {
+    if (dt == TH_F32) ((float*)out)[at] = v;
+    else if (dt == TH_F16) ((_Float16*)out)[at] = (_Float16)v;
+    else ((__bf16*)out)[at] = (__bf16)v;
+}
+
+__device__ __forceinline__ void kv_store_out4(void* out, th_dtype dt, size_t at, kv_f32x4_t v) {
+    if (dt == TH_F32) {
+        *(kv_f32x4_t*)((float*)out + at) = v;
+    } else if (dt == TH_F16) {
+        typedef _Float16 h4 __attribute__((ext_vector_type(4)));
+        *(h4*)((_Float16*)out + at) = h4{(_Float16)v[0], (_Float16)v[1], (_Float16)v[2], (_Float16)v[3]};
+    } else {
+        typedef __bf16 b4 __attribute__((ext_vector_type(4)));
+        *(b4*)((__bf16*)out + at) = b4{(__bf16)v[0], (__bf16)v[1], (__bf16)v[2], (__bf16)v[3]};
+    }
+}
+
+// Key j of an item's numbers, and the row of its K and V.
+__device__ __forceinline__ int kv_key(const KvItem& it, int j) { return j + (j >= it.sink_end ? it.gap : 0); }
+__device__ __forceinline__ uint32_t kv_row(const KvPages& p, const int* table, int h, int key) {
+    const uint32_t page = (uint32_t)table[key >> p.shift];
+    return ((page * p.n_kv_heads + h) << p.shift) + (key & ((1 << p.shift) - 1));
+}
+// Whether the row at position pos sees the key.
+__device__ __forceinline__ bool kv_sees(int key, int pos, int window, int sinks) {
+    return key <= pos && (window == 0 || key > pos - window || key < sinks);
+}
+
+// Where the sums of a token's row go: the record, or the result itself.
+__device__ __forceinline__ size_t kv_record(const KvItem& it, const KvTok& t, int n_heads, int head) {
+    const int s = (it.rec & KV_REC_OWN) ? (it.rec & ~KV_REC_OWN) + (t.own_n & 0xFFFF) : it.rec;
+    return ((size_t)t.rec + s) * n_heads + head;
+}
+
+// One row over some of an item's keys by one wave in plain f32, for rows
+// whose MFMA sums are not finite: an infinity times a part that is zero is NaN
+// there, and hidden keys carry weight zero rather than being left out.  Blocks of `block` numbers every `step`
+// from `from` on.  Lane l ends with dims l, l + 64, ...; m and l are every lane's.
+template <typename E, int DE>
+__device__ __noinline__ void kv_row_plain(const KvAttnArgs& a, const KvItem& it, const int* table, int h, size_t q_at, int pos,
+                                          int from, int block, int step, float& m, float& l, float (&acc)[DE]) {
+    const int lane = threadIdx.x & 63, hd = a.pages.hd;
+    float qv[DE];
+    m = -INFINITY;
+    l = 0.0f;
+#pragma unroll
+    for (int e = 0; e < DE; e++) {
+        acc[e] = 0.0f;
+        qv[e] = lane + 64 * e < hd ? kv_load_q(a.q, a.qdt, q_at + lane + 64 * e) : 0.0f;
+    }
+    for (int base = from; base < it.j1; base += step) {
+        for (int j = base; j < min(it.j1, base + block); j++) {
+            const int key = kv_key(it, j);
+            if (!kv_sees(key, pos, a.window, a.sinks)) continue;
+            const size_t row = (size_t)kv_row(a.pages, table, h, key) * hd;
+            float d = 0.0f;
+#pragma unroll
+            for (int e = 0; e < DE; e++)
+                if (lane + 64 * e < hd) d += qv[e] * (float)((const E*)a.pages.k)[row + lane + 64 * e];
+            const float s = wave_sum(d) * a.scale, mn = fmaxf(m, s), ref = mn == -INFINITY ? 0.0f : mn;
+            const float p = kv_exp2(s - ref), f = kv_exp2(m - ref);
+            l = l * f + p;
+#pragma unroll
+            for (int e = 0; e < DE; e++)
+                acc[e] = acc[e] * f + p * (lane + 64 * e < hd ? (float)((const E*)a.pages.v)[row + lane + 64 * e] : 0.0f);
+            m = mn;
+        }
+    }
+}
+
+}  // namespace th

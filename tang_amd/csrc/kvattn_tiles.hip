@@ -1,0 +1,269 @@
+// Attention over a paged cache for tiles of up to 128 rows (new tokens x query
+// heads of one kv head): prompts, and shared prefixes whose sequences' rows make
+// up one tile.
+//
+// Workgroup = (item, kv head); its four waves have 32 rows each and share blocks
+// of keys in LDS, the next block's loads in flight meanwhile.  The products are
+// transposed as in kvattn_rows.hip, on the 32x32x16 MFMA: S^T = K.Q^T leaves lane (h, c) of
+// row c the keys 8i + 4h .. + 3 of each 32, and the numbering of the
+// contraction in O^T += V^T.P^T follows that (slots 8h .. 8h + 7 of a step of 16 keys are
+// keys 4h .. 4h + 3 and 8 + 4h ..), so probabilities never leave their lane.
+#include <algorithm>
+#include <type_traits>
+
+#include "kvattn.hpp"
+
+namespace th {
+
+template <int D, typename E, int NP, bool PAD>
+__global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void kv_attn_tiles_kernel(KvAttnArgs a) {
+    typedef typename KvVec<E>::x8 x8;
+    // LDS rows of K end in 16 bytes (16-byte reads of 16 rows then meet all banks),
+    // those of V in 64 (four rows of 32 bytes, as the transposing reads take them)
+    constexpr int KB = D <= 128 ? 64 : 32, KT = KB / 32, NS = D / 16, NDT = D / 32, LK = D + 8, LV = D + 32, CPR = D / 8;
+    constexpr int NL = KB * CPR / 256, DE = D / 64;
+    __shared__ __align__(16) E ks[KB * LK], vs[KB * LV];
+    const KvPlanHead& head = *(const KvPlanHead*)a.plan;
+    const KvTok* toks = (const KvTok*)(a.plan + KV_HEAD_WORDS);
+    const KvItem* items = (const KvItem*)(a.plan + head.tile_items);
+    const int kvh = a.pages.n_kv_heads, hk = blockIdx.x % kvh, G = a.n_heads / kvh, hd = PAD ? a.pages.hd : D, nch = hd / 8;
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int h = lane >> 5, c = lane & 31;
+    for (int n = blockIdx.x / kvh; n < head.n_tile_items; n += gridDim.x / kvh) {
+        const KvItem it = items[n];
+        const int R = it.ntok * G, row = min(wave * 32 + c, R - 1);
+        const bool live = wave * 32 + c < R;
+        const KvTok tok = toks[it.tok0 + row / G];
+        const int hq = hk * G + row % G;
+        const int* table = a.pages.table + (size_t)it.seq * a.pages.pages_per_seq;
+        // the wave's lowest and highest positions: which blocks need no mask, and which no work
+        int p_lo = tok.pos, p_hi = tok.pos;
+#pragma unroll
+        for (int x = 16; x > 0; x >>= 1) {
+            p_lo = min(p_lo, __shfl_xor(p_lo, x, 64));
+            p_hi = max(p_hi, __shfl_xor(p_hi, x, 64));
+        }
+        p_lo = __builtin_amdgcn_readfirstlane(p_lo);
+        p_hi = __builtin_amdgcn_readfirstlane(p_hi);
+
+        uint32_t rn[NL];
+        auto find = [&](int j0) {
+#pragma unroll
+            for (int i = 0; i < NL; i++)
+                rn[i] = kv_row(a.pages, table, hk, kv_key(it, min(j0 + (tid + 256 * i) / CPR, it.j1 - 1)));
+        };
+        kv_u4_t kr[NL], vr[NL];
+        const int chunk = PAD ? min(tid % CPR, nch - 1) : tid % CPR;
+        auto load = [&]() {
+#pragma unroll
+            for (int i = 0; i < NL; i++) {
+                const size_t at = (size_t)rn[i] * hd + chunk * 8;
+                kr[i] = *(const kv_u4_t*)((const E*)a.pages.k + at);
+                vr[i] = *(const kv_u4_t*)((const E*)a.pages.v + at);
+            }
+        };
+        find(it.j0);
+        load();
+        find(it.j0 + KB);
+
+        // the queries: B operand, lane (h, c) dims 16s + 8h.. of row c
+        x8 q[NP][NS];
+        int qe = 0;
+        const size_t q_at = ((size_t)tok.row * a.n_heads + hq) * hd;
+        if constexpr (NP == 1) {
+#pragma unroll
+            for (int s = 0; s < NS; s++) {
+                q[0][s] = *(const x8*)((const E*)a.q + q_at + (PAD ? min(2 * s + h, nch - 1) : 2 * s + h) * 8);
+                if (PAD && 2 * s + h >= nch) q[0][s] = x8{};
+            }
+        } else {
+            float mx = 0.0f;
+            for (int s = 0; s < NS; s++) {
+                float x[8];
+                kv_load_q8(a.q, a.qdt, q_at + (PAD ? min(2 * s + h, nch - 1) : 2 * s + h) * 8, x);
+#pragma unroll
+                for (int i = 0; i < 8; i++) mx = fmaxf(mx, fabsf(x[i]));
+            }
+            mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
+            qe = range_exp(mx, KV_Q_TOP);
+#pragma unroll
+            for (int s = 0; s < NS; s++) {
+                float x[8];
+                kv_load_q8(a.q, a.qdt, q_at + (PAD ? min(2 * s + h, nch - 1) : 2 * s + h) * 8, x);
+#pragma unroll
+                for (int i = 0; i < 8; i++) {
+                    E part[NP];
+                    kv_split<E, NP>(PAD && 2 * s + h >= nch ? 0.0f : __builtin_amdgcn_ldexpf(x[i], -qe), part);
+#pragma unroll
+                    for (int u = 0; u < NP; u++) q[u][s][i] = part[u];
+                }
+            }
+        }
+        const float scale = NP == 1 ? a.scale : __builtin_amdgcn_ldexpf(a.scale, qe);
+        float m = -INFINITY, l = 0.0f;
+        kv_f32x16_t o[NDT];
+#pragma unroll
+        for (int t = 0; t < NDT; t++)
+#pragma unroll
+            for (int i = 0; i < 16; i++) o[t][i] = 0.0f;
+
+        for (int j = it.j0; j < it.j1; j += KB) {
+            __syncthreads();  // the previous block's reads are done
+#pragma unroll
+            for (int i = 0; i < NL; i++) {
+                const int key = (tid + 256 * i) / CPR;
+                *(kv_u4_t*)(ks + key * LK + tid % CPR * 8) = kr[i];
+                *(kv_u4_t*)(vs + key * LV + tid % CPR * 8) = vr[i];
+            }
+            __syncthreads();
+            load();  // the next block (past the last: its last row again)
+            find(j + 2 * KB);
+            const int k_lo = kv_key(it, j), k_hi = kv_key(it, min(j + KB, it.j1) - 1);
+            if (k_lo > p_hi) continue;  // wave-uniform: every key is behind this wave's rows
+            kv_f32x16_t s[KT];
+#pragma unroll
+            for (int t = 0; t < KT; t++) {
+#pragma unroll
+                for (int i = 0; i < 16; i++) s[t][i] = 0.0f;
+#pragma unroll
+                for (int x = 0; x < NS; x++) {
+                    const x8 ka = *(const x8*)(ks + (t * 32 + c) * LK + x * 16 + 8 * h);
+#pragma unroll
+                    for (int u = NP - 1; u >= 0; u--) s[t] = kv_mfma32(ka, q[u][x], s[t]);
+                }
+            }
+            kv_mfma_wait();
+            const bool whole = j + KB <= it.j1 && k_hi <= p_lo &&
+                               (a.window == 0 || k_lo > p_hi - a.window || (k_hi < a.sinks));
+            float bm = -INFINITY;
+            if (whole) {
+#pragma unroll
+                for (int t = 0; t < KT; t++)
+#pragma unroll
+                    for (int i = 0; i < 16; i++) {
+                        s[t][i] *= scale;
+                        bm = fmaxf(bm, s[t][i]);
+                    }
+            } else {
+#pragma unroll
+                for (int t = 0; t < KT; t++)
+#pragma unroll
+                    for (int i = 0; i < 16; i++) {
+                        const int jj = j + t * 32 + 8 * (i >> 2) + 4 * h + (i & 3);
+                        const bool seen = jj < it.j1 && kv_sees(kv_key(it, jj), tok.pos, a.window, a.sinks);
+                        s[t][i] = seen ? s[t][i] * scale : -INFINITY;
+                        bm = fmaxf(bm, s[t][i]);
+                    }
+            }
+            bm = fmaxf(bm, __shfl_xor(bm, 32, 64));
+            const float mn = fmaxf(m, bm), ref = mn == -INFINITY ? 0.0f : mn, f = kv_exp2(m - ref);
+            float ps = 0.0f;
+            x8 p[NP][KT * 2];
+#pragma unroll
+            for (int t = 0; t < KT; t++)
+#pragma unroll
+                for (int i = 0; i < 16; i++) {
+                    const float e = kv_exp2(s[t][i] - ref);
+                    ps += e;
+                    E part[NP];
+                    kv_split<E, NP>(NP == 1 ? e : e * KV_P_UP, part);
+#pragma unroll
+                    for (int u = 0; u < NP; u++) p[u][2 * t + (i >> 3)][i & 7] = part[u];
+                }
+            l = l * f + ps;  // this lane's keys; the row's two lanes meet at the end
+            m = mn;
+            // The block sums up by itself and meets the sums so far in plain additions
+            // (an MFMA truncates what it adds to a larger sum).
+#pragma unroll
+            for (int dt = 0; dt < NDT; dt++) {
+                kv_f32x16_t d;
+#pragma unroll
+                for (int i = 0; i < 16; i++) d[i] = 0.0f;
+#pragma unroll
+                for (int x = 0; x < KT * 2; x++) {
+                    kv_s4_t w[2];
+#pragma unroll
+                    for (int y = 0; y < 2; y++)
+                        w[y] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                            (kv_lds_s4_t*)(vs + (16 * x + 8 * y + 4 * h + ((lane & 15) >> 2)) * LV + dt * 32 + (c & 16) +
+                                           4 * (lane & 3)));
+                    typedef short s8 __attribute__((ext_vector_type(8)));
+                    const x8 va = __builtin_bit_cast(x8, (s8){w[0][0], w[0][1], w[0][2], w[0][3], w[1][0], w[1][1], w[1][2], w[1][3]});
+#pragma unroll
+                    for (int u = NP - 1; u >= 0; u--) d = kv_mfma32(va, p[u][x], d);
+                }
+#pragma unroll
+                for (int i = 0; i < 16; i++) o[dt][i] = __builtin_fmaf(o[dt][i], f, d[i]);
+            }
+        }
+        l += __shfl_xor(l, 32, 64);
+        bool fine = l == l;
+#pragma unroll
+        for (int t = 0; t < NDT; t++)
+#pragma unroll
+            for (int i = 0; i < 16; i++) {
+                if constexpr (NP > 1) o[t][i] *= 1.0f / KV_P_UP;
+                fine &= fabsf(o[t][i]) <= 3.402823466e38f;
+            }
+        const size_t rec = it.rec < 0 ? 0 : kv_record(it, tok, a.n_heads, hq);
+        if (live) {
+            const float inv = it.rec < 0 ? 1.0f / l : 1.0f;
+#pragma unroll
+            for (int t = 0; t < NDT; t++)
+#pragma unroll
+                for (int i = 0; i < 16; i += 4) {
+                    const int d = t * 32 + 2 * i + 4 * h;
+                    if (PAD && d >= hd) continue;
+                    const kv_f32x4_t x = {o[t][i] * inv, o[t][i + 1] * inv, o[t][i + 2] * inv, o[t][i + 3] * inv};
+                    if (it.rec < 0) kv_store_out4(a.out, a.odt, q_at + d, x);
+                    else *(kv_f32x4_t*)(a.rec_o + rec * hd + d) = x;
+                }
+            if (it.rec >= 0 && h == 0) a.rec_ml[rec] = make_float2(m, l);
+        }
+        uint64_t todo = __ballot(live && !fine);
+        todo = (todo | (todo >> 32)) & 0xFFFFFFFFull;
+        for (; todo; todo &= todo - 1) {
+            const int rw = wave * 32 + (int)__builtin_ctzll(todo);
+            const KvTok t = toks[it.tok0 + rw / G];
+            const int hx = hk * G + rw % G;
+            const size_t at = ((size_t)t.row * a.n_heads + hx) * hd;
+            float pm, pl, acc[DE];
+            kv_row_plain<E, DE>(a, it, table, hk, at, t.pos, it.j0, KB, KB, pm, pl, acc);
+            const size_t rx = it.rec < 0 ? 0 : kv_record(it, t, a.n_heads, hx);
+#pragma unroll
+            for (int e = 0; e < DE; e++) {
+                if (lane + 64 * e >= hd) continue;
+                if (it.rec < 0) kv_store_out(a.out, a.odt, at + lane + 64 * e, acc[e] / pl);
+                else a.rec_o[rx * hd + lane + 64 * e] = acc[e];
+            }
+            if (it.rec >= 0 && lane == 0) a.rec_ml[rx] = make_float2(pm, pl);
+        }
+    }
+}
+
+template <int D, typename E>
+static void tiles_launch(const KvAttnArgs& a, unsigned grid, hipStream_t s) {
+    constexpr int WIDE = kv_wide_parts<E>();
+    const th_dtype own = std::is_same<E, __bf16>::value ? TH_BF16 : TH_F16;
+    const bool one = a.qdt == own && a.odt == own, pad = a.pages.hd != D;
+    if (one && pad) TH_LAUNCH((kv_attn_tiles_kernel<D, E, 1, true>), dim3(grid), dim3(256), 0, s, a);
+    else if (one) TH_LAUNCH((kv_attn_tiles_kernel<D, E, 1, false>), dim3(grid), dim3(256), 0, s, a);
+    else if (pad) TH_LAUNCH((kv_attn_tiles_kernel<D, E, WIDE, true>), dim3(grid), dim3(256), 0, s, a);
+    else TH_LAUNCH((kv_attn_tiles_kernel<D, E, WIDE, false>), dim3(grid), dim3(256), 0, s, a);
+    TH_LAUNCH_CHECK();
+}
+
+void launch_kv_attn_tiles(const KvAttnArgs& a, th_dtype cache, size_t grid, hipStream_t s) {
+    if (grid == 0) return;
+    const unsigned g = (unsigned)(grid * a.pages.n_kv_heads);
+    auto with = [&](auto e) {
+        typedef decltype(e) E;
+        if (a.pages.hd <= 64) tiles_launch<64, E>(a, g, s);
+        else if (a.pages.hd <= 128) tiles_launch<128, E>(a, g, s);
+        else tiles_launch<256, E>(a, g, s);
+    };
+    if (cache == TH_F16) with((_Float16)0);
+    else with((__bf16)0.0f);
+}
+
+}  // namespace th

@@ -67,6 +67,14 @@ pub struct th_moe {
     _private: [u8; 0],
 }
 #[repr(C)]
+pub struct th_kv_cache {
+    _private: [u8; 0],
+}
+#[repr(C)]
+pub struct th_kv_batch {
+    _private: [u8; 0],
+}
+#[repr(C)]
 pub struct th_graph {
     _private: [u8; 0],
 }
@@ -112,6 +120,39 @@ pub struct th_sampling_config {
     pub repetition_penalty: f64,
     pub stop_token: i64,
     pub max_tokens: usize,
+}
+
+// th_rope_rows, th_kv_append: how pairs lie; th_rope_scaling.kind
+pub const TH_ROPE_INTERLEAVED: c_int = 0;
+pub const TH_ROPE_HALF: c_int = 1;
+pub const TH_ROPE_PLAIN: c_int = 0;
+pub const TH_ROPE_LINEAR: c_int = 1;
+pub const TH_ROPE_BASE: c_int = 2;
+pub const TH_ROPE_BANDS: c_int = 3;
+pub const TH_ROPE_RAMP: c_int = 4;
+
+#[repr(C)]
+#[derive(Clone, Copy)]
+pub struct th_rope_scaling {
+    pub kind: c_int,
+    pub factor: f64,
+    pub low: f64,
+    pub high: f64,
+    pub warmth: f64,
+    pub original_len: usize,
+}
+
+#[repr(C)]
+#[derive(Clone, Copy)]
+pub struct th_kv_cache_config {
+    pub dtype: c_int,
+    pub n_layers: usize,
+    pub n_kv_heads: usize,
+    pub head_dim: usize,
+    pub page_size: usize,
+    pub n_pages: usize,
+    pub max_seqs: usize,
+    pub max_len: usize,
 }
 
 // th_expr_node.op: the tang-expr node kinds (crates/tang-expr/src/node.rs:58-90)
@@ -227,6 +268,27 @@ extern "C" {
     pub fn th_moe_init_synthetic(moe: *mut th_moe, seed: u64) -> c_int;
     pub fn th_moe_forward(moe: *mut th_moe, h: *const th_buffer, T: usize, out: *mut th_buffer, topk_idx: *mut th_buffer, topk_w: *mut th_buffer) -> c_int;
     pub fn th_mla_decode(dev: *mut th_device, q_nope: *const th_buffer, q_rope: *const th_buffer, cache: *const th_buffer, B: usize, H: usize, L: usize, dn: usize, dr: usize, r: usize, dv: usize, w_uk: *const th_qweight, w_uv: *const th_qweight, sm_scale: f32, out: *mut th_buffer) -> c_int;
+    pub fn th_buffer_ptr(buf: *const th_buffer, ptr: *mut *mut c_void) -> c_int;
+    pub fn th_rope_tables_scaled(rot_dim: usize, max_seq: usize, base: f64, s: *const th_rope_scaling, cos_table: *mut f32, sin_table: *mut f32) -> c_int;
+    pub fn th_rope_rows(dev: *mut th_device, in_: *const th_buffer, cos_buf: *const th_buffer, sin_buf: *const th_buffer, positions: *const th_buffer, start_pos: usize, n_rows: usize, n_heads: usize, head_dim: usize, rot_dim: usize, layout: c_int, out: *mut th_buffer) -> c_int;
+    pub fn th_kv_cache_create(dev: *mut th_device, cfg: *const th_kv_cache_config, out: *mut *mut th_kv_cache) -> c_int;
+    pub fn th_kv_cache_destroy(c: *mut th_kv_cache) -> c_int;
+    pub fn th_kv_cache_info(c: *const th_kv_cache, pages_vacant: *mut usize, seqs_vacant: *mut usize) -> c_int;
+    pub fn th_kv_cache_pages(c: *mut th_kv_cache, layer: usize, k: *mut *mut c_void, v: *mut *mut c_void) -> c_int;
+    pub fn th_kv_cache_compact(c: *mut th_kv_cache, n_moved: *mut usize) -> c_int;
+    pub fn th_kv_seq_create(c: *mut th_kv_cache, n: usize, seqs: *mut i32) -> c_int;
+    pub fn th_kv_seq_free(c: *mut th_kv_cache, seqs: *const i32, n: usize) -> c_int;
+    pub fn th_kv_seq_len(c: *const th_kv_cache, seq: i32, len: *mut usize) -> c_int;
+    pub fn th_kv_seq_resize(c: *mut th_kv_cache, seq: i32, len: usize) -> c_int;
+    pub fn th_kv_seq_fork(c: *mut th_kv_cache, seq: i32, len: usize, n: usize, children: *mut i32) -> c_int;
+    pub fn th_kv_seq_select(c: *mut th_kv_cache, seq: i32, positions: *const u32, n: usize) -> c_int;
+    pub fn th_kv_seq_read(c: *mut th_kv_cache, seq: i32, layer: usize, from: usize, n: usize, k: *mut th_buffer, v: *mut th_buffer) -> c_int;
+    pub fn th_kv_batch_create(c: *mut th_kv_cache, max_seqs: usize, max_rows: usize, n_heads: usize, out: *mut *mut th_kv_batch) -> c_int;
+    pub fn th_kv_batch_destroy(b: *mut th_kv_batch) -> c_int;
+    pub fn th_kv_batch_begin(b: *mut th_kv_batch, seqs: *const i32, n_new: *const u32, n: usize) -> c_int;
+    pub fn th_kv_batch_trim(b: *mut th_kv_batch, n_keep: *const u32, n: usize) -> c_int;
+    pub fn th_kv_append(b: *mut th_kv_batch, layer: usize, q: *const th_buffer, k: *const th_buffer, v: *const th_buffer, cos_buf: *const th_buffer, sin_buf: *const th_buffer, positions: *const th_buffer, rot_dim: usize, layout: c_int, q_out: *mut th_buffer) -> c_int;
+    pub fn th_kv_batch_attention(b: *mut th_kv_batch, layer: usize, q: *const th_buffer, window: usize, n_sinks: usize, scale: f32, out: *mut th_buffer) -> c_int;
     pub fn th_synth_seed(base: u64, layer: u64, tensor: u64) -> u64;
     pub fn th_synth_q4(seed: u64, rows: usize, cols: usize, smin: f32, smax: f32, nib: *mut u8, scales_f16: *mut u16) -> c_int;
     pub fn th_synth_q8_rowwise(seed: u64, rows: usize, cols: usize, smin: f32, smax: f32, q: *mut i8, row_scale: *mut f32) -> c_int;

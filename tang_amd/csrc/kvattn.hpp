@@ -67,19 +67,31 @@ __device__ __forceinline__ float kv_load_q(const void* q, th_dtype dt, size_t at
     return (float)((const __bf16*)q)[at];
 }
 
-__device__ __forceinline__ void kv_load_q8(const void* q, th_dtype dt, size_t at, float (&v)[8]) {
+// N pieces of eight values of a row as f32, all on their way before the first is used;
+// piece i starts at `at` + 8 * chunk(i) (zeros where chunk(i) says no).
+template <int N, typename F>
+__device__ __forceinline__ void kv_load_row(const void* q, th_dtype dt, size_t at, F&& chunk, float (&x)[N][8]) {
     if (dt == TH_F32) {
-        const kv_f32x4_t a = *(const kv_f32x4_t*)((const float*)q + at), b = *(const kv_f32x4_t*)((const float*)q + at + 4);
+        kv_f32x4_t v[N][2];
 #pragma unroll
-        for (int i = 0; i < 4; i++) { v[i] = a[i]; v[4 + i] = b[i]; }
-    } else if (dt == TH_F16) {
-        const KvVec<_Float16>::x8 a = *(const KvVec<_Float16>::x8*)((const _Float16*)q + at);
+        for (int i = 0; i < N; i++)
 #pragma unroll
-        for (int i = 0; i < 8; i++) v[i] = (float)a[i];
+            for (int y = 0; y < 2; y++) v[i][y] = *(const kv_f32x4_t*)((const float*)q + at + 8 * chunk(i) + 4 * y);
+#pragma unroll
+        for (int i = 0; i < N; i++)
+#pragma unroll
+            for (int e = 0; e < 8; e++) x[i][e] = v[i][e >> 2][e & 3];
     } else {
-        const KvVec<__bf16>::x8 a = *(const KvVec<__bf16>::x8*)((const __bf16*)q + at);
+        kv_u4_t v[N];
 #pragma unroll
-        for (int i = 0; i < 8; i++) v[i] = (float)a[i];
+        for (int i = 0; i < N; i++) v[i] = *(const kv_u4_t*)((const uint16_t*)q + at + 8 * chunk(i));
+#pragma unroll
+        for (int i = 0; i < N; i++)
+#pragma unroll
+            for (int e = 0; e < 8; e++) {
+                const uint16_t u = (uint16_t)(v[i][e >> 1] >> (16 * (e & 1)));
+                x[i][e] = dt == TH_F16 ? (float)__builtin_bit_cast(_Float16, u) : __uint_as_float((uint32_t)u << 16);
+            }
     }
 }
 
@@ -101,18 +113,38 @@ __device__ __forceinline__ void kv_store_out4(void* out, th_dtype dt, size_t at,
     }
 }
 
-// Key j of an item's numbers, and the row of its K and V.
+// An item, in scalar registers (the workgroup's waves all have the same).
+__device__ __forceinline__ KvItem kv_item(const KvItem* items, int n) {
+    const kv_u4_t a = ((const kv_u4_t*)(items + n))[0], b = ((const kv_u4_t*)(items + n))[1];
+    auto one = [](uint32_t x) { return (int)__builtin_amdgcn_readfirstlane(x); };
+    return KvItem{one(a[0]), one(a[1]), one(a[2]), one(a[3]), one(b[0]), one(b[1]), one(b[2]), one(b[3])};
+}
+
+// Key j of an item's numbers; the page that it is in; the row of its K and V.
+// (A page number is used an iteration after its load was issued: its wait would wait for every load before it.)
 __device__ __forceinline__ int kv_key(const KvItem& it, int j) { return j + (j >= it.sink_end ? it.gap : 0); }
-__device__ __forceinline__ uint32_t kv_row(const KvPages& p, const int* table, int h, int key) {
-    const uint32_t page = (uint32_t)table[key >> p.shift];
-    return ((page * p.n_kv_heads + h) << p.shift) + (key & ((1 << p.shift) - 1));
+__device__ __forceinline__ uint32_t kv_row(const KvPages& p, int page, int h, int key) {
+    return (((uint32_t)page * p.n_kv_heads + h) << p.shift) + (key & ((1 << p.shift) - 1));
 }
 // Whether the row at position pos sees the key.
 __device__ __forceinline__ bool kv_sees(int key, int pos, int window, int sinks) {
-    return key <= pos && (window == 0 || key > pos - window || key < sinks);
+    return (key <= pos) & ((window == 0) | (key > pos - window) | (key < sinks));
 }
+// The same in an item's numbers: the row sees number j if j <= hi and not from <= j <= to.
+struct KvSeen {
+    int hi, from, to;
+    __device__ __forceinline__ KvSeen(const KvItem& it, int pos, int window, int sinks) {
+        // the last number whose key is at most x
+        auto upto = [&](int x) { return x < it.sink_end ? x : max(it.sink_end - 1, x - it.gap); };
+        hi = min(upto(pos), it.j1 - 1);
+        from = upto(sinks - 1) + 1;
+        to = window ? upto(pos - window) : -1;
+    }
+};
 
-// Where the sums of a token's row go: the record, or the result itself.
+// Split work: a piece of a token's keys leaves, for each query head, its sums and {maximum,
+// sum of weights} in a record; a kernel of its own joins them in the records' order.  (Joined by the piece that arrives last,
+// with stores and loads past the XCDs' L2s: 28.8 us against 16.2 + 6.2 for one row of 8192 keys, 32 heads of 128 on 8.)
 __device__ __forceinline__ size_t kv_record(const KvItem& it, const KvTok& t, int n_heads, int head) {
     const int s = (it.rec & KV_REC_OWN) ? (it.rec & ~KV_REC_OWN) + (t.own_n & 0xFFFF) : it.rec;
     return ((size_t)t.rec + s) * n_heads + head;
@@ -123,7 +155,7 @@ __device__ __forceinline__ size_t kv_record(const KvItem& it, const KvTok& t, in
 // there, and hidden keys carry weight zero rather than being left out.  Blocks of `block` numbers every `step`
 // from `from` on.  Lane l ends with dims l, l + 64, ...; m and l are every lane's.
 template <typename E, int DE>
-__device__ __noinline__ void kv_row_plain(const KvAttnArgs& a, const KvItem& it, const int* table, int h, size_t q_at, int pos,
+__device__ __forceinline__ void kv_row_plain(const KvAttnArgs& a, const KvItem& it, const int* table, int h, size_t q_at, int pos,
                                           int from, int block, int step, float& m, float& l, float (&acc)[DE]) {
     const int lane = threadIdx.x & 63, hd = a.pages.hd;
     float qv[DE];
@@ -138,7 +170,7 @@ __device__ __noinline__ void kv_row_plain(const KvAttnArgs& a, const KvItem& it,
         for (int j = base; j < min(it.j1, base + block); j++) {
             const int key = kv_key(it, j);
             if (!kv_sees(key, pos, a.window, a.sinks)) continue;
-            const size_t row = (size_t)kv_row(a.pages, table, h, key) * hd;
+            const size_t row = (size_t)kv_row(a.pages, table[key >> a.pages.shift], h, key) * hd;
             float d = 0.0f;
 #pragma unroll
             for (int e = 0; e < DE; e++)

@@ -1,5 +1,5 @@
 // Attention over a paged cache for at most 16 rows (new tokens x query heads of
-// one kv head): decode steps, and the merge of split work.
+// one kv head): decode steps; and the join of split work.
 //
 //   o = sum_j 2^(s_j - m) v_j / sum_j 2^(s_j - m),  s_j = q.k_j * scale * log2(e)
 //
@@ -30,25 +30,32 @@ __global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void kv_attn_rows_kernel(KvA
     constexpr size_t REGION = std::max((size_t)KB * LD * 2, (size_t)16 * D * 4);
     __shared__ __align__(16) char lds[4 * REGION];
     __shared__ float sm[4][16], sl[4][16], sM[16];
-    const KvPlanHead& head = *(const KvPlanHead*)a.plan;
-    const KvTok* toks = (const KvTok*)(a.plan + KV_HEAD_WORDS);
-    const KvItem* items = (const KvItem*)(a.plan + head.rows_items);
+    const KvTok* toks = a.toks;
     const int kvh = a.pages.n_kv_heads, h = blockIdx.x % kvh, G = a.n_heads / kvh, hd = PAD ? a.pages.hd : D, nch = hd / 8;
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int g = lane >> 4, r = lane & 15;
     E* vs = (E*)(lds + wave * REGION);
-    for (int n = blockIdx.x / kvh; n < head.n_rows_items; n += gridDim.x / kvh) {
-        const KvItem it = items[n];
+    // the first item is read before it is known to be there (the list has room for the grid)
+    const int count = __builtin_amdgcn_readfirstlane(*a.n_items);
+    int n = blockIdx.x / kvh;
+    KvItem it = kv_item(a.items, n);
+    for (; n < count; it = kv_item(a.items, n)) {
         const int R = it.ntok * G, row = min(r, R - 1);
         const KvTok tok = toks[it.tok0 + row / G];
         const int* table = a.pages.table + (size_t)it.seq * a.pages.pages_per_seq;
         auto q_at = [&](const KvTok& t, int rw) { return ((size_t)t.row * a.n_heads + h * G + rw % G) * hd; };
 
-        // this block's K and V rows: lane (g, r) finds keys r and 16 + r
+        // the pages and rows of a block's keys: lane (g, r) has keys r and 16 + r
+        int pg[2];
         uint32_t rn[2];
+        auto key_of = [&](int j0, int t) { return kv_key(it, min(j0 + 16 * t + r, it.j1 - 1)); };
         auto find = [&](int j0) {
 #pragma unroll
-            for (int t = 0; t < 2; t++) rn[t] = kv_row(a.pages, table, h, kv_key(it, min(j0 + 16 * t + r, it.j1 - 1)));
+            for (int t = 0; t < 2; t++) pg[t] = table[key_of(j0, t) >> a.pages.shift];
+        };
+        auto place = [&](int j0) {
+#pragma unroll
+            for (int t = 0; t < 2; t++) rn[t] = kv_row(a.pages, pg[t], h, key_of(j0, t));
         };
         kv_u4_t k[2][NK], v[VL];
         auto load_k = [&]() {
@@ -69,9 +76,10 @@ __global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void kv_attn_rows_kernel(KvA
         };
         int j = it.j0 + wave * KB;
         find(j);
+        place(j);
+        find(j + 4 * KB);
         load_k();
         load_v();
-        find(j + 4 * KB);
 
         // the queries: B operand, lane (g, r) dims 32c + 8g.. of row r
         x8 q[NP][NK];
@@ -84,15 +92,14 @@ __global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void kv_attn_rows_kernel(KvA
             }
         } else {
             float x[NK][8], mx = 0.0f;
+            kv_load_row<NK>(a.q, a.qdt, q_at(tok, row), [&](int c) { return PAD ? min(4 * c + g, nch - 1) : 4 * c + g; }, x);
 #pragma unroll
-            for (int c = 0; c < NK; c++) {
-                kv_load_q8(a.q, a.qdt, q_at(tok, row) + (PAD ? min(4 * c + g, nch - 1) : 4 * c + g) * 8, x[c]);
+            for (int c = 0; c < NK; c++)
 #pragma unroll
                 for (int i = 0; i < 8; i++) {
                     if (PAD && 4 * c + g >= nch) x[c][i] = 0.0f;
                     mx = fmaxf(mx, fabsf(x[c][i]));
                 }
-            }
             mx = fmaxf(mx, __shfl_xor(mx, 16, 64));
             mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
             qe = range_exp(mx, KV_Q_TOP);
@@ -107,6 +114,7 @@ __global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void kv_attn_rows_kernel(KvA
                 }
         }
         const float scale = NP == 1 ? a.scale : __builtin_amdgcn_ldexpf(a.scale, qe);
+        const KvSeen see(it, tok.pos, a.window, a.sinks);
         float m = -INFINITY, l = 0.0f;
         kv_f32x4_t o[NDT];
 #pragma unroll
@@ -122,19 +130,22 @@ __global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void kv_attn_rows_kernel(KvA
 #pragma unroll
                     for (int c = 0; c < NK; c++) s[t] = kv_mfma16(__builtin_bit_cast(x8, k[t][c]), q[u][c], s[t]);
             }
-            load_k();  // of the next block (past the last: its last row again)
+            // the next block (past the last: its last row again)
+            place(j + 4 * KB);
+            find(j + 8 * KB);
+            load_k();
             float bm = -INFINITY;
+            const int hi = see.hi - j - 4 * g, from = see.from - j - 4 * g, to = see.to - j - 4 * g;
 #pragma unroll
             for (int t = 0; t < 2; t++)
 #pragma unroll
                 for (int i = 0; i < 4; i++) {
-                    const int jj = j + 16 * t + 4 * g + i;
-                    const bool seen = jj < it.j1 && kv_sees(kv_key(it, jj), tok.pos, a.window, a.sinks);
-                    s[t][i] = seen ? s[t][i] * scale : -INFINITY;
+                    const int x = 16 * t + i;
+                    s[t][i] = (x <= hi) & ((x < from) | (x > to)) ? s[t][i] : -INFINITY;
                     bm = fmaxf(bm, s[t][i]);
                 }
             bm = fmaxf(bm, __shfl_xor(bm, 16, 64));
-            bm = fmaxf(bm, __shfl_xor(bm, 32, 64));
+            bm = fmaxf(bm, __shfl_xor(bm, 32, 64)) * scale;
             const float mn = fmaxf(m, bm), ref = mn == -INFINITY ? 0.0f : mn, f = kv_exp2(m - ref);
             float ps = 0.0f;
             x8 p[NP];
@@ -142,7 +153,7 @@ __global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void kv_attn_rows_kernel(KvA
             for (int t = 0; t < 2; t++)
 #pragma unroll
                 for (int i = 0; i < 4; i++) {
-                    const float e = kv_exp2(s[t][i] - ref);
+                    const float e = kv_exp2(__builtin_fmaf(s[t][i], scale, -ref));
                     ps += e;
                     E part[NP];
                     kv_split<E, NP>(NP == 1 ? e : e * KV_P_UP, part);
@@ -156,7 +167,6 @@ __global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void kv_attn_rows_kernel(KvA
                 *(kv_u4_t*)(vs + (lane + 64 * i) / CPR * LD + lane % CPR * 8) = v[i];
             wave_lds_fence();
             load_v();
-            find(j + 8 * KB);
 #pragma unroll
             for (int dt = 0; dt < NDT; dt++) {
                 // lane r addresses four dims of key r >> 2 of its group's four, and gets its dim of all four
@@ -231,58 +241,101 @@ __global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void kv_attn_rows_kernel(KvA
                 if (d == 0) a.rec_ml[rec] = make_float2(sM[rw], sl[0][rw]);
             }
         }
+        n += gridDim.x / kvh;
+        if (n >= count) break;
         __syncthreads();  // the next item writes these rows
     }
 }
 
-// One wave per (token, query head): the records of its pieces joined in order.
-template <int DE>
-__global__ __launch_bounds__(256) void kv_attn_merge_kernel(KvAttnArgs a) {
-    const KvPlanHead& head = *(const KvPlanHead*)a.plan;
-    const KvTok* toks = (const KvTok*)(a.plan + KV_HEAD_WORDS);
-    const int* list = a.plan + head.merge;
-    const int lane = threadIdx.x & 63, hd = a.pages.hd;
-    const int total = head.n_merge * a.n_heads;
-    for (int x = blockIdx.x * 4 + (threadIdx.x >> 6); x < total; x += gridDim.x * 4) {
-        const KvTok t = toks[list[x / a.n_heads]];
-        const int hq = x % a.n_heads, n = t.own_n >> 16;
+// Records joined: WR waves for each (token, query head), wave w the records w, w + WR, ...
+// with lane l on dims DE l .. ; the waves meet in LDS.  Few rows take all four waves of a
+// workgroup (latency: one round of loads for 64 records), many one wave each.
+template <int DE, int WR>
+__global__ __launch_bounds__(256) void kv_attn_join_kernel(KvAttnArgs a, const int* __restrict__ list) {
+    constexpr int U = DE == 4 ? 8 : 16, RPB = 4 / WR;
+    __shared__ float sA[WR > 1 ? 4 : 1][64 * DE], sM[4], sL[4];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), hd = a.pages.hd, d0 = lane * DE;
+    const int total = *a.n_items * a.n_heads, part = wave % WR;
+    const size_t step = (size_t)a.n_heads * hd;
+    for (int x0 = blockIdx.x * RPB; x0 < total; x0 += gridDim.x * RPB) {
+        const int x = min(x0 + wave / WR, total - 1), hq = x % a.n_heads;
+        const KvTok t = a.toks[list[x / a.n_heads]];
+        const int n = t.own_n >> 16, mine = (n - part + WR - 1) / WR;  // this wave's records
         const float2* ml = a.rec_ml + (size_t)t.rec * a.n_heads + hq;
-        const float* po = a.rec_o + ((size_t)t.rec * a.n_heads + hq) * hd;
-        const size_t step = (size_t)a.n_heads * hd;
-        // lane s looks at records s, s + 64, ...
+        const float* po = a.rec_o + ((size_t)t.rec * a.n_heads + hq) * hd + (d0 < hd ? d0 : 0);
         float M = -INFINITY, L = 0.0f, A[DE];
-        for (int s = lane; s < n; s += 64) M = fmaxf(M, ml[(size_t)s * a.n_heads].x);
-        M = wave_max(M);
 #pragma unroll
         for (int e = 0; e < DE; e++) A[e] = 0.0f;
-        for (int s0 = 0; s0 < n; s0 += 64) {
-            float2 w = make_float2(0.0f, 0.0f);
-            if (s0 + lane < n) w = ml[(size_t)(s0 + lane) * a.n_heads];
-            const float f = w.x == -INFINITY && w.y == 0.0f ? 0.0f : kv_exp2(w.x - M);
-            L += f * w.y;
-            const int here = min(64, n - s0);
-            for (int u0 = 0; u0 < here; u0 += 8) {
-                float v[8][DE];
+        for (int s0 = 0; s0 < mine; s0 += U) {
+            typedef float vec __attribute__((ext_vector_type(DE == 1 ? 2 : DE)));
+            float v[U][DE];
 #pragma unroll
-                for (int u = 0; u < 8; u++)
+            for (int u = 0; u < U; u++) {
+                const float* p = po + (size_t)(min(s0 + u, mine - 1) * WR + part) * step;
+                if constexpr (DE == 1) v[u][0] = *p;
+                else {
+                    const vec w = *(const vec*)p;
 #pragma unroll
-                    for (int e = 0; e < DE; e++)
-                        v[u][e] = lane + 64 * e < hd ? po[(size_t)(s0 + min(u0 + u, here - 1)) * step + lane + 64 * e] : 0.0f;
+                    for (int e = 0; e < DE; e++) v[u][e] = w[e];
+                }
+            }
+            const int sl = s0 + (lane & (U - 1));
+            const float2 w = ml[(size_t)(min(sl, mine - 1) * WR + part) * a.n_heads];
+            const bool none = sl >= mine || (w.x == -INFINITY && w.y == 0.0f);  // no record, or one without a key that the row sees
+            const float mn = fmaxf(M, group_max<16>(none ? -INFINITY : w.x)), ref = mn == -INFINITY ? 0.0f : mn;
+            const float f = none ? 0.0f : kv_exp2(w.x - ref), back = kv_exp2(M - ref);
+            L = L * back + (lane < U ? f * w.y : 0.0f);
 #pragma unroll
-                for (int u = 0; u < 8; u++) {
-                    const float fu = __shfl(f, u0 + u < here ? u0 + u : 0, 64);
-                    if (u0 + u < here) {
+            for (int e = 0; e < DE; e++) A[e] *= back;
+            M = mn;
 #pragma unroll
-                        for (int e = 0; e < DE; e++) A[e] = __builtin_fmaf(fu, v[u][e], A[e]);
-                    }
+            for (int u = 0; u < U; u++) {
+                const float fu = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(f), u));
+                if (s0 + u < mine) {
+#pragma unroll
+                    for (int e = 0; e < DE; e++) A[e] = __builtin_fmaf(fu, v[u][e], A[e]);
                 }
             }
         }
         L = wave_sum(L);
+        if constexpr (WR > 1) {
+            __syncthreads();  // the last row's sums have been read
 #pragma unroll
-        for (int e = 0; e < DE; e++)
-            if (lane + 64 * e < hd) kv_store_out(a.out, a.odt, ((size_t)t.row * a.n_heads + hq) * hd + lane + 64 * e, A[e] / L);
+            for (int e = 0; e < DE; e++) sA[wave][d0 + e] = A[e];
+            if (lane == 0) { sM[wave] = M; sL[wave] = L; }
+            __syncthreads();
+            if (wave > 0) continue;
+            M = fmaxf(fmaxf(sM[0], sM[1]), fmaxf(sM[2], sM[3]));
+            L = 0.0f;
+#pragma unroll
+            for (int e = 0; e < DE; e++) A[e] = 0.0f;
+#pragma unroll
+            for (int w = 0; w < WR; w++) {
+                const float f = sM[w] == -INFINITY && sL[w] == 0.0f ? 0.0f : kv_exp2(sM[w] - M);
+                L = __builtin_fmaf(f, sL[w], L);
+#pragma unroll
+                for (int e = 0; e < DE; e++) A[e] = f == 0.0f ? A[e] : __builtin_fmaf(f, sA[w][d0 + e], A[e]);
+            }
+        }
+        if (d0 < hd && x == x0 + wave / WR) {
+#pragma unroll
+            for (int e = 0; e < DE; e++) kv_store_out(a.out, a.odt, ((size_t)t.row * a.n_heads + hq) * hd + d0 + e, A[e] / L);
+        }
     }
+}
+
+void launch_kv_attn_join(const KvAttnArgs& a, const int* list, size_t grid, hipStream_t s) {
+    if (grid == 0) return;
+    const size_t rows = grid * a.n_heads;
+    auto with = [&](auto de) {
+        constexpr int DE = decltype(de)::value;
+        if (rows <= 1024) TH_LAUNCH((kv_attn_join_kernel<DE, 4>), dim3((unsigned)rows), dim3(256), 0, s, a, list);
+        else TH_LAUNCH((kv_attn_join_kernel<DE, 1>), dim3((unsigned)ceil_div(rows, (size_t)4)), dim3(256), 0, s, a, list);
+    };
+    if (a.pages.hd <= 64) with(std::integral_constant<int, 1>{});
+    else if (a.pages.hd <= 128) with(std::integral_constant<int, 2>{});
+    else with(std::integral_constant<int, 4>{});
+    TH_LAUNCH_CHECK();
 }
 
 template <int D, typename E>
@@ -308,15 +361,6 @@ void launch_kv_attn_rows(const KvAttnArgs& a, th_dtype cache, size_t grid, hipSt
     };
     if (cache == TH_F16) with((_Float16)0);
     else with((__bf16)0.0f);
-}
-
-void launch_kv_attn_merge(const KvAttnArgs& a, size_t grid, hipStream_t s) {
-    if (grid == 0) return;
-    const unsigned g = (unsigned)ceil_div(grid * a.n_heads, (size_t)4);
-    if (a.pages.hd <= 64) TH_LAUNCH(kv_attn_merge_kernel<1>, dim3(g), dim3(256), 0, s, a);
-    else if (a.pages.hd <= 128) TH_LAUNCH(kv_attn_merge_kernel<2>, dim3(g), dim3(256), 0, s, a);
-    else TH_LAUNCH(kv_attn_merge_kernel<4>, dim3(g), dim3(256), 0, s, a);
-    TH_LAUNCH_CHECK();
 }
 
 }  // namespace th

@@ -18,53 +18,62 @@ namespace th {
 template <int D, typename E, int NP, bool PAD>
 __global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void kv_attn_tiles_kernel(KvAttnArgs a) {
     typedef typename KvVec<E>::x8 x8;
+    constexpr int KB = D <= 64 || (D <= 128 && NP == 1) ? 64 : 32, KT = KB / 32, NS = D / 16, NDT = D / 32, CPR = D / 8;
+    constexpr int NL = KB * CPR / 256, RPI = 64 / CPR, DE = D / 64;
     // LDS rows of K end in 16 bytes (16-byte reads of 16 rows then meet all banks),
-    // those of V in 64 (four rows of 32 bytes, as the transposing reads take them)
-    constexpr int KB = D <= 128 ? 64 : 32, KT = KB / 32, NS = D / 16, NDT = D / 32, LK = D + 8, LV = D + 32, CPR = D / 8;
-    constexpr int NL = KB * CPR / 256, DE = D / 64;
-    __shared__ __align__(16) E ks[KB * LK], vs[KB * LV];
-    const KvPlanHead& head = *(const KvPlanHead*)a.plan;
-    const KvTok* toks = (const KvTok*)(a.plan + KV_HEAD_WORDS);
-    const KvItem* items = (const KvItem*)(a.plan + head.tile_items);
+    // those of V in 64 (the transposing reads take 32 bytes of each of four rows).
+    // Two blocks: one is filled while the other is read.
+    constexpr int LK = D + 8, LV = D + 32;
+    __shared__ __align__(16) E lds[2][KB * (LK + LV)];
+    const KvTok* toks = a.toks;
     const int kvh = a.pages.n_kv_heads, hk = blockIdx.x % kvh, G = a.n_heads / kvh, hd = PAD ? a.pages.hd : D, nch = hd / 8;
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int h = lane >> 5, c = lane & 31;
-    for (int n = blockIdx.x / kvh; n < head.n_tile_items; n += gridDim.x / kvh) {
-        const KvItem it = items[n];
-        const int R = it.ntok * G, row = min(wave * 32 + c, R - 1);
-        const bool live = wave * 32 + c < R;
-        const KvTok tok = toks[it.tok0 + row / G];
-        const int hq = hk * G + row % G;
+    // the first item is read before it is known to be there (the list has room for the grid)
+    const int count = __builtin_amdgcn_readfirstlane(*a.n_items);
+    int n = blockIdx.x / kvh;
+    KvItem it = kv_item(a.items, n);
+    for (; n < count; it = kv_item(a.items, n)) {
         const int* table = a.pages.table + (size_t)it.seq * a.pages.pages_per_seq;
-        // the wave's lowest and highest positions: which blocks need no mask, and which no work
-        int p_lo = tok.pos, p_hi = tok.pos;
-#pragma unroll
-        for (int x = 16; x > 0; x >>= 1) {
-            p_lo = min(p_lo, __shfl_xor(p_lo, x, 64));
-            p_hi = max(p_hi, __shfl_xor(p_hi, x, 64));
-        }
-        p_lo = __builtin_amdgcn_readfirstlane(p_lo);
-        p_hi = __builtin_amdgcn_readfirstlane(p_hi);
-
-        uint32_t rn[NL];
+        // piece i of this thread: 16 bytes of row (tid + 256 i) / CPR
+        int pg[NL];
+        kv_u4_t kr[NL], vr[NL];
+        auto key_of = [&](int j0, int i) { return kv_key(it, min(j0 + (tid + 256 * i) / CPR, it.j1 - 1)); };
         auto find = [&](int j0) {
 #pragma unroll
-            for (int i = 0; i < NL; i++)
-                rn[i] = kv_row(a.pages, table, hk, kv_key(it, min(j0 + (tid + 256 * i) / CPR, it.j1 - 1)));
+            for (int i = 0; i < NL; i++) pg[i] = table[key_of(j0, i) >> a.pages.shift];
         };
-        kv_u4_t kr[NL], vr[NL];
-        const int chunk = PAD ? min(tid % CPR, nch - 1) : tid % CPR;
-        auto load = [&]() {
+        auto load = [&](int j0) {
 #pragma unroll
             for (int i = 0; i < NL; i++) {
-                const size_t at = (size_t)rn[i] * hd + chunk * 8;
+                const size_t at = (size_t)kv_row(a.pages, pg[i], hk, key_of(j0, i)) * hd + (PAD ? min(tid % CPR, nch - 1) : tid % CPR) * 8;
                 kr[i] = *(const kv_u4_t*)((const E*)a.pages.k + at);
                 vr[i] = *(const kv_u4_t*)((const E*)a.pages.v + at);
             }
         };
         find(it.j0);
-        load();
+        load(it.j0);
         find(it.j0 + KB);
+
+        const int R = it.ntok * G, row = min(wave * 32 + c, R - 1);
+        const bool live = wave * 32 + c < R;
+        const KvTok tok = toks[it.tok0 + row / G];
+        const int hq = hk * G + row % G;
+        // which blocks need no mask, and which no work, for this wave's rows
+        const KvSeen see(it, tok.pos, a.window, a.sinks);
+        int hi_lo = see.hi, hi_hi = see.hi, to_lo = see.to, to_hi = see.to;
+#pragma unroll
+        for (int x = 16; x > 0; x >>= 1) {
+            hi_lo = min(hi_lo, __shfl_xor(hi_lo, x, 64));
+            hi_hi = max(hi_hi, __shfl_xor(hi_hi, x, 64));
+            to_lo = min(to_lo, __shfl_xor(to_lo, x, 64));
+            to_hi = max(to_hi, __shfl_xor(to_hi, x, 64));
+        }
+        hi_lo = __builtin_amdgcn_readfirstlane(hi_lo);
+        hi_hi = __builtin_amdgcn_readfirstlane(hi_hi);
+        to_lo = __builtin_amdgcn_readfirstlane(to_lo);
+        to_hi = __builtin_amdgcn_readfirstlane(to_hi);
+        const int hidden = __builtin_amdgcn_readfirstlane(see.from);  // the same for all rows
 
         // the queries: B operand, lane (h, c) dims 16s + 8h.. of row c
         x8 q[NP][NS];
@@ -77,27 +86,26 @@ __global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void kv_attn_tiles_kernel(Kv
                 if (PAD && 2 * s + h >= nch) q[0][s] = x8{};
             }
         } else {
-            float mx = 0.0f;
-            for (int s = 0; s < NS; s++) {
-                float x[8];
-                kv_load_q8(a.q, a.qdt, q_at + (PAD ? min(2 * s + h, nch - 1) : 2 * s + h) * 8, x);
+            float x[NS][8], mx = 0.0f;
+            kv_load_row<NS>(a.q, a.qdt, q_at, [&](int s) { return PAD ? min(2 * s + h, nch - 1) : 2 * s + h; }, x);
 #pragma unroll
-                for (int i = 0; i < 8; i++) mx = fmaxf(mx, fabsf(x[i]));
-            }
+            for (int s = 0; s < NS; s++)
+#pragma unroll
+                for (int i = 0; i < 8; i++) {
+                    if (PAD && 2 * s + h >= nch) x[s][i] = 0.0f;
+                    mx = fmaxf(mx, fabsf(x[s][i]));
+                }
             mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
             qe = range_exp(mx, KV_Q_TOP);
 #pragma unroll
-            for (int s = 0; s < NS; s++) {
-                float x[8];
-                kv_load_q8(a.q, a.qdt, q_at + (PAD ? min(2 * s + h, nch - 1) : 2 * s + h) * 8, x);
+            for (int s = 0; s < NS; s++)
 #pragma unroll
                 for (int i = 0; i < 8; i++) {
                     E part[NP];
-                    kv_split<E, NP>(PAD && 2 * s + h >= nch ? 0.0f : __builtin_amdgcn_ldexpf(x[i], -qe), part);
+                    kv_split<E, NP>(__builtin_amdgcn_ldexpf(x[s][i], -qe), part);
 #pragma unroll
                     for (int u = 0; u < NP; u++) q[u][s][i] = part[u];
                 }
-            }
         }
         const float scale = NP == 1 ? a.scale : __builtin_amdgcn_ldexpf(a.scale, qe);
         float m = -INFINITY, l = 0.0f;
@@ -107,19 +115,8 @@ __global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void kv_attn_tiles_kernel(Kv
 #pragma unroll
             for (int i = 0; i < 16; i++) o[t][i] = 0.0f;
 
-        for (int j = it.j0; j < it.j1; j += KB) {
-            __syncthreads();  // the previous block's reads are done
-#pragma unroll
-            for (int i = 0; i < NL; i++) {
-                const int key = (tid + 256 * i) / CPR;
-                *(kv_u4_t*)(ks + key * LK + tid % CPR * 8) = kr[i];
-                *(kv_u4_t*)(vs + key * LV + tid % CPR * 8) = vr[i];
-            }
-            __syncthreads();
-            load();  // the next block (past the last: its last row again)
-            find(j + 2 * KB);
-            const int k_lo = kv_key(it, j), k_hi = kv_key(it, min(j + KB, it.j1) - 1);
-            if (k_lo > p_hi) continue;  // wave-uniform: every key is behind this wave's rows
+        auto block = [&](const E* ks, const E* vs, int j) {
+            if (j > hi_hi || (j >= hidden && j + KB - 1 <= to_lo)) return;  // wave-uniform: no row sees any of it
             kv_f32x16_t s[KT];
 #pragma unroll
             for (int t = 0; t < KT; t++) {
@@ -133,29 +130,22 @@ __global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void kv_attn_tiles_kernel(Kv
                 }
             }
             kv_mfma_wait();
-            const bool whole = j + KB <= it.j1 && k_hi <= p_lo &&
-                               (a.window == 0 || k_lo > p_hi - a.window || (k_hi < a.sinks));
-            float bm = -INFINITY;
-            if (whole) {
+            if (j + KB - 1 > hi_lo || (j <= to_hi && j + KB - 1 >= hidden)) {
+                const int hi = see.hi - j - 4 * h, from = see.from - j - 4 * h, to = see.to - j - 4 * h;
 #pragma unroll
                 for (int t = 0; t < KT; t++)
 #pragma unroll
                     for (int i = 0; i < 16; i++) {
-                        s[t][i] *= scale;
-                        bm = fmaxf(bm, s[t][i]);
-                    }
-            } else {
-#pragma unroll
-                for (int t = 0; t < KT; t++)
-#pragma unroll
-                    for (int i = 0; i < 16; i++) {
-                        const int jj = j + t * 32 + 8 * (i >> 2) + 4 * h + (i & 3);
-                        const bool seen = jj < it.j1 && kv_sees(kv_key(it, jj), tok.pos, a.window, a.sinks);
-                        s[t][i] = seen ? s[t][i] * scale : -INFINITY;
-                        bm = fmaxf(bm, s[t][i]);
+                        const int x = t * 32 + 8 * (i >> 2) + (i & 3);
+                        s[t][i] = (x <= hi) & ((x < from) | (x > to)) ? s[t][i] : -INFINITY;
                     }
             }
-            bm = fmaxf(bm, __shfl_xor(bm, 32, 64));
+            float bm = -INFINITY;
+#pragma unroll
+            for (int t = 0; t < KT; t++)
+#pragma unroll
+                for (int i = 0; i < 16; i++) bm = fmaxf(bm, s[t][i]);
+            bm = fmaxf(bm, __shfl_xor(bm, 32, 64)) * scale;
             const float mn = fmaxf(m, bm), ref = mn == -INFINITY ? 0.0f : mn, f = kv_exp2(m - ref);
             float ps = 0.0f;
             x8 p[NP][KT * 2];
@@ -163,7 +153,7 @@ __global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void kv_attn_tiles_kernel(Kv
             for (int t = 0; t < KT; t++)
 #pragma unroll
                 for (int i = 0; i < 16; i++) {
-                    const float e = kv_exp2(s[t][i] - ref);
+                    const float e = kv_exp2(__builtin_fmaf(s[t][i], scale, -ref));
                     ps += e;
                     E part[NP];
                     kv_split<E, NP>(NP == 1 ? e : e * KV_P_UP, part);
@@ -195,7 +185,22 @@ __global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void kv_attn_tiles_kernel(Kv
 #pragma unroll
                 for (int i = 0; i < 16; i++) o[dt][i] = __builtin_fmaf(o[dt][i], f, d[i]);
             }
+        };
+        for (int j = it.j0, b = 0; j < it.j1; j += KB, b ^= 1) {
+            E *ks = lds[b], *vs = ks + KB * LK;
+#pragma unroll
+            for (int i = 0; i < NL; i++) {
+                const int k = (tid + 256 * i) / CPR;
+                *(kv_u4_t*)(ks + k * LK + tid % CPR * 8) = kr[i];
+                *(kv_u4_t*)(vs + k * LV + tid % CPR * 8) = vr[i];
+            }
+            // behind the barrier the block is whole, and the other buffer's reads (a block ago) are done
+            __syncthreads();
+            load(j + KB);  // past the last: its last row again
+            find(j + 2 * KB);
+            block(ks, vs, j);
         }
+        kv_mfma_wait();
         l += __shfl_xor(l, 32, 64);
         bool fine = l == l;
 #pragma unroll
@@ -238,6 +243,9 @@ __global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void kv_attn_tiles_kernel(Kv
             }
             if (it.rec >= 0 && lane == 0) a.rec_ml[rx] = make_float2(pm, pl);
         }
+        n += gridDim.x / kvh;
+        if (n >= count) break;
+        __syncthreads();  // the next item's first block goes where this one's last may be read
     }
 }
 

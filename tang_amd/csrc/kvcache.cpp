@@ -48,7 +48,7 @@ static void require_open(const th_kv_cache* c, const char* what) {
 
 // Calls that change tables are made between replays, not recorded.
 static void require_eager(const th_kv_cache* c, const char* what) {
-    if (stream_capturing(c->dev->stream))
+    if (c->dev->capturing)
         throw Error(TH_ERR_INVALID, std::string(what) + ": changes the cache's tables and cannot be captured");
 }
 
@@ -78,8 +78,9 @@ static uint32_t* stage(th_kv_cache* c, size_t bytes, th_kv_stage*& st) {
     return (uint32_t*)st->host;
 }
 
-// The table entries that changed, and `words` to dst, in stream order.
-static void upload(th_kv_cache* c, const uint32_t* words, size_t n_words, void* dst) {
+// The table entries that changed, and `words` to the runs' places in dst, in stream order.
+static void upload(th_kv_cache* c, const uint32_t* words, const KvRuns& runs, void* dst) {
+    const size_t n_words = (size_t)runs.words();
     size_t pairs = 0;
     for (const auto& d : c->dirty) pairs += d.second;
     const size_t total = 2 * pairs + n_words;
@@ -94,12 +95,18 @@ static void upload(th_kv_cache* c, const uint32_t* words, size_t n_words, void* 
             to[at++] = (uint32_t)c->mirror[d.first + i];
         }
     if (n_words) std::memcpy(to + at, words, n_words * 4);
-    launch_kv_upload(w, st ? to : nullptr, (int)pairs, c->table, (int)n_words, (uint32_t*)dst, c->dev->stream);
+    launch_kv_upload(w, st ? to : nullptr, (int)pairs, c->table, runs, (uint32_t*)dst, c->dev->stream);
     if (st) {
         TH_HIP(hipEventRecord(st->done, c->dev->stream));
         st->used = true;
     }
     c->dirty.clear();
+}
+
+static KvRuns one_run(size_t n) {
+    KvRuns r;
+    r.n[0] = (int)n;
+    return r;
 }
 
 // {from, to} pages, every layer's K and V.
@@ -113,7 +120,7 @@ static void copy_pages(th_kv_cache* c, const std::vector<uint32_t>& pairs) {
         return;
     }
     uint32_t* dev = (uint32_t*)device_scratch(c->dev, 8 * n);
-    upload(c, pairs.data(), 2 * n, dev);
+    upload(c, pairs.data(), one_run(2 * n), dev);
     launch_kv_copy_pages(c->pool, c->page_bytes, c->n_pages, planes, dev, n, c->dev->stream);
 }
 
@@ -206,6 +213,7 @@ struct PlanTile { KvItem it; bool small, own; };
 
 // Shared prefixes shorter than this are read by each sequence.
 constexpr size_t KV_MIN_PREFIX = 128;
+constexpr size_t KV_MIN_ROWS_KEYS = 256, KV_MIN_TILE_KEYS = 256;
 
 class PlanMaker {
    public:
@@ -213,21 +221,23 @@ class PlanMaker {
         : b_(b), c_(b->cache), G_(b->n_heads / b->cache->n_kv_heads), window_(window), sinks_(sinks) {}
 
     void make() {
-        order();
-        for (size_t i = 0; i < tiles_.size(); i++) keys_[tiles_[i].small] += (size_t)(tiles_[i].it.j1 - tiles_[i].it.j0);
-        for (size_t scale = 1;; scale *= 2)
-            if (split(scale)) return;
+        order(true);
+        for (size_t scale = 1; !split(scale); scale *= 2) {
+            // nothing is split any more, and two records a token are still too many
+            if (scale > c_->max_len) order(false);
+        }
     }
 
-    // head, tokens, rows items, tile items, merge list
-    std::vector<uint32_t> words;
-    size_t n_items[2] = {0, 0}, n_merge = 0;  // [0] tiles, [1] rows
+    std::vector<uint32_t> words;  // head, tokens, rows items, tile items, joined tokens
+    size_t n_toks = 0, n_items[2] = {0, 0}, n_joins = 0;  // items: [0] tiles, [1] rows
 
    private:
     const int* table(int s) const { return c_->mirror.data() + (size_t)s * c_->pages_per_seq; }
 
     // Sequences whose first pages are the same, next to each other; the tokens in that order.
-    void order() {
+    void order(bool shared_prefixes) {
+        toks_.clear();
+        tiles_.clear();
         const size_t B = b_->seqs.size(), ps = c_->page_size;
         std::vector<size_t> row(B + 1, 0);
         for (size_t i = 0; i < B; i++) row[i + 1] = row[i] + b_->n[i];
@@ -235,7 +245,7 @@ class PlanMaker {
         std::unordered_map<int, size_t> by_page;
         for (size_t i = 0; i < B; i++) {
             if (b_->n[i] == 0) continue;
-            const bool can = b_->start[i] >= KV_MIN_PREFIX;
+            const bool can = shared_prefixes && b_->start[i] >= KV_MIN_PREFIX;
             const int first = can ? table(b_->seqs[i])[0] : -1;
             if (can && c_->refs[first] > 1) {
                 auto [at, fresh] = by_page.try_emplace(first, groups.size());
@@ -269,6 +279,8 @@ class PlanMaker {
                 at += b_->n[i];
             }
         }
+        keys_[0] = keys_[1] = 0;
+        for (const PlanTile& t : tiles_) keys_[t.small] += (size_t)(t.it.j1 - t.it.j0);
     }
 
     // Tokens [tok0, tok0 + n) against keys [from, to) of a sequence.
@@ -307,11 +319,12 @@ class PlanMaker {
 
     bool split(size_t scale) {
         const size_t kvh = c_->n_kv_heads, cus = (size_t)c_->dev->num_cus;
-        // Keys of a piece.  Rows items: the chip's 2 * CUs workgroups share the keys evenly, a
-        // workgroup has at least two 32-key blocks for each of its waves.  Tiles: the same with four blocks of 64.
+        // Keys of a piece.  The chip holds 2 * CUs workgroups at a time: pieces are a quarter of an even
+        // share, so that uneven lengths level out, but no less than a block for each wave (rows items) or
+        // four blocks (tiles).
         size_t per[2];
-        per[0] = round_up(std::max<size_t>(256, ceil_div(keys_[0] * kvh, 2 * cus)), 64) * scale;
-        per[1] = round_up(std::max<size_t>(256, ceil_div(keys_[1] * kvh, 2 * cus)), 128) * scale;
+        per[1] = round_up(std::max<size_t>(KV_MIN_ROWS_KEYS, ceil_div(keys_[1] * kvh, 8 * cus)), 64) * scale;
+        per[0] = round_up(std::max<size_t>(KV_MIN_TILE_KEYS, ceil_div(keys_[0] * kvh, 4 * cus)), 64) * scale;
         std::vector<int> shared(toks_.size(), 0), own(toks_.size(), 0), pieces(tiles_.size());
         size_t extra = 0;
         for (size_t i = 0; i < tiles_.size(); i++) {
@@ -323,7 +336,6 @@ class PlanMaker {
         }
         // The tokens of one tile have one count of records each kind, whatever tiles hold their other keys.
         size_t recs = 0;
-        std::vector<int> merge;
         for (size_t i = 0; i < toks_.size(); i++) {
             if (shared[i] + own[i] <= 1) continue;
             recs += (size_t)(shared[i] + own[i]);
@@ -357,14 +369,14 @@ class PlanMaker {
         }
         if (recs > b_->max_recs || tiles_.size() + extra > b_->max_items) return false;
         size_t rec = 0;
+        std::vector<int> joins;
         for (size_t i = 0; i < toks_.size(); i++) {
             KvTok& t = toks_[i];
             t.rec = (int)rec;
             t.own_n = shared[i] | (shared[i] + own[i]) << 16;
-            if (recorded[i]) {
-                rec += (size_t)(shared[i] + own[i]);
-                merge.push_back((int)i);
-            }
+            if (!recorded[i]) continue;
+            rec += (size_t)(shared[i] + own[i]);
+            joins.push_back((int)i);
         }
         std::vector<KvItem> items[2];
         for (size_t i = 0; i < tiles_.size(); i++) {
@@ -381,26 +393,27 @@ class PlanMaker {
             }
         }
         // the longest first: the last workgroups to start are short
-        std::stable_sort(items[0].begin(), items[0].end(), [](const KvItem& x, const KvItem& y) { return x.j1 - x.j0 > y.j1 - y.j0; });
-        KvPlanHead head = {};
-        head.n_rows_items = (int)items[1].size();
-        head.n_tile_items = (int)items[0].size();
-        head.n_merge = (int)merge.size();
-        head.rows_items = KV_HEAD_WORDS + (int)(toks_.size() * sizeof(KvTok) / 4);
-        head.tile_items = head.rows_items + (int)(items[1].size() * sizeof(KvItem) / 4);
-        head.merge = head.tile_items + (int)(items[0].size() * sizeof(KvItem) / 4);
-        words.resize((size_t)head.merge + merge.size());
-        std::memcpy(words.data(), &head, sizeof(head));
-        auto put = [&](size_t at, const void* p, size_t bytes) {
-            if (bytes) std::memcpy(words.data() + at, p, bytes);
-        };
-        put(KV_HEAD_WORDS, toks_.data(), toks_.size() * sizeof(KvTok));
-        put((size_t)head.rows_items, items[1].data(), items[1].size() * sizeof(KvItem));
-        put((size_t)head.tile_items, items[0].data(), items[0].size() * sizeof(KvItem));
-        put((size_t)head.merge, merge.data(), merge.size() * 4);
+        for (auto& v : items)
+            std::stable_sort(v.begin(), v.end(), [](const KvItem& x, const KvItem& y) { return x.j1 - x.j0 > y.j1 - y.j0; });
+        n_toks = toks_.size();
         n_items[0] = items[0].size();
         n_items[1] = items[1].size();
-        n_merge = merge.size();
+        n_joins = joins.size();
+        KvPlanHead head = {};
+        head.n_joins = (int)n_joins;
+        head.n_rows_items = (int)n_items[1];
+        head.n_tile_items = (int)n_items[0];
+        words.resize(KV_HEAD_WORDS + n_toks * sizeof(KvTok) / 4 + (n_items[0] + n_items[1]) * sizeof(KvItem) / 4 + n_joins);
+        uint32_t* to = words.data();
+        auto put = [&](const void* p, size_t bytes) {
+            if (bytes) std::memcpy(to, p, bytes);
+            to += bytes / 4;
+        };
+        put(&head, sizeof(head));
+        put(toks_.data(), n_toks * sizeof(KvTok));
+        put(items[1].data(), n_items[1] * sizeof(KvItem));
+        put(items[0].data(), n_items[0] * sizeof(KvItem));
+        put(joins.data(), n_joins * 4);
         return true;
     }
 
@@ -412,19 +425,32 @@ class PlanMaker {
     size_t keys_[2] = {0, 0};
 };
 
-static size_t plan_words(const th_kv_batch* b) {
-    return KV_HEAD_WORDS + b->max_rows * (sizeof(KvTok) / 4 + 1) + b->max_items * sizeof(KvItem) / 4;
-}
+// Where a plan's parts are, in words.
+static size_t plan_toks(const th_kv_batch*) { return KV_HEAD_WORDS; }
+static size_t plan_rows(const th_kv_batch* b) { return plan_toks(b) + b->max_rows * sizeof(KvTok) / 4; }
+static size_t plan_tiles(const th_kv_batch* b) { return plan_rows(b) + b->max_items * sizeof(KvItem) / 4; }
+static size_t plan_joins(const th_kv_batch* b) { return plan_tiles(b) + b->max_items * sizeof(KvItem) / 4; }
+static size_t plan_words(const th_kv_batch* b) { return plan_joins(b) + b->max_rows; }
 
 static void build_plan(th_kv_batch* b, std::pair<size_t, size_t> key, th_kv_batch::Plan& p) {
     p.built = false;
     PlanMaker m(b, key.first, key.second);
     m.make();
-    TH_REQUIRE(m.words.size() <= plan_words(b), "attention plan exceeds its block");
-    upload(b->cache, m.words.data(), m.words.size(), p.block);
+    KvRuns runs;
+    runs.n[0] = KV_HEAD_WORDS;
+    runs.n[1] = (int)(m.n_toks * sizeof(KvTok) / 4);
+    runs.at[1] = (int)plan_toks(b);
+    runs.n[2] = (int)(m.n_items[1] * sizeof(KvItem) / 4);
+    runs.at[2] = (int)plan_rows(b);
+    runs.n[3] = (int)(m.n_items[0] * sizeof(KvItem) / 4);
+    runs.at[3] = (int)plan_tiles(b);
+    runs.n[4] = (int)m.n_joins;
+    runs.at[4] = (int)plan_joins(b);
+    TH_REQUIRE(m.n_items[0] <= b->max_items && m.n_items[1] <= b->max_items, "attention plan exceeds its block");
+    upload(b->cache, m.words.data(), runs, p.block);
     p.n_tile_items = m.n_items[0];
     p.n_rows_items = m.n_items[1];
-    p.n_merge = m.n_merge;
+    p.n_joins = m.n_joins;
     p.built = true;
 }
 
@@ -602,7 +628,7 @@ int th_kv_cache_compact(th_kv_cache* c, size_t* n_moved) {
             }
             if (any) c->seqs[s].version = ++c->versions;
         }
-        upload(c, nullptr, 0, nullptr);
+        upload(c, nullptr, KvRuns(), nullptr);
     }
     if (n_moved) *n_moved = pairs.size() / 2;
     TH_API_END
@@ -713,7 +739,7 @@ int th_kv_seq_select(th_kv_cache* c, int32_t seq, const uint32_t* positions, siz
     touch(c, seq, 0, pages);
     if (n) {
         uint32_t* dev = (uint32_t*)device_scratch(c->dev, w.size() * 4);
-        upload(c, w.data(), w.size(), dev);
+        upload(c, w.data(), one_run(w.size()), dev);
         launch_kv_gather_rows(c->pool, c->n_pages, (int)(2 * c->n_layers), (int)c->n_kv_heads, c->shift, c->hd * 2, dev, dev + n, n,
                               c->dev->stream);
     }
@@ -734,7 +760,7 @@ int th_kv_seq_read(th_kv_cache* c, int32_t seq, size_t layer, size_t from, size_
     DeviceScope scope(c->dev);
     if (!c->dirty.empty()) {
         require_eager(c, __func__);
-        upload(c, nullptr, 0, nullptr);
+        upload(c, nullptr, KvRuns(), nullptr);
     }
     launch_kv_read(layer_pages(c, layer), seq, from, n, c->hd * 2, k->ptr, v->ptr, c->dev->stream);
     TH_API_END
@@ -754,13 +780,20 @@ int th_kv_batch_create(th_kv_cache* c, size_t max_seqs, size_t max_rows, size_t 
     b->max_seqs = max_seqs;
     b->max_rows = max_rows;
     b->n_heads = n_heads;
-    TH_HIP(hipMalloc((void**)&b->block, 16 + max_rows * sizeof(KvRow)));
-    // Pieces of attention work that a plan may have (split() stays below), and the
-    // records of tokens whose work is split: two for each row (a shared
-    // prefix and the own keys) and 4096 for the splits of few long rows.
+    // Pieces of attention work that a plan may have, and the records of tokens whose work
+    // is split (a plan that would need more splits less), 1 GiB of them at most.
     const size_t G = n_heads / c->n_kv_heads;
-    b->max_recs = 2 * max_rows + 4096;
+    b->max_recs = std::max<size_t>(64, std::min<size_t>(8192, ((size_t)1 << 30) / (n_heads * c->hd * 4)));
     b->max_items = 2 * (max_seqs + ceil_div(max_rows, std::max<size_t>(1, KV_TILE / G))) + 4096;
+    try {
+        TH_HIP(hipMalloc((void**)&b->block, 16 + max_rows * sizeof(KvRow)));
+        TH_HIP(hipMalloc((void**)&b->rec_o, b->max_recs * n_heads * c->hd * 4));
+        TH_HIP(hipMalloc((void**)&b->rec_ml, b->max_recs * n_heads * 8));
+    } catch (...) {
+        for (void* p : {(void*)b->block, (void*)b->rec_o, (void*)b->rec_ml})
+            if (p) (void)hipFree(p);
+        throw;
+    }
     c->live++;
     *out = b.release();
     TH_API_END
@@ -832,7 +865,7 @@ int th_kv_batch_begin(th_kv_batch* b, const int32_t* seqs, const uint32_t* n_new
     }
     b->rows = rows;
     copy_pages(c, copies);
-    upload(c, words.data(), words.size(), b->block);
+    upload(c, words.data(), one_run(words.size()), b->block);
     for (auto& p : b->plans) build_plan(b, p.first, p.second);
     b->begun = true;
     TH_API_END
@@ -859,7 +892,7 @@ int th_kv_append(th_kv_batch* b, size_t layer, const th_buffer* q, const th_buff
     TH_REQUIRE((q == nullptr) == (q_out == nullptr), "q and q_out go together");
     DeviceScope scope(c->dev);
     // a captured call runs on whatever the batch begins with later
-    const size_t rows = stream_capturing(c->dev->stream) ? b->max_rows : b->rows;
+    const size_t rows = c->dev->capturing ? b->max_rows : b->rows;
     const size_t kv = rows * c->n_kv_heads * c->hd, qn = rows * b->n_heads * c->hd;
     require_x(c, k, kv, "k");
     require_x(c, v, kv, "v");
@@ -891,7 +924,7 @@ int th_kv_batch_attention(th_kv_batch* b, size_t layer, const th_buffer* q, size
     TH_REQUIRE(q != out, "out must not be q");
     TH_REQUIRE(std::isfinite(scale) && scale >= 0.0f, "scale must be finite and not negative");
     DeviceScope scope(c->dev);
-    const bool capturing = stream_capturing(c->dev->stream);
+    const bool capturing = c->dev->capturing;
     const size_t n = (capturing ? b->max_rows : b->rows) * b->n_heads * c->hd;
     require_x(c, q, n, "q");
     require_x(c, out, n, "out");
@@ -902,10 +935,6 @@ int th_kv_batch_attention(th_kv_batch* b, size_t layer, const th_buffer* q, size
     auto at = b->plans.find(key);
     if (at == b->plans.end() || !at->second.built) {
         TH_REQUIRE(!capturing, "make the call once before it is captured");
-        if (!b->rec_o) {
-            TH_HIP(hipMalloc((void**)&b->rec_o, b->max_recs * b->n_heads * c->hd * sizeof(float)));
-        }
-        if (!b->rec_ml) TH_HIP(hipMalloc((void**)&b->rec_ml, b->max_recs * b->n_heads * sizeof(float2)));
         th_kv_batch::Plan& p = b->plans[key];
         if (!p.block) TH_HIP(hipMalloc((void**)&p.block, plan_words(b) * 4));
         build_plan(b, key, p);
@@ -914,7 +943,7 @@ int th_kv_batch_attention(th_kv_batch* b, size_t layer, const th_buffer* q, size
     const th_kv_batch::Plan& p = at->second;
     KvAttnArgs a;
     a.pages = layer_pages(c, layer);
-    a.plan = p.block;
+    a.toks = (const KvTok*)(p.block + plan_toks(b));
     a.q = q->ptr;
     a.out = out->ptr;
     a.qdt = q->dtype;
@@ -925,15 +954,20 @@ int th_kv_batch_attention(th_kv_batch* b, size_t layer, const th_buffer* q, size
     a.scale = (scale > 0.0f ? scale : 1.0f / std::sqrt((float)c->hd)) * 1.44269504f;
     a.rec_o = b->rec_o;
     a.rec_ml = b->rec_ml;
+    const KvPlanHead* head = (const KvPlanHead*)p.block;
     // A captured call runs whatever plan the batch has at replay: every kernel, on grids that walk
     // their lists.
-    const size_t some = std::max<size_t>(1, ceil_div(4 * (size_t)c->dev->num_cus, c->n_kv_heads));
+    const size_t some = std::min(b->max_items, ceil_div(4 * (size_t)c->dev->num_cus, c->n_kv_heads));
     const size_t tiles = capturing ? std::max(p.n_tile_items, some) : p.n_tile_items;
     const size_t rows = capturing ? std::max(p.n_rows_items, some) : p.n_rows_items;
-    const size_t merge = capturing ? std::max(p.n_merge, std::min<size_t>(b->max_rows, 1024)) : p.n_merge;
+    a.n_items = &head->n_tile_items;
+    a.items = (const KvItem*)(p.block + plan_tiles(b));
     launch_kv_attn_tiles(a, c->dtype, tiles, c->dev->stream);
+    a.n_items = &head->n_rows_items;
+    a.items = (const KvItem*)(p.block + plan_rows(b));
     launch_kv_attn_rows(a, c->dtype, rows, c->dev->stream);
-    launch_kv_attn_merge(a, merge, c->dev->stream);
+    a.n_items = &head->n_joins;
+    launch_kv_attn_join(a, p.block + plan_joins(b), capturing ? std::min<size_t>(b->max_rows, 1024) : p.n_joins, c->dev->stream);
     TH_API_END
 }
 

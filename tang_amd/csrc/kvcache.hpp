@@ -26,7 +26,7 @@ struct KvPages {
 struct KvRow { int seq, pos; };
 
 // A token of an attention plan: its row in the batch, its position, its first
-// record, and where its own keys' records start (low half) and how many records it has
+// record (-1: none), and where its own keys' records start (low half) and how many records it has
 // (high half).
 struct KvTok { int row, pos, rec, own_n; };
 
@@ -38,14 +38,16 @@ struct KvTok { int row, pos, rec, own_n; };
 struct KvItem { int tok0, ntok, seq, j0, j1, sink_end, gap, rec; };
 constexpr int KV_REC_OWN = 1 << 30;
 
-// An attention plan's block in device memory: these words, then tokens, rows
-// items, tile items and the tokens whose records are merged.
-struct KvPlanHead { int n_rows_items, n_tile_items, n_merge, rows_items, tile_items, merge, pad[2]; };
+// An attention plan in device memory: counts, tokens, the two kernels'
+// items and the tokens whose records are joined, each part at a place of its own that does not change with the step.
+struct KvPlanHead { int n_rows_items, n_tile_items, n_joins, pad; };
 constexpr int KV_HEAD_WORDS = sizeof(KvPlanHead) / 4;
 
 struct KvAttnArgs {
     KvPages pages;
-    const int* plan;
+    const int* n_items;   // of the kernel's items (the join: of tokens)
+    const KvItem* items;
+    const KvTok* toks;
     const void* q;
     void* out;
     th_dtype qdt, odt;
@@ -63,9 +65,15 @@ struct KvAttnArgs {
 constexpr int KV_ARG_WORDS = 224;
 struct KvWords { uint32_t w[KV_ARG_WORDS]; };
 
-// table[index] = value for n_pairs pairs, then n_words words to dst; both come
+// Runs of words that follow one another in an upload's source: their lengths and where each goes.
+struct KvRuns {
+    static constexpr int MAX = 5;
+    int n[MAX] = {}, at[MAX] = {};
+    __host__ __device__ int words() const { return n[0] + n[1] + n[2] + n[3] + n[4]; }
+};
+// table[index] = value for n_pairs pairs, then runs of words to dst; both come
 // from src (device-visible host memory) or, where that is null, from w.
-void launch_kv_upload(const KvWords& w, const uint32_t* src, int n_pairs, int* table, int n_words, uint32_t* dst,
+void launch_kv_upload(const KvWords& w, const uint32_t* src, int n_pairs, int* table, const KvRuns& runs, uint32_t* dst,
                       hipStream_t s);
 // Whole pages, every layer's K and V.  pairs (device): {from, to}.
 void launch_kv_copy_pages(void* pool, size_t page_bytes, size_t n_pages, int n_planes, const uint32_t* pairs, size_t n,
@@ -96,7 +104,7 @@ void launch_rope_rows(const KvRopeArgs& a, size_t n_rows, hipStream_t s);
 // grid: how many items the launch covers at a time (the kernels walk the rest).
 void launch_kv_attn_rows(const KvAttnArgs& a, th_dtype cache, size_t grid, hipStream_t s);
 void launch_kv_attn_tiles(const KvAttnArgs& a, th_dtype cache, size_t grid, hipStream_t s);
-void launch_kv_attn_merge(const KvAttnArgs& a, size_t grid, hipStream_t s);
+void launch_kv_attn_join(const KvAttnArgs& a, const int* list, size_t grid, hipStream_t s);
 
 // Rows (tokens x query heads of a kv head) that one item has at most.
 constexpr int KV_ROWS = 16, KV_TILE = 128;
@@ -169,11 +177,11 @@ struct th_kv_batch {
     int* block = nullptr;      // device: the number of rows (16 bytes), then KvRow[max_rows]
     struct Plan {
         int* block = nullptr;  // device
-        size_t n_rows_items = 0, n_tile_items = 0, n_merge = 0;
+        size_t n_rows_items = 0, n_tile_items = 0, n_joins = 0;
         bool built = false;    // for the batch as it is begun
     };
     std::map<std::pair<size_t, size_t>, Plan> plans;  // by window and sinks
-    float* rec_o = nullptr;    // records of split work, allocated with the first plan
+    float* rec_o = nullptr;    // records of split work
     float2* rec_ml = nullptr;
     size_t max_recs = 0, max_items = 0;
 };

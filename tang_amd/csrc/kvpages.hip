@@ -17,23 +17,30 @@ typedef uint32_t kv_u32x4_t __attribute__((ext_vector_type(4)));
 // need no copy, no staging memory and no event.  More comes from pinned host
 // memory, which the kernel reads across the bus by itself.
 __global__ __launch_bounds__(256) void kv_upload_kernel(KvWords w, const uint32_t* __restrict__ src, int n_pairs,
-                                                        int* __restrict__ table, int n_words, uint32_t* __restrict__ dst) {
+                                                        int* __restrict__ table, KvRuns runs, uint32_t* __restrict__ dst) {
     const int i0 = blockIdx.x * 256 + threadIdx.x, step = gridDim.x * 256;
-    if (src) {
-        for (int i = i0; i < n_pairs; i += step) table[src[2 * i]] = (int)src[2 * i + 1];
-        for (int i = i0; i < n_words; i += step) dst[i] = src[2 * n_pairs + i];
-    } else {
-        for (int i = i0; i < n_pairs; i += step) table[w.w[2 * i]] = (int)w.w[2 * i + 1];
-        for (int i = i0; i < n_words; i += step) dst[i] = w.w[2 * n_pairs + i];
+    for (int i = i0; i < n_pairs; i += step) {
+        if (src) table[src[2 * i]] = (int)src[2 * i + 1];
+        else table[w.w[2 * i]] = (int)w.w[2 * i + 1];
+    }
+    const int n_words = runs.words();
+    for (int i = i0; i < n_words; i += step) {
+        int to = i, end = 0;
+#pragma unroll
+        for (int r = 0; r < KvRuns::MAX; r++) {
+            if (i >= end) to = runs.at[r] + i - end;
+            end += runs.n[r];
+        }
+        dst[to] = src ? src[2 * n_pairs + i] : w.w[2 * n_pairs + i];
     }
 }
 
-void launch_kv_upload(const KvWords& w, const uint32_t* src, int n_pairs, int* table, int n_words, uint32_t* dst,
+void launch_kv_upload(const KvWords& w, const uint32_t* src, int n_pairs, int* table, const KvRuns& runs, uint32_t* dst,
                       hipStream_t s) {
-    const size_t n = (size_t)n_pairs + n_words;
+    const size_t n = (size_t)n_pairs + runs.words();
     if (n == 0) return;
     TH_LAUNCH(kv_upload_kernel, dim3((unsigned)std::min<size_t>(ceil_div(n, 256), 64)), dim3(256), 0, s, w, src, n_pairs, table,
-              n_words, dst);
+              runs, dst);
     TH_LAUNCH_CHECK();
 }
 

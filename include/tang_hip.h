@@ -468,7 +468,7 @@ typedef struct {
     th_dtype dtype;    /* TH_F16 or TH_BF16 */
     size_t n_layers, n_kv_heads;
     size_t head_dim;   /* a multiple of 8, at most 256 */
-    size_t page_size;  /* positions: a power of two from 8 to 1024 */
+    size_t page_size;  /* positions: a power of two from 16 to 1024 */
     size_t n_pages, max_seqs;
     size_t max_len;    /* of a sequence, at most 2^28 */
 } th_kv_cache_config;

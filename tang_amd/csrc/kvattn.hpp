@@ -54,6 +54,13 @@ constexpr float KV_P_UP = 16384.0f;
 
 __device__ __forceinline__ float kv_exp2(float x) { return __builtin_amdgcn_exp2f(x); }
 
+// A value that the compiler takes for a new one: what is computed from it stays where it is written. (Addresses that
+// a few instructions make again for each block would else fill registers for the whole loop.)
+__device__ __forceinline__ int kv_fresh(int x) {
+    asm volatile("" : "+v"(x));
+    return x;
+}
+
 // Chain of MFMAs before a branch: what follows may read their results.
 __device__ __forceinline__ void kv_mfma_wait() {
     __builtin_amdgcn_sched_barrier(0);
@@ -85,13 +92,14 @@ __device__ __forceinline__ void kv_load_row(const void* q, th_dtype dt, size_t a
         kv_u4_t v[N];
 #pragma unroll
         for (int i = 0; i < N; i++) v[i] = *(const kv_u4_t*)((const uint16_t*)q + at + 8 * chunk(i));
+        auto widen = [&](auto f) {
 #pragma unroll
-        for (int i = 0; i < N; i++)
+            for (int i = 0; i < N; i++)
 #pragma unroll
-            for (int e = 0; e < 8; e++) {
-                const uint16_t u = (uint16_t)(v[i][e >> 1] >> (16 * (e & 1)));
-                x[i][e] = dt == TH_F16 ? (float)__builtin_bit_cast(_Float16, u) : __uint_as_float((uint32_t)u << 16);
-            }
+                for (int e = 0; e < 8; e++) x[i][e] = f((uint16_t)(v[i][e >> 1] >> (16 * (e & 1))));
+        };
+        if (dt == TH_F16) widen([](uint16_t u) { return (float)__builtin_bit_cast(_Float16, u); });
+        else widen([](uint16_t u) { return __uint_as_float((uint32_t)u << 16); });
     }
 }
 
@@ -120,12 +128,57 @@ __device__ __forceinline__ KvItem kv_item(const KvItem* items, int n) {
     return KvItem{one(a[0]), one(a[1]), one(a[2]), one(a[3]), one(b[0]), one(b[1]), one(b[2]), one(b[3])};
 }
 
-// Key j of an item's numbers; the page that it is in; the row of its K and V.
-// (A page number is used an iteration after its load was issued: its wait would wait for every load before it.)
+// Key j of an item's numbers.
 __device__ __forceinline__ int kv_key(const KvItem& it, int j) { return j + (j >= it.sink_end ? it.gap : 0); }
 __device__ __forceinline__ uint32_t kv_row(const KvPages& p, int page, int h, int key) {
     return (((uint32_t)page * p.n_kv_heads + h) << p.shift) + (key & ((1 << p.shift) - 1));
 }
+
+// Where an item's keys lie.  Sixteen numbers from a multiple of 16 on are sixteen
+// neighbouring rows of one page (pages, hidden runs and pieces begin at multiples of 16), so
+// addresses are a scalar for sixteen rows and constants of the lane.  One load finds the pages of
+// the next 64 such groups, one a lane, a window ahead of their use.
+struct KvGroups {
+    const int* table;
+    int pages, next, base, last;  // this lane's pages; first group of the window; last group of the item
+    __device__ __forceinline__ int find(const KvPages& p, const KvItem& it, int b) const {
+        return table[kv_key(it, 16 * min(b + (int)(threadIdx.x & 63), last)) >> p.shift];
+    }
+    __device__ __forceinline__ KvGroups(const KvPages& p, const KvItem& it) {
+        table = p.table + (size_t)it.seq * p.pages_per_seq;
+        base = it.j0 >> 4;
+        last = max(it.j1 - 1, it.j0) >> 4;
+        pages = find(p, it, base);
+        next = pages;
+        if (base + 64 <= last) next = find(p, it, base + 64);
+    }
+    // before the rows of a block that begins at group b: blocks lie in one window each
+    __device__ __forceinline__ void reach(const KvPages& p, const KvItem& it, int b) {
+        if (b < base + 64 || b > last) return;  // (behind the end: the last group again)
+        base += 64;
+        pages = next;
+        if (base + 64 <= last) next = find(p, it, base + 64);
+    }
+    // element offset of group b's first row
+    __device__ __forceinline__ size_t at(const KvPages& p, const KvItem& it, int h, int hd, int b) const {
+        b = min(b, last);
+        const int page = __builtin_amdgcn_readlane(pages, min(b - base, 63));
+        return (size_t)kv_row(p, page, h, kv_key(it, 16 * b)) * hd;
+    }
+};
+// 16 bytes at a scalar place plus a lane's byte offset.
+template <typename E>
+__device__ __forceinline__ kv_u4_t kv_load16(const void* base, size_t at, uint32_t off) {
+    return *(const kv_u4_t*)((const char*)((const E*)base + at) + off);
+}
+
+// Largest of three (two fmaxf take up to four more instructions: each first quiets its operands).
+__device__ __forceinline__ float kv_max3(float a, float b, float c) {
+    float r;
+    asm("v_max3_f32 %0, %1, %2, %3" : "=v"(r) : "v"(a), "v"(b), "v"(c));
+    return r;
+}
+
 // Whether the row at position pos sees the key.
 __device__ __forceinline__ bool kv_sees(int key, int pos, int window, int sinks) {
     return (key <= pos) & ((window == 0) | (key > pos - window) | (key < sinks));

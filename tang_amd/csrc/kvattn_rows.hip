@@ -42,42 +42,34 @@ __global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void kv_attn_rows_kernel(KvA
     for (; n < count; it = kv_item(a.items, n)) {
         const int R = it.ntok * G, row = min(r, R - 1);
         const KvTok tok = toks[it.tok0 + row / G];
-        const int* table = a.pages.table + (size_t)it.seq * a.pages.pages_per_seq;
+        KvGroups groups(a.pages, it);
         auto q_at = [&](const KvTok& t, int rw) { return ((size_t)t.row * a.n_heads + h * G + rw % G) * hd; };
 
-        // the pages and rows of a block's keys: lane (g, r) has keys r and 16 + r
-        int pg[2];
-        uint32_t rn[2];
-        auto key_of = [&](int j0, int t) { return kv_key(it, min(j0 + 16 * t + r, it.j1 - 1)); };
-        auto find = [&](int j0) {
-#pragma unroll
-            for (int t = 0; t < 2; t++) pg[t] = table[key_of(j0, t) >> a.pages.shift];
-        };
-        auto place = [&](int j0) {
-#pragma unroll
-            for (int t = 0; t < 2; t++) rn[t] = kv_row(a.pages, pg[t], h, key_of(j0, t));
-        };
+        // K: lane (g, r) has row r of each group, pieces 4c + g.  V: piece lane + 64 i of the block.
         kv_u4_t k[2][NK], v[VL];
+        size_t at[2];
+        auto place = [&](int j0) {
+            groups.reach(a.pages, it, j0 >> 4);
+#pragma unroll
+            for (int t = 0; t < 2; t++) at[t] = groups.at(a.pages, it, h, hd, (j0 >> 4) + t);
+        };
         auto load_k = [&]() {
 #pragma unroll
-            for (int t = 0; t < 2; t++) {
-                const E* p = (const E*)a.pages.k + (size_t)rn[t] * hd;
+            for (int t = 0; t < 2; t++)
 #pragma unroll
-                for (int c = 0; c < NK; c++) k[t][c] = *(const kv_u4_t*)(p + (PAD ? min(4 * c + g, nch - 1) : 4 * c + g) * 8);
-            }
+                for (int c = 0; c < NK; c++)
+                    k[t][c] = kv_load16<E>(a.pages.k, at[t], (uint32_t)(r * hd + (PAD ? min(4 * c + g, nch - 1) : 4 * c + g) * 8) * 2);
         };
         auto load_v = [&]() {
 #pragma unroll
-            for (int i = 0; i < VL; i++) {  // 16-byte piece lane + 64 i of the block
-                const int key = (lane + 64 * i) / CPR, c = lane % CPR;
-                const uint32_t rw = __shfl(rn[(64 * i / CPR) >> 4], key & 15, 64);
-                v[i] = *(const kv_u4_t*)((const E*)a.pages.v + (size_t)rw * hd + (PAD ? min(c, nch - 1) : c) * 8);
+            for (int i = 0; i < VL; i++) {
+                constexpr int RPI = 64 / CPR;  // rows a load covers
+                const int c = lane % CPR, row = lane / CPR + RPI * i % 16;
+                v[i] = kv_load16<E>(a.pages.v, at[RPI * i / 16], (uint32_t)(row * hd + (PAD ? min(c, nch - 1) : c) * 8) * 2);
             }
         };
         int j = it.j0 + wave * KB;
-        find(j);
         place(j);
-        find(j + 4 * KB);
         load_k();
         load_v();
 
@@ -130,9 +122,8 @@ __global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void kv_attn_rows_kernel(KvA
 #pragma unroll
                     for (int c = 0; c < NK; c++) s[t] = kv_mfma16(__builtin_bit_cast(x8, k[t][c]), q[u][c], s[t]);
             }
-            // the next block (past the last: its last row again)
+            // the next block (past the last: its last group again)
             place(j + 4 * KB);
-            find(j + 8 * KB);
             load_k();
             float bm = -INFINITY;
             const int hi = see.hi - j - 4 * g, from = see.from - j - 4 * g, to = see.to - j - 4 * g;
@@ -204,7 +195,7 @@ __global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void kv_attn_rows_kernel(KvA
             for (int rw = 0; rw < R; rw++) {
                 const KvTok t = toks[it.tok0 + rw / G];
                 float pm, pl, acc[DE];
-                kv_row_plain<E, DE>(a, it, table, h, q_at(t, rw), t.pos, it.j0 + wave * KB, KB, 4 * KB, pm, pl, acc);
+                kv_row_plain<E, DE>(a, it, groups.table, h, q_at(t, rw), t.pos, it.j0 + wave * KB, KB, 4 * KB, pm, pl, acc);
 #pragma unroll
                 for (int e = 0; e < DE; e++) mo[rw * D + lane + 64 * e] = acc[e];
                 if (lane == 0) { sm[wave][rw] = pm; sl[wave][rw] = pl; }

@@ -34,31 +34,28 @@ __global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void kv_attn_tiles_kernel(Kv
     int n = blockIdx.x / kvh;
     KvItem it = kv_item(a.items, n);
     for (; n < count; it = kv_item(a.items, n)) {
-        const int* table = a.pages.table + (size_t)it.seq * a.pages.pages_per_seq;
-        // piece i of this thread: 16 bytes of row (tid + 256 i) / CPR
-        int pg[NL];
-        kv_u4_t kr[NL], vr[NL];
-        auto key_of = [&](int j0, int i) { return kv_key(it, min(j0 + (tid + 256 * i) / CPR, it.j1 - 1)); };
-        auto find = [&](int j0) {
-#pragma unroll
-            for (int i = 0; i < NL; i++) pg[i] = table[key_of(j0, i) >> a.pages.shift];
-        };
-        auto load = [&](int j0) {
-#pragma unroll
-            for (int i = 0; i < NL; i++) {
-                const size_t at = (size_t)kv_row(a.pages, pg[i], hk, key_of(j0, i)) * hd + (PAD ? min(tid % CPR, nch - 1) : tid % CPR) * 8;
-                kr[i] = *(const kv_u4_t*)((const E*)a.pages.k + at);
-                vr[i] = *(const kv_u4_t*)((const E*)a.pages.v + at);
-            }
-        };
-        find(it.j0);
-        load(it.j0);
-        find(it.j0 + KB);
-
+        KvGroups groups(a.pages, it);
         const int R = it.ntok * G, row = min(wave * 32 + c, R - 1);
         const bool live = wave * 32 + c < R;
         const KvTok tok = toks[it.tok0 + row / G];
         const int hq = hk * G + row % G;
+        // piece i of this thread: 16 bytes of row (tid + 256 i) / CPR
+        kv_u4_t kr[NL], vr[NL];
+        constexpr int RPI = 256 / CPR;  // rows a load of the workgroup covers
+        const uint32_t off = (uint32_t)(tid / CPR % 16 * hd + (PAD ? min(tid % CPR, nch - 1) : tid % CPR) * 8) * 2;
+        auto load = [&](int j0) {
+            groups.reach(a.pages, it, j0 >> 4);
+#pragma unroll
+            for (int i = 0; i < NL; i++) {
+                const int group = RPI * i / 16 + (RPI > 16 ? wave * RPI / 64 : 0);
+                const size_t at = groups.at(a.pages, it, hk, hd, (j0 >> 4) + group);
+                const uint32_t o = off + (uint32_t)(RPI < 16 ? RPI * i % 16 * hd * 2 : 0);
+                kr[i] = kv_load16<E>(a.pages.k, at, o);
+                vr[i] = kv_load16<E>(a.pages.v, at, o);
+            }
+        };
+        load(it.j0);
+
         // which blocks need no mask, and which no work, for this wave's rows
         const KvSeen see(it, tok.pos, a.window, a.sinks);
         int hi_lo = see.hi, hi_hi = see.hi, to_lo = see.to, to_hi = see.to;
@@ -117,16 +114,32 @@ __global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void kv_attn_tiles_kernel(Kv
 
         auto block = [&](const E* ks, const E* vs, int j) {
             if (j > hi_hi || (j >= hidden && j + KB - 1 <= to_lo)) return;  // wave-uniform: no row sees any of it
+            const int ln = kv_fresh(lane);
+            // S^T.  The operands of a step are read while the step before it is in the MFMAs.
             kv_f32x16_t s[KT];
+            {
+                constexpr int XS = NS < 2 ? 1 : 2, STEPS = KT * NS / XS;
+                const E* kp = ks + (ln & 31) * LK + 8 * (ln >> 5);
+                x8 ka[2][XS];
+                auto read = [&](int i) {
 #pragma unroll
-            for (int t = 0; t < KT; t++) {
+                    for (int y = 0; y < XS; y++) ka[i & 1][y] = *(const x8*)(kp + (i * XS / NS) * 32 * LK + (i * XS % NS + y) * 16);
+                };
+                read(0);
 #pragma unroll
-                for (int i = 0; i < 16; i++) s[t][i] = 0.0f;
+                for (int t = 0; t < KT; t++)
 #pragma unroll
-                for (int x = 0; x < NS; x++) {
-                    const x8 ka = *(const x8*)(ks + (t * 32 + c) * LK + x * 16 + 8 * h);
+                    for (int e = 0; e < 16; e++) s[t][e] = 0.0f;
 #pragma unroll
-                    for (int u = NP - 1; u >= 0; u--) s[t] = kv_mfma32(ka, q[u][x], s[t]);
+                for (int i = 0; i < STEPS; i++) {
+                    if (i + 1 < STEPS) read(i + 1);
+                    __builtin_amdgcn_sched_barrier(0);
+                    const int t = i * XS / NS;
+#pragma unroll
+                    for (int y = 0; y < XS; y++)
+#pragma unroll
+                        for (int u = NP - 1; u >= 0; u--) s[t] = kv_mfma32(ka[i & 1][y], q[u][i * XS % NS + y], s[t]);
+                    __builtin_amdgcn_sched_barrier(0);
                 }
             }
             kv_mfma_wait();
@@ -140,13 +153,31 @@ __global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void kv_attn_tiles_kernel(Kv
                         s[t][i] = (x <= hi) & ((x < from) | (x > to)) ? s[t][i] : -INFINITY;
                     }
             }
-            float bm = -INFINITY;
+            float bm = kv_max3(s[0][0], s[0][1], s[0][2]);
 #pragma unroll
-            for (int t = 0; t < KT; t++)
+            for (int i = 3; i < KT * 16 - 1; i += 2) bm = kv_max3(bm, s[i >> 4][i & 15], s[(i + 1) >> 4][(i + 1) & 15]);
+            bm = kv_max3(bm, s[KT - 1][15], __shfl_xor(kv_max3(bm, bm, s[KT - 1][15]), 32, 64)) * scale;
+            float f = 1.0f;
+            if constexpr (NP == 1) {
+                // The sums' reference follows the maximum only when that has risen by 2^6: weights up to
+                // 64 have the same relative rounding, and the sums are seldom rescaled.
+                if (__any(bm > m + 6.0f)) {
+                    const float mn = fmaxf(m, bm);
+                    f = kv_exp2(m - (mn == -INFINITY ? 0.0f : mn));
+                    m = mn;
 #pragma unroll
-                for (int i = 0; i < 16; i++) bm = fmaxf(bm, s[t][i]);
-            bm = fmaxf(bm, __shfl_xor(bm, 32, 64)) * scale;
-            const float mn = fmaxf(m, bm), ref = mn == -INFINITY ? 0.0f : mn, f = kv_exp2(m - ref);
+                    for (int t = 0; t < NDT; t++)
+#pragma unroll
+                        for (int i = 0; i < 16; i++) o[t][i] *= f;
+                    l *= f;
+                }
+            } else {
+                const float mn = fmaxf(m, bm);
+                f = kv_exp2(m - (mn == -INFINITY ? 0.0f : mn));
+                m = mn;
+                l *= f;
+            }
+            const float ref = m == -INFINITY ? 0.0f : m;
             float ps = 0.0f;
             x8 p[NP][KT * 2];
 #pragma unroll
@@ -160,44 +191,61 @@ __global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void kv_attn_tiles_kernel(Kv
 #pragma unroll
                     for (int u = 0; u < NP; u++) p[u][2 * t + (i >> 3)][i & 7] = part[u];
                 }
-            l = l * f + ps;  // this lane's keys; the row's two lanes meet at the end
-            m = mn;
-            // The block sums up by itself and meets the sums so far in plain additions
-            // (an MFMA truncates what it adds to a larger sum).
+            l += ps;  // this lane's keys; the row's two lanes meet at the end
+            // An MFMA truncates what it adds to a larger sum: f32 results add a block's sum to
+            // the sums so far in plain additions.  (Results of 16 bits do not see it: a step of 2^-24 for 16 keys,
+            // over the 16384 keys that a piece has at most.)
+            {
+                typedef short s8 __attribute__((ext_vector_type(8)));
+                constexpr int XS = 2, PER = KT * 2 / XS, STEPS = NDT * PER;
+                // lane 4k + i of sixteen addresses four dims of key k and gets its dim of four keys
+                const E* vp = vs + (4 * (ln >> 5) + ((ln & 15) >> 2)) * LV + (ln & 16) + 4 * (ln & 3);
+                s8 va[2][XS];
+                auto read = [&](int i) {
 #pragma unroll
-            for (int dt = 0; dt < NDT; dt++) {
+                    for (int y = 0; y < XS; y++) {
+                        kv_s4_t w[2];
+#pragma unroll
+                        for (int z = 0; z < 2; z++)
+                            w[z] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                                (kv_lds_s4_t*)(vp + (16 * (i % PER * XS + y) + 8 * z) * LV + i / PER * 32));
+                        va[i & 1][y] = s8{w[0][0], w[0][1], w[0][2], w[0][3], w[1][0], w[1][1], w[1][2], w[1][3]};
+                    }
+                };
+                read(0);
                 kv_f32x16_t d;
 #pragma unroll
-                for (int i = 0; i < 16; i++) d[i] = 0.0f;
+                for (int i = 0; i < STEPS; i++) {
+                    const int dt = i / PER, x0 = i % PER * XS;
+                    if (x0 == 0) {
 #pragma unroll
-                for (int x = 0; x < KT * 2; x++) {
-                    kv_s4_t w[2];
+                        for (int e = 0; e < 16; e++) d[e] = NP == 1 ? o[dt][e] : 0.0f;
+                    }
+                    if (i + 1 < STEPS) read(i + 1);
+                    __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-                    for (int y = 0; y < 2; y++)
-                        w[y] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-                            (kv_lds_s4_t*)(vs + (16 * x + 8 * y + 4 * h + ((lane & 15) >> 2)) * LV + dt * 32 + (c & 16) +
-                                           4 * (lane & 3)));
-                    typedef short s8 __attribute__((ext_vector_type(8)));
-                    const x8 va = __builtin_bit_cast(x8, (s8){w[0][0], w[0][1], w[0][2], w[0][3], w[1][0], w[1][1], w[1][2], w[1][3]});
+                    for (int y = 0; y < XS; y++)
 #pragma unroll
-                    for (int u = NP - 1; u >= 0; u--) d = kv_mfma32(va, p[u][x], d);
+                        for (int u = NP - 1; u >= 0; u--) d = kv_mfma32(__builtin_bit_cast(x8, va[i & 1][y]), p[u][x0 + y], d);
+                    if (x0 + XS == KT * 2) {
+#pragma unroll
+                        for (int e = 0; e < 16; e++) o[dt][e] = NP == 1 ? d[e] : __builtin_fmaf(o[dt][e], f, d[e]);
+                    }
+                    if (i + 1 < STEPS) __builtin_amdgcn_sched_barrier(0);
                 }
-#pragma unroll
-                for (int i = 0; i < 16; i++) o[dt][i] = __builtin_fmaf(o[dt][i], f, d[i]);
             }
         };
         for (int j = it.j0, b = 0; j < it.j1; j += KB, b ^= 1) {
             E *ks = lds[b], *vs = ks + KB * LK;
+            const int ti = kv_fresh(tid);
 #pragma unroll
             for (int i = 0; i < NL; i++) {
-                const int k = (tid + 256 * i) / CPR;
-                *(kv_u4_t*)(ks + k * LK + tid % CPR * 8) = kr[i];
-                *(kv_u4_t*)(vs + k * LV + tid % CPR * 8) = vr[i];
+                *(kv_u4_t*)(ks + ti / CPR * LK + ti % CPR * 8 + i * RPI * LK) = kr[i];
+                *(kv_u4_t*)(vs + ti / CPR * LV + ti % CPR * 8 + i * RPI * LV) = vr[i];
             }
             // behind the barrier the block is whole, and the other buffer's reads (a block ago) are done
             __syncthreads();
-            load(j + KB);  // past the last: its last row again
-            find(j + 2 * KB);
+            load(j + KB);  // past the last: its last group again
             block(ks, vs, j);
         }
         kv_mfma_wait();
@@ -233,7 +281,7 @@ __global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void kv_attn_tiles_kernel(Kv
             const int hx = hk * G + rw % G;
             const size_t at = ((size_t)t.row * a.n_heads + hx) * hd;
             float pm, pl, acc[DE];
-            kv_row_plain<E, DE>(a, it, table, hk, at, t.pos, it.j0, KB, KB, pm, pl, acc);
+            kv_row_plain<E, DE>(a, it, groups.table, hk, at, t.pos, it.j0, KB, KB, pm, pl, acc);
             const size_t rx = it.rec < 0 ? 0 : kv_record(it, t, a.n_heads, hx);
 #pragma unroll
             for (int e = 0; e < DE; e++) {

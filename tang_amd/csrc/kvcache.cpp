@@ -213,7 +213,7 @@ struct PlanTile { KvItem it; bool small, own; };
 
 // Shared prefixes shorter than this are read by each sequence.
 constexpr size_t KV_MIN_PREFIX = 128;
-constexpr size_t KV_MIN_ROWS_KEYS = 256, KV_MIN_TILE_KEYS = 256;
+constexpr size_t KV_MIN_ROWS_KEYS = 256, KV_MIN_TILE_KEYS = 256, KV_MAX_TILE_KEYS = 16384 * 4 / 5;
 
 class PlanMaker {
    public:
@@ -297,10 +297,11 @@ class PlanMaker {
             const size_t end = std::min(to, (size_t)hi + 1);
             size_t sink_end = end, main = end;  // hidden: [sink_end, main)
             if (window_ && (size_t)lo + 1 > window_) {
-                main = std::max(from, (size_t)lo + 1 - window_);
-                sink_end = std::max(from, std::min(sinks_, end));
-                if (main > end) main = end;
-                if (sink_end >= main) sink_end = main = end;
+                // (the run begins and ends at multiples of 16: rows mask what is left of it)
+                main = std::max(from, ((size_t)lo + 1 - window_) / 16 * 16);
+                sink_end = std::max(from, round_up(std::min(sinks_, end), 16));
+                if (sink_end >= std::min(main, end)) sink_end = main = end;
+                main = std::min(main, end);
             }
             const size_t keys = sink_end - from + (end - main);
             if (end <= from || keys == 0) continue;
@@ -325,6 +326,8 @@ class PlanMaker {
         size_t per[2];
         per[1] = round_up(std::max<size_t>(KV_MIN_ROWS_KEYS, ceil_div(keys_[1] * kvh, 8 * cus)), 64) * scale;
         per[0] = round_up(std::max<size_t>(KV_MIN_TILE_KEYS, ceil_div(keys_[0] * kvh, 4 * cus)), 64) * scale;
+        // (sums of 16-bit results stay in the MFMAs for a piece of tiles)
+        per[0] = std::min(per[0], KV_MAX_TILE_KEYS);
         std::vector<int> shared(toks_.size(), 0), own(toks_.size(), 0), pieces(tiles_.size());
         size_t extra = 0;
         for (size_t i = 0; i < tiles_.size(); i++) {
@@ -513,8 +516,8 @@ int th_kv_cache_create(th_device* dev, const th_kv_cache_config* cfg, th_kv_cach
     TH_REQUIRE(!dev->closed, "the device was destroyed");
     TH_REQUIRE(cfg->n_layers > 0 && cfg->n_kv_heads > 0 && cfg->head_dim > 0 && cfg->n_pages > 0 && cfg->max_seqs > 0 && cfg->max_len > 0,
                "every size must be positive");
-    TH_REQUIRE(cfg->page_size >= 8 && cfg->page_size <= 1024 && (cfg->page_size & (cfg->page_size - 1)) == 0,
-               "page_size must be a power of two from 8 to 1024");
+    TH_REQUIRE(cfg->page_size >= 16 && cfg->page_size <= 1024 && (cfg->page_size & (cfg->page_size - 1)) == 0,
+               "page_size must be a power of two from 16 to 1024");
     if (cfg->dtype != TH_F16 && cfg->dtype != TH_BF16)
         throw Error(TH_ERR_UNSUPPORTED, "th_kv_cache_create: the cache holds f16 or bf16");
     if (cfg->head_dim % 8 != 0 || cfg->head_dim > 256)

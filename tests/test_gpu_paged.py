@@ -175,7 +175,7 @@ TYPES = [(F32, F16, F32), (F16, F16, F16), (BF16, BF16, BF16), (F32, BF16, F32),
 @pytest.mark.parametrize("qdt,cdt,odt", TYPES, ids=lambda t: NAMES[t])
 @pytest.mark.parametrize("kh,G,hd,page,starts,news", [
     (2, 1, 64, 16, [0], [1]),                                  # the first position
-    (1, 4, 128, 8, [0, 31, 32, 33, 127, 300], [1] * 6),        # block and page ends
+    (1, 4, 128, 32, [0, 31, 32, 33, 127, 300], [1] * 6),        # block and page ends
     (2, 7, 128, 16, [15, 500, 0, 90], [2, 1, 3, 0]),           # a few new ones, none
     (3, 3, 80, 32, [100, 3], [5, 1]),                          # 80 of 128 dims
     (2, 1, 256, 16, [70, 260], [1, 16]),
@@ -379,7 +379,7 @@ def test_kv_attention_agrees_on_rows_read_out(dev):
 # ---------------------------------------------------------------------------
 
 
-@pytest.mark.parametrize("page,hd,dt", [(8, 8, F16), (16, 128, BF16), (64, 40, F16)])
+@pytest.mark.parametrize("page,hd,dt", [(16, 8, F16), (16, 128, BF16), (64, 40, F16)])
 def test_moves_of_pages(dev, page, hd, dt):
     """Random growth, forks, cuts, selections, frees and compactions: every sequence
     keeps its own rows, and no page is lost."""
@@ -431,10 +431,10 @@ def test_moves_of_pages(dev, page, hd, dt):
 def test_many_moves_at_once(dev):
     """More pages than a launch's arguments hold: forks that all write, a compaction of all."""
     rng = np.random.default_rng(1)
-    m = Model(dev, 1, 64, 8, 900, 300, 1, 400, F16)
+    m = Model(dev, 1, 64, 16, 900, 300, 1, 800, F16)
     a, gap = m.create(), m.create()
     m.fill(rng, [a], [13])
-    m.cache.seq_resize(gap, 399)
+    m.cache.seq_resize(gap, 799)
     m.rows[gap] = None
     children = m.cache.seq_fork(a, 200)
     for s in children:
@@ -640,7 +640,7 @@ def test_refusals(dev):
     _refused(uns, dev.kv_cache, 1, 1, 64, 16, 4, 1, 64, F32)
     _refused(uns, dev.kv_cache, 1, 1, 12, 16, 4, 1, 64)
     _refused(uns, dev.kv_cache, 1, 1, 264, 16, 4, 1, 64)
-    for args in [(0, 1, 64, 16, 4, 1, 64), (1, 0, 64, 16, 4, 1, 64), (1, 1, 64, 24, 4, 1, 64), (1, 1, 64, 4, 4, 1, 64), (1, 1, 64, 16, 0, 1, 64),
+    for args in [(0, 1, 64, 16, 4, 1, 64), (1, 0, 64, 16, 4, 1, 64), (1, 1, 64, 24, 4, 1, 64), (1, 1, 64, 8, 4, 1, 64), (1, 1, 64, 16, 0, 1, 64),
                  (1, 1, 64, 16, 4, 0, 64), (1, 1, 64, 16, 4, 1, 0), (1, 1, 64, 16, 1 << 28, 1, 64), (1, 1, 64, 16, 4, 1, 1 << 29)]:
         _refused(bad, dev.kv_cache, *args)
     c = dev.kv_cache(2, 2, 64, 16, 8, 3, 100)

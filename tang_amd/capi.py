@@ -9,6 +9,7 @@ reference panics instead).
 The shared library must have been built (tang_amd/build.py); importing this
 module without it raises, so no caller can silently fall back to CPU code.
 """
+import array
 import ctypes
 import os
 
@@ -555,7 +556,8 @@ class KvCache:
         return list(out[:n])
 
     def seq_free(self, seqs):
-        check(lib().th_kv_seq_free(self.handle, (ctypes.c_int32 * max(len(seqs), 1))(*seqs), len(seqs)))
+        s = array.array("i", seqs)
+        check(lib().th_kv_seq_free(self.handle, s.buffer_info()[0], len(s)))
 
     def seq_len(self, seq):
         n = ctypes.c_size_t()
@@ -597,29 +599,45 @@ class KvCache:
             pass
 
 
+def _handle(buf):
+    return None if buf is None else buf.handle
+
+
 class KvBatch:
     """New positions of several sequences of a cache, step by step (th_kv_batch_*)."""
 
     def __init__(self, cache, max_seqs, max_rows, n_heads):
         self.cache = cache
-        h = ctypes.c_void_p()
-        check(lib().th_kv_batch_create(cache.handle, max_seqs, max_rows, n_heads, ctypes.byref(h)))
+        h, L = ctypes.c_void_p(), lib()
+        check(L.th_kv_batch_create(cache.handle, max_seqs, max_rows, n_heads, ctypes.byref(h)))
         self.handle = h
+        # a step is many short calls
+        self._begin, self._trim, self._append, self._attention = (L.th_kv_batch_begin, L.th_kv_batch_trim, L.th_kv_append,
+                                                                  L.th_kv_batch_attention)
 
     def begin(self, seqs, n_new):
-        assert len(seqs) == len(n_new)
-        n = max(len(seqs), 1)
-        check(lib().th_kv_batch_begin(self.handle, (ctypes.c_int32 * n)(*seqs), (ctypes.c_uint32 * n)(*n_new), len(seqs)))
+        s, n = array.array("i", seqs), array.array("I", n_new)
+        assert len(s) == len(n)
+        rc = self._begin(self.handle, s.buffer_info()[0], n.buffer_info()[0], len(s))
+        if rc:
+            check(rc)
 
     def trim(self, n_keep):
-        check(lib().th_kv_batch_trim(self.handle, (ctypes.c_uint32 * max(len(n_keep), 1))(*n_keep), len(n_keep)))
+        n = array.array("I", n_keep)
+        rc = self._trim(self.handle, n.buffer_info()[0], len(n))
+        if rc:
+            check(rc)
 
-    def append(self, layer, q, k, v, q_out, cos_buf=None, sin_buf=None, rot_dim=0, layout=0, positions=None):
-        h = [b.handle if b is not None else None for b in (q, k, v, cos_buf, sin_buf, positions)]
-        check(lib().th_kv_append(self.handle, layer, *h, rot_dim, layout, q_out.handle if q_out is not None else None))
+    def append(self, layer, q, k, v, q_out, cos_buf=None, sin_buf=None, rot_dim=0, layout=ROPE_INTERLEAVED, positions=None):
+        rc = self._append(self.handle, layer, _handle(q), k.handle, v.handle, _handle(cos_buf), _handle(sin_buf), _handle(positions),
+                          rot_dim, layout, _handle(q_out))
+        if rc:
+            check(rc)
 
     def attention(self, layer, q, out, window=0, sinks=0, scale=0.0):
-        check(lib().th_kv_batch_attention(self.handle, layer, q.handle, window, sinks, scale, out.handle))
+        rc = self._attention(self.handle, layer, q.handle, window, sinks, scale, out.handle)
+        if rc:
+            check(rc)
 
     def free(self):
         if self.handle:

@@ -229,7 +229,7 @@ class PlanMaker {
     }
 
     std::vector<uint32_t> words;  // head, tokens, rows items, tile items, joined tokens
-    size_t n_toks = 0, n_items[2] = {0, 0}, n_joins = 0;  // items: [0] tiles, [1] rows
+    size_t n_toks = 0, n_items[2] = {0, 0}, n_joins = 0, n_recs = 0;  // items: [0] tiles, [1] rows
 
    private:
     const int* table(int s) const { return c_->mirror.data() + (size_t)s * c_->pages_per_seq; }
@@ -402,6 +402,7 @@ class PlanMaker {
         n_items[0] = items[0].size();
         n_items[1] = items[1].size();
         n_joins = joins.size();
+        n_recs = rec;
         KvPlanHead head = {};
         head.n_joins = (int)n_joins;
         head.n_rows_items = (int)n_items[1];
@@ -454,6 +455,7 @@ static void build_plan(th_kv_batch* b, std::pair<size_t, size_t> key, th_kv_batc
     p.n_tile_items = m.n_items[0];
     p.n_rows_items = m.n_items[1];
     p.n_joins = m.n_joins;
+    p.n_recs = m.n_recs;
     p.built = true;
 }
 
@@ -957,20 +959,20 @@ int th_kv_batch_attention(th_kv_batch* b, size_t layer, const th_buffer* q, size
     a.scale = (scale > 0.0f ? scale : 1.0f / std::sqrt((float)c->hd)) * 1.44269504f;
     a.rec_o = b->rec_o;
     a.rec_ml = b->rec_ml;
-    const KvPlanHead* head = (const KvPlanHead*)p.block;
-    // A captured call runs whatever plan the batch has at replay: every kernel, on grids that walk
-    // their lists.
-    const size_t some = std::min(b->max_items, ceil_div(4 * (size_t)c->dev->num_cus, c->n_kv_heads));
-    const size_t tiles = capturing ? std::max(p.n_tile_items, some) : p.n_tile_items;
-    const size_t rows = capturing ? std::max(p.n_rows_items, some) : p.n_rows_items;
-    a.n_items = &head->n_tile_items;
-    a.items = (const KvItem*)(p.block + plan_tiles(b));
-    launch_kv_attn_tiles(a, c->dtype, tiles, c->dev->stream);
-    a.n_items = &head->n_rows_items;
-    a.items = (const KvItem*)(p.block + plan_rows(b));
-    launch_kv_attn_rows(a, c->dtype, rows, c->dev->stream);
-    a.n_items = &head->n_joins;
-    launch_kv_attn_join(a, p.block + plan_joins(b), capturing ? std::min<size_t>(b->max_rows, 1024) : p.n_joins, c->dev->stream);
+    a.head = (const KvPlanHead*)p.block;
+    a.rows_items = (const KvItem*)(p.block + plan_rows(b));
+    a.tile_items = (const KvItem*)(p.block + plan_tiles(b));
+    const size_t items = p.n_tile_items + p.n_rows_items;
+    if (capturing) {
+        // whatever plan the batch has at replay: every kernel, on grids that walk their lists
+        launch_kv_attn_both(a, c->dtype, std::max(items, ceil_div(4 * (size_t)c->dev->num_cus, c->n_kv_heads)), c->dev->stream);
+        launch_kv_attn_join(a, p.block + plan_joins(b), std::min<size_t>(b->max_rows, 1024), p.n_recs, c->dev->stream);
+    } else {
+        if (p.n_tile_items && p.n_rows_items) launch_kv_attn_both(a, c->dtype, items, c->dev->stream);
+        else if (p.n_tile_items) launch_kv_attn_tiles(a, c->dtype, items, c->dev->stream);
+        else launch_kv_attn_rows(a, c->dtype, items, c->dev->stream);
+        launch_kv_attn_join(a, p.block + plan_joins(b), p.n_joins, p.n_recs, c->dev->stream);
+    }
     TH_API_END
 }
 

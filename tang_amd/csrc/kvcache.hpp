@@ -45,9 +45,9 @@ constexpr int KV_HEAD_WORDS = sizeof(KvPlanHead) / 4;
 
 struct KvAttnArgs {
     KvPages pages;
-    const int* n_items;   // of the kernel's items (the join: of tokens)
-    const KvItem* items;
+    const KvPlanHead* head;
     const KvTok* toks;
+    const KvItem *rows_items, *tile_items;
     const void* q;
     void* out;
     th_dtype qdt, odt;
@@ -104,7 +104,9 @@ void launch_rope_rows(const KvRopeArgs& a, size_t n_rows, hipStream_t s);
 // grid: how many items the launch covers at a time (the kernels walk the rest).
 void launch_kv_attn_rows(const KvAttnArgs& a, th_dtype cache, size_t grid, hipStream_t s);
 void launch_kv_attn_tiles(const KvAttnArgs& a, th_dtype cache, size_t grid, hipStream_t s);
-void launch_kv_attn_join(const KvAttnArgs& a, const int* list, size_t grid, hipStream_t s);
+void launch_kv_attn_both(const KvAttnArgs& a, th_dtype cache, size_t grid, hipStream_t s);
+// n: tokens to join, n_recs: their records (by which the kernel is chosen).
+void launch_kv_attn_join(const KvAttnArgs& a, const int* list, size_t n, size_t n_recs, hipStream_t s);
 
 // Rows (tokens x query heads of a kv head) that one item has at most.
 constexpr int KV_ROWS = 16, KV_TILE = 128;
@@ -177,7 +179,7 @@ struct th_kv_batch {
     int* block = nullptr;      // device: the number of rows (16 bytes), then KvRow[max_rows]
     struct Plan {
         int* block = nullptr;  // device
-        size_t n_rows_items = 0, n_tile_items = 0, n_joins = 0;
+        size_t n_rows_items = 0, n_tile_items = 0, n_joins = 0, n_recs = 0;
         bool built = false;    // for the batch as it is begun
     };
     std::map<std::pair<size_t, size_t>, Plan> plans;  // by window and sinks

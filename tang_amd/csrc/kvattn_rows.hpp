@@ -154,14 +154,14 @@ __device__ __forceinline__ void kv_rows_item(const KvAttnArgs& a, const KvItem& 
             *(kv_u4_t*)(vs + (lane + 64 * i) / CPR * LD + lane % CPR * 8) = v[i];
         wave_lds_fence();
         load_v();
+        kv_lds_s4_t* vp = (kv_lds_s4_t*)(vs + (4 * g + (r >> 2)) * LD + 4 * (r & 3));
 #pragma unroll
         for (int dt = 0; dt < NDT; dt++) {
             // lane r addresses four dims of key r >> 2 of its group's four, and gets its dim of all four
             kv_s4_t w[2];
 #pragma unroll
             for (int t = 0; t < 2; t++)
-                w[t] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-                    (kv_lds_s4_t*)(vs + (16 * t + 4 * g + (r >> 2)) * LD + dt * 16 + 4 * (r & 3)));
+                w[t] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(vp + (16 * t * LD + dt * 16) / 4);
             typedef short s8 __attribute__((ext_vector_type(8)));
             const x8 va = __builtin_bit_cast(x8, (s8){w[0][0], w[0][1], w[0][2], w[0][3], w[1][0], w[1][1], w[1][2], w[1][3]});
             kv_f32x4_t d = {0.0f, 0.0f, 0.0f, 0.0f};

@@ -202,7 +202,7 @@ __device__ __forceinline__ void kv_tiles_item(const KvAttnArgs& a, const KvItem&
             typedef short s8 __attribute__((ext_vector_type(8)));
             constexpr int XS = 2, PER = KT * 2 / XS, STEPS = NDT * PER;
             // lane 4k + i of sixteen addresses four dims of key k and gets its dim of four keys
-            const E* vp = vs + (4 * (ln >> 5) + ((ln & 15) >> 2)) * LV + (ln & 16) + 4 * (ln & 3);
+            kv_lds_s4_t* vp = (kv_lds_s4_t*)(vs + (4 * (ln >> 5) + ((ln & 15) >> 2)) * LV + (ln & 16) + 4 * (ln & 3));
             s8 va[2][XS];
             auto read = [&](int i) {
 #pragma unroll
@@ -210,8 +210,7 @@ __device__ __forceinline__ void kv_tiles_item(const KvAttnArgs& a, const KvItem&
                     kv_s4_t w[2];
 #pragma unroll
                     for (int z = 0; z < 2; z++)
-                        w[z] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-                            (kv_lds_s4_t*)(vp + (16 * (i % PER * XS + y) + 8 * z) * LV + i / PER * 32));
+                        w[z] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(vp + ((16 * (i % PER * XS + y) + 8 * z) * LV + i / PER * 32) / 4);
                     va[i & 1][y] = s8{w[0][0], w[0][1], w[0][2], w[0][3], w[1][0], w[1][1], w[1][2], w[1][3]};
                 }
             };

@@ -325,7 +325,7 @@ class PlanMaker {
         // four blocks (tiles).
         size_t per[2];
         per[1] = round_up(std::max<size_t>(KV_MIN_ROWS_KEYS, ceil_div(keys_[1] * kvh, 8 * cus)), 64) * scale;
-        per[0] = round_up(std::max<size_t>(KV_MIN_TILE_KEYS, ceil_div(keys_[0] * kvh, 4 * cus)), 64) * scale;
+        per[0] = round_up(std::max<size_t>(KV_MIN_TILE_KEYS, ceil_div(keys_[0] * kvh, cus * 3 / 2)), 64) * scale;
         // (sums of 16-bit results stay in the MFMAs for a piece of tiles)
         per[0] = std::min(per[0], KV_MAX_TILE_KEYS);
         std::vector<int> shared(toks_.size(), 0), own(toks_.size(), 0), pieces(tiles_.size());

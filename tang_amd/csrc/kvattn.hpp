@@ -203,8 +203,19 @@ __device__ __forceinline__ size_t kv_record(const KvItem& it, const KvTok& t, in
     return ((size_t)t.rec + s) * n_heads + head;
 }
 
+// Whether a row's sums of weights stand.  A weight's exponent is fma(q.k, scale, -m) with m rounded, so all weights
+// share a factor of up to 2^(|m| 2^-24): no more than 2^(1/16) up to the bound, and past any type's range for the largest m.
+__device__ __forceinline__ bool kv_fine(float m, float l) {
+    return (l == l) & ((fabsf(m) <= 1048576.0f) | (m == -INFINITY));
+}
+// q.k * scale rounded, as m is: never one operation with the subtraction that follows.
+__device__ __forceinline__ float kv_score(float d, float scale) {
+#pragma clang fp contract(off)
+    return d * scale;
+}
+
 // One row over some of an item's keys by one wave in plain f32, for rows
-// whose MFMA sums are not finite: an infinity times a part that is zero is NaN
+// whose MFMA sums are not finite or whose scores are huge: an infinity times a part that is zero is NaN
 // there, and hidden keys carry weight zero rather than being left out.  Blocks of `block` numbers every `step`
 // from `from` on.  Lane l ends with dims l, l + 64, ...; m and l are every lane's.
 template <typename E, int DE>
@@ -228,7 +239,7 @@ __device__ __forceinline__ void kv_row_plain(const KvAttnArgs& a, const KvItem& 
 #pragma unroll
             for (int e = 0; e < DE; e++)
                 if (lane + 64 * e < hd) d += qv[e] * (float)((const E*)a.pages.k)[row + lane + 64 * e];
-            const float s = wave_sum(d) * a.scale, mn = fmaxf(m, s), ref = mn == -INFINITY ? 0.0f : mn;
+            const float s = kv_score(wave_sum(d), a.scale), mn = fmaxf(m, s), ref = mn == -INFINITY ? 0.0f : mn;
             const float p = kv_exp2(s - ref), f = kv_exp2(m - ref);
             l = l * f + p;
 #pragma unroll

@@ -147,8 +147,8 @@ void launch_kv_attn_join(const KvAttnArgs& a, const int* list, size_t n, size_t 
     const size_t rows = n * a.n_heads;
     auto with = [&](auto de) {
         constexpr int DE = decltype(de)::value, LPR = 8 * DE;
-        if (rows <= 1024 || n_recs >= 8 * n) TH_LAUNCH((kv_attn_join_few_kernel<DE>), dim3((unsigned)rows), dim3(256), 0, s, a, list);
-        else TH_LAUNCH((kv_attn_join_many_kernel<LPR>), dim3((unsigned)ceil_div(rows, (size_t)(256 / LPR))), dim3(256), 0, s, a, list);
+        if (rows <= 1024 || n_recs >= 8 * n) TH_LAUNCH((kv_attn_join_few_kernel<DE>), dim3((unsigned)std::min(rows, KV_MAX_BLOCKS)), dim3(256), 0, s, a, list);
+        else TH_LAUNCH((kv_attn_join_many_kernel<LPR>), dim3((unsigned)std::min(ceil_div(rows, (size_t)(256 / LPR)), KV_MAX_BLOCKS)), dim3(256), 0, s, a, list);
     };
     if (a.pages.hd <= 64) with(std::integral_constant<int, 1>{});
     else if (a.pages.hd <= 128) with(std::integral_constant<int, 2>{});
@@ -170,7 +170,7 @@ static void rows_launch(const KvAttnArgs& a, unsigned grid, hipStream_t s) {
 
 void launch_kv_attn_rows(const KvAttnArgs& a, th_dtype cache, size_t grid, hipStream_t s) {
     if (grid == 0) return;
-    const unsigned g = (unsigned)(grid * a.pages.n_kv_heads);
+    const unsigned g = (unsigned)(std::min(grid, KV_MAX_BLOCKS / a.pages.n_kv_heads) * a.pages.n_kv_heads);
     auto with = [&](auto e) {
         typedef decltype(e) E;
         if (a.pages.hd <= 64) rows_launch<64, E>(a, g, s);

@@ -174,7 +174,7 @@ __device__ __forceinline__ void kv_rows_item(const KvAttnArgs& a, const KvItem& 
     }
     l += __shfl_xor(l, 16, 64);
     l += __shfl_xor(l, 32, 64);
-    bool fine = l == l;
+    bool fine = kv_fine(m, l);
 #pragma unroll
     for (int t = 0; t < NDT; t++)
 #pragma unroll

@@ -35,7 +35,7 @@ static void tiles_launch(const KvAttnArgs& a, unsigned grid, hipStream_t s) {
 
 void launch_kv_attn_tiles(const KvAttnArgs& a, th_dtype cache, size_t grid, hipStream_t s) {
     if (grid == 0) return;
-    const unsigned g = (unsigned)(grid * a.pages.n_kv_heads);
+    const unsigned g = (unsigned)(std::min(grid, KV_MAX_BLOCKS / a.pages.n_kv_heads) * a.pages.n_kv_heads);
     auto with = [&](auto e) {
         typedef decltype(e) E;
         if (a.pages.hd <= 64) tiles_launch<64, E>(a, g, s);

@@ -252,7 +252,7 @@ __device__ __forceinline__ void kv_tiles_item(const KvAttnArgs& a, const KvItem&
     }
     kv_mfma_wait();
     l += __shfl_xor(l, 32, 64);
-    bool fine = l == l;
+    bool fine = kv_fine(m, l);
 #pragma unroll
     for (int t = 0; t < NDT; t++)
 #pragma unroll

@@ -213,6 +213,7 @@ struct PlanTile { KvItem it; bool small, own; };
 
 // Shared prefixes shorter than this are read by each sequence.
 constexpr size_t KV_MIN_PREFIX = 128;
+constexpr size_t KV_MAX_PLANS = 16;
 constexpr size_t KV_MIN_ROWS_KEYS = 256, KV_MIN_TILE_KEYS = 256, KV_MAX_TILE_KEYS = 16384 * 4 / 5;
 
 class PlanMaker {
@@ -436,7 +437,7 @@ static size_t plan_tiles(const th_kv_batch* b) { return plan_rows(b) + b->max_it
 static size_t plan_joins(const th_kv_batch* b) { return plan_tiles(b) + b->max_items * sizeof(KvItem) / 4; }
 static size_t plan_words(const th_kv_batch* b) { return plan_joins(b) + b->max_rows; }
 
-static void build_plan(th_kv_batch* b, std::pair<size_t, size_t> key, th_kv_batch::Plan& p) {
+static void build_plan(th_kv_batch* b, const th_kv_batch::Key& key, th_kv_batch::Plan& p) {
     p.built = false;
     PlanMaker m(b, key.first, key.second);
     m.make();
@@ -457,6 +458,27 @@ static void build_plan(th_kv_batch* b, std::pair<size_t, size_t> key, th_kv_batc
     p.n_joins = m.n_joins;
     p.n_recs = m.n_recs;
     p.built = true;
+}
+
+// Room for another plan: of its own, or, where there are many, that of one that no graph reads (uploads
+// are in stream order, behind the calls that read the old plan).
+static std::map<th_kv_batch::Key, th_kv_batch::Plan>::iterator add_plan(th_kv_batch* b, const th_kv_batch::Key& key) {
+    th_kv_batch::Plan p;
+    if (b->plans.size() >= KV_MAX_PLANS) {
+        auto old = std::find_if(b->plans.begin(), b->plans.end(), [](const auto& x) { return !x.second.captured; });
+        if (old != b->plans.end()) {
+            p.block = old->second.block;
+            b->plans.erase(old);
+        }
+    }
+    if (!p.block) {
+        const hipError_t e = hipMalloc((void**)&p.block, plan_words(b) * 4);
+        if (e != hipSuccess) {
+            (void)hipGetLastError();
+            throw Error(e == hipErrorOutOfMemory ? TH_ERR_OOM : TH_ERR_HIP, "no memory for an attention plan");
+        }
+    }
+    return b->plans.emplace(key, p).first;
 }
 
 // The batch as it was begun, and still so.
@@ -559,6 +581,7 @@ int th_kv_cache_create(th_device* dev, const th_kv_cache_config* cfg, th_kv_cach
     } catch (...) {
         if (c->pool) (void)hipFree(c->pool);
         if (c->table) (void)hipFree(c->table);
+        (void)hipGetLastError();  // the next launch's check must not find it
         throw;
     }
     device_retain(dev);
@@ -661,9 +684,11 @@ int th_kv_seq_free(th_kv_cache* c, const int32_t* seqs, size_t n) {
     TH_API_BEGIN
     require_open(c, __func__);
     TH_REQUIRE(seqs || n == 0, "null argument");
+    std::vector<char> seen(c->seqs.size(), 0);
     for (size_t i = 0; i < n; i++) {
         the_seq(c, seqs[i], __func__);
-        for (size_t k = 0; k < i; k++) TH_REQUIRE(seqs[k] != seqs[i], "a sequence twice");
+        TH_REQUIRE(!seen[seqs[i]], "a sequence twice");
+        seen[seqs[i]] = 1;
     }
     for (size_t i = 0; i < n; i++) {
         shrink(c, seqs[i], 0);
@@ -797,6 +822,7 @@ int th_kv_batch_create(th_kv_cache* c, size_t max_seqs, size_t max_rows, size_t 
     } catch (...) {
         for (void* p : {(void*)b->block, (void*)b->rec_o, (void*)b->rec_ml})
             if (p) (void)hipFree(p);
+        (void)hipGetLastError();
         throw;
     }
     c->live++;
@@ -871,7 +897,11 @@ int th_kv_batch_begin(th_kv_batch* b, const int32_t* seqs, const uint32_t* n_new
     b->rows = rows;
     copy_pages(c, copies);
     upload(c, words.data(), one_run(words.size()), b->block);
-    for (auto& p : b->plans) build_plan(b, p.first, p.second);
+    // graphs read their plans at replay; the others are built by the step's first call that needs them
+    for (auto& p : b->plans) {
+        p.second.built = false;
+        if (p.second.captured) build_plan(b, p.first, p.second);
+    }
     b->begun = true;
     TH_API_END
 }
@@ -936,15 +966,14 @@ int th_kv_batch_attention(th_kv_batch* b, size_t layer, const th_buffer* q, size
     // a window as long as any sequence hides nothing, and without one there are no sinks
     if (window >= c->max_len) window = 0;
     n_sinks = window ? std::min(n_sinks, c->max_len) : 0;
-    const std::pair<size_t, size_t> key(window, n_sinks);
+    const th_kv_batch::Key key(window, n_sinks);
     auto at = b->plans.find(key);
     if (at == b->plans.end() || !at->second.built) {
         TH_REQUIRE(!capturing, "make the call once before it is captured");
-        th_kv_batch::Plan& p = b->plans[key];
-        if (!p.block) TH_HIP(hipMalloc((void**)&p.block, plan_words(b) * 4));
-        build_plan(b, key, p);
-        at = b->plans.find(key);
+        if (at == b->plans.end()) at = add_plan(b, key);
+        build_plan(b, key, at->second);
     }
+    at->second.captured |= capturing;
     const th_kv_batch::Plan& p = at->second;
     KvAttnArgs a;
     a.pages = layer_pages(c, layer);

@@ -101,7 +101,8 @@ void launch_kv_append(const KvRopeArgs& a, const KvPages& p, th_dtype cache, con
                       size_t n_rows, hipStream_t s);
 void launch_rope_rows(const KvRopeArgs& a, size_t n_rows, hipStream_t s);
 
-// grid: how many items the launch covers at a time (the kernels walk the rest).
+// grid: how many items the launch covers at a time (the kernels walk the rest; a launch has below 2^32 threads).
+constexpr size_t KV_MAX_BLOCKS = (size_t)1 << 23;
 void launch_kv_attn_rows(const KvAttnArgs& a, th_dtype cache, size_t grid, hipStream_t s);
 void launch_kv_attn_tiles(const KvAttnArgs& a, th_dtype cache, size_t grid, hipStream_t s);
 void launch_kv_attn_both(const KvAttnArgs& a, th_dtype cache, size_t grid, hipStream_t s);
@@ -181,8 +182,10 @@ struct th_kv_batch {
         int* block = nullptr;  // device
         size_t n_rows_items = 0, n_tile_items = 0, n_joins = 0, n_recs = 0;
         bool built = false;    // for the batch as it is begun
+        bool captured = false; // a graph may read it
     };
-    std::map<std::pair<size_t, size_t>, Plan> plans;  // by window and sinks
+    typedef std::pair<size_t, size_t> Key;  // window, sinks
+    std::map<Key, Plan> plans;
     float* rec_o = nullptr;    // records of split work
     float2* rec_ml = nullptr;
     size_t max_recs = 0, max_items = 0;

@@ -5,6 +5,7 @@ import oracle
 from tang_amd import capi
 
 EPS = {capi.F32: 2.0 ** -24, capi.F16: 2.0 ** -11, capi.BF16: 2.0 ** -8}  # half a step, relative
+LEAST = {capi.F32: 2.0 ** -150, capi.F16: 2.0 ** -25, capi.BF16: 2.0 ** -134}  # half of the smallest step
 
 
 def to_bits(x, dt):
@@ -75,12 +76,11 @@ def attention_bound(q, k, v, pos, qdt, cdt, odt, window=0, sinks=0, scale=None):
     q, k, v = (np.asarray(t, np.float64) for t in (q, k, v))
     H, KH, D, n = q.shape[1], k.shape[1], q.shape[2], k.shape[0]
     scale = 1.0 / np.sqrt(D) if scale is None else scale
-    A = max(np.abs(q[:, h]) @ np.abs(k[:, h // (H // KH)]).T for h in range(1)).max() if n else 0.0
-    for h in range(H):
-        A = max(A, (np.abs(q[:, h]) @ np.abs(k[:, h // (H // KH)]).T).max())
+    A = max((np.abs(q[:, h]) @ np.abs(k[:, h // (H // KH)]).T).max() for h in range(H))
     A *= scale
     u, parts = 2.0 ** -23, 1 if qdt == cdt == odt else 3
     e = (4 + parts * D / 16 + 8) * u * A + 2.0 ** -22 + (n / 32 + 24) * u
     top = np.abs(v).max()
-    once = EPS[cdt] * top if qdt == cdt == odt else 0.0
-    return 2.0 * e * top + once + EPS[odt] * top
+    # (of n weights, those below the type's normal range are off by half its smallest step)
+    once = (EPS[cdt] + n * LEAST[cdt]) * top if qdt == cdt == odt else 0.0
+    return 2.0 * e * top + once + max(EPS[odt] * top, LEAST[odt])

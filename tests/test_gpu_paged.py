@@ -374,6 +374,67 @@ def test_kv_attention_agrees_on_rows_read_out(dev):
     assert np.abs(got - want).max() <= tol
 
 
+@pytest.mark.parametrize("qdt,cdt", [(F32, F16), (F16, F16), (F32, BF16), (BF16, BF16)], ids=lambda t: NAMES[t])
+@pytest.mark.parametrize("start,new", [(50, 1), (10, 90)])
+def test_small_and_large_values(dev, qdt, cdt, start, new):
+    """Keys and values among the smallest of the cache's type (f16's below its normal range), queries that make up for
+    it, and rows of tiny and of huge queries."""
+    rng = np.random.default_rng(start + new)
+    m = Model(dev, 1, 64, 16, 20, 1, 1, 200, cdt, heads=2)
+    s = m.create()
+    small = 2.0 ** -17
+    for n in (start, new):
+        m.begin([s], [n])
+        k, v = (rounded(_normal(rng, n, 1, 64) * small, cdt) for _ in range(2))
+        m.batch.append(0, None, dev.upload(to_bits(k, cdt), cdt), dev.upload(to_bits(v, cdt), cdt), None)
+        m.rows[s] = np.concatenate((m.rows[s], np.stack((k, v))[None]), 2)
+    q = rounded(_normal(rng, new, 2, 64) * np.float32(2.0 ** 13), qdt)
+    m.attend(rng, qdt, F32 if qdt == F32 else qdt, q=q)
+    if qdt == F32:
+        q[0] *= np.float32(2.0 ** -100)
+        q[new // 2] = np.float32(2.0 ** 90) * np.sign(q[new // 2])
+        _, got = m.attend(rng, q=q, check=False)
+        kk, vv = m.rows[s][0]
+        want = attention(q, kk, vv, np.arange(start, start + new))
+        row = [i for i in range(new) if i != new // 2]
+        if row:
+            tol = attention_bound(q[row], kk, vv, np.arange(start, start + new)[row], qdt, cdt, qdt)
+            assert np.abs(got[row] - want[row]).max() <= tol
+        # scores of 2^80 and more: all weight on the largest, which f32 sums of 64 products (2^-17 of the terms' sum) must tell
+        # from the second
+        p = np.sort(np.einsum("hd,nd->hn", q[new // 2].astype(np.float64), kk[:start + new // 2 + 1, 0].astype(np.float64)), -1)
+        scale = np.abs(q[new // 2]).astype(np.float64) @ np.abs(kk[:, 0]).max(0)
+        clear = (p[:, -1] - p[:, -2]) > scale * 2.0 ** -17
+        assert clear.any()
+        assert np.array_equal(got[new // 2][clear], want[new // 2][clear].astype(np.float32))
+
+
+def test_beyond_four_gibibytes(dev):
+    """Pages behind 2^32 bytes of a layer's keys: attention, append, copies, gathers and reads."""
+    rng = np.random.default_rng(2)
+    pages = 140100  # of 32 KiB: 4.6 GB of keys, as much of values
+    m = Model(dev, 8, 128, 16, pages, 8, 1, 140000 * 16, F16, heads=16, rows=300)
+    first = m.cache.seq_create()[0]
+    m.cache.seq_resize(first, 139950 * 16)
+    a, b = m.create(), m.create()
+    m.fill(rng, [a, b], [70, 3])
+    m.fill(rng, [a, b], [1, 40])
+    m.attend(rng)
+    c = m.cache.seq_fork(a, 2)
+    for s in c:
+        m.rows[s] = m.rows[a].copy()
+    m.fill(rng, c, [1, 30])
+    m.attend(rng)
+    m.cache.seq_select(c[0], np.arange(50, 10, -1))
+    m.rows[c[0]] = m.rows[c[0]][:, :, 50:10:-1].copy()
+    m.check()
+    m.cache.seq_free([first])
+    assert m.cache.compact() > 0
+    m.check()
+    m.batch.free()
+    m.cache.free()
+
+
 # ---------------------------------------------------------------------------
 # Pages
 # ---------------------------------------------------------------------------
@@ -581,6 +642,42 @@ def test_captured_steps(dev, cdt, qdt):
                 big.append(l, None, kk, kk, None)
             m.cache.seq_free(extra)
     graph.free()
+
+
+def test_many_windows(dev):
+    """More windows than a batch keeps plans for, in turns over steps; one is captured and stays."""
+    rng = np.random.default_rng(61)
+    m = Model(dev, 1, 64, 16, 60, 2, 1, 600, F16, heads=2, rows=4)
+    s = m.create()
+    for _ in range(100):
+        m.fill(rng, [s], [4])
+    m.fill(rng, [s], [1])
+    q, out = dev.alloc(4 * 128), dev.alloc(4 * 128)
+    m.batch.attention(0, q, out, 50, 1)
+    graph = dev.capture(lambda: m.batch.attention(0, q, out, 50, 1))
+    for step in range(3):
+        for window in range(1, 60, 2):
+            m.attend(rng, window=window, sinks=window % 3)
+        m.fill(rng, [s], [2 + step])
+        x = _normal(rng, 4, 2, 64)
+        q.upload(x)
+        graph.launch()
+        dev.sync()
+        n = 2 + step
+        k, v = m.rows[s][0]
+        args = (x[:n], k, v, np.arange(k.shape[0] - n, k.shape[0]))
+        err = np.abs(out.to_numpy().reshape(x.shape)[:n] - attention(*args, 50, 1)).max()
+        assert err <= attention_bound(*args, F32, F16, F32, 50, 1)
+    graph.free()
+
+
+def test_out_of_memory_leaves_no_trace(dev):
+    """A cache that does not fit is refused, and the calls behind it work."""
+    _refused(capi.TH_ERR_OOM, dev.kv_cache, 1024, 8, 256, 1024, 4096, 1, 64)  # 33 TB
+    m = Model(dev, 1, 64, 16, 10, 2, 1, 100, F16)
+    s = m.create()
+    m.fill(np.random.default_rng(1), [s], [20])
+    m.check()
 
 
 def test_two_batches_and_two_handles(dev):

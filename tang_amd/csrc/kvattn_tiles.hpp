@@ -24,8 +24,10 @@ struct KvTiles {
     static constexpr size_t LDS = (size_t)2 * KB * (LK + LV) * 2;
 };
 
-// One item by a workgroup.
-template <int D, typename E, int NP, bool PAD>
+// One item by a workgroup.  ADD: a block's sum of values is added to the sums so far in plain additions, since an
+// MFMA truncates what it adds to a larger sum.  Results of 16 bits do not see that (a step of 2^-24 for 16 keys) over the
+// KV_LONG_ITEM keys that an item without ADD has at most.
+template <int D, typename E, int NP, bool PAD, bool ADD>
 __device__ __forceinline__ void kv_tiles_item(const KvAttnArgs& a, const KvItem& it, int hk, char* lds_) {
     typedef KvTiles<D, NP> T;
     typedef typename KvVec<E>::x8 x8;
@@ -195,9 +197,6 @@ __device__ __forceinline__ void kv_tiles_item(const KvAttnArgs& a, const KvItem&
                 for (int u = 0; u < NP; u++) p[u][2 * t + (i >> 3)][i & 7] = part[u];
             }
         l += ps;  // this lane's keys; the row's two lanes meet at the end
-        // An MFMA truncates what it adds to a larger sum: f32 results add a block's sum to
-        // the sums so far in plain additions.  (Results of 16 bits do not see it: a step of 2^-24 for 16 keys,
-        // over the 16384 keys that a piece has at most.)
         {
             typedef short s8 __attribute__((ext_vector_type(8)));
             constexpr int XS = 2, PER = KT * 2 / XS, STEPS = NDT * PER;
@@ -221,7 +220,7 @@ __device__ __forceinline__ void kv_tiles_item(const KvAttnArgs& a, const KvItem&
                 const int dt = i / PER, x0 = i % PER * XS;
                 if (x0 == 0) {
 #pragma unroll
-                    for (int e = 0; e < 16; e++) d[e] = NP == 1 ? o[dt][e] : 0.0f;
+                    for (int e = 0; e < 16; e++) d[e] = ADD ? 0.0f : o[dt][e];
                 }
                 if (i + 1 < STEPS) read(i + 1);
                 __builtin_amdgcn_sched_barrier(0);
@@ -231,7 +230,7 @@ __device__ __forceinline__ void kv_tiles_item(const KvAttnArgs& a, const KvItem&
                     for (int u = NP - 1; u >= 0; u--) d = kv_mfma32(__builtin_bit_cast(x8, va[i & 1][y]), p[u][x0 + y], d);
                 if (x0 + XS == KT * 2) {
 #pragma unroll
-                    for (int e = 0; e < 16; e++) o[dt][e] = NP == 1 ? d[e] : __builtin_fmaf(o[dt][e], f, d[e]);
+                    for (int e = 0; e < 16; e++) o[dt][e] = !ADD ? d[e] : NP == 1 ? o[dt][e] + d[e] : __builtin_fmaf(o[dt][e], f, d[e]);
                 }
                 if (i + 1 < STEPS) __builtin_amdgcn_sched_barrier(0);
             }

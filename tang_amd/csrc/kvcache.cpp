@@ -214,7 +214,7 @@ struct PlanTile { KvItem it; bool small, own; };
 // Shared prefixes shorter than this are read by each sequence.
 constexpr size_t KV_MIN_PREFIX = 128;
 constexpr size_t KV_MAX_PLANS = 16;
-constexpr size_t KV_MIN_ROWS_KEYS = 256, KV_MIN_TILE_KEYS = 256, KV_MAX_TILE_KEYS = 16384 * 4 / 5;
+constexpr size_t KV_MIN_ROWS_KEYS = 256, KV_MIN_TILE_KEYS = 256;
 
 class PlanMaker {
    public:
@@ -230,6 +230,7 @@ class PlanMaker {
     }
 
     std::vector<uint32_t> words;  // head, tokens, rows items, tile items, joined tokens
+    bool far = false;                              // an item of tiles has more than KV_LONG_ITEM keys
     size_t n_toks = 0, n_items[2] = {0, 0}, n_joins = 0, n_recs = 0;  // items: [0] tiles, [1] rows
 
    private:
@@ -327,8 +328,9 @@ class PlanMaker {
         size_t per[2];
         per[1] = round_up(std::max<size_t>(KV_MIN_ROWS_KEYS, ceil_div(keys_[1] * kvh, 8 * cus)), 64) * scale;
         per[0] = round_up(std::max<size_t>(KV_MIN_TILE_KEYS, ceil_div(keys_[0] * kvh, cus * 3 / 2)), 64) * scale;
-        // (sums of 16-bit results stay in the MFMAs for a piece of tiles)
-        per[0] = std::min(per[0], KV_MAX_TILE_KEYS);
+        // Where there are records for it, no tile's piece is so long that it needs additions of its own (a quarter
+        // more than `per` is one piece).
+        if (scale == 1) per[0] = std::min(per[0], KV_LONG_ITEM * 4 / 5);
         std::vector<int> shared(toks_.size(), 0), own(toks_.size(), 0), pieces(tiles_.size());
         size_t extra = 0;
         for (size_t i = 0; i < tiles_.size(); i++) {
@@ -399,6 +401,7 @@ class PlanMaker {
         // the longest first: the last workgroups to start are short
         for (auto& v : items)
             std::stable_sort(v.begin(), v.end(), [](const KvItem& x, const KvItem& y) { return x.j1 - x.j0 > y.j1 - y.j0; });
+        far = !items[0].empty() && (size_t)(items[0][0].j1 - items[0][0].j0) > KV_LONG_ITEM;
         n_toks = toks_.size();
         n_items[0] = items[0].size();
         n_items[1] = items[1].size();
@@ -457,6 +460,7 @@ static void build_plan(th_kv_batch* b, const th_kv_batch::Key& key, th_kv_batch:
     p.n_rows_items = m.n_items[1];
     p.n_joins = m.n_joins;
     p.n_recs = m.n_recs;
+    p.far = m.far;
     p.built = true;
 }
 
@@ -994,11 +998,12 @@ int th_kv_batch_attention(th_kv_batch* b, size_t layer, const th_buffer* q, size
     const size_t items = p.n_tile_items + p.n_rows_items;
     if (capturing) {
         // whatever plan the batch has at replay: every kernel, on grids that walk their lists
-        launch_kv_attn_both(a, c->dtype, std::max(items, ceil_div(4 * (size_t)c->dev->num_cus, c->n_kv_heads)), c->dev->stream);
+        launch_kv_attn_both(a, c->dtype, std::max(items, ceil_div(4 * (size_t)c->dev->num_cus, c->n_kv_heads)),
+                            c->max_len > KV_LONG_ITEM, c->dev->stream);
         launch_kv_attn_join(a, p.block + plan_joins(b), std::min<size_t>(b->max_rows, 1024), p.n_recs, c->dev->stream);
     } else {
-        if (p.n_tile_items && p.n_rows_items) launch_kv_attn_both(a, c->dtype, items, c->dev->stream);
-        else if (p.n_tile_items) launch_kv_attn_tiles(a, c->dtype, items, c->dev->stream);
+        if (p.n_tile_items && p.n_rows_items) launch_kv_attn_both(a, c->dtype, items, p.far, c->dev->stream);
+        else if (p.n_tile_items) launch_kv_attn_tiles(a, c->dtype, items, p.far, c->dev->stream);
         else launch_kv_attn_rows(a, c->dtype, items, c->dev->stream);
         launch_kv_attn_join(a, p.block + plan_joins(b), p.n_joins, p.n_recs, c->dev->stream);
     }

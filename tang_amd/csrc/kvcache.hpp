@@ -102,10 +102,12 @@ void launch_kv_append(const KvRopeArgs& a, const KvPages& p, th_dtype cache, con
 void launch_rope_rows(const KvRopeArgs& a, size_t n_rows, hipStream_t s);
 
 // grid: how many items the launch covers at a time (the kernels walk the rest; a launch has below 2^32 threads).
+// far: a tile item may have more than KV_LONG_ITEM keys.
+constexpr size_t KV_LONG_ITEM = 16384;
 constexpr size_t KV_MAX_BLOCKS = (size_t)1 << 23;
 void launch_kv_attn_rows(const KvAttnArgs& a, th_dtype cache, size_t grid, hipStream_t s);
-void launch_kv_attn_tiles(const KvAttnArgs& a, th_dtype cache, size_t grid, hipStream_t s);
-void launch_kv_attn_both(const KvAttnArgs& a, th_dtype cache, size_t grid, hipStream_t s);
+void launch_kv_attn_tiles(const KvAttnArgs& a, th_dtype cache, size_t grid, bool far, hipStream_t s);
+void launch_kv_attn_both(const KvAttnArgs& a, th_dtype cache, size_t grid, bool far, hipStream_t s);
 // n: tokens to join, n_recs: their records (by which the kernel is chosen).
 void launch_kv_attn_join(const KvAttnArgs& a, const int* list, size_t n, size_t n_recs, hipStream_t s);
 
@@ -181,6 +183,7 @@ struct th_kv_batch {
     struct Plan {
         int* block = nullptr;  // device
         size_t n_rows_items = 0, n_tile_items = 0, n_joins = 0, n_recs = 0;
+        bool far = false;      // an item of tiles has more than KV_LONG_ITEM keys
         bool built = false;    // for the batch as it is begun
         bool captured = false; // a graph may read it
     };

@@ -211,6 +211,30 @@ def test_attention_split_over_long_sequences(dev, qdt, cdt, kh, G, hd, start, ne
     m.attend(rng, qdt, qdt, 2000, 4)
 
 
+@pytest.mark.parametrize("qdt,cdt", [(F16, F16), (BF16, BF16), (F32, F16)])
+@pytest.mark.parametrize("other", [0, 1])
+def test_long_prompt_without_splits(dev, qdt, cdt, other):
+    """So many rows that records for pieces run out: items of more keys than the MFMAs' own sums are for. Values about
+    one would show sums that drift. (other: a second sequence's decode step in the same launch)"""
+    rng = np.random.default_rng(other)
+    m = Model(dev, 1, 64, 64, 400, 2, 1, 24000, cdt, heads=2, rows=16000)
+    s, t = m.create(), m.create()
+    for step in ([s, t], [16000, 0]), ([s, t], [4200, other]):
+        m.begin(*step)
+        n = sum(step[1])
+        k, v = rounded(_normal(rng, n, 1, 64), cdt), rounded(1.0 + 0.125 * _normal(rng, n, 1, 64), cdt)
+        m.batch.append(0, None, dev.upload(to_bits(k, cdt), cdt), dev.upload(to_bits(v, cdt), cdt), None)
+        m.rows[s] = np.concatenate((m.rows[s], np.stack((k, v))[None, :, :step[1][0]]), 2)
+        m.rows[t] = np.concatenate((m.rows[t], np.stack((k, v))[None, :, step[1][0]:]), 2)
+    q, got = m.attend(rng, qdt, qdt, check=False)
+    k, v = m.rows[s][0]
+    rows = [0, 1, 63, 64, 2000, 4111, 4199]
+    args = (q[rows], k, v, 16000 + np.array(rows))
+    assert np.abs(got[rows] - attention(*args)).max() <= attention_bound(*args, qdt, cdt, qdt)
+    if other:
+        assert np.abs(got[4200] - m.rows[t][0, 1, 0]).max() <= 2 * EPS[qdt] * 2.0
+
+
 def test_f32_queries_keep_their_precision(dev):
     """An f16 rounding of queries and probabilities (2^-12 of each on the average)
     shows in the results; parts that leave 2^-24 must show at most a 64th of that."""

@@ -62,44 +62,65 @@ static th_kv_cache::Seq& the_seq(th_kv_cache* c, int32_t s, const char* what) {
 // Uploads
 // ---------------------------------------------------------------------------
 
-static uint32_t* stage(th_kv_cache* c, size_t bytes, th_kv_stage*& st) {
-    st = &c->stages[c->next_stage++ % 8];
-    if (st->used) TH_HIP(hipEventSynchronize(st->done));
-    st->used = false;
-    if (!st->done) TH_HIP(hipEventCreateWithFlags(&st->done, hipEventDisableTiming));
-    if (st->bytes < bytes) {
-        if (st->host) TH_HIP(hipHostFree(st->host));
-        st->host = nullptr;
-        st->bytes = 0;
-        const size_t want = std::max(bytes + bytes / 2, (size_t)64 << 10);
-        TH_HIP(hipHostMalloc(&st->host, want, hipHostMallocDefault));
-        st->bytes = want;
+static void stage_alloc(th_kv_stage& st, size_t bytes) {
+    if (st.host) TH_HIP(hipHostFree(st.host));
+    st.host = nullptr;
+    st.bytes = 0;
+    const hipError_t e = hipHostMalloc(&st.host, bytes, hipHostMallocDefault);
+    if (e != hipSuccess) {
+        st.host = nullptr;
+        (void)hipGetLastError();
+        throw Error(TH_ERR_OOM, "no pinned memory for uploads");
     }
-    return (uint32_t*)st->host;
+    st.bytes = bytes;
 }
 
-// The table entries that changed, and `words` to the runs' places in dst, in stream order.
-static void upload(th_kv_cache* c, const uint32_t* words, const KvRuns& runs, void* dst) {
-    const size_t n_words = (size_t)runs.words();
+// Room for an upload: behind the last one, or in the next stage when this one is full.  A stage's event is recorded
+// once, when it is left (an event for each upload cost 1.5 us of a step's host time).
+static uint32_t* stage(th_kv_cache* c, size_t bytes) {
+    bytes = round_up(bytes, 16);
+    th_kv_stage* st = &c->stages[c->stage_at];
+    if (st->at + bytes > st->bytes) {
+        if (st->at) {
+            if (!st->done) TH_HIP(hipEventCreateWithFlags(&st->done, hipEventDisableTiming));
+            TH_HIP(hipEventRecord(st->done, c->dev->stream));
+            st->busy = true;
+            c->stage_at = (c->stage_at + 1) % KV_STAGES;
+            st = &c->stages[c->stage_at];
+        }
+        if (st->busy) TH_HIP(hipEventSynchronize(st->done));
+        st->busy = false;
+        st->at = 0;
+        if (st->bytes < bytes) stage_alloc(*st, bytes + bytes / 2);
+    }
+    uint32_t* to = (uint32_t*)((char*)st->host + st->at);
+    st->at += bytes;
+    return to;
+}
+
+// The table entries that changed, and `words` to the runs' places in dst, in stream order; and copies of pages
+// ({from, to}, at most KV_ARG_COPIES) in the same launch.
+static void upload(th_kv_cache* c, const uint32_t* words, const KvRuns& runs, void* dst, const std::vector<uint32_t>* copies = nullptr) {
+    const size_t n_words = (size_t)runs.words(), n_copies = copies ? copies->size() / 2 : 0;
     size_t pairs = 0;
     for (const auto& d : c->dirty) pairs += d.second;
     const size_t total = 2 * pairs + n_words;
-    if (total == 0) return;
+    if (total + n_copies == 0) return;
     KvWords w;
-    th_kv_stage* st = nullptr;
-    uint32_t* to = total <= KV_ARG_WORDS ? w.w : stage(c, total * 4, st);
-    size_t at = 0;
+    if (n_copies) std::copy(copies->begin(), copies->end(), w.w);
+    const bool far = 2 * n_copies + total > KV_ARG_WORDS;
+    uint32_t *const from = far ? stage(c, total * 4) : w.w + 2 * n_copies, *to = from;
     for (const auto& d : c->dirty)
         for (uint32_t i = 0; i < d.second; i++) {
-            to[at++] = d.first + i;
-            to[at++] = (uint32_t)c->mirror[d.first + i];
+            *to++ = d.first + i;
+            *to++ = (uint32_t)c->mirror[d.first + i];
         }
-    if (n_words) std::memcpy(to + at, words, n_words * 4);
-    launch_kv_upload(w, st ? to : nullptr, (int)pairs, c->table, runs, (uint32_t*)dst, c->dev->stream);
-    if (st) {
-        TH_HIP(hipEventRecord(st->done, c->dev->stream));
-        st->used = true;
-    }
+    if (n_words) std::memcpy(to, words, n_words * 4);
+    if (n_copies)
+        launch_kv_copy_upload(c->pool, c->page_bytes, c->n_pages, (int)(2 * c->n_layers), w, n_copies, far ? from : nullptr, (int)pairs,
+                              c->table, runs, (uint32_t*)dst, c->dev->stream);
+    else
+        launch_kv_upload(w, far ? from : nullptr, (int)pairs, c->table, runs, (uint32_t*)dst, c->dev->stream);
     c->dirty.clear();
 }
 
@@ -109,19 +130,17 @@ static KvRuns one_run(size_t n) {
     return r;
 }
 
-// {from, to} pages, every layer's K and V.
-static void copy_pages(th_kv_cache* c, const std::vector<uint32_t>& pairs) {
+// Copies of pages ({from, to}), then the table and `words` as in upload.
+static void copy_upload(th_kv_cache* c, const std::vector<uint32_t>& pairs, const uint32_t* words, const KvRuns& runs, void* dst) {
     const size_t n = pairs.size() / 2;
-    const int planes = (int)(2 * c->n_layers);
-    if (2 * n <= KV_ARG_WORDS) {
-        KvWords w;
-        std::copy(pairs.begin(), pairs.end(), w.w);
-        launch_kv_copy_pages_args(c->pool, c->page_bytes, c->n_pages, planes, w, n, c->dev->stream);
+    if (n <= KV_ARG_COPIES) {
+        upload(c, words, runs, dst, &pairs);
         return;
     }
     uint32_t* dev = (uint32_t*)device_scratch(c->dev, 8 * n);
     upload(c, pairs.data(), one_run(2 * n), dev);
-    launch_kv_copy_pages(c->pool, c->page_bytes, c->n_pages, planes, dev, n, c->dev->stream);
+    launch_kv_copy_pages(c->pool, c->page_bytes, c->n_pages, (int)(2 * c->n_layers), dev, n, c->dev->stream);
+    upload(c, words, runs, dst);
 }
 
 // ---------------------------------------------------------------------------
@@ -582,7 +601,10 @@ int th_kv_cache_create(th_device* dev, const th_kv_cache_config* cfg, th_kv_cach
         TH_HIP(hipMemset(c->table, 0, c->mirror.size() * 4));
         TH_HIP(hipMemset(c->pool, 0, bytes));
         TH_HIP(hipDeviceSynchronize());
+        for (th_kv_stage& st : c->stages) stage_alloc(st, (size_t)64 << 10);
     } catch (...) {
+        for (th_kv_stage& st : c->stages)
+            if (st.host) (void)hipHostFree(st.host);
         if (c->pool) (void)hipFree(c->pool);
         if (c->table) (void)hipFree(c->table);
         (void)hipGetLastError();  // the next launch's check must not find it
@@ -639,7 +661,7 @@ int th_kv_cache_compact(th_kv_cache* c, size_t* n_moved) {
         moved[p] = (int)hole++;
     }
     if (!pairs.empty()) {
-        copy_pages(c, pairs);
+        copy_upload(c, pairs, nullptr, KvRuns(), nullptr);
         for (size_t i = 0; i < pairs.size(); i += 2) {
             const int from = (int)pairs[i], to = (int)pairs[i + 1];
             c->refs[to] = c->refs[from];
@@ -725,7 +747,7 @@ int th_kv_seq_resize(th_kv_cache* c, int32_t seq, size_t len) {
     std::vector<uint32_t> copies;
     grow(c, seq, len, copies);
     c->seqs[seq].version = ++c->versions;
-    copy_pages(c, copies);
+    if (!copies.empty()) copy_upload(c, copies, nullptr, KvRuns(), nullptr);
     TH_API_END
 }
 
@@ -899,8 +921,7 @@ int th_kv_batch_begin(th_kv_batch* b, const int32_t* seqs, const uint32_t* n_new
         }
     }
     b->rows = rows;
-    copy_pages(c, copies);
-    upload(c, words.data(), one_run(words.size()), b->block);
+    copy_upload(c, copies, words.data(), one_run(words.size()), b->block);
     // graphs read their plans at replay; the others are built by the step's first call that needs them
     for (auto& p : b->plans) {
         p.second.built = false;

@@ -62,7 +62,8 @@ struct KvAttnArgs {
 // ---------------------------------------------------------------------------
 
 // Words that go into a kernel's argument block.
-constexpr int KV_ARG_WORDS = 224;
+constexpr int KV_ARG_WORDS = 224, KV_ARG_COPIES = KV_ARG_WORDS / 2;
+constexpr unsigned KV_STAGES = 8;
 struct KvWords { uint32_t w[KV_ARG_WORDS]; };
 
 // Runs of words that follow one another in an upload's source: their lengths and where each goes.
@@ -78,8 +79,9 @@ void launch_kv_upload(const KvWords& w, const uint32_t* src, int n_pairs, int* t
 // Whole pages, every layer's K and V.  pairs (device): {from, to}.
 void launch_kv_copy_pages(void* pool, size_t page_bytes, size_t n_pages, int n_planes, const uint32_t* pairs, size_t n,
                           hipStream_t s);
-void launch_kv_copy_pages_args(void* pool, size_t page_bytes, size_t n_pages, int n_planes, const KvWords& w, size_t n,
-                               hipStream_t s);
+// n copies whose pairs are the first of w, and an upload whose words follow them there or are in src.
+void launch_kv_copy_upload(void* pool, size_t page_bytes, size_t n_pages, int n_planes, const KvWords& w, size_t n,
+                           const uint32_t* src, int n_pairs, int* table, const KvRuns& runs, uint32_t* dst, hipStream_t s);
 // Rows: place i of the pages to[] takes the row that is at place from[i] of the
 // line of all places, every layer's K and V.
 void launch_kv_gather_rows(void* pool, size_t n_pages, int n_planes, int n_kv_heads, int shift, size_t row_bytes,
@@ -137,12 +139,12 @@ struct DeviceScope {
 // The objects behind the handles
 // ---------------------------------------------------------------------------
 
-// Pinned memory that uploads pass through; `done` says when it is free again.
+// Pinned memory that uploads pass through, one behind the other; once it is left (busy), `done` says when it is free again.
 struct th_kv_stage {
     void* host = nullptr;
-    size_t bytes = 0;
+    size_t bytes = 0, at = 0;
     hipEvent_t done = nullptr;
-    bool used = false;
+    bool busy = false;
 };
 
 struct th_kv_cache {
@@ -165,8 +167,8 @@ struct th_kv_cache {
     size_t n_vacant = 0, hint = 0;
     std::vector<std::pair<uint32_t, uint32_t>> dirty;  // table entries to upload: first, count
     uint64_t versions = 0;
-    th_kv_stage stages[8];
-    unsigned next_stage = 0;
+    th_kv_stage stages[th::KV_STAGES];
+    unsigned stage_at = 0;
     int live = 1;  // the handle, and the batches
     bool closed = false;
 };

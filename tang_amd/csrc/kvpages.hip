@@ -16,13 +16,9 @@ typedef uint32_t kv_u32x4_t __attribute__((ext_vector_type(4)));
 // A step's tables and plans are some hundred words: as launch arguments they
 // need no copy, no staging memory and no event.  More comes from pinned host
 // memory, which the kernel reads across the bus by itself.
-__global__ __launch_bounds__(256) void kv_upload_kernel(KvWords w, const uint32_t* __restrict__ src, int n_pairs,
-                                                        int* __restrict__ table, KvRuns runs, uint32_t* __restrict__ dst) {
-    const int i0 = blockIdx.x * 256 + threadIdx.x, step = gridDim.x * 256;
-    for (int i = i0; i < n_pairs; i += step) {
-        if (src) table[src[2 * i]] = (int)src[2 * i + 1];
-        else table[w.w[2 * i]] = (int)w.w[2 * i + 1];
-    }
+__device__ __forceinline__ void kv_upload_words(int i0, int step, const uint32_t* src, int n_pairs, int* table, const KvRuns& runs,
+                                                uint32_t* dst) {
+    for (int i = i0; i < n_pairs; i += step) table[src[2 * i]] = (int)src[2 * i + 1];
     const int n_words = runs.words();
     for (int i = i0; i < n_words; i += step) {
         int to = i, end = 0;
@@ -31,8 +27,13 @@ __global__ __launch_bounds__(256) void kv_upload_kernel(KvWords w, const uint32_
             if (i >= end) to = runs.at[r] + i - end;
             end += runs.n[r];
         }
-        dst[to] = src ? src[2 * n_pairs + i] : w.w[2 * n_pairs + i];
+        dst[to] = src[2 * n_pairs + i];
     }
+}
+
+__global__ __launch_bounds__(256) void kv_upload_kernel(KvWords w, const uint32_t* src, int n_pairs, int* table, KvRuns runs,
+                                                        uint32_t* dst) {
+    kv_upload_words(blockIdx.x * 256 + threadIdx.x, gridDim.x * 256, src ? src : w.w, n_pairs, table, runs, dst);
 }
 
 void launch_kv_upload(const KvWords& w, const uint32_t* src, int n_pairs, int* table, const KvRuns& runs, uint32_t* dst,
@@ -72,9 +73,15 @@ __global__ __launch_bounds__(256) void kv_copy_pages_kernel(char* __restrict__ p
     kv_copy_piece(pool, page_bytes, n_pages, pairs[2 * blockIdx.x], pairs[2 * blockIdx.x + 1]);
 }
 
-__global__ __launch_bounds__(256) void kv_copy_pages_args_kernel(char* __restrict__ pool, size_t page_bytes, size_t n_pages,
-                                                                 KvWords w) {
-    kv_copy_piece(pool, page_bytes, n_pages, w.w[2 * blockIdx.x], w.w[2 * blockIdx.x + 1]);
+// A step whose sequences get copies of shared pages: the copies and the upload touch different memory, so they share a
+// launch (2.4 us of host time); the upload is the work of one more plane.
+__global__ __launch_bounds__(256) void kv_copy_upload_kernel(char* __restrict__ pool, size_t page_bytes, size_t n_pages, KvWords w,
+                                                             const uint32_t* src, int n_pairs, int* table, KvRuns runs, uint32_t* dst) {
+    if (blockIdx.z + 1 < gridDim.z)
+        kv_copy_piece(pool, page_bytes, n_pages, w.w[2 * blockIdx.x], w.w[2 * blockIdx.x + 1]);
+    else
+        kv_upload_words((blockIdx.y * gridDim.x + blockIdx.x) * 256 + threadIdx.x, gridDim.x * gridDim.y * 256,
+                        src ? src : w.w + 2 * gridDim.x, n_pairs, table, runs, dst);
 }
 
 void launch_kv_copy_pages(void* pool, size_t page_bytes, size_t n_pages, int n_planes, const uint32_t* pairs, size_t n,
@@ -85,12 +92,11 @@ void launch_kv_copy_pages(void* pool, size_t page_bytes, size_t n_pages, int n_p
     TH_LAUNCH_CHECK();
 }
 
-void launch_kv_copy_pages_args(void* pool, size_t page_bytes, size_t n_pages, int n_planes, const KvWords& w, size_t n,
-                               hipStream_t s) {
-    if (n == 0) return;
-    TH_LAUNCH(kv_copy_pages_args_kernel,
-              dim3((unsigned)n, (unsigned)ceil_div(page_bytes, (size_t)KV_COPY_BYTES), (unsigned)n_planes), dim3(256), 0, s,
-              (char*)pool, page_bytes, n_pages, w);
+void launch_kv_copy_upload(void* pool, size_t page_bytes, size_t n_pages, int n_planes, const KvWords& w, size_t n,
+                           const uint32_t* src, int n_pairs, int* table, const KvRuns& runs, uint32_t* dst, hipStream_t s) {
+    TH_LAUNCH(kv_copy_upload_kernel,
+              dim3((unsigned)n, (unsigned)ceil_div(page_bytes, (size_t)KV_COPY_BYTES), (unsigned)n_planes + 1), dim3(256), 0, s,
+              (char*)pool, page_bytes, n_pages, w, src, n_pairs, table, runs, dst);
     TH_LAUNCH_CHECK();
 }
 

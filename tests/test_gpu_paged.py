@@ -537,6 +537,30 @@ def test_many_moves_at_once(dev):
     m.check()
 
 
+def test_uploads_ahead_of_the_stream(dev):
+    """200 forks of a long sequence, 1.6 MB of table entries, behind work that keeps the stream busy: every child's row
+    goes to its own page, whatever of the uploads' memory is reused by then."""
+    rng = np.random.default_rng(8)
+    m = Model(dev, 1, 64, 16, 1300, 201, 1, 17000, F16, rows=16008)
+    s = m.create()
+    m.fill(rng, [s], [16008])
+    q = dev.alloc(16008 * 64, F16)
+    out = dev.alloc(16008 * 64, F16)
+    for _ in range(60):
+        m.batch.attention(0, q, out)
+    kids = []
+    rows = [[dev.upload(to_bits(np.full((1, 1, 64), x, np.float32), F16), F16) for x in (i + 1, -i - 1)] for i in range(200)]
+    for k, v in rows:
+        kids += m.cache.seq_fork(s, 1)
+        m.begin(kids[-1:], [1])
+        m.batch.append(0, None, k, v, None)
+    for i, c in enumerate(kids):
+        for w, b in enumerate(m.cache.seq_read(c, 0, 16000)):
+            got = from_bits(b.to_numpy(), F16).reshape(9, 64)
+            assert np.array_equal(got[:8], m.rows[s][0, w, 16000:, 0]), (i, w)
+            assert (got[8] == (i + 1 if w == 0 else -i - 1)).all(), (i, w)
+
+
 def test_pages_are_handed_out_lowest_first_and_addressed(dev):
     m = Model(dev, 2, 64, 16, 10, 4, 2, 160, F16)
     k0, v0 = m.cache.page_pointers(0)

@@ -514,7 +514,7 @@ int th_kv_batch_trim(th_kv_batch* b, const uint32_t* n_keep, size_t n);
  * any of them (it may be q, with q's type).  A row's position is its place in its sequence, or positions[row] where
  * that is given (as in th_rope_rows).  rot_dim 0 rotates nothing (tables may be NULL);
  * q and q_out may be NULL together.  Captured: buffers for max_rows rows, and a
- * replay runs on the batch as it last began. */
+ * replay runs on the batch as it last began (rows behind the tables' end get NaN pairs then). */
 int th_kv_append(th_kv_batch* b, size_t layer, const th_buffer* q, const th_buffer* k, const th_buffer* v,
                  const th_buffer* cos_buf, const th_buffer* sin_buf, const th_buffer* positions, size_t rot_dim,
                  int layout, th_buffer* q_out);

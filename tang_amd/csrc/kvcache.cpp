@@ -98,29 +98,39 @@ static uint32_t* stage(th_kv_cache* c, size_t bytes) {
     return to;
 }
 
+// Table entries of a sequence to upload: first and count.  (What it no longer has is read by nobody.)
+static std::pair<size_t, size_t> changed(const th_kv_cache::Seq& q) {
+    const size_t end = std::min(q.dirty_to, q.n_pages);
+    return {q.dirty_from, end > q.dirty_from ? end - q.dirty_from : 0};
+}
+
 // The table entries that changed, and `words` to the runs' places in dst, in stream order; and copies of pages
 // ({from, to}, at most KV_ARG_COPIES) in the same launch.
 static void upload(th_kv_cache* c, const uint32_t* words, const KvRuns& runs, void* dst, const std::vector<uint32_t>* copies = nullptr) {
     const size_t n_words = (size_t)runs.words(), n_copies = copies ? copies->size() / 2 : 0;
     size_t pairs = 0;
-    for (const auto& d : c->dirty) pairs += d.second;
+    for (const int32_t s : c->dirty) pairs += changed(c->seqs[s]).second;
     const size_t total = 2 * pairs + n_words;
     if (total + n_copies == 0) return;
     KvWords w;
     if (n_copies) std::copy(copies->begin(), copies->end(), w.w);
     const bool far = 2 * n_copies + total > KV_ARG_WORDS;
     uint32_t *const from = far ? stage(c, total * 4) : w.w + 2 * n_copies, *to = from;
-    for (const auto& d : c->dirty)
-        for (uint32_t i = 0; i < d.second; i++) {
-            *to++ = d.first + i;
-            *to++ = (uint32_t)c->mirror[d.first + i];
+    for (const int32_t s : c->dirty) {
+        const auto d = changed(c->seqs[s]);
+        const size_t at = (size_t)s * c->pages_per_seq + d.first;
+        for (size_t i = at; i < at + d.second; i++) {
+            *to++ = (uint32_t)i;
+            *to++ = (uint32_t)c->mirror[i];
         }
+    }
     if (n_words) std::memcpy(to, words, n_words * 4);
     if (n_copies)
         launch_kv_copy_upload(c->pool, c->page_bytes, c->n_pages, (int)(2 * c->n_layers), w, n_copies, far ? from : nullptr, (int)pairs,
                               c->table, runs, (uint32_t*)dst, c->dev->stream);
     else
         launch_kv_upload(w, far ? from : nullptr, (int)pairs, c->table, runs, (uint32_t*)dst, c->dev->stream);
+    for (const int32_t s : c->dirty) c->seqs[s].dirty_to = 0;
     c->dirty.clear();
 }
 
@@ -168,7 +178,14 @@ static void drop_page(th_kv_cache* c, int p) {
 static int* seq_table(th_kv_cache* c, int32_t s) { return c->mirror.data() + (size_t)s * c->pages_per_seq; }
 
 static void touch(th_kv_cache* c, int32_t s, size_t first, size_t n) {
-    if (n) c->dirty.emplace_back((uint32_t)((size_t)s * c->pages_per_seq + first), (uint32_t)n);
+    if (n == 0) return;
+    th_kv_cache::Seq& q = c->seqs[s];
+    if (q.dirty_to == 0) {
+        c->dirty.push_back(s);
+        q.dirty_from = first;
+    }
+    q.dirty_from = std::min(q.dirty_from, first);
+    q.dirty_to = std::max(q.dirty_to, first + n);
 }
 
 // What growing a sequence to `len` takes: pages, and whether its last one has to be
@@ -561,6 +578,7 @@ int th_kv_cache_create(th_device* dev, const th_kv_cache_config* cfg, th_kv_cach
     TH_API_BEGIN
     TH_REQUIRE(dev && cfg && out, "null argument");
     TH_REQUIRE(!dev->closed, "the device was destroyed");
+    TH_REQUIRE(!dev->capturing, "a cache cannot be made while work is captured");
     TH_REQUIRE(cfg->n_layers > 0 && cfg->n_kv_heads > 0 && cfg->head_dim > 0 && cfg->n_pages > 0 && cfg->max_seqs > 0 && cfg->max_len > 0,
                "every size must be positive");
     TH_REQUIRE(cfg->page_size >= 16 && cfg->page_size <= 1024 && (cfg->page_size & (cfg->page_size - 1)) == 0,
@@ -586,7 +604,7 @@ int th_kv_cache_create(th_device* dev, const th_kv_cache_config* cfg, th_kv_cach
     c->max_seqs = cfg->max_seqs;
     c->max_len = cfg->max_len;
     c->pages_per_seq = std::min(ceil_div(cfg->max_len, cfg->page_size), cfg->n_pages);
-    TH_REQUIRE(c->max_seqs * c->pages_per_seq < (size_t)1 << 31, "page tables exceed 2^31 entries");
+    TH_REQUIRE(c->max_seqs * c->pages_per_seq < (size_t)1 << 29, "page tables exceed 2^29 entries");
     c->page_bytes = c->n_kv_heads * c->page_size * c->hd * 2;
     c->mirror.assign(c->max_seqs * c->pages_per_seq, 0);
     c->seqs.resize(c->max_seqs);
@@ -826,6 +844,7 @@ int th_kv_batch_create(th_kv_cache* c, size_t max_seqs, size_t max_rows, size_t 
     TH_API_BEGIN
     require_open(c, __func__);
     TH_REQUIRE(out, "null argument");
+    TH_REQUIRE(!c->dev->capturing, "a batch cannot be made while work is captured");
     TH_REQUIRE(max_seqs > 0 && max_seqs <= c->max_seqs, "max_seqs must be from 1 to the cache's");
     TH_REQUIRE(max_rows > 0 && max_rows <= (size_t)1 << 24, "max_rows must be from 1 to 2^24");
     TH_REQUIRE(n_heads > 0 && n_heads % c->n_kv_heads == 0, "n_heads must be a multiple of the cache's kv heads");

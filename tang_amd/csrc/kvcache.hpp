@@ -159,13 +159,14 @@ struct th_kv_cache {
     struct Seq {
         bool used = false;
         size_t len = 0, n_pages = 0;
+        size_t dirty_from = 0, dirty_to = 0;  // table entries to upload, if any (dirty_to > 0)
         uint64_t version = 0;  // changes whenever a batch begun on the sequence no longer fits it
     };
     std::vector<Seq> seqs;
     std::vector<int> refs;         // sequences that have the page
     std::vector<uint64_t> vacant;  // a bit for each page without any
     size_t n_vacant = 0, hint = 0;
-    std::vector<std::pair<uint32_t, uint32_t>> dirty;  // table entries to upload: first, count
+    std::vector<int32_t> dirty;    // sequences with table entries to upload
     uint64_t versions = 0;
     th_kv_stage stages[th::KV_STAGES];
     unsigned stage_at = 0;

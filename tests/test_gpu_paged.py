@@ -537,6 +537,26 @@ def test_many_moves_at_once(dev):
     m.check()
 
 
+def test_forks_that_go_again_before_a_step(dev):
+    """Thousands of forks, resizes and frees without a step between: what is left of them is all that the next one uploads."""
+    rng = np.random.default_rng(9)
+    m = Model(dev, 1, 8, 16, 60, 6, 1, 500, F16)
+    s = m.create()
+    m.fill(rng, [s], [300])
+    for i in range(3000):
+        kids = m.cache.seq_fork(s, 3, 16 * (1 + i % 18))
+        m.cache.seq_resize(kids[0], 16 * (i % 5))
+        m.cache.seq_resize(kids[1], 400)
+        m.cache.seq_free(kids)
+    kid = m.cache.seq_fork(s, 1, 100)[0]
+    m.rows[kid] = m.rows[s][:, :, :100].copy()
+    other = m.create()
+    m.cache.seq_resize(kid, 50)
+    m.rows[kid] = m.rows[kid][:, :, :50]
+    m.fill(rng, [other, kid, s], [33, 70, 1])
+    m.check()
+
+
 def test_uploads_ahead_of_the_stream(dev):
     """200 forks of a long sequence, 1.6 MB of table entries, behind work that keeps the stream busy: every child's row
     goes to its own page, whatever of the uploads' memory is reused by then."""
@@ -874,6 +894,8 @@ def test_what_cannot_be_captured(dev):
         _refused(capi.TH_ERR_INVALID, c.seq_resize, s, 20)
         _refused(capi.TH_ERR_INVALID, c.seq_select, s, [0])
         _refused(capi.TH_ERR_INVALID, c.compact)
+        _refused(capi.TH_ERR_INVALID, dev.kv_cache, 1, 1, 64, 16, 8, 2, 100)
+        _refused(capi.TH_ERR_INVALID, c.batch, 2, 8, 2)
         _refused(capi.TH_ERR_INVALID, b.attention, 0, x, y, 6)  # a window that has no plan yet
         _refused(capi.TH_ERR_INVALID, b.attention, 0, dev_small, y, 5)  # fewer than max_rows rows
         b.attention(0, x, y, 5)

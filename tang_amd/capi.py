@@ -11,6 +11,7 @@ module without it raises, so no caller can silently fall back to CPU code.
 """
 import array
 import ctypes
+import gc
 import os
 
 import numpy as np
@@ -703,17 +704,23 @@ class HipComputeDevice:
     def capture(self, fn):
         """Record the library calls fn() makes on this device's stream into a
         Graph (th_capture_begin / th_capture_end)."""
-        check(lib().th_capture_begin(self.handle))
-        h = ctypes.c_void_p()
+        collecting = gc.isenabled()
+        gc.disable()  # a buffer that the collector frees in the middle would end the capture
         try:
-            fn()
-        except BaseException:
-            # end the capture (the stream must leave capture mode) and drop its graph
-            if lib().th_capture_end(self.handle, ctypes.byref(h)) == 0 and h:
-                lib().th_graph_destroy(h)
-            raise
-        check(lib().th_capture_end(self.handle, ctypes.byref(h)))
-        return Graph(h)
+            check(lib().th_capture_begin(self.handle))
+            h = ctypes.c_void_p()
+            try:
+                fn()
+            except BaseException:
+                # end the capture (the stream must leave capture mode) and drop its graph
+                if lib().th_capture_end(self.handle, ctypes.byref(h)) == 0 and h:
+                    lib().th_graph_destroy(h)
+                raise
+            check(lib().th_capture_end(self.handle, ctypes.byref(h)))
+            return Graph(h)
+        finally:
+            if collecting:
+                gc.enable()
 
     # -- quantized weights
     def q4_upload_blocks(self, blocks, rows, cols, scale_dtype=F32):

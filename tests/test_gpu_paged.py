@@ -1,6 +1,7 @@
 """The paged key/value cache: rotary positions into its pages, attention over
 them, and the moves of pages, against plain 64-bit statements (paged_ref)."""
 import ctypes
+import gc
 
 import numpy as np
 import pytest
@@ -904,6 +905,27 @@ def test_what_cannot_be_captured(dev):
     g = dev.capture(inside)
     g.launch()
     dev.sync()
+    g.free()
+
+
+def test_garbage_does_not_end_a_capture(dev):
+    """Buffers in a cycle of references, which the collector frees when so many objects have been made."""
+    x, y = dev.upload(np.ones(8, np.float32)), dev.upload(np.full(8, 2.0, np.float32))
+
+    def inside():
+        for _ in range(2):
+            dev.add_assign(x, y)
+            objects = [[i] for i in range(100000)]  # the collector's thresholds are passed
+            assert objects
+
+    cycle = [dev.alloc(64)]
+    cycle.append(cycle)
+    del cycle
+    assert gc.isenabled()
+    g = dev.capture(inside)
+    assert gc.isenabled()
+    g.launch()
+    assert np.array_equal(x.to_numpy(), np.full(8, 5.0, np.float32))
     g.free()
 
 

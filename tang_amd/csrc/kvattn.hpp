@@ -75,7 +75,7 @@ __device__ __forceinline__ float kv_load_q(const void* q, th_dtype dt, size_t at
 }
 
 // N pieces of eight values of a row as f32, all on their way before the first is used;
-// piece i starts at `at` + 8 * chunk(i) (zeros where chunk(i) says no).
+// piece i starts at `at` + 8 * chunk(i).
 template <int N, typename F>
 __device__ __forceinline__ void kv_load_row(const void* q, th_dtype dt, size_t at, F&& chunk, float (&x)[N][8]) {
     if (dt == TH_F32) {
@@ -216,7 +216,8 @@ __device__ __forceinline__ float kv_score(float d, float scale) {
 
 // One row over some of an item's keys by one wave in plain f32, for rows
 // whose MFMA sums are not finite or whose scores are huge: an infinity times a part that is zero is NaN
-// there, and hidden keys carry weight zero rather than being left out.  Blocks of `block` numbers every `step`
+// there, and hidden keys carry weight zero rather than being left out.  (A key a wave at a time: hundreds of times slower
+// than the MFMAs, for rows that no sound model makes.)  Blocks of `block` numbers every `step`
 // from `from` on.  Lane l ends with dims l, l + 64, ...; m and l are every lane's.
 template <typename E, int DE>
 __device__ __forceinline__ void kv_row_plain(const KvAttnArgs& a, const KvItem& it, const int* table, int h, size_t q_at, int pos,

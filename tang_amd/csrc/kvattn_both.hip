@@ -1,6 +1,7 @@
 // Tile and rows items in one launch: a shared prefix's tiles and the sequences' own
 // keys, prompts next to decode steps.  Tiles come first (they take longest), rows items fill what
-// they leave; two launches would each end with a part of the chip idle.
+// they leave; two launches would each end with a part of the chip idle (64 rows on a shared prefix of 8192: 112 us
+// against 119 in two launches, eight on one of 992: 25 against 32).
 #include <algorithm>
 #include <type_traits>
 

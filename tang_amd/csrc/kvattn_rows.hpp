@@ -9,6 +9,11 @@
 // takes K as it lies in memory as the first operand and leaves lane (g, r) the
 // scores of row r for keys 4g..4g+3 of each 16, which is the operand that
 // O^T += V^T.P^T wants; V^T comes out of row-major LDS by transposing reads.
+//
+// A step over long caches is bound by the reads of K and V: 48 sequences of 100 to 16000 positions (bf16, 32 heads of
+// 128 on 8) take 120 us, 5.4 TB/s, with a block of loads in flight for each wave and two workgroups a CU.
+// Eight waves to a workgroup read slower (143 us).  One sequence of 8192 positions is bound by latency: item,
+// pages, first rows, two blocks, the waves' join take 11 us, the records' join 4.5 us.
 #pragma once
 
 #include "kvattn.hpp"

@@ -250,6 +250,10 @@ struct PlanTile { KvItem it; bool small, own; };
 // Shared prefixes shorter than this are read by each sequence.
 constexpr size_t KV_MIN_PREFIX = 128;
 constexpr size_t KV_MAX_PLANS = 16;
+// Least keys of a piece.  Rows items: two blocks for each of the four waves; one of them makes the join longer than the
+// pieces get shorter (one row of 8192 keys, 32 heads of 128 on 8, four layers: 62 us, with 128 71, with 512 67,
+// with 1024 83; 24 rows with a window of 1000: 22 us, with 512 25.5, unsplit 23.7).  Tiles: eight samples of a prompt
+// of 992 take 32 us, with 512 40.
 constexpr size_t KV_MIN_ROWS_KEYS = 256, KV_MIN_TILE_KEYS = 256;
 
 class PlanMaker {
@@ -358,9 +362,10 @@ class PlanMaker {
 
     bool split(size_t scale) {
         const size_t kvh = c_->n_kv_heads, cus = (size_t)c_->dev->num_cus;
-        // Keys of a piece.  The chip holds 2 * CUs workgroups at a time: pieces are a quarter of an even
-        // share, so that uneven lengths level out, but no less than a block for each wave (rows items) or
-        // four blocks (tiles).
+        // Keys of a piece.  The chip holds 2 * CUs workgroups at a time.  Rows items are a quarter of an even share, so
+        // that uneven lengths level out.  Tiles are longer, since each of their pieces leaves 128 rows of
+        // records: 1.5 pieces a CU (six ragged prompt chunks behind a window 49 us, 64 rows on a prefix
+        // of 8192 99 us; with 4 a CU 59 and 112, with 2 54 and 109, with 1 59 and 95).
         size_t per[2];
         per[1] = round_up(std::max<size_t>(KV_MIN_ROWS_KEYS, ceil_div(keys_[1] * kvh, 8 * cus)), 64) * scale;
         per[0] = round_up(std::max<size_t>(KV_MIN_TILE_KEYS, ceil_div(keys_[0] * kvh, cus * 3 / 2)), 64) * scale;
@@ -411,14 +416,14 @@ class PlanMaker {
         }
         if (recs > b_->max_recs || tiles_.size() + extra > b_->max_items) return false;
         size_t rec = 0;
-        std::vector<int> joins;
+        std::vector<KvTok> joins;
         for (size_t i = 0; i < toks_.size(); i++) {
             KvTok& t = toks_[i];
             t.rec = (int)rec;
             t.own_n = shared[i] | (shared[i] + own[i]) << 16;
             if (!recorded[i]) continue;
             rec += (size_t)(shared[i] + own[i]);
-            joins.push_back((int)i);
+            joins.push_back(t);
         }
         std::vector<KvItem> items[2];
         for (size_t i = 0; i < tiles_.size(); i++) {
@@ -447,7 +452,7 @@ class PlanMaker {
         head.n_joins = (int)n_joins;
         head.n_rows_items = (int)n_items[1];
         head.n_tile_items = (int)n_items[0];
-        words.resize(KV_HEAD_WORDS + n_toks * sizeof(KvTok) / 4 + (n_items[0] + n_items[1]) * sizeof(KvItem) / 4 + n_joins);
+        words.resize(KV_HEAD_WORDS + n_toks * sizeof(KvTok) / 4 + (n_items[0] + n_items[1]) * sizeof(KvItem) / 4 + n_joins * sizeof(KvTok) / 4);
         uint32_t* to = words.data();
         auto put = [&](const void* p, size_t bytes) {
             if (bytes) std::memcpy(to, p, bytes);
@@ -457,7 +462,7 @@ class PlanMaker {
         put(toks_.data(), n_toks * sizeof(KvTok));
         put(items[1].data(), n_items[1] * sizeof(KvItem));
         put(items[0].data(), n_items[0] * sizeof(KvItem));
-        put(joins.data(), n_joins * 4);
+        put(joins.data(), n_joins * sizeof(KvTok));
         return true;
     }
 
@@ -474,7 +479,8 @@ static size_t plan_toks(const th_kv_batch*) { return KV_HEAD_WORDS; }
 static size_t plan_rows(const th_kv_batch* b) { return plan_toks(b) + b->max_rows * sizeof(KvTok) / 4; }
 static size_t plan_tiles(const th_kv_batch* b) { return plan_rows(b) + b->max_items * sizeof(KvItem) / 4; }
 static size_t plan_joins(const th_kv_batch* b) { return plan_tiles(b) + b->max_items * sizeof(KvItem) / 4; }
-static size_t plan_words(const th_kv_batch* b) { return plan_joins(b) + b->max_rows; }
+// (the join kernels read an entry before they know whether it is there: up to 32 rows behind the last)
+static size_t plan_words(const th_kv_batch* b) { return plan_joins(b) + (b->max_rows + 32) * sizeof(KvTok) / 4; }
 
 static void build_plan(th_kv_batch* b, const th_kv_batch::Key& key, th_kv_batch::Plan& p) {
     p.built = false;
@@ -488,7 +494,7 @@ static void build_plan(th_kv_batch* b, const th_kv_batch::Key& key, th_kv_batch:
     runs.at[2] = (int)plan_rows(b);
     runs.n[3] = (int)(m.n_items[0] * sizeof(KvItem) / 4);
     runs.at[3] = (int)plan_tiles(b);
-    runs.n[4] = (int)m.n_joins;
+    runs.n[4] = (int)(m.n_joins * sizeof(KvTok) / 4);
     runs.at[4] = (int)plan_joins(b);
     TH_REQUIRE(m.n_items[0] <= b->max_items && m.n_items[1] <= b->max_items, "attention plan exceeds its block");
     upload(b->cache, m.words.data(), runs, p.block);
@@ -1040,12 +1046,12 @@ int th_kv_batch_attention(th_kv_batch* b, size_t layer, const th_buffer* q, size
         // whatever plan the batch has at replay: every kernel, on grids that walk their lists
         launch_kv_attn_both(a, c->dtype, std::max(items, ceil_div(4 * (size_t)c->dev->num_cus, c->n_kv_heads)),
                             c->max_len > KV_LONG_ITEM, c->dev->stream);
-        launch_kv_attn_join(a, p.block + plan_joins(b), std::min<size_t>(b->max_rows, 1024), p.n_recs, c->dev->stream);
+        launch_kv_attn_join(a, (const KvTok*)(p.block + plan_joins(b)), std::min<size_t>(b->max_rows, 1024), p.n_recs, c->dev->stream);
     } else {
         if (p.n_tile_items && p.n_rows_items) launch_kv_attn_both(a, c->dtype, items, p.far, c->dev->stream);
         else if (p.n_tile_items) launch_kv_attn_tiles(a, c->dtype, items, p.far, c->dev->stream);
         else launch_kv_attn_rows(a, c->dtype, items, c->dev->stream);
-        launch_kv_attn_join(a, p.block + plan_joins(b), p.n_joins, p.n_recs, c->dev->stream);
+        launch_kv_attn_join(a, (const KvTok*)(p.block + plan_joins(b)), p.n_joins, p.n_recs, c->dev->stream);
     }
     TH_API_END
 }

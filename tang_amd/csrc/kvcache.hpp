@@ -111,7 +111,7 @@ void launch_kv_attn_rows(const KvAttnArgs& a, th_dtype cache, size_t grid, hipSt
 void launch_kv_attn_tiles(const KvAttnArgs& a, th_dtype cache, size_t grid, bool far, hipStream_t s);
 void launch_kv_attn_both(const KvAttnArgs& a, th_dtype cache, size_t grid, bool far, hipStream_t s);
 // n: tokens to join, n_recs: their records (by which the kernel is chosen).
-void launch_kv_attn_join(const KvAttnArgs& a, const int* list, size_t n, size_t n_recs, hipStream_t s);
+void launch_kv_attn_join(const KvAttnArgs& a, const KvTok* list, size_t n, size_t n_recs, hipStream_t s);
 
 // Rows (tokens x query heads of a kv head) that one item has at most.
 constexpr int KV_ROWS = 16, KV_TILE = 128;

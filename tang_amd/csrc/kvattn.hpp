@@ -247,6 +247,7 @@ __device__ __forceinline__ void kv_row_plain(const KvAttnArgs& a, const KvItem& 
             for (int e = 0; e < DE; e++)
                 acc[e] = acc[e] * f + p * (lane + 64 * e < hd ? (float)((const E*)a.pages.v)[row + lane + 64 * e] : 0.0f);
             m = mn;
+            if (l != l) return;  // a NaN among the weights: the row's sums are NaN for good
         }
     }
 }

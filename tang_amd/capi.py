@@ -618,7 +618,8 @@ class KvBatch:
 
     def begin(self, seqs, n_new):
         s, n = array.array("i", seqs), array.array("I", n_new)
-        assert len(s) == len(n)
+        if len(s) != len(n):
+            raise ValueError("one count for each sequence")
         rc = self._begin(self.handle, s.buffer_info()[0], n.buffer_info()[0], len(s))
         if rc:
             check(rc)

@@ -234,6 +234,20 @@ def test_long_prompt_without_splits(dev, qdt, cdt, other):
     assert np.abs(got[rows] - attention(*args)).max() <= attention_bound(*args, qdt, cdt, qdt)
     if other:
         assert np.abs(got[4200] - m.rows[t][0, 1, 0]).max() <= 2 * EPS[qdt] * 2.0
+    # replayed, with buffers for all 16000 rows that the batch may have
+    wide = np.zeros((16000, 2, 64), np.float32)
+    wide[:len(q)] = q
+    qb, out = dev.upload(to_bits(wide, qdt), qdt), dev.upload(to_bits(wide, qdt), qdt)
+    g = dev.capture(lambda: m.batch.attention(0, qb, out))
+    for _ in range(2):
+        g.launch()
+        dev.sync()
+        again = from_bits(out.to_numpy(), qdt).reshape(wide.shape)
+        assert np.abs(again[rows] - attention(*args)).max() <= attention_bound(*args, qdt, cdt, qdt)
+        assert not again[len(q):].any()  # rows behind the last stay as they were
+    g.free()
+    with pytest.raises(ValueError):
+        m.batch.begin([s, t], [1])
 
 
 def test_f32_queries_keep_their_precision(dev):

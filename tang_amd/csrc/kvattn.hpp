@@ -14,8 +14,14 @@ typedef short kv_s4_t __attribute__((ext_vector_type(4)));
 typedef __attribute__((address_space(3))) kv_s4_t kv_lds_s4_t;
 
 template <typename E> struct KvVec;
-template <> struct KvVec<_Float16> { typedef _Float16 x8 __attribute__((ext_vector_type(8))); };
-template <> struct KvVec<__bf16> { typedef __bf16 x8 __attribute__((ext_vector_type(8))); };
+template <> struct KvVec<_Float16> {
+    typedef _Float16 x8 __attribute__((ext_vector_type(8)));
+    typedef _Float16 x2 __attribute__((ext_vector_type(2)));
+};
+template <> struct KvVec<__bf16> {
+    typedef __bf16 x8 __attribute__((ext_vector_type(8)));
+    typedef __bf16 x2 __attribute__((ext_vector_type(2)));
+};
 
 __device__ __forceinline__ kv_f32x4_t kv_mfma16(KvVec<_Float16>::x8 a, KvVec<_Float16>::x8 b, kv_f32x4_t c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
@@ -45,6 +51,25 @@ __device__ __forceinline__ void kv_split(float x, E (&part)[NP]) {
     for (int i = 0; i < NP; i++) {
         part[i] = (E)x;
         x -= (float)part[i];
+    }
+}
+// The parts of x * up and y * up, up a power of two, as pairs.  Each rest is one operation on x itself, and the first
+// pair a new value to the compiler, which would else make half of it twice.
+template <typename E, int NP>
+__device__ __forceinline__ void kv_split_pair(float x, float y, float up, typename KvVec<E>::x2 (&part)[NP]) {
+    typedef typename KvVec<E>::x2 x2;
+    part[0] = x2{(E)(x * up), (E)(y * up)};
+    if constexpr (NP > 1) {
+        uint32_t pair = __builtin_bit_cast(uint32_t, part[0]);
+        asm("" : "+v"(pair));
+        part[0] = __builtin_bit_cast(x2, pair);
+        float r = __builtin_fmaf(x, up, -(float)part[0][0]), s = __builtin_fmaf(y, up, -(float)part[0][1]);
+#pragma unroll
+        for (int i = 1; i < NP; i++) {
+            part[i] = x2{(E)r, (E)s};
+            r -= (float)part[i][0];
+            s -= (float)part[i][1];
+        }
     }
 }
 // f16 parts keep their bits if the largest is near the type's end: queries are brought to

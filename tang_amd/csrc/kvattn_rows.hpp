@@ -144,13 +144,17 @@ __device__ __forceinline__ void kv_rows_item(const KvAttnArgs& a, const KvItem& 
 #pragma unroll
         for (int t = 0; t < 2; t++)
 #pragma unroll
-            for (int i = 0; i < 4; i++) {
-                const float e = kv_exp2(__builtin_fmaf(s[t][i], scale, -ref));
-                ps += e;
-                E part[NP];
-                kv_split<E, NP>(NP == 1 ? e : e * KV_P_UP, part);
+            for (int i = 0; i < 4; i += 2) {
+                const float e0 = kv_exp2(__builtin_fmaf(s[t][i], scale, -ref)), e1 = kv_exp2(__builtin_fmaf(s[t][i + 1], scale, -ref));
+                ps += e0;
+                ps += e1;
+                typename KvVec<E>::x2 part[NP];
+                kv_split_pair<E, NP>(e0, e1, NP == 1 ? 1.0f : KV_P_UP, part);
 #pragma unroll
-                for (int u = 0; u < NP; u++) p[u][4 * t + i] = part[u];
+                for (int u = 0; u < NP; u++) {
+                    p[u][4 * t + i] = part[u][0];
+                    p[u][4 * t + i + 1] = part[u][1];
+                }
             }
         l = l * f + ps;  // this lane's keys; the row's lanes meet at the end
         m = mn;

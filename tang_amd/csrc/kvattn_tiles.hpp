@@ -9,7 +9,7 @@
 // contraction in O^T += V^T.P^T follows that (slots 8h .. 8h + 7 of a step of 16 keys are
 // keys 4h .. 4h + 3 and 8 + 4h ..), so probabilities never leave their lane.
 //
-// Bound by the SIMDs' issue: the MFMAs' time and the softmax's vector instructions (some eight for a score) add up.
+// Bound by the SIMDs' issue: the MFMAs' time and the softmax's vector instructions (four for a score, six with two parts) add up.
 // A prompt of 8192 (bf16, 32 heads of 128 on 8): 612 us, 900 TFLOP/s of what rows see, where a large matrix product
 // reaches 1231.  Eight waves in two phases, wave priorities, two chains of MFMAs and blocks of 32 keys
 // with three workgroups a CU gave nothing more.  f32 queries on an f16 cache take twice the MFMAs.
@@ -193,13 +193,17 @@ __device__ __forceinline__ void kv_tiles_item(const KvAttnArgs& a, const KvItem&
 #pragma unroll
         for (int t = 0; t < KT; t++)
 #pragma unroll
-            for (int i = 0; i < 16; i++) {
-                const float e = kv_exp2(__builtin_fmaf(s[t][i], scale, -ref));
-                ps += e;
-                E part[NP];
-                kv_split<E, NP>(NP == 1 ? e : e * KV_P_UP, part);
+            for (int i = 0; i < 16; i += 2) {
+                const float e0 = kv_exp2(__builtin_fmaf(s[t][i], scale, -ref)), e1 = kv_exp2(__builtin_fmaf(s[t][i + 1], scale, -ref));
+                ps += e0;
+                ps += e1;
+                typename KvVec<E>::x2 part[NP];
+                kv_split_pair<E, NP>(e0, e1, NP == 1 ? 1.0f : KV_P_UP, part);
 #pragma unroll
-                for (int u = 0; u < NP; u++) p[u][2 * t + (i >> 3)][i & 7] = part[u];
+                for (int u = 0; u < NP; u++) {
+                    p[u][2 * t + (i >> 3)][i & 7] = part[u][0];
+                    p[u][2 * t + (i >> 3)][(i & 7) + 1] = part[u][1];
+                }
             }
         l += ps;  // this lane's keys; the row's two lanes meet at the end
         {

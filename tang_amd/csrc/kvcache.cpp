@@ -104,33 +104,63 @@ static std::pair<size_t, size_t> changed(const th_kv_cache::Seq& q) {
     return {q.dirty_from, end > q.dirty_from ? end - q.dirty_from : 0};
 }
 
+// How many of a fork's first entries the device copies from the row it was forked from.  That row holds them as long as
+// nothing is uploaded; one that changes in this very upload is not read, and the entries go up like any others.
+static size_t copied_row(const th_kv_cache* c, const th_kv_cache::Seq& q) {
+    const size_t n = std::min(q.row_n, q.n_pages);
+    if (n == 0) return 0;
+    const th_kv_cache::Seq& o = c->seqs[q.row_of];
+    return o.row_n > 0 || (o.dirty_to > 0 && o.dirty_from < n) ? 0 : n;
+}
+
 // The table entries that changed, and `words` to the runs' places in dst, in stream order; and copies of pages
 // ({from, to}, at most KV_ARG_COPIES) in the same launch.
 static void upload(th_kv_cache* c, const uint32_t* words, const KvRuns& runs, void* dst, const std::vector<uint32_t>* copies = nullptr) {
     const size_t n_words = (size_t)runs.words(), n_copies = copies ? copies->size() / 2 : 0;
-    size_t pairs = 0;
-    for (const int32_t s : c->dirty) pairs += changed(c->seqs[s]).second;
-    const size_t total = 2 * pairs + n_words;
+    size_t pairs = 0, rows = 0;
+    for (const int32_t s : c->dirty) {
+        const th_kv_cache::Seq& q = c->seqs[s];
+        const size_t n = copied_row(c, q);
+        rows += n > 0;
+        pairs += changed(q).second + (n ? 0 : std::min(q.row_n, q.n_pages));
+    }
+    const size_t total = 3 * rows + 2 * pairs + n_words;
     if (total + n_copies == 0) return;
     KvWords w;
     if (n_copies) std::copy(copies->begin(), copies->end(), w.w);
     const bool far = 2 * n_copies + total > KV_ARG_WORDS;
-    uint32_t *const from = far ? stage(c, total * 4) : w.w + 2 * n_copies, *to = from;
-    for (const int32_t s : c->dirty) {
-        const auto d = changed(c->seqs[s]);
-        const size_t at = (size_t)s * c->pages_per_seq + d.first;
-        for (size_t i = at; i < at + d.second; i++) {
+    uint32_t *const from = far ? stage(c, total * 4) : w.w + 2 * n_copies, *row = from, *to = from + 3 * rows;
+    auto entries = [&](size_t at, size_t n) {
+        for (size_t i = at; i < at + n; i++) {
             *to++ = (uint32_t)i;
             *to++ = (uint32_t)c->mirror[i];
         }
+    };
+    for (const int32_t s : c->dirty) {
+        const th_kv_cache::Seq& q = c->seqs[s];
+        const size_t at = (size_t)s * c->pages_per_seq;
+        if (const size_t n = copied_row(c, q)) {
+            *row++ = (uint32_t)(q.row_of * c->pages_per_seq);
+            *row++ = (uint32_t)at;
+            *row++ = (uint32_t)n;
+        } else {
+            entries(at, std::min(q.row_n, q.n_pages));
+        }
+        const auto d = changed(q);
+        entries(at + d.first, d.second);
     }
     if (n_words) std::memcpy(to, words, n_words * 4);
+    const KvTableWork work{far ? from : nullptr, (int)rows, (int)pairs, c->table};
     if (n_copies)
-        launch_kv_copy_upload(c->pool, c->page_bytes, c->n_pages, (int)(2 * c->n_layers), w, n_copies, far ? from : nullptr, (int)pairs,
-                              c->table, runs, (uint32_t*)dst, c->dev->stream);
+        launch_kv_copy_upload(c->pool, c->page_bytes, c->n_pages, (int)(2 * c->n_layers), w, n_copies, work, runs, (uint32_t*)dst,
+                              c->dev->stream);
     else
-        launch_kv_upload(w, far ? from : nullptr, (int)pairs, c->table, runs, (uint32_t*)dst, c->dev->stream);
-    for (const int32_t s : c->dirty) c->seqs[s].dirty_to = 0;
+        launch_kv_upload(w, work, runs, (uint32_t*)dst, c->dev->stream);
+    for (const int32_t s : c->dirty) {
+        th_kv_cache::Seq& q = c->seqs[s];
+        q.dirty_from = q.dirty_to = q.row_n = 0;
+        q.listed = false;
+    }
     c->dirty.clear();
 }
 
@@ -177,15 +207,22 @@ static void drop_page(th_kv_cache* c, int p) {
 
 static int* seq_table(th_kv_cache* c, int32_t s) { return c->mirror.data() + (size_t)s * c->pages_per_seq; }
 
+static void list(th_kv_cache* c, int32_t s) {
+    if (!c->seqs[s].listed) c->dirty.push_back(s);
+    c->seqs[s].listed = true;
+}
+
 static void touch(th_kv_cache* c, int32_t s, size_t first, size_t n) {
     if (n == 0) return;
     th_kv_cache::Seq& q = c->seqs[s];
-    if (q.dirty_to == 0) {
-        c->dirty.push_back(s);
-        q.dirty_from = first;
+    list(c, s);
+    size_t end = first + n;
+    if (first < q.row_n) {  // the rest of a copied row goes up with the entries from here on
+        end = std::max(end, q.row_n);
+        q.row_n = first;
     }
-    q.dirty_from = std::min(q.dirty_from, first);
-    q.dirty_to = std::max(q.dirty_to, first + n);
+    q.dirty_from = q.dirty_to ? std::min(q.dirty_from, first) : first;
+    q.dirty_to = std::max(q.dirty_to, end);
 }
 
 // What growing a sequence to `len` takes: pages, and whether its last one has to be
@@ -724,6 +761,7 @@ int th_kv_seq_create(th_kv_cache* c, size_t n, int32_t* seqs) {
         th_kv_cache::Seq& q = c->seqs[got[i]];
         q.used = true;
         q.len = q.n_pages = 0;
+        q.dirty_from = q.dirty_to = q.row_n = 0;
         q.version = ++c->versions;
         seqs[i] = got[i];
     }
@@ -784,11 +822,19 @@ int th_kv_seq_fork(th_kv_cache* c, int32_t seq, size_t len, size_t n, int32_t* c
     check_status(th_kv_seq_create(c, n, children));
     const size_t pages = ceil_div(len, c->page_size);
     const int* from = seq_table(c, seq);
+    const bool row = c->seqs[seq].row_n == 0 && c->seqs[seq].dirty_to == 0;  // the device has the parent's row
     for (size_t i = 0; i < n; i++) {
+        th_kv_cache::Seq& q = c->seqs[children[i]];
         std::copy(from, from + pages, seq_table(c, children[i]));
-        touch(c, children[i], 0, pages);
-        c->seqs[children[i]].len = len;
-        c->seqs[children[i]].n_pages = pages;
+        q.len = len;
+        q.n_pages = pages;
+        if (row && pages) {
+            q.row_of = seq;
+            q.row_n = pages;
+            list(c, children[i]);
+        } else {
+            touch(c, children[i], 0, pages);
+        }
     }
     for (size_t p = 0; p < pages; p++) c->refs[from[p]] += (int)n;
     TH_API_END

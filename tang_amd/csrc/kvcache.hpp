@@ -72,16 +72,21 @@ struct KvRuns {
     int n[MAX] = {}, at[MAX] = {};
     __host__ __device__ int words() const { return n[0] + n[1] + n[2] + n[3] + n[4]; }
 };
-// table[index] = value for n_pairs pairs, then runs of words to dst; both come
-// from src (device-visible host memory) or, where that is null, from w.
-void launch_kv_upload(const KvWords& w, const uint32_t* src, int n_pairs, int* table, const KvRuns& runs, uint32_t* dst,
-                      hipStream_t s);
+// Changes of a table: n_rows times {from, to, n} (n entries copied from one place to another; none of a place that changes),
+// n_pairs times {index, value}, then an upload's words; all from src (device-visible host memory) or, where that is null,
+// from a launch's arguments.
+struct KvTableWork {
+    const uint32_t* src;
+    int n_rows, n_pairs;
+    int* table;
+};
+void launch_kv_upload(const KvWords& w, const KvTableWork& work, const KvRuns& runs, uint32_t* dst, hipStream_t s);
 // Whole pages, every layer's K and V.  pairs (device): {from, to}.
 void launch_kv_copy_pages(void* pool, size_t page_bytes, size_t n_pages, int n_planes, const uint32_t* pairs, size_t n,
                           hipStream_t s);
 // n copies whose pairs are the first of w, and an upload whose words follow them there or are in src.
 void launch_kv_copy_upload(void* pool, size_t page_bytes, size_t n_pages, int n_planes, const KvWords& w, size_t n,
-                           const uint32_t* src, int n_pairs, int* table, const KvRuns& runs, uint32_t* dst, hipStream_t s);
+                           const KvTableWork& work, const KvRuns& runs, uint32_t* dst, hipStream_t s);
 // Rows: place i of the pages to[] takes the row that is at place from[i] of the
 // line of all places, every layer's K and V.
 void launch_kv_gather_rows(void* pool, size_t n_pages, int n_planes, int n_kv_heads, int shift, size_t row_bytes,
@@ -159,7 +164,11 @@ struct th_kv_cache {
     struct Seq {
         bool used = false;
         size_t len = 0, n_pages = 0;
-        size_t dirty_from = 0, dirty_to = 0;  // table entries to upload, if any (dirty_to > 0)
+        // to upload: entries [dirty_from, dirty_to), if any (dirty_to > 0), and the first row_n, which are those of row_of's
+        // row on the device
+        size_t dirty_from = 0, dirty_to = 0, row_n = 0;
+        int32_t row_of = 0;
+        bool listed = false;  // in `dirty`
         uint64_t version = 0;  // changes whenever a batch begun on the sequence no longer fits it
     };
     std::vector<Seq> seqs;

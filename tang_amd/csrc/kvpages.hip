@@ -16,9 +16,17 @@ typedef uint32_t kv_u32x4_t __attribute__((ext_vector_type(4)));
 // A step's tables and plans are some hundred words: as launch arguments they
 // need no copy, no staging memory and no event.  More comes from pinned host
 // memory, which the kernel reads across the bus by itself.
-__device__ __forceinline__ void kv_upload_words(int i0, int step, const uint32_t* src, int n_pairs, int* table, const KvRuns& runs,
-                                                uint32_t* dst) {
-    for (int i = i0; i < n_pairs; i += step) table[src[2 * i]] = (int)src[2 * i + 1];
+__device__ __forceinline__ void kv_upload_words(int block, int blocks, const uint32_t* src, const KvTableWork& work,
+                                                const KvRuns& runs, uint32_t* dst) {
+    const int i0 = block * 256 + threadIdx.x, step = blocks * 256;
+    for (int r = block; r < work.n_rows; r += blocks) {
+        const int *from = work.table + src[3 * r], n = (int)src[3 * r + 2];
+        int* to = work.table + src[3 * r + 1];
+        for (int i = threadIdx.x; i < n; i += 256) to[i] = from[i];
+    }
+    src += 3 * work.n_rows;
+    for (int i = i0; i < work.n_pairs; i += step) work.table[src[2 * i]] = (int)src[2 * i + 1];
+    src += 2 * work.n_pairs;
     const int n_words = runs.words();
     for (int i = i0; i < n_words; i += step) {
         int to = i, end = 0;
@@ -27,21 +35,18 @@ __device__ __forceinline__ void kv_upload_words(int i0, int step, const uint32_t
             if (i >= end) to = runs.at[r] + i - end;
             end += runs.n[r];
         }
-        dst[to] = src[2 * n_pairs + i];
+        dst[to] = src[i];
     }
 }
 
-__global__ __launch_bounds__(256) void kv_upload_kernel(KvWords w, const uint32_t* src, int n_pairs, int* table, KvRuns runs,
-                                                        uint32_t* dst) {
-    kv_upload_words(blockIdx.x * 256 + threadIdx.x, gridDim.x * 256, src ? src : w.w, n_pairs, table, runs, dst);
+__global__ __launch_bounds__(256) void kv_upload_kernel(KvWords w, KvTableWork work, KvRuns runs, uint32_t* dst) {
+    kv_upload_words(blockIdx.x, gridDim.x, work.src ? work.src : w.w, work, runs, dst);
 }
 
-void launch_kv_upload(const KvWords& w, const uint32_t* src, int n_pairs, int* table, const KvRuns& runs, uint32_t* dst,
-                      hipStream_t s) {
-    const size_t n = (size_t)n_pairs + runs.words();
+void launch_kv_upload(const KvWords& w, const KvTableWork& work, const KvRuns& runs, uint32_t* dst, hipStream_t s) {
+    const size_t n = std::max(ceil_div((size_t)work.n_pairs + runs.words(), 256), (size_t)work.n_rows);
     if (n == 0) return;
-    TH_LAUNCH(kv_upload_kernel, dim3((unsigned)std::min<size_t>(ceil_div(n, 256), 64)), dim3(256), 0, s, w, src, n_pairs, table,
-              runs, dst);
+    TH_LAUNCH(kv_upload_kernel, dim3((unsigned)std::min<size_t>(n, 64)), dim3(256), 0, s, w, work, runs, dst);
     TH_LAUNCH_CHECK();
 }
 
@@ -76,12 +81,12 @@ __global__ __launch_bounds__(256) void kv_copy_pages_kernel(char* __restrict__ p
 // A step whose sequences get copies of shared pages: the copies and the upload touch different memory, so they share a
 // launch (2.4 us of host time); the upload is the work of one more plane.
 __global__ __launch_bounds__(256) void kv_copy_upload_kernel(char* __restrict__ pool, size_t page_bytes, size_t n_pages, KvWords w,
-                                                             const uint32_t* src, int n_pairs, int* table, KvRuns runs, uint32_t* dst) {
+                                                             KvTableWork work, KvRuns runs, uint32_t* dst) {
     if (blockIdx.z + 1 < gridDim.z)
         kv_copy_piece(pool, page_bytes, n_pages, w.w[2 * blockIdx.x], w.w[2 * blockIdx.x + 1]);
     else
-        kv_upload_words((blockIdx.y * gridDim.x + blockIdx.x) * 256 + threadIdx.x, gridDim.x * gridDim.y * 256,
-                        src ? src : w.w + 2 * gridDim.x, n_pairs, table, runs, dst);
+        kv_upload_words(blockIdx.y * gridDim.x + blockIdx.x, gridDim.x * gridDim.y, work.src ? work.src : w.w + 2 * gridDim.x, work, runs,
+                        dst);
 }
 
 void launch_kv_copy_pages(void* pool, size_t page_bytes, size_t n_pages, int n_planes, const uint32_t* pairs, size_t n,
@@ -93,10 +98,10 @@ void launch_kv_copy_pages(void* pool, size_t page_bytes, size_t n_pages, int n_p
 }
 
 void launch_kv_copy_upload(void* pool, size_t page_bytes, size_t n_pages, int n_planes, const KvWords& w, size_t n,
-                           const uint32_t* src, int n_pairs, int* table, const KvRuns& runs, uint32_t* dst, hipStream_t s) {
+                           const KvTableWork& work, const KvRuns& runs, uint32_t* dst, hipStream_t s) {
     TH_LAUNCH(kv_copy_upload_kernel,
               dim3((unsigned)n, (unsigned)ceil_div(page_bytes, (size_t)KV_COPY_BYTES), (unsigned)n_planes + 1), dim3(256), 0, s,
-              (char*)pool, page_bytes, n_pages, w, src, n_pairs, table, runs, dst);
+              (char*)pool, page_bytes, n_pages, w, work, runs, dst);
     TH_LAUNCH_CHECK();
 }
 

@@ -572,6 +572,42 @@ def test_forks_that_go_again_before_a_step(dev):
     m.check()
 
 
+@pytest.mark.parametrize("seed", range(6))
+def test_any_order_of_forks_and_changes(dev, seed):
+    """Forks of forks, parents that shrink, go, or come again as something else, before anything of it is uploaded."""
+    rng = np.random.default_rng(seed)
+    m = Model(dev, 1, 8, 16, 150, 12, 1, 600, F16)
+    m.fill(rng, [m.create()], [400])
+    for i in range(250):
+        live = list(m.rows)
+        s = live[rng.integers(len(live))]
+        have = m.rows[s].shape[2]
+        kind = rng.integers(6)
+        if kind == 0 and len(live) > 2:
+            m.cache.seq_free([s])
+            del m.rows[s]
+        elif kind == 1 and len(live) < 11:
+            n = int(rng.integers(0, have + 1))
+            for c in m.cache.seq_fork(s, int(rng.integers(1, 13 - len(live))), n):
+                m.rows[c] = m.rows[s][:, :, :n].copy()
+        elif kind == 2 and rng.random() < 0.3:
+            n = int(rng.integers(have // 2, have + 1))
+            m.cache.seq_resize(s, n)
+            m.rows[s] = m.rows[s][:, :, :n]
+        elif kind == 3 and rng.random() < 0.3 and have and m.cache.info()[0] > 40:
+            at = rng.integers(0, have, int(rng.integers(1, min(have, 100) + 1)))
+            m.cache.seq_select(s, at)
+            m.rows[s] = m.rows[s][:, :, at]
+        elif kind == 4 and rng.random() < 0.2:
+            m.cache.compact()
+        elif kind == 5 and m.cache.info()[0] > 30:
+            some = [x for x in live if m.rows[x].shape[2] < 500][:3]
+            m.fill(rng, some, [int(rng.integers(0, 40)) for _ in some])
+        if i % 9 == 8:
+            m.check()
+    m.check()
+
+
 def test_uploads_ahead_of_the_stream(dev):
     """200 forks of a long sequence, 1.6 MB of table entries, behind work that keeps the stream busy: every child's row
     goes to its own page, whatever of the uploads' memory is reused by then."""

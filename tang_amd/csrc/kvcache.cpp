@@ -722,7 +722,7 @@ int th_kv_cache_compact(th_kv_cache* c, size_t* n_moved) {
         moved[p] = (int)hole++;
     }
     if (!pairs.empty()) {
-        copy_upload(c, pairs, nullptr, KvRuns(), nullptr);
+        if (pairs.size() / 2 > KV_ARG_COPIES) device_scratch(c->dev, 4 * pairs.size());  // there before anything changes
         for (size_t i = 0; i < pairs.size(); i += 2) {
             const int from = (int)pairs[i], to = (int)pairs[i + 1];
             c->refs[to] = c->refs[from];
@@ -743,7 +743,7 @@ int th_kv_cache_compact(th_kv_cache* c, size_t* n_moved) {
             }
             if (any) c->seqs[s].version = ++c->versions;
         }
-        upload(c, nullptr, KvRuns(), nullptr);
+        copy_upload(c, pairs, nullptr, KvRuns(), nullptr);
     }
     if (n_moved) *n_moved = pairs.size() / 2;
     TH_API_END

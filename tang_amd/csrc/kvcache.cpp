@@ -402,7 +402,8 @@ class PlanMaker {
         // Keys of a piece.  The chip holds 2 * CUs workgroups at a time.  Rows items are a quarter of an even share, so
         // that uneven lengths level out.  Tiles are longer, since each of their pieces leaves 128 rows of
         // records: 1.5 pieces a CU (six ragged prompt chunks behind a window 49 us, 64 rows on a prefix
-        // of 8192 99 us; with 4 a CU 59 and 112, with 2 54 and 109, with 1 59 and 95).
+        // of 8192 99 us, 512 tokens beside 32 decode steps 146 us, 128 rows on a prefix of 16000 115 us; with 4 a CU 59 and
+        // 112, with 2 54 and 109, with 1 59, 95, 138 and 126).
         size_t per[2];
         per[1] = round_up(std::max<size_t>(KV_MIN_ROWS_KEYS, ceil_div(keys_[1] * kvh, 8 * cus)), 64) * scale;
         per[0] = round_up(std::max<size_t>(KV_MIN_TILE_KEYS, ceil_div(keys_[0] * kvh, cus * 3 / 2)), 64) * scale;

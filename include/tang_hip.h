@@ -521,9 +521,9 @@ int th_kv_append(th_kv_batch* b, size_t layer, const th_buffer* q, const th_buff
 /* Attention of the step's rows over the pages: the row at place p of its sequence
  * sees keys j <= p with window == 0, j > p - window or j < n_sinks.  q and out
  * [rows][n_heads][head_dim], each f32, f16 or bf16, query head h reads kv head
- * h / (n_heads / n_kv_heads); scores times scale (0: 1/sqrt(head_dim)), softmax and sums in f32.  q and out of
- * the cache's type take probabilities rounded to it; any other mix keeps f32's
- * precision.  Pages that sequences of the batch share from their start on are read once for all.
+ * h / (n_heads / n_kv_heads); scores times scale (0: 1/sqrt(head_dim)), softmax and sums in f32.  With q and out of
+ * the cache's type, more than 16 rows (new positions x query heads of a kv head) taken together, as in prompts and on shared
+ * prefixes, have probabilities rounded to it, in the dividend and the divisor alike; all else keeps f32's precision or, for such types, 2^-18.  Pages that sequences of the batch share from their start on are read once for all.
  * Captured (after the same call has been made once): buffers for max_rows rows, and
  * a replay runs on the batch as it last began. */
 int th_kv_batch_attention(th_kv_batch* b, size_t layer, const th_buffer* q, size_t window, size_t n_sinks, float scale,

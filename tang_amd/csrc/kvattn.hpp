@@ -41,8 +41,9 @@ __device__ __forceinline__ kv_f32x16_t kv_mfma32(KvVec<__bf16>::x8 a, KvVec<__bf
 // takes the bits that the ones before left, rounded to nearest.  Two f16 are off by
 // 2^-24 of the value at most (2^-12 is left behind the first, and 2^-12 of that), three
 // bf16 by 2^-27: an f32's own rounding or less.  NP = 1 is for queries and
-// results of the cache's type: the one rounding of a probability (2^-11 f16, 2^-8 bf16
-// at most half a step each) is that of a result.
+// results of the cache's type.  Their weights are two values in rows items, which leaves 2^-18 (bf16) or less and is hidden behind the
+// reads of K and V (48 ragged sequences 120 us with one and with two), and one in tiles, where a second takes half as many MFMAs again (a prompt of 8192
+// in bf16: 605 us, with two 807).  Its rounding, half a step, comes on top of the result's own half step, for each weight in a direction of its own.
 template <typename E> constexpr int kv_wide_parts() { return sizeof(E) == 2 && std::is_same<E, __bf16>::value ? 3 : 2; }
 
 template <typename E, int NP>
@@ -76,6 +77,15 @@ __device__ __forceinline__ void kv_split_pair(float x, float y, float up, typena
 // [2^14, 2^15) by a power of two for each row, probabilities (at most 1) by 2^14.
 constexpr int KV_Q_TOP = 15;
 constexpr float KV_P_UP = 16384.0f;
+// sum + a pair's two values, in f32.  The divisor sums the weights as they went into the product, rounded: the quotient is then a mean
+// with weights that add up to one, whatever way they were all rounded (equal values give that value).  One instruction, where
+// adding the unrounded weights takes two.
+__device__ __forceinline__ float kv_add_pair(KvVec<_Float16>::x2 a, float sum) {
+    return __builtin_amdgcn_fdot2(a, KvVec<_Float16>::x2{(_Float16)1.0f, (_Float16)1.0f}, sum, false);
+}
+__device__ __forceinline__ float kv_add_pair(KvVec<__bf16>::x2 a, float sum) {
+    return __builtin_amdgcn_fdot2_f32_bf16(a, KvVec<__bf16>::x2{(__bf16)1.0f, (__bf16)1.0f}, sum, false);
+}
 
 __device__ __forceinline__ float kv_exp2(float x) { return __builtin_amdgcn_exp2f(x); }
 

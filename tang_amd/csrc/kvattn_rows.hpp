@@ -34,6 +34,7 @@ __device__ __forceinline__ void kv_rows_item(const KvAttnArgs& a, const KvItem& 
     typedef KvRows<D> W;
     typedef typename KvVec<E>::x8 x8;
     constexpr int NK = W::NK, NDT = W::NDT, LD = W::LD, KB = W::KB, CPR = W::CPR, VL = W::VL, DE = D / 64;
+    constexpr int PP = NP == 1 ? 2 : NP;  // parts of a weight (kvattn.hpp)
     constexpr size_t REGION = W::REGION;
     float(*sm)[16] = (float(*)[16])(lds + 4 * REGION), (*sl)[16] = sm + 4, *sM = sl[4];
     const KvTok* toks = a.toks;
@@ -140,7 +141,7 @@ __device__ __forceinline__ void kv_rows_item(const KvAttnArgs& a, const KvItem& 
         bm = fmaxf(bm, __shfl_xor(bm, 32, 64)) * scale;
         const float mn = fmaxf(m, bm), ref = mn == -INFINITY ? 0.0f : mn, f = kv_exp2(m - ref);
         float ps = 0.0f;
-        x8 p[NP];
+        x8 p[PP];
 #pragma unroll
         for (int t = 0; t < 2; t++)
 #pragma unroll
@@ -148,10 +149,10 @@ __device__ __forceinline__ void kv_rows_item(const KvAttnArgs& a, const KvItem& 
                 const float e0 = kv_exp2(__builtin_fmaf(s[t][i], scale, -ref)), e1 = kv_exp2(__builtin_fmaf(s[t][i + 1], scale, -ref));
                 ps += e0;
                 ps += e1;
-                typename KvVec<E>::x2 part[NP];
-                kv_split_pair<E, NP>(e0, e1, NP == 1 ? 1.0f : KV_P_UP, part);
+                typename KvVec<E>::x2 part[PP];
+                kv_split_pair<E, PP>(e0, e1, NP == 1 ? 1.0f : KV_P_UP, part);
 #pragma unroll
-                for (int u = 0; u < NP; u++) {
+                for (int u = 0; u < PP; u++) {
                     p[u][4 * t + i] = part[u][0];
                     p[u][4 * t + i + 1] = part[u][1];
                 }
@@ -175,7 +176,7 @@ __device__ __forceinline__ void kv_rows_item(const KvAttnArgs& a, const KvItem& 
             const x8 va = __builtin_bit_cast(x8, (s8){w[0][0], w[0][1], w[0][2], w[0][3], w[1][0], w[1][1], w[1][2], w[1][3]});
             kv_f32x4_t d = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-            for (int u = NP - 1; u >= 0; u--) d = kv_mfma16(va, p[u], d);
+            for (int u = PP - 1; u >= 0; u--) d = kv_mfma16(va, p[u], d);
 #pragma unroll
             for (int i = 0; i < 4; i++) o[dt][i] = __builtin_fmaf(o[dt][i], f, d[i]);
         }

@@ -30,8 +30,9 @@ struct KvTiles {
 };
 
 // One item by a workgroup.  ADD: a block's sum of values is added to the sums so far in plain additions, since an
-// MFMA truncates what it adds to a larger sum.  Results of 16 bits do not see that (a step of 2^-24 for 16 keys) over the
-// KV_LONG_ITEM keys that an item without ADD has at most.  (Without ADD the sums cost no vector instruction.)
+// MFMA truncates what it adds to a larger sum.  Results of 16 bits do not see that over the KV_LONG_ITEM keys that an item
+// without ADD has at most: 1024 steps of 16 keys lose up to 2^-23 of the sum so far each, which is 3e-5 of values of one sign, next to a
+// rounding of 5e-4 (f16) or 4e-3 (bf16).  (Without ADD the sums cost no vector instruction.)
 template <int D, typename E, int NP, bool PAD, bool ADD>
 __device__ __forceinline__ void kv_tiles_item(const KvAttnArgs& a, const KvItem& it, int hk, char* lds_) {
     typedef KvTiles<D, NP> T;
@@ -195,10 +196,14 @@ __device__ __forceinline__ void kv_tiles_item(const KvAttnArgs& a, const KvItem&
 #pragma unroll
             for (int i = 0; i < 16; i += 2) {
                 const float e0 = kv_exp2(__builtin_fmaf(s[t][i], scale, -ref)), e1 = kv_exp2(__builtin_fmaf(s[t][i + 1], scale, -ref));
-                ps += e0;
-                ps += e1;
                 typename KvVec<E>::x2 part[NP];
                 kv_split_pair<E, NP>(e0, e1, NP == 1 ? 1.0f : KV_P_UP, part);
+                if constexpr (NP == 1) {
+                    ps = kv_add_pair(part[0], ps);
+                } else {
+                    ps += e0;
+                    ps += e1;
+                }
 #pragma unroll
                 for (int u = 0; u < NP; u++) {
                     p[u][2 * t + (i >> 3)][i & 7] = part[u][0];

@@ -77,6 +77,13 @@ __device__ __forceinline__ void kv_split_pair(float x, float y, float up, typena
 // [2^14, 2^15) by a power of two for each row, probabilities (at most 1) by 2^14.
 constexpr int KV_Q_TOP = 15;
 constexpr float KV_P_UP = 16384.0f;
+// Weights of queries and results of the cache's type are taken against a reference that lies KV_*_LOW below the running
+// maximum, so that f16's largest come near 2^15 (in tiles the reference may lag by 2^KV_LAG): a weight of 2^-14 of the largest would
+// else lose bits below f16's normal range, and one of 2^-25 all of them, and together such weights can be most of a row.  bf16 has f32's range.
+constexpr float KV_LAG = 6.0f;
+template <typename E> constexpr float kv_rows_low() { return std::is_same<E, _Float16>::value ? 15.0f : 0.0f; }
+template <typename E> constexpr float kv_tiles_low() { return std::is_same<E, _Float16>::value ? 15.0f - KV_LAG : 0.0f; }
+
 // sum + a pair's two values, in f32.  The divisor sums the weights as they went into the product, rounded: the quotient is then a mean
 // with weights that add up to one, whatever way they were all rounded (equal values give that value).  One instruction, where
 // adding the unrounded weights takes two.

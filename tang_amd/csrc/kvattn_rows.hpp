@@ -139,6 +139,7 @@ __device__ __forceinline__ void kv_rows_item(const KvAttnArgs& a, const KvItem& 
             }
         bm = fmaxf(bm, __shfl_xor(bm, 16, 64));
         bm = fmaxf(bm, __shfl_xor(bm, 32, 64)) * scale;
+        if constexpr (NP == 1) bm -= kv_rows_low<E>();
         const float mn = fmaxf(m, bm), ref = mn == -INFINITY ? 0.0f : mn, f = kv_exp2(m - ref);
         float ps = 0.0f;
         x8 p[PP];

@@ -172,7 +172,8 @@ __device__ __forceinline__ void kv_tiles_item(const KvAttnArgs& a, const KvItem&
         if constexpr (NP == 1) {
             // The sums' reference follows the maximum only when that has risen by 2^6: weights up to
             // 64 have the same relative rounding, and the sums are seldom rescaled.
-            if (__any(bm > m + 6.0f)) {
+            bm -= kv_tiles_low<E>();
+            if (__any(bm > m + KV_LAG)) {
                 const float mn = fmaxf(m, bm);
                 f = kv_exp2(m - (mn == -INFINITY ? 0.0f : mn));
                 m = mn;

@@ -460,7 +460,7 @@ int th_rope_rows(th_device* dev, const th_buffer* in, const th_buffer* cos_buf, 
  * layer; a sequence is a list of pages that grows with it, lowest vacant page first.  Forks share
  * pages, and a page that is shared is copied when one of its sequences writes
  * to it.  Bookkeeping is the host's: calls that change sequences cost no
- * synchronisation, and are made between replays of captured graphs, not recorded.
+ * synchronisation, and are made between replays of captured graphs, not recorded.  One that finds no memory changes nothing.
  * All calls on a cache are its device handle's: one host thread, one stream. */
 typedef struct th_kv_cache th_kv_cache;
 typedef struct th_kv_batch th_kv_batch;
@@ -505,7 +505,8 @@ int th_kv_batch_create(th_kv_cache* c, size_t max_seqs, size_t max_rows, size_t 
 int th_kv_batch_destroy(th_kv_batch* b);
 /* Begins a step: sequence seqs[i] (none twice) grows by n_new[i] >= 0 positions.
  * Rows of the step's buffers are the new positions, sequence by sequence in this
- * order.  Refused as a whole if pages or lengths do not suffice (TH_ERR_OOM, TH_ERR_INVALID). */
+ * order.  Refused as a whole if pages, memory or lengths do not suffice (TH_ERR_OOM, TH_ERR_OOM, TH_ERR_INVALID):
+ * sequences and the batch are then as they were. */
 int th_kv_batch_begin(th_kv_batch* b, const int32_t* seqs, const uint32_t* n_new, size_t n);
 /* Ends it: sequence i keeps its first n_keep[i] new positions (rejected drafts go). */
 int th_kv_batch_trim(th_kv_batch* b, const uint32_t* n_keep, size_t n);

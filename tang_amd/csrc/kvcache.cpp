@@ -63,22 +63,20 @@ static th_kv_cache::Seq& the_seq(th_kv_cache* c, int32_t s, const char* what) {
 // ---------------------------------------------------------------------------
 
 static void stage_alloc(th_kv_stage& st, size_t bytes) {
-    if (st.host) TH_HIP(hipHostFree(st.host));
-    st.host = nullptr;
-    st.bytes = 0;
-    const hipError_t e = hipHostMalloc(&st.host, bytes, hipHostMallocDefault);
-    if (e != hipSuccess) {
-        st.host = nullptr;
+    void* host = nullptr;
+    if (hipHostMalloc(&host, bytes, hipHostMallocDefault) != hipSuccess) {
         (void)hipGetLastError();
         throw Error(TH_ERR_OOM, "no pinned memory for uploads");
     }
+    if (st.host) (void)hipHostFree(st.host);
+    st.host = host;
     st.bytes = bytes;
 }
 
-// Room for an upload: behind the last one, or in the next stage when this one is full.  A stage's event is recorded
+// Room for a call's uploads: behind the last one's, or in the next stage when this one is full.  A stage's event is recorded
 // once, when it is left (an event for each upload cost 1.5 us of a step's host time).
-static uint32_t* stage(th_kv_cache* c, size_t bytes) {
-    bytes = round_up(bytes, 16);
+static char* stage(th_kv_cache* c, size_t bytes) {
+    if (bytes == 0) return nullptr;
     th_kv_stage* st = &c->stages[c->stage_at];
     if (st->at + bytes > st->bytes) {
         if (st->at) {
@@ -93,7 +91,7 @@ static uint32_t* stage(th_kv_cache* c, size_t bytes) {
         st->at = 0;
         if (st->bytes < bytes) stage_alloc(*st, bytes + bytes / 2);
     }
-    uint32_t* to = (uint32_t*)((char*)st->host + st->at);
+    char* to = (char*)st->host + st->at;
     st->at += bytes;
     return to;
 }
@@ -113,23 +111,38 @@ static size_t copied_row(const th_kv_cache* c, const th_kv_cache::Seq& q) {
     return o.row_n > 0 || (o.dirty_to > 0 && o.dirty_from < n) ? 0 : n;
 }
 
-// The table entries that changed, and `words` to the runs' places in dst, in stream order; and copies of pages
-// ({from, to}, at most KV_ARG_COPIES) in the same launch.
-static void upload(th_kv_cache* c, const uint32_t* words, const KvRuns& runs, void* dst, const std::vector<uint32_t>* copies = nullptr) {
-    const size_t n_words = (size_t)runs.words(), n_copies = copies ? copies->size() / 2 : 0;
-    size_t pairs = 0, rows = 0;
+// What an upload of the table holds: copies of rows, and entries.
+struct TableSize {
+    size_t rows = 0, pairs = 0;
+    size_t words() const { return 3 * rows + 2 * pairs; }
+};
+static TableSize table_size(const th_kv_cache* c) {
+    TableSize t;
     for (const int32_t s : c->dirty) {
         const th_kv_cache::Seq& q = c->seqs[s];
         const size_t n = copied_row(c, q);
-        rows += n > 0;
-        pairs += changed(q).second + (n ? 0 : std::min(q.row_n, q.n_pages));
+        t.rows += n > 0;
+        t.pairs += changed(q).second + (n ? 0 : std::min(q.row_n, q.n_pages));
     }
-    const size_t total = 3 * rows + 2 * pairs + n_words;
+    return t;
+}
+
+// Staging memory of an upload of so many words next to copies of pages: none where all fit a launch's arguments.
+static size_t staged(size_t words, size_t n_copies = 0) { return 2 * n_copies + words > KV_ARG_WORDS ? round_up(words * 4, 16) : 0; }
+
+// The table entries that changed, and `words` to the runs' places in dst, in stream order; and copies of pages
+// ({from, to}, at most KV_ARG_COPIES) in the same launch.  room: staged() bytes, taken before (stage), and moved behind them.
+static void upload(th_kv_cache* c, const uint32_t* words, const KvRuns& runs, void* dst, char*& room,
+                   const std::vector<uint32_t>* copies = nullptr) {
+    const size_t n_words = (size_t)runs.words(), n_copies = copies ? copies->size() / 2 : 0;
+    const TableSize table = table_size(c);
+    const size_t rows = table.rows, pairs = table.pairs, total = table.words() + n_words;
     if (total + n_copies == 0) return;
     KvWords w;
     if (n_copies) std::copy(copies->begin(), copies->end(), w.w);
-    const bool far = 2 * n_copies + total > KV_ARG_WORDS;
-    uint32_t *const from = far ? stage(c, total * 4) : w.w + 2 * n_copies, *row = from, *to = from + 3 * rows;
+    const size_t far = staged(total, n_copies);
+    uint32_t *const from = far ? (uint32_t*)room : w.w + 2 * n_copies, *row = from, *to = from + 3 * rows;
+    room += far;
     auto entries = [&](size_t at, size_t n) {
         for (size_t i = at; i < at + n; i++) {
             *to++ = (uint32_t)i;
@@ -170,17 +183,29 @@ static KvRuns one_run(size_t n) {
     return r;
 }
 
-// Copies of pages ({from, to}), then the table and `words` as in upload.
-static void copy_upload(th_kv_cache* c, const std::vector<uint32_t>& pairs, const uint32_t* words, const KvRuns& runs, void* dst) {
+// What a call sends: copies of pages ({from, to}), then the table and `words` as in upload.  The memory for it is taken first (here, as the
+// tables stand), so that a call that finds none has sent nothing and can put back what it changed.
+struct Sending {
+    char* room = nullptr;
+    uint32_t* pairs = nullptr;  // device: copies beyond those that a launch's arguments hold
+};
+// more: staging bytes of uploads behind these
+static Sending prepare(th_kv_cache* c, const std::vector<uint32_t>& pairs, size_t n_words, size_t more = 0) {
+    const size_t n = pairs.size() / 2, table = table_size(c).words();
+    Sending to;
+    if (n > KV_ARG_COPIES) to.pairs = (uint32_t*)device_scratch(c->dev, 8 * n);
+    to.room = stage(c, (n > KV_ARG_COPIES ? staged(table + 2 * n) + staged(n_words) : staged(table + n_words, n)) + more);
+    return to;
+}
+static void send(th_kv_cache* c, Sending& to, const std::vector<uint32_t>& pairs, const uint32_t* words, const KvRuns& runs, void* dst) {
     const size_t n = pairs.size() / 2;
     if (n <= KV_ARG_COPIES) {
-        upload(c, words, runs, dst, &pairs);
+        upload(c, words, runs, dst, to.room, &pairs);
         return;
     }
-    uint32_t* dev = (uint32_t*)device_scratch(c->dev, 8 * n);
-    upload(c, pairs.data(), one_run(2 * n), dev);
-    launch_kv_copy_pages(c->pool, c->page_bytes, c->n_pages, (int)(2 * c->n_layers), dev, n, c->dev->stream);
-    upload(c, words, runs, dst);
+    upload(c, pairs.data(), one_run(2 * n), to.pairs, to.room);
+    launch_kv_copy_pages(c->pool, c->page_bytes, c->n_pages, (int)(2 * c->n_layers), to.pairs, n, c->dev->stream);
+    upload(c, words, runs, dst, to.room);
 }
 
 // ---------------------------------------------------------------------------
@@ -233,7 +258,7 @@ static bool must_copy(const th_kv_cache* c, int32_t s, size_t len) {
     return c->refs[c->mirror[(size_t)s * c->pages_per_seq + q.n_pages - 1]] > 1;
 }
 
-// Grows a sequence; the pages are there (counted before).
+// Grows a sequence; the pages are there (counted before), and room in `copies`: nothing here fails.
 static void grow(th_kv_cache* c, int32_t s, size_t len, std::vector<uint32_t>& copies) {
     th_kv_cache::Seq& q = c->seqs[s];
     int* t = seq_table(c, s);
@@ -249,6 +274,29 @@ static void grow(th_kv_cache* c, int32_t s, size_t len, std::vector<uint32_t>& c
     while (q.n_pages < need) t[q.n_pages++] = take_page(c);
     touch(c, s, had, q.n_pages - had);
     q.len = len;
+}
+
+// A sequence as it was before it grew, and back to that, where the rest of the call found no memory.
+struct SeqWas {
+    size_t len, n_pages;
+    uint64_t version;
+    int last;  // page (-1: none)
+};
+static SeqWas seq_was(th_kv_cache* c, int32_t s) {
+    const th_kv_cache::Seq& q = c->seqs[s];
+    return {q.len, q.n_pages, q.version, q.n_pages ? seq_table(c, s)[q.n_pages - 1] : -1};
+}
+static void ungrow(th_kv_cache* c, int32_t s, const SeqWas& was) {
+    th_kv_cache::Seq& q = c->seqs[s];
+    int* t = seq_table(c, s);
+    while (q.n_pages > was.n_pages) drop_page(c, t[--q.n_pages]);
+    if (was.n_pages && t[was.n_pages - 1] != was.last) {
+        drop_page(c, t[was.n_pages - 1]);
+        t[was.n_pages - 1] = was.last;
+        c->refs[was.last]++;
+    }
+    q.len = was.len;
+    q.version = was.version;
 }
 
 static void shrink(th_kv_cache* c, int32_t s, size_t len) {
@@ -317,15 +365,15 @@ class PlanMaker {
     void order(bool shared_prefixes) {
         toks_.clear();
         tiles_.clear();
-        const size_t B = b_->seqs.size(), ps = c_->page_size;
+        const size_t B = b_->step.seqs.size(), ps = c_->page_size;
         std::vector<size_t> row(B + 1, 0);
-        for (size_t i = 0; i < B; i++) row[i + 1] = row[i] + b_->n[i];
+        for (size_t i = 0; i < B; i++) row[i + 1] = row[i] + b_->step.n[i];
         std::vector<std::vector<size_t>> groups;
         std::unordered_map<int, size_t> by_page;
         for (size_t i = 0; i < B; i++) {
-            if (b_->n[i] == 0) continue;
-            const bool can = shared_prefixes && b_->start[i] >= KV_MIN_PREFIX;
-            const int first = can ? table(b_->seqs[i])[0] : -1;
+            if (b_->step.n[i] == 0) continue;
+            const bool can = shared_prefixes && b_->step.start[i] >= KV_MIN_PREFIX;
+            const int first = can ? table(b_->step.seqs[i])[0] : -1;
             if (can && c_->refs[first] > 1) {
                 auto [at, fresh] = by_page.try_emplace(first, groups.size());
                 if (!fresh) {
@@ -338,24 +386,24 @@ class PlanMaker {
         for (const auto& g : groups) {
             size_t common = 0;
             if (g.size() > 1) {
-                common = b_->start[g[0]] / ps;
-                const int* t0 = table(b_->seqs[g[0]]);
+                common = b_->step.start[g[0]] / ps;
+                const int* t0 = table(b_->step.seqs[g[0]]);
                 for (size_t k = 1; k < g.size() && common; k++) {
-                    const int* t = table(b_->seqs[g[k]]);
-                    const size_t most = std::min(common, b_->start[g[k]] / ps);
+                    const int* t = table(b_->step.seqs[g[k]]);
+                    const size_t most = std::min(common, b_->step.start[g[k]] / ps);
                     common = (size_t)(std::mismatch(t, t + most, t0).first - t);
                 }
                 if (common * ps < KV_MIN_PREFIX) common = 0;
             }
             const size_t tok0 = toks_.size();
             for (size_t i : g)
-                for (size_t j = 0; j < b_->n[i]; j++)
-                    toks_.push_back(KvTok{(int)(row[i] + j), (int)(b_->start[i] + j), 0, 0});
-            if (common) tile(tok0, toks_.size() - tok0, b_->seqs[g[0]], 0, common * ps, false);
+                for (size_t j = 0; j < b_->step.n[i]; j++)
+                    toks_.push_back(KvTok{(int)(row[i] + j), (int)(b_->step.start[i] + j), 0, 0});
+            if (common) tile(tok0, toks_.size() - tok0, b_->step.seqs[g[0]], 0, common * ps, false);
             size_t at = tok0;
             for (size_t i : g) {
-                tile(at, b_->n[i], b_->seqs[i], common * ps, b_->start[i] + b_->n[i], true);
-                at += b_->n[i];
+                tile(at, b_->step.n[i], b_->step.seqs[i], common * ps, b_->step.start[i] + b_->step.n[i], true);
+                at += b_->step.n[i];
             }
         }
         keys_[0] = keys_[1] = 0;
@@ -520,10 +568,7 @@ static size_t plan_joins(const th_kv_batch* b) { return plan_tiles(b) + b->max_i
 // (the join kernels read an entry before they know whether it is there: up to 32 rows behind the last)
 static size_t plan_words(const th_kv_batch* b) { return plan_joins(b) + (b->max_rows + 32) * sizeof(KvTok) / 4; }
 
-static void build_plan(th_kv_batch* b, const th_kv_batch::Key& key, th_kv_batch::Plan& p) {
-    p.built = false;
-    PlanMaker m(b, key.first, key.second);
-    m.make();
+static KvRuns plan_runs(const th_kv_batch* b, const PlanMaker& m) {
     KvRuns runs;
     runs.n[0] = KV_HEAD_WORDS;
     runs.n[1] = (int)(m.n_toks * sizeof(KvTok) / 4);
@@ -535,13 +580,25 @@ static void build_plan(th_kv_batch* b, const th_kv_batch::Key& key, th_kv_batch:
     runs.n[4] = (int)(m.n_joins * sizeof(KvTok) / 4);
     runs.at[4] = (int)plan_joins(b);
     TH_REQUIRE(m.n_items[0] <= b->max_items && m.n_items[1] <= b->max_items, "attention plan exceeds its block");
-    upload(b->cache, m.words.data(), runs, p.block);
+    return runs;
+}
+
+static void send_plan(th_kv_batch* b, const PlanMaker& m, const KvRuns& runs, th_kv_batch::Plan& p, char*& room) {
+    upload(b->cache, m.words.data(), runs, p.block, room);
     p.n_tile_items = m.n_items[0];
     p.n_rows_items = m.n_items[1];
     p.n_joins = m.n_joins;
     p.n_recs = m.n_recs;
     p.far = m.far;
     p.built = true;
+}
+
+static void build_plan(th_kv_batch* b, const th_kv_batch::Key& key, th_kv_batch::Plan& p) {
+    PlanMaker m(b, key.first, key.second);
+    m.make();
+    const KvRuns runs = plan_runs(b, m);
+    char* room = stage(b->cache, staged(table_size(b->cache).words() + m.words.size()));
+    send_plan(b, m, runs, p, room);
 }
 
 // Room for another plan: of its own, or, where there are many, that of one that no graph reads (uploads
@@ -572,9 +629,9 @@ static void require_begun(const th_kv_batch* b, size_t layer, const char* what) 
     const th_kv_cache* c = b->cache;
     if (!b->begun) throw Error(TH_ERR_INVALID, std::string(what) + ": the batch has not begun");
     if (layer >= c->n_layers) throw Error(TH_ERR_INVALID, std::string(what) + ": no layer " + std::to_string(layer));
-    for (size_t i = 0; i < b->seqs.size(); i++)
-        if (!c->seqs[b->seqs[i]].used || c->seqs[b->seqs[i]].version != b->versions[i])
-            throw Error(TH_ERR_INVALID, std::string(what) + ": sequence " + std::to_string(b->seqs[i]) +
+    for (size_t i = 0; i < b->step.seqs.size(); i++)
+        if (!c->seqs[b->step.seqs[i]].used || c->seqs[b->step.seqs[i]].version != b->step.versions[i])
+            throw Error(TH_ERR_INVALID, std::string(what) + ": sequence " + std::to_string(b->step.seqs[i]) +
                                             " has changed since the batch began");
 }
 
@@ -652,6 +709,7 @@ int th_kv_cache_create(th_device* dev, const th_kv_cache_config* cfg, th_kv_cach
     c->page_bytes = c->n_kv_heads * c->page_size * c->hd * 2;
     c->mirror.assign(c->max_seqs * c->pages_per_seq, 0);
     c->seqs.resize(c->max_seqs);
+    c->dirty.reserve(c->max_seqs);
     c->refs.assign(c->n_pages, 0);
     c->vacant.assign(ceil_div(c->n_pages, 64), ~0ull);
     if (c->n_pages % 64) c->vacant.back() = (1ull << (c->n_pages % 64)) - 1;
@@ -719,32 +777,45 @@ int th_kv_cache_compact(th_kv_cache* c, size_t* n_moved) {
         if (c->refs[p] == 0) continue;
         while (c->refs[hole] > 0) hole++;
         pairs.push_back((uint32_t)p);
-        pairs.push_back((uint32_t)hole);
-        moved[p] = (int)hole++;
+        pairs.push_back((uint32_t)hole++);
     }
     if (!pairs.empty()) {
-        if (pairs.size() / 2 > KV_ARG_COPIES) device_scratch(c->dev, 4 * pairs.size());  // there before anything changes
-        for (size_t i = 0; i < pairs.size(); i += 2) {
-            const int from = (int)pairs[i], to = (int)pairs[i + 1];
-            c->refs[to] = c->refs[from];
-            c->refs[from] = 0;
-            c->vacant[from / 64] |= 1ull << (from % 64);
-            c->vacant[to / 64] &= ~(1ull << (to % 64));
-        }
-        c->hint = 0;
-        for (size_t s = 0; s < c->seqs.size(); s++) {
-            if (!c->seqs[s].used) continue;
-            int* t = seq_table(c, (int32_t)s);
-            bool any = false;
-            for (size_t i = 0; i < c->seqs[s].n_pages; i++) {
-                if (moved[t[i]] < 0) continue;
-                t[i] = moved[t[i]];
-                touch(c, (int32_t)s, i, 1);
-                any = true;
+        std::vector<uint64_t> versions(c->seqs.size());
+        for (size_t s = 0; s < c->seqs.size(); s++) versions[s] = c->seqs[s].version;
+        // moves pages in the books: those of `pairs` from their item `from` to the other
+        auto move = [&](int from) {
+            for (size_t i = 0; i < pairs.size(); i += 2) {
+                const int a = (int)pairs[i + from], z = (int)pairs[i + 1 - from];
+                c->refs[z] = c->refs[a];
+                c->refs[a] = 0;
+                c->vacant[a / 64] |= 1ull << (a % 64);
+                c->vacant[z / 64] &= ~(1ull << (z % 64));
+                moved[a] = z;
             }
-            if (any) c->seqs[s].version = ++c->versions;
+            c->hint = 0;
+            for (size_t s = 0; s < c->seqs.size(); s++) {
+                if (!c->seqs[s].used) continue;
+                int* t = seq_table(c, (int32_t)s);
+                bool any = false;
+                for (size_t i = 0; i < c->seqs[s].n_pages; i++) {
+                    if (moved[t[i]] < 0) continue;
+                    t[i] = moved[t[i]];
+                    touch(c, (int32_t)s, i, 1);
+                    any = true;
+                }
+                if (any) c->seqs[s].version = from ? versions[s] : ++c->versions;
+            }
+            for (size_t i = 0; i < pairs.size(); i += 2) moved[pairs[i + from]] = -1;
+        };
+        move(0);
+        Sending to;
+        try {
+            to = prepare(c, pairs, 0);
+        } catch (...) {
+            move(1);
+            throw;
         }
-        copy_upload(c, pairs, nullptr, KvRuns(), nullptr);
+        send(c, to, pairs, nullptr, KvRuns(), nullptr);
     }
     if (n_moved) *n_moved = pairs.size() / 2;
     TH_API_END
@@ -808,9 +879,20 @@ int th_kv_seq_resize(th_kv_cache* c, int32_t seq, size_t len) {
     const size_t need = ceil_div(len, c->page_size) - q.n_pages + (must_copy(c, seq, len) ? 1 : 0);
     if (need > c->n_vacant) no_pages(__func__, need, c->n_vacant);
     std::vector<uint32_t> copies;
+    copies.reserve(2);
+    const SeqWas was = seq_was(c, seq);
     grow(c, seq, len, copies);
     c->seqs[seq].version = ++c->versions;
-    if (!copies.empty()) copy_upload(c, copies, nullptr, KvRuns(), nullptr);
+    if (!copies.empty()) {
+        Sending to;
+        try {
+            to = prepare(c, copies, 0);
+        } catch (...) {
+            ungrow(c, seq, was);
+            throw;
+        }
+        send(c, to, copies, nullptr, KvRuns(), nullptr);
+    }
     TH_API_END
 }
 
@@ -857,16 +939,33 @@ int th_kv_seq_select(th_kv_cache* c, int32_t seq, const uint32_t* positions, siz
     for (size_t i = 0; i < n; i++)
         w[i] = (uint32_t)(((size_t)t[positions[i] >> c->shift] << c->shift) + (positions[i] & (c->page_size - 1)));
     // the rows go to pages of their own: the old ones may be shared, and order is free
-    std::vector<int> fresh(pages);
-    for (size_t p = 0; p < pages; p++) w[n + p] = (uint32_t)(fresh[p] = take_page(c));
-    shrink(c, seq, 0);
-    std::copy(fresh.begin(), fresh.end(), t);
-    c->seqs[seq].len = n;
-    c->seqs[seq].n_pages = pages;
-    touch(c, seq, 0, pages);
+    th_kv_cache::Seq& q = c->seqs[seq];
+    const SeqWas was = seq_was(c, seq);
+    const std::vector<int> old(t, t + q.n_pages);
+    auto put = [&](size_t len, size_t n_pages, uint64_t version) {
+        q.len = len;
+        q.n_pages = n_pages;
+        q.version = version;
+        touch(c, seq, 0, n_pages);
+    };
+    for (size_t p = 0; p < pages; p++) w[n + p] = (uint32_t)(t[p] = take_page(c));
+    put(n, pages, ++c->versions);
+    uint32_t* dev = nullptr;
+    char* room = nullptr;
+    try {
+        if (n) {
+            dev = (uint32_t*)device_scratch(c->dev, w.size() * 4);
+            room = stage(c, staged(table_size(c).words() + w.size()));
+        }
+    } catch (...) {
+        for (size_t p = 0; p < pages; p++) drop_page(c, t[p]);
+        std::copy(old.begin(), old.end(), t);
+        put(was.len, was.n_pages, was.version);
+        throw;
+    }
+    for (const int p : old) drop_page(c, p);
     if (n) {
-        uint32_t* dev = (uint32_t*)device_scratch(c->dev, w.size() * 4);
-        upload(c, w.data(), one_run(w.size()), dev);
+        upload(c, w.data(), one_run(w.size()), dev, room);
         launch_kv_gather_rows(c->pool, c->n_pages, (int)(2 * c->n_layers), (int)c->n_kv_heads, c->shift, c->hd * 2, dev, dev + n, n,
                               c->dev->stream);
     }
@@ -887,7 +986,8 @@ int th_kv_seq_read(th_kv_cache* c, int32_t seq, size_t layer, size_t from, size_
     DeviceScope scope(c->dev);
     if (!c->dirty.empty()) {
         require_eager(c, __func__);
-        upload(c, nullptr, KvRuns(), nullptr);
+        char* room = stage(c, staged(table_size(c).words()));
+        upload(c, nullptr, KvRuns(), nullptr, room);
     }
     launch_kv_read(layer_pages(c, layer), seq, from, n, c->hd * 2, k->ptr, v->ptr, c->dev->stream);
     TH_API_END
@@ -969,36 +1069,57 @@ int th_kv_batch_begin(th_kv_batch* b, const int32_t* seqs, const uint32_t* n_new
     TH_REQUIRE(rows <= b->max_rows, "more new positions than max_rows");
     if (need > c->n_vacant) no_pages(__func__, need, c->n_vacant);
     DeviceScope scope(c->dev);
-    b->begun = false;
     std::vector<uint32_t> copies, words(4 + rows * sizeof(KvRow) / 4);
-    b->seqs.assign(seqs, seqs + n);
-    b->n.assign(n_new, n_new + n);
-    b->start.resize(n);
-    b->versions.resize(n);
+    copies.reserve(2 * n);
     words[0] = (uint32_t)rows;
+    th_kv_batch::Step step;
+    step.seqs.assign(seqs, seqs + n);
+    step.n.assign(n_new, n_new + n);
+    step.start.resize(n);
+    step.versions.resize(n);
+    step.rows = rows;
+    std::vector<SeqWas> was(n);
     size_t at = 4;
-    b->top = 0;
     for (size_t i = 0; i < n; i++) {
         th_kv_cache::Seq& q = c->seqs[seqs[i]];
-        b->start[i] = q.len;
+        was[i] = seq_was(c, seqs[i]);
+        step.start[i] = q.len;
         if (n_new[i]) {
             grow(c, seqs[i], q.len + n_new[i], copies);
             q.version = ++c->versions;
-            b->top = std::max(b->top, q.len);
+            step.top = std::max(step.top, q.len);
         }
-        b->versions[i] = q.version;
+        step.versions[i] = q.version;
         for (size_t j = 0; j < n_new[i]; j++) {
             words[at++] = (uint32_t)seqs[i];
-            words[at++] = (uint32_t)(b->start[i] + j);
+            words[at++] = (uint32_t)(step.start[i] + j);
         }
     }
-    b->rows = rows;
-    copy_upload(c, copies, words.data(), one_run(words.size()), b->block);
+    std::swap(b->step, step);
     // graphs read their plans at replay; the others are built by the step's first call that needs them
-    for (auto& p : b->plans) {
-        p.second.built = false;
-        if (p.second.captured) build_plan(b, p.first, p.second);
+    struct Made { th_kv_batch::Plan* plan; PlanMaker maker; KvRuns runs; };
+    std::vector<Made> made;
+    Sending to;
+    try {
+        size_t more = 0;
+        for (auto& p : b->plans) {
+            if (!p.second.captured) continue;
+            made.push_back({&p.second, PlanMaker(b, p.first.first, p.first.second), {}});
+            Made& m = made.back();
+            m.maker.make();
+            m.runs = plan_runs(b, m.maker);
+            more += staged(m.maker.words.size());
+        }
+        to = prepare(c, copies, words.size(), more);
+    } catch (...) {
+        std::swap(b->step, step);
+        for (size_t i = n; i-- > 0;) ungrow(c, seqs[i], was[i]);
+        throw;
     }
+    b->begun = false;
+    for (auto& p : b->plans) p.second.built = false;
+    send(c, to, copies, words.data(), one_run(words.size()), b->block);
+    for (Made& m : made) send_plan(b, m.maker, m.runs, *m.plan, to.room);
     b->begun = true;
     TH_API_END
 }
@@ -1007,10 +1128,10 @@ int th_kv_batch_trim(th_kv_batch* b, const uint32_t* n_keep, size_t n) {
     TH_API_BEGIN
     require_begun(b, 0, __func__);
     TH_REQUIRE(n_keep || n == 0, "null argument");
-    TH_REQUIRE(n == b->seqs.size(), "one count for each sequence of the batch");
-    for (size_t i = 0; i < n; i++) TH_REQUIRE(n_keep[i] <= b->n[i], "more kept than were new");
+    TH_REQUIRE(n == b->step.seqs.size(), "one count for each sequence of the batch");
+    for (size_t i = 0; i < n; i++) TH_REQUIRE(n_keep[i] <= b->step.n[i], "more kept than were new");
     for (size_t i = 0; i < n; i++)
-        if (n_keep[i] < b->n[i]) shrink(b->cache, b->seqs[i], b->start[i] + n_keep[i]);
+        if (n_keep[i] < b->step.n[i]) shrink(b->cache, b->step.seqs[i], b->step.start[i] + n_keep[i]);
     b->begun = false;
     TH_API_END
 }
@@ -1024,7 +1145,7 @@ int th_kv_append(th_kv_batch* b, size_t layer, const th_buffer* q, const th_buff
     TH_REQUIRE((q == nullptr) == (q_out == nullptr), "q and q_out go together");
     DeviceScope scope(c->dev);
     // a captured call runs on whatever the batch begins with later
-    const size_t rows = c->dev->capturing ? b->max_rows : b->rows;
+    const size_t rows = c->dev->capturing ? b->max_rows : b->step.rows;
     const size_t kv = rows * c->n_kv_heads * c->hd, qn = rows * b->n_heads * c->hd;
     require_x(c, k, kv, "k");
     require_x(c, v, kv, "v");
@@ -1035,7 +1156,7 @@ int th_kv_append(th_kv_batch* b, size_t layer, const th_buffer* q, const th_buff
         require_x(c, q_out, qn, "q_out");
         TH_REQUIRE(q_out != k && q_out != v, "q_out must not be k or v");
     }
-    rope_args(a, c->dev, cos_t, sin_t, positions, rows, c->hd, rot_dim, layout, b->top);
+    rope_args(a, c->dev, cos_t, sin_t, positions, rows, c->hd, rot_dim, layout, b->step.top);
     a.q = q ? q->ptr : nullptr;
     a.k = k->ptr;
     a.v = v->ptr;
@@ -1057,7 +1178,7 @@ int th_kv_batch_attention(th_kv_batch* b, size_t layer, const th_buffer* q, size
     TH_REQUIRE(std::isfinite(scale) && scale >= 0.0f, "scale must be finite and not negative");
     DeviceScope scope(c->dev);
     const bool capturing = c->dev->capturing;
-    const size_t n = (capturing ? b->max_rows : b->rows) * b->n_heads * c->hd;
+    const size_t n = (capturing ? b->max_rows : b->step.rows) * b->n_heads * c->hd;
     require_x(c, q, n, "q");
     require_x(c, out, n, "out");
     // a window as long as any sequence hides nothing, and without one there are no sinks

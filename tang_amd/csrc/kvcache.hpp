@@ -175,7 +175,7 @@ struct th_kv_cache {
     std::vector<int> refs;         // sequences that have the page
     std::vector<uint64_t> vacant;  // a bit for each page without any
     size_t n_vacant = 0, hint = 0;
-    std::vector<int32_t> dirty;    // sequences with table entries to upload
+    std::vector<int32_t> dirty;    // sequences with table entries to upload (room for all is there)
     uint64_t versions = 0;
     th_kv_stage stages[th::KV_STAGES];
     unsigned stage_at = 0;
@@ -186,10 +186,12 @@ struct th_kv_cache {
 struct th_kv_batch {
     th_kv_cache* cache = nullptr;
     size_t max_seqs = 0, max_rows = 0, n_heads = 0;
-    std::vector<int> seqs;
-    std::vector<size_t> start, n;
-    std::vector<uint64_t> versions;
-    size_t rows = 0, top = 0;  // new rows, and one past the highest position
+    struct Step {
+        std::vector<int> seqs;
+        std::vector<size_t> start, n;
+        std::vector<uint64_t> versions;
+        size_t rows = 0, top = 0;  // new rows, and one past the highest position
+    } step;
     bool begun = false;
     int* block = nullptr;      // device: the number of rows (16 bytes), then KvRow[max_rows]
     struct Plan {

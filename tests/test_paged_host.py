@@ -1,0 +1,104 @@
+"""The paged cache's bookkeeping without a GPU: calls that find no memory leave everything as it was."""
+import os
+
+import numpy as np
+import pytest
+
+from host_cache import CLANG, Cache, Refused, build
+from tang_amd import capi
+
+pytestmark = pytest.mark.skipif(not os.path.exists(CLANG), reason="needs ROCm's clang++")
+
+
+@pytest.fixture(scope="module")
+def lib(tmp_path_factory):
+    return build(tmp_path_factory.mktemp("host"))
+
+
+class _Setup:
+    """A long sequence, 150 forks of it that end inside a shared page, one that has been written behind, a batch that has begun (and whose
+    attention a graph has), vacant pages before live ones."""
+
+    def __init__(self, L):
+        rng = self.rng = np.random.default_rng(1)
+        c = self.c = Cache(L, layers=2, pages=24000, seqs=170, max_len=160000)
+        self.b = c.batch(160, 12000)
+        gap, self.a = c.created(2)
+        c.resize(gap, 160000)
+        c.grow(rng, self.b, [self.a], [10005])
+        c.grow(rng, self.b, [self.a], [11000])
+        self.kids = c.fork(self.a, 150, 21003)
+        self.other, self.begun = c.created(2)
+        c.grow(rng, self.b, [self.other], [30])
+        c.free([gap])
+        self.b2 = c.batch(160, 12000)
+        c.begin(self.b2, [self.begun], [20])
+        c.attend(self.b2, 20)
+        # another batch, with a plan that a graph reads
+        self.c.begin(self.b, [], [])
+        c.attend(self.b, 0)
+        q = c.buffer(12000 * 8), c.buffer(12000 * 8)
+        c.call("th_capture_begin", c.dev)
+        c.call("th_kv_batch_attention", self.b, 0, q[0], 0, 0, 0.0, q[1])
+        c.new("th_capture_end", c.dev)
+        c.fill(rng, self.b2, [self.begun], [20])
+
+
+def _begin_forks(S):
+    news = [1] * len(S.kids) + [9000]
+    S.c.begin(S.b, S.kids + [S.other], news)
+    return lambda: S.c.fill(S.rng, S.b, S.kids + [S.other], news)
+
+
+def _begin_few(S):
+    S.c.begin(S.b, [S.kids[3], S.a, S.other], [40, 11000, 0])
+    return lambda: S.c.fill(S.rng, S.b, [S.kids[3], S.a, S.other], [40, 11000, 0])
+
+
+def _resize(S):
+    S.c.resize(S.kids[5], 160000)
+    S.c.resize(S.kids[5], 21003)
+    return lambda: None
+
+
+def _select(S):
+    keep = S.rng.permutation(21005)[:20500]
+    S.c.select(S.a, keep)
+    S.c.rows[S.a] = S.c.rows[S.a][:, :, keep]
+    return lambda: None
+
+
+def _compact(S):
+    assert S.c.compact() > 1000
+    return lambda: None
+
+
+@pytest.mark.parametrize("act,least", [(_begin_forks, 3), (_begin_few, 1), (_resize, 1), (_select, 2), (_compact, 2)])
+def test_calls_that_find_no_memory_change_nothing(lib, act, least):
+    """Every allocation of a call fails in turn: the call is refused, lengths, pages, rows, the books and begun batches are as they were, and
+    the same call works afterwards."""
+    for fail in range(50):
+        S = _Setup(lib)
+        c, before = S.c, S.c.info()
+        rows = dict(c.rows)
+        lib.host_fail(fail)
+        try:
+            act(S)
+            refused = False
+        except Refused as e:
+            assert e.code == capi.TH_ERR_OOM
+            refused = True
+        finally:
+            lib.host_fail(-1)
+        if not refused:
+            break
+        assert c.info() == before, fail
+        c.rows = rows
+        c.attend(S.b2, 20)  # still begun
+        c.check((act.__name__, fail, "refused"))
+        act(S)()
+        c.check((act.__name__, fail, "again"))
+        c.call("th_kv_batch_destroy", S.b)
+        c.call("th_kv_batch_destroy", S.b2)
+        c.close()
+    assert fail >= least, "too few allocations to have been looked at"

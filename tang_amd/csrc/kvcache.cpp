@@ -456,8 +456,8 @@ class PlanMaker {
         per[1] = round_up(std::max<size_t>(KV_MIN_ROWS_KEYS, ceil_div(keys_[1] * kvh, 8 * cus)), 64) * scale;
         per[0] = round_up(std::max<size_t>(KV_MIN_TILE_KEYS, ceil_div(keys_[0] * kvh, cus * 3 / 2)), 64) * scale;
         // Where there are records for it, no tile's piece is so long that it needs additions of its own (a quarter
-        // more than `per` is one piece).
-        if (scale == 1) per[0] = std::min(per[0], KV_LONG_ITEM * 4 / 5);
+        // more than `per` is one piece).  A multiple of 64 like any other: pieces begin at blocks, and the last of many shall have keys left.
+        if (scale == 1) per[0] = std::min(per[0], KV_LONG_ITEM * 4 / 5 / 64 * 64);
         std::vector<int> shared(toks_.size(), 0), own(toks_.size(), 0), pieces(tiles_.size());
         size_t extra = 0;
         for (size_t i = 0; i < tiles_.size(); i++) {

@@ -1,0 +1,101 @@
+"""Plans of attention over the paged cache, made without a GPU: what their items cover, and how the work is cut."""
+import os
+
+import numpy as np
+import pytest
+
+from host_cache import CLANG, Cache, build
+
+pytestmark = pytest.mark.skipif(not os.path.exists(CLANG), reason="needs ROCm's clang++")
+
+OWN = 1 << 30
+
+
+@pytest.fixture(scope="module")
+def lib(tmp_path_factory):
+    return build(tmp_path_factory.mktemp("host"))
+
+
+def _plan(c, b, seqs, news, heads, window=0, sinks=0):
+    """A step's plan, checked: every key that a token sees is in one of its items, every item has keys of its sequence, every record of
+    a token is written once. Returns (rows items, tile items)."""
+    c.attend(b, sum(news), heads, window, sinks)
+    toks, rows, tiles, joins = c.plan(sum(news))
+    G = heads // c.kh
+    starts = {s: c.length(s) - n for s, n in zip(seqs, news)}
+    at = [(s, starts[s] + j) for s, n in zip(seqs, news) for j in range(n)]
+    assert sorted(toks[:, 0]) == list(range(len(at)))
+    assert all(at[t[0]][1] == t[1] for t in toks)
+    seen, recs = [[] for _ in toks], [[] for _ in toks]
+    for items, most in ((rows, 16), (tiles, 128)):
+        for tok0, ntok, seq, j0, j1, sink_end, gap, rec in items.tolist():
+            assert ntok > 0 and ntok * G <= most
+            assert j0 < j1, "an item without keys"
+            last = j1 - 1 + (gap if j1 - 1 >= sink_end else 0)
+            assert last < c.length(seq) and j0 % 16 == 0
+            for t in range(tok0, tok0 + ntok):
+                for lo, hi, g in ((j0, min(j1, sink_end), 0), (max(j0, sink_end), j1, gap)):
+                    if lo < hi:
+                        seen[t].append((lo + g, hi + g))
+                if rec < 0:
+                    recs[t].append(None)
+                else:
+                    recs[t].append((rec & ~OWN) + (toks[t, 3] & 0xFFFF if rec & OWN else 0))
+    joined = {tuple(j) for j in joins.tolist()}
+    for t, (row, pos, first, own_n) in enumerate(toks.tolist()):
+        ranges = sorted(seen[t])
+        assert all(a[1] <= b[0] for a, b in zip(ranges, ranges[1:]))
+        cover = np.zeros(pos + 1, bool)
+        for a, z in ranges:
+            cover[a:z] = True
+        j = np.arange(pos + 1)
+        need = (j > pos - window) | (j < sinks) if window else j >= 0
+        assert (cover | ~need).all(), (row, pos)
+        if (row, pos, first, own_n) in joined:
+            assert sorted(recs[t]) == list(range(own_n >> 16))
+        else:
+            assert recs[t] == [None]
+    spans = sorted((j[2], j[2] + (j[3] >> 16)) for j in joined)
+    assert all(a[1] <= b[0] for a, b in zip(spans, spans[1:]))
+    return rows, tiles
+
+
+def test_pieces_of_a_very_long_sequence_have_keys(lib):
+    """5.2 million keys in pieces of 13107 that begin at multiples of 64: 400 of 13120 were all, and the 401st began behind the sequence's end,
+    where the kernel looks up a page before it sees that there is nothing to do."""
+    n = 400 * 13107 + 100
+    c = Cache(lib, pages=n // 16 + 2, seqs=1, max_len=n)
+    b = c.batch(1, 17)
+    s = c.create()
+    c.resize(s, n - 17)
+    c.begin(b, [s], [17])
+    _plan(c, b, [s], [17], 1)
+    c.call("th_kv_batch_destroy", b)
+    c.close()
+
+
+@pytest.mark.parametrize("seed", range(30))
+def test_plans_cover_what_rows_see(lib, seed):
+    rng = np.random.default_rng(seed)
+    kh, G = int(rng.choice([1, 2])), int(rng.choice([1, 2, 3, 7, 16, 40]))
+    page = int(rng.choice([16, 64, 256]))
+    c = Cache(lib, kh=kh, page=page, pages=40000 // page + 400, seqs=40, max_len=9000)
+    b = c.batch(40, 3000, kh * G)
+    first = c.created(int(rng.integers(1, 4)))
+    for s in first:
+        c.resize(s, int(rng.integers(1, 4000)))
+    seqs = list(first)
+    for s in first:
+        if rng.random() < 0.6:
+            seqs += c.fork(s, int(rng.integers(1, 9)), int(rng.integers(0, c.length(s) + 1)))
+    for s in seqs:
+        if rng.random() < 0.5:
+            c.resize(s, c.length(s) + int(rng.integers(0, 300)))
+    seqs = [seqs[i] for i in rng.permutation(len(seqs))]
+    news = [int(rng.choice([0, 1, 1, 2, 5, int(rng.integers(1, 120))])) for _ in seqs]
+    c.begin(b, seqs, news)
+    for window, sinks in [(0, 0), (1, 0), (300, 4), (50, 70), (1000, 0)]:
+        if sum(news):
+            _plan(c, b, seqs, news, kh * G, window, sinks)
+    c.call("th_kv_batch_destroy", b)
+    c.close()

@@ -347,10 +347,13 @@ class PlanMaker {
         : b_(b), c_(b->cache), G_(b->n_heads / b->cache->n_kv_heads), window_(window), sinks_(sinks) {}
 
     void make() {
-        order(true);
-        for (size_t scale = 1; !split(scale); scale *= 2) {
-            // nothing is split any more, and two records a token are still too many
-            if (scale > c_->max_len) order(false);
+        order();
+        // Pieces of one kind get longer, those that take more of what does not suffice.  Unsplit work fits: order() has seen to it.
+        for (size_t scale[2] = {1, 1};;) {
+            const int longer = split(scale);
+            if (longer < 0) return;
+            TH_REQUIRE(scale[longer] <= c_->max_len, "an unsplit plan exceeds its block");
+            scale[longer] *= 2;
         }
     }
 
@@ -361,24 +364,32 @@ class PlanMaker {
    private:
     const int* table(int s) const { return c_->mirror.data() + (size_t)s * c_->pages_per_seq; }
 
-    // Sequences whose first pages are the same, next to each other; the tokens in that order.
-    void order(bool shared_prefixes) {
-        toks_.clear();
-        tiles_.clear();
+    // Sequences whose first pages are the same, next to each other; the tokens in that order.  Tokens that share a prefix take two
+    // records at least; they get three quarters of all, so that long sequences can be split whatever else is in the batch, and
+    // sequences beyond that read the prefix by themselves.
+    void order() {
         const size_t B = b_->step.seqs.size(), ps = c_->page_size;
         std::vector<size_t> row(B + 1, 0);
         for (size_t i = 0; i < B; i++) row[i + 1] = row[i] + b_->step.n[i];
         std::vector<std::vector<size_t>> groups;
         std::unordered_map<int, size_t> by_page;
+        size_t left = b_->max_recs * 3 / 8;
         for (size_t i = 0; i < B; i++) {
-            if (b_->step.n[i] == 0) continue;
-            const bool can = shared_prefixes && b_->step.start[i] >= KV_MIN_PREFIX;
+            const size_t n = b_->step.n[i];
+            if (n == 0) continue;
+            const bool can = b_->step.start[i] >= KV_MIN_PREFIX;
             const int first = can ? table(b_->step.seqs[i])[0] : -1;
             if (can && c_->refs[first] > 1) {
                 auto [at, fresh] = by_page.try_emplace(first, groups.size());
                 if (!fresh) {
-                    groups[at->second].push_back(i);
-                    continue;
+                    std::vector<size_t>& g = groups[at->second];
+                    const size_t other = g.size() == 1 ? b_->step.n[g[0]] : 0;
+                    if (n + other <= left) {
+                        left -= n + other;
+                        g.push_back(i);
+                        continue;
+                    }
+                    if (n < other) at->second = groups.size();  // shorter ones may share with this one
                 }
             }
             groups.push_back({i});
@@ -445,7 +456,8 @@ class PlanMaker {
         }
     }
 
-    bool split(size_t scale) {
+    // Cuts the tiles into pieces.  -1: done; else the kind of items (0 tiles, 1 rows) whose pieces have to be longer.
+    int split(const size_t (&scale)[2]) {
         const size_t kvh = c_->n_kv_heads, cus = (size_t)c_->dev->num_cus;
         // Keys of a piece.  The chip holds 2 * CUs workgroups at a time.  Rows items are a quarter of an even share, so
         // that uneven lengths level out.  Tiles are longer, since each of their pieces leaves 128 rows of
@@ -453,18 +465,19 @@ class PlanMaker {
         // of 8192 99 us, 512 tokens beside 32 decode steps 146 us, 128 rows on a prefix of 16000 115 us; with 4 a CU 59 and
         // 112, with 2 54 and 109, with 1 59, 95, 138 and 126).
         size_t per[2];
-        per[1] = round_up(std::max<size_t>(KV_MIN_ROWS_KEYS, ceil_div(keys_[1] * kvh, 8 * cus)), 64) * scale;
-        per[0] = round_up(std::max<size_t>(KV_MIN_TILE_KEYS, ceil_div(keys_[0] * kvh, cus * 3 / 2)), 64) * scale;
+        per[1] = round_up(std::max<size_t>(KV_MIN_ROWS_KEYS, ceil_div(keys_[1] * kvh, 8 * cus)), 64) * scale[1];
+        per[0] = round_up(std::max<size_t>(KV_MIN_TILE_KEYS, ceil_div(keys_[0] * kvh, cus * 3 / 2)), 64) * scale[0];
         // Where there are records for it, no tile's piece is so long that it needs additions of its own (a quarter
         // more than `per` is one piece).  A multiple of 64 like any other: pieces begin at blocks, and the last of many shall have keys left.
-        if (scale == 1) per[0] = std::min(per[0], KV_LONG_ITEM * 4 / 5 / 64 * 64);
+        if (scale[0] == 1) per[0] = std::min(per[0], KV_LONG_ITEM * 4 / 5 / 64 * 64);
         std::vector<int> shared(toks_.size(), 0), own(toks_.size(), 0), pieces(tiles_.size());
-        size_t extra = 0;
+        size_t extra[2] = {0, 0}, more[2] = {0, 0};  // items and records that splitting takes
         for (size_t i = 0; i < tiles_.size(); i++) {
             const PlanTile& t = tiles_[i];
             const size_t keys = (size_t)(t.it.j1 - t.it.j0), p = per[t.small];
             pieces[i] = (int)(keys <= p + p / 4 ? 1 : ceil_div(keys, p));
-            extra += (size_t)pieces[i] - 1;
+            extra[t.small] += (size_t)pieces[i] - 1;
+            more[t.small] += ((size_t)pieces[i] - 1) * t.it.ntok;
             for (int k = 0; k < t.it.ntok; k++) (t.own ? own : shared)[t.it.tok0 + k] = pieces[i];
         }
         // The tokens of one tile have one count of records each kind, whatever tiles hold their other keys.
@@ -500,7 +513,8 @@ class PlanMaker {
                 again = true;
             }
         }
-        if (recs > b_->max_recs || tiles_.size() + extra > b_->max_items) return false;
+        if (recs > b_->max_recs) return more[1] > more[0];
+        if (tiles_.size() + extra[0] + extra[1] > b_->max_items) return extra[1] > extra[0];
         size_t rec = 0;
         std::vector<KvTok> joins;
         for (size_t i = 0; i < toks_.size(); i++) {
@@ -549,7 +563,7 @@ class PlanMaker {
         put(items[1].data(), n_items[1] * sizeof(KvItem));
         put(items[0].data(), n_items[0] * sizeof(KvItem));
         put(joins.data(), n_joins * sizeof(KvTok));
-        return true;
+        return -1;
     }
 
     const th_kv_batch* b_;

@@ -99,3 +99,43 @@ def test_plans_cover_what_rows_see(lib, seed):
             _plan(c, b, seqs, news, kh * G, window, sinks)
     c.call("th_kv_batch_destroy", b)
     c.close()
+
+
+def _longest(items):
+    return int((items[:, 4] - items[:, 3]).max(initial=0))
+
+
+@pytest.mark.parametrize("new,shared", [(400, 1), (600, 0)])
+def test_long_prompts_on_a_prefix_leave_decode_steps_split(lib, new, shared):
+    """Eight forks of 2000 positions with 400 or 600 new ones each, more than records are there for with the longer, next to a decode step at
+    100000: its keys are cut into pieces all the same. As many of the forks as fit share the prefix."""
+    c = Cache(lib, pages=8000, seqs=12, max_len=131072)
+    b = c.batch(12, 6000, 4)
+    a, far = c.created(2)
+    c.resize(a, 2000)
+    c.resize(far, 100000)
+    kids = c.fork(a, 8, 2000)
+    news = [new] * 8 + [1]
+    c.begin(b, kids + [far], news)
+    rows, tiles = _plan(c, b, kids + [far], news, 4)
+    assert _longest(rows) <= 2048
+    prefix = tiles[tiles[:, 4] <= 2000]
+    assert len(prefix) and (shared or prefix[:, 1].sum() < 2 * 8 * new)
+    c.call("th_kv_batch_destroy", b)
+    c.close()
+
+
+def test_thousands_of_rows_on_a_prefix(lib):
+    """More forks than records are there for: those that fit share the prefix, whatever came first."""
+    c = Cache(lib, pages=3000, seqs=1100, max_len=4096)
+    b = c.batch(1100, 6000, 2)
+    a = c.create()
+    c.resize(a, 1600)
+    kids = c.fork(a, 1001, 1600)
+    news = [1500] + [4] * 1000
+    c.begin(b, kids, news)
+    rows, tiles = _plan(c, b, kids, news, 2)
+    prefix = tiles[(tiles[:, 3] < 1600) & (tiles[:, 4] <= 1600)]
+    assert prefix[:, 1].sum() >= 3000
+    c.call("th_kv_batch_destroy", b)
+    c.close()

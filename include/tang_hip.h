@@ -524,7 +524,10 @@ int th_kv_append(th_kv_batch* b, size_t layer, const th_buffer* q, const th_buff
  * [rows][n_heads][head_dim], each f32, f16 or bf16, query head h reads kv head
  * h / (n_heads / n_kv_heads); scores times scale (0: 1/sqrt(head_dim)), softmax and sums in f32.  With q and out of
  * the cache's type, more than 16 rows (new positions x query heads of a kv head) taken together, as in prompts and on shared
- * prefixes, have probabilities rounded to it, in the dividend and the divisor alike; all else keeps f32's precision or, for such types, 2^-18.  Pages that sequences of the batch share from their start on are read once for all.
+ * prefixes, have probabilities rounded to it, in the dividend and the divisor alike; all else keeps f32's precision or, for such types, 2^-18.  Sequences
+ * of the batch that share (by th_kv_seq_fork) the pages of their first 128 positions at least are a group: the pages that all of a group have in
+ * common from the start on are read once for it (a member that left early shortens them for the others; some thousand new
+ * positions on shared pages at most).
  * Captured (after the same call has been made once): buffers for max_rows rows, and
  * a replay runs on the batch as it last began. */
 int th_kv_batch_attention(th_kv_batch* b, size_t layer, const th_buffer* q, size_t window, size_t n_sinks, float scale,

@@ -364,7 +364,8 @@ class PlanMaker {
    private:
     const int* table(int s) const { return c_->mirror.data() + (size_t)s * c_->pages_per_seq; }
 
-    // Sequences whose first pages are the same, next to each other; the tokens in that order.  Tokens that share a prefix take two
+    // Sequences whose first KV_MIN_PREFIX positions are in the same pages, next to each other; the tokens in that order.  A group reads as
+    // tiles what all its sequences have in common.  Tokens that share a prefix take two
     // records at least; they get three quarters of all, so that long sequences can be split whatever else is in the batch, and
     // sequences beyond that read the prefix by themselves.
     void order() {
@@ -377,8 +378,10 @@ class PlanMaker {
         for (size_t i = 0; i < B; i++) {
             const size_t n = b_->step.n[i];
             if (n == 0) continue;
+            // (the page that holds the last position of the shortest prefix: forks that have it in common have all before it, and
+            // those that only share less belong to other groups)
             const bool can = b_->step.start[i] >= KV_MIN_PREFIX;
-            const int first = can ? table(b_->step.seqs[i])[0] : -1;
+            const int first = can ? table(b_->step.seqs[i])[(KV_MIN_PREFIX - 1) / ps] : -1;
             if (can && c_->refs[first] > 1) {
                 auto [at, fresh] = by_page.try_emplace(first, groups.size());
                 if (!fresh) {

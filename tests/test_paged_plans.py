@@ -139,3 +139,24 @@ def test_thousands_of_rows_on_a_prefix(lib):
     assert prefix[:, 1].sum() >= 3000
     c.call("th_kv_batch_destroy", b)
     c.close()
+
+
+@pytest.mark.parametrize("page", [16, 64])
+def test_documents_behind_a_short_common_start(lib, page):
+    """Two documents behind the same 64 positions, four answers to each: each document is read once."""
+    c = Cache(lib, page=page, pages=4000 // page + 60, seqs=12, max_len=2048)
+    b = c.batch(12, 100, 2)
+    start = c.create()
+    c.resize(start, 64)
+    docs = c.fork(start, 2, 64)
+    seqs = []
+    for d in docs:
+        c.resize(d, 1280)
+        seqs += c.fork(d, 4, 1280)
+    seqs = seqs[::2] + seqs[1::2]
+    c.begin(b, seqs, [1] * 8)
+    rows, tiles = _plan(c, b, seqs, [1] * 8, 2)
+    keys = sum(int((t[:, 4] - t[:, 3]).sum()) for t in (rows, tiles))
+    assert keys == 2 * 1280 + 8
+    c.call("th_kv_batch_destroy", b)
+    c.close()

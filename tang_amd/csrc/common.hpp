@@ -138,6 +138,8 @@ struct th_device {
     // name them: they stay until the last such graph goes.
     int graphs = 0;          // captured graphs, and a capture in progress
     bool capturing = false;  // between th_capture_begin and th_capture_end
+    uint64_t captures = 0;   // captures begun so far: the number of the last one
+    std::vector<uint64_t> graph_ids;  // numbers of those that are among `graphs`
     std::vector<void*> retired;
     int live = 0;          // buffers, weights and engines that hold this device
     bool closed = false;   // th_device_destroy ran; the struct waits for live == 0
@@ -167,6 +169,7 @@ inline void device_drain(th_device* d) {
 // A captured sequence of library calls (th_capture_begin / th_capture_end).
 struct th_graph {
     th_device* dev = nullptr;
+    uint64_t id = 0;  // of th_device::captures
     hipGraphExec_t exec = nullptr;
 };
 

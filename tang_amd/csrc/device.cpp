@@ -76,7 +76,8 @@ int* device_counters(th_device* dev, size_t n) {
 
 // One captured graph (or open capture) less: with the last one the outgrown
 // blocks go.  The device's work is drained.
-static void graph_gone(th_device* d) {
+static void graph_gone(th_device* d, uint64_t id) {
+    d->graph_ids.erase(std::remove(d->graph_ids.begin(), d->graph_ids.end(), id), d->graph_ids.end());
     if (--d->graphs > 0) return;
     for (void* p : d->retired) (void)hipFree(p);
     d->retired.clear();
@@ -347,6 +348,7 @@ int th_capture_begin(th_device* d) {
     TH_HIP(hipStreamBeginCapture(d->stream, hipStreamCaptureModeThreadLocal));
     d->capturing = true;
     d->graphs++;
+    d->graph_ids.push_back(++d->captures);
     TH_API_END
 }
 
@@ -364,11 +366,12 @@ int th_capture_end(th_device* d, th_graph** out) {
     d->capturing = false;
     if (e != hipSuccess && open) {
         device_drain(d);
-        graph_gone(d);
+        graph_gone(d, d->captures);
     }
     TH_HIP(e);
     th_graph* r = new th_graph();
     r->dev = d;
+    r->id = d->captures;
     r->exec = ge;
     device_retain(d);
     *out = r;
@@ -388,8 +391,9 @@ int th_graph_destroy(th_graph* g) {
     device_drain(g->dev);
     (void)hipGraphExecDestroy(g->exec);
     th_device* d = g->dev;
+    const uint64_t id = g->id;
     delete g;
-    graph_gone(d);
+    graph_gone(d, id);
     device_release(d);
     TH_API_END
 }

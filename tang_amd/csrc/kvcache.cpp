@@ -618,16 +618,32 @@ static void build_plan(th_kv_batch* b, const th_kv_batch::Key& key, th_kv_batch:
     send_plan(b, m, runs, p, room);
 }
 
-// Room for another plan: of its own, or, where there are many, that of one that no graph reads (uploads
+// Whether a graph that is still there may read the plan.
+static bool captured(const th_device* d, th_kv_batch::Plan& p) {
+    auto gone = [&](uint64_t id) { return std::find(d->graph_ids.begin(), d->graph_ids.end(), id) == d->graph_ids.end(); };
+    p.graphs.erase(std::remove_if(p.graphs.begin(), p.graphs.end(), gone), p.graphs.end());
+    return !p.graphs.empty();
+}
+
+// Room for another plan: of its own, or, where there are KV_MAX_PLANS that no graph reads, that of one of them (uploads
 // are in stream order, behind the calls that read the old plan).
 static std::map<th_kv_batch::Key, th_kv_batch::Plan>::iterator add_plan(th_kv_batch* b, const th_kv_batch::Key& key) {
+    th_device* d = b->cache->dev;
     th_kv_batch::Plan p;
-    if (b->plans.size() >= KV_MAX_PLANS) {
-        auto old = std::find_if(b->plans.begin(), b->plans.end(), [](const auto& x) { return !x.second.captured; });
-        if (old != b->plans.end()) {
-            p.block = old->second.block;
-            b->plans.erase(old);
+    size_t spare = 0;
+    for (auto& x : b->plans) spare += !captured(d, x.second);
+    for (auto at = b->plans.begin(); at != b->plans.end() && spare >= KV_MAX_PLANS;) {
+        if (!at->second.graphs.empty()) {
+            ++at;
+            continue;
         }
+        if (p.block) {  // left by graphs that are gone
+            device_drain(d);
+            free_drained(d, p.block);
+        }
+        p.block = at->second.block;
+        at = b->plans.erase(at);
+        spare--;
     }
     if (!p.block) {
         const hipError_t e = hipMalloc((void**)&p.block, plan_words(b) * 4);
@@ -1120,7 +1136,7 @@ int th_kv_batch_begin(th_kv_batch* b, const int32_t* seqs, const uint32_t* n_new
     try {
         size_t more = 0;
         for (auto& p : b->plans) {
-            if (!p.second.captured) continue;
+            if (!captured(c->dev, p.second)) continue;
             made.push_back({&p.second, PlanMaker(b, p.first.first, p.first.second), {}});
             Made& m = made.back();
             m.maker.make();
@@ -1208,7 +1224,7 @@ int th_kv_batch_attention(th_kv_batch* b, size_t layer, const th_buffer* q, size
         if (at == b->plans.end()) at = add_plan(b, key);
         build_plan(b, key, at->second);
     }
-    at->second.captured |= capturing;
+    if (capturing && (at->second.graphs.empty() || at->second.graphs.back() != c->dev->captures)) at->second.graphs.push_back(c->dev->captures);
     const th_kv_batch::Plan& p = at->second;
     KvAttnArgs a;
     a.pages = layer_pages(c, layer);

@@ -199,7 +199,7 @@ struct th_kv_batch {
         size_t n_rows_items = 0, n_tile_items = 0, n_joins = 0, n_recs = 0;
         bool far = false;      // an item of tiles has more than KV_LONG_ITEM keys
         bool built = false;    // for the batch as it is begun
-        bool captured = false; // a graph may read it
+        std::vector<uint64_t> graphs;  // th_graph::id of those that may read it (and of some that are gone)
     };
     typedef std::pair<size_t, size_t> Key;  // window, sinks
     std::map<Key, Plan> plans;

@@ -205,6 +205,7 @@ int th_device_destroy(th_device* d) {
 int th_capture_begin(th_device* d) {
     d->capturing = true;
     d->graphs++;
+    d->graph_ids.push_back(++d->captures);
     return TH_OK;
 }
 int th_capture_end(th_device* d, th_graph** out) {
@@ -212,10 +213,12 @@ int th_capture_end(th_device* d, th_graph** out) {
     device_retain(d);
     *out = new th_graph();
     (*out)->dev = d;
+    (*out)->id = d->captures;
     return TH_OK;
 }
 int th_graph_destroy(th_graph* g) {
     th_device* d = g->dev;
+    d->graph_ids.erase(std::find(d->graph_ids.begin(), d->graph_ids.end(), g->id));
     delete g;
     d->graphs--;
     device_release(d);
@@ -245,7 +248,7 @@ void host_fail(long which) { g_fail = which; }
 long host_allocs(void) { return g_allocs; }
 size_t host_bytes(void) { return g_bytes; }
 long host_launches(void) { return g_launches; }
-// The last attention call's plan: sizes {tokens' pointer count unknown here: joins, rows items, tile items}, then copies of its parts.
+// The last attention call's plan: how many rows items, tile items and joined tokens it has, and copies of its parts.
 void host_plan_sizes(int* n) {
     n[0] = g_plan.head->n_rows_items;
     n[1] = g_plan.head->n_tile_items;

@@ -102,3 +102,43 @@ def test_calls_that_find_no_memory_change_nothing(lib, act, least):
         c.call("th_kv_batch_destroy", S.b2)
         c.close()
     assert fail >= least, "too few allocations to have been looked at"
+
+
+def test_plans_of_graphs_that_are_gone(lib):
+    """A step rebuilds the plans that captured graphs read, and no others: not those of a graph that was destroyed. Their memory is used for
+    other windows."""
+    c = Cache(lib, pages=40, seqs=2, max_len=600)
+    b = c.batch(2, 4)
+    s = c.create()
+    c.resize(s, 300)
+    c.begin(b, [s], [1])
+    q, o = c.buffer(4 * 8), c.buffer(4 * 8)
+
+    def step():
+        n = lib.host_launches()
+        c.begin(b, [s], [1])
+        return lib.host_launches() - n
+
+    graphs = []
+    for windows in (range(10, 20), range(20, 30), range(10, 13)):
+        for w in windows:
+            c.attend(b, 1, window=w)
+        c.call("th_capture_begin", c.dev)
+        for w in windows:
+            for _ in range(2):
+                c.call("th_kv_batch_attention", b, 0, q, w, 0, 0.0, o)
+        graphs.append(c.new("th_capture_end", c.dev))
+    assert step() == 1 + 20
+    c.call("th_graph_destroy", graphs[0])
+    assert step() == 1 + 13
+    c.call("th_graph_destroy", graphs[1])
+    assert step() == 1 + 3
+    asked = lib.host_bytes()
+    for w in range(30, 60):
+        c.attend(b, 1, window=w)
+    assert lib.host_bytes() == asked  # no memory for new plans
+    assert step() == 1 + 3
+    c.call("th_graph_destroy", graphs[2])
+    assert step() == 1
+    c.call("th_kv_batch_destroy", b)
+    c.close()

@@ -1328,6 +1328,7 @@ int th_rope_rows(th_device* dev, const th_buffer* in, const th_buffer* cos_t, co
     auto ok = [&](const th_buffer* b) { return (b->dtype == TH_F32 || b->dtype == TH_F16 || b->dtype == TH_BF16) && b->dev == dev; };
     TH_REQUIRE(ok(in) && ok(out), "buffers must be f32, f16 or bf16, of this device handle");
     TH_REQUIRE(n_heads <= (size_t)1 << 20 && head_dim <= (size_t)1 << 16 && n_rows < (size_t)1 << 31, "sizes out of range");
+    TH_REQUIRE(n_heads * ceil_div(head_dim, 8) < (size_t)1 << 31, "sizes out of range: a row of 2^34 elements");
     TH_REQUIRE(n_rows == 0 || start_pos <= SIZE_MAX - n_rows, "sizes out of range");
     require_len_any(in, n_rows * n_heads * head_dim, "input");
     require_len_any(out, n_rows * n_heads * head_dim, "out");

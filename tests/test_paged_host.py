@@ -142,3 +142,17 @@ def test_plans_of_graphs_that_are_gone(lib):
     assert step() == 1
     c.call("th_kv_batch_destroy", b)
     c.close()
+
+
+def test_rows_of_rotary_positions_that_pass_32_bits(lib):
+    """2^20 heads of 2^14 dims make 2^31 threads of a row, which the kernel counts in 32 bits: refused, before the buffers are looked at."""
+    c = Cache(lib)
+    x, t = c.buffer(64), c.buffer(64, capi.F32)
+    for heads, hd in ((1 << 20, 1 << 14), (1 << 20, 1 << 16), (1 << 18, 1 << 16)):
+        with pytest.raises(Refused, match="sizes out of range") as e:
+            c.call("th_rope_rows", c.dev, x, t, t, None, 0, 1, heads, hd, 2, 0, x)
+        assert e.value.code == capi.TH_ERR_INVALID
+    with pytest.raises(Refused, match="too small"):
+        c.call("th_rope_rows", c.dev, x, t, t, None, 0, 1, (1 << 18) - 1, 1 << 16, 2, 0, x)
+    c.call("th_rope_rows", c.dev, x, t, t, None, 0, 1, 1, 64, 2, 0, x)
+    c.close()

@@ -91,10 +91,12 @@ __global__ __launch_bounds__(256) void kv_copy_upload_kernel(char* __restrict__ 
 
 void launch_kv_copy_pages(void* pool, size_t page_bytes, size_t n_pages, int n_planes, const uint32_t* pairs, size_t n,
                           hipStream_t s) {
-    if (n == 0) return;
-    TH_LAUNCH(kv_copy_pages_kernel, dim3((unsigned)n, (unsigned)ceil_div(page_bytes, (size_t)KV_COPY_BYTES), (unsigned)n_planes),
-              dim3(256), 0, s, (char*)pool, page_bytes, n_pages, pairs);
-    TH_LAUNCH_CHECK();
+    // (a launch has below 2^32 threads: more pages go in slices)
+    for (size_t at = 0; at < n; at += KV_MAX_BLOCKS) {
+        const dim3 grid((unsigned)std::min(n - at, KV_MAX_BLOCKS), (unsigned)ceil_div(page_bytes, (size_t)KV_COPY_BYTES), (unsigned)n_planes);
+        TH_LAUNCH(kv_copy_pages_kernel, grid, dim3(256), 0, s, (char*)pool, page_bytes, n_pages, pairs + 2 * at);
+        TH_LAUNCH_CHECK();
+    }
 }
 
 void launch_kv_copy_upload(void* pool, size_t page_bytes, size_t n_pages, int n_planes, const KvWords& w, size_t n,
@@ -133,11 +135,13 @@ __global__ __launch_bounds__(256) void kv_gather_rows_kernel(char* __restrict__ 
 
 void launch_kv_gather_rows(void* pool, size_t n_pages, int n_planes, int n_kv_heads, int shift, size_t row_bytes,
                            const uint32_t* from, const uint32_t* to, size_t n, hipStream_t s) {
-    if (n == 0) return;
-    TH_LAUNCH(kv_gather_rows_kernel,
-              dim3((unsigned)ceil_div(n, (size_t)1 << shift), (unsigned)n_kv_heads, (unsigned)n_planes), dim3(256), 0, s, (char*)pool,
-              n_pages, n_kv_heads, shift, (int)(row_bytes / 16), from, to, (int)n);
-    TH_LAUNCH_CHECK();
+    const size_t pages = ceil_div(n, (size_t)1 << shift);
+    for (size_t at = 0; at < pages; at += KV_MAX_BLOCKS) {
+        const dim3 grid((unsigned)std::min(pages - at, KV_MAX_BLOCKS), (unsigned)n_kv_heads, (unsigned)n_planes);
+        TH_LAUNCH(kv_gather_rows_kernel, grid, dim3(256), 0, s, (char*)pool, n_pages, n_kv_heads, shift, (int)(row_bytes / 16),
+                  from + (at << shift), to + at, (int)(n - (at << shift)));
+        TH_LAUNCH_CHECK();
+    }
 }
 
 __global__ __launch_bounds__(256) void kv_read_kernel(KvPages p, int seq, size_t from, size_t total, int cpr,

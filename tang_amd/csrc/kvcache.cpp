@@ -340,6 +340,8 @@ constexpr size_t KV_MAX_PLANS = 16;
 // with 1024 83; 24 rows with a window of 1000: 22 us, with 512 25.5, unsplit 23.7).  Tiles: eight samples of a prompt
 // of 992 take 32 us, with 512 40.
 constexpr size_t KV_MIN_ROWS_KEYS = 256, KV_MIN_TILE_KEYS = 256;
+constexpr size_t KV_ROWS_SHARE = 8;  // pieces of rows items a CU (PlanMaker::split)
+constexpr size_t KV_LONG_PIECE = KV_LONG_ITEM * 4 / 5 / 64 * 64;
 
 class PlanMaker {
    public:
@@ -468,11 +470,11 @@ class PlanMaker {
         // of 8192 99 us, 512 tokens beside 32 decode steps 146 us, 128 rows on a prefix of 16000 115 us; with 4 a CU 59 and
         // 112, with 2 54 and 109, with 1 59, 95, 138 and 126).
         size_t per[2];
-        per[1] = round_up(std::max<size_t>(KV_MIN_ROWS_KEYS, ceil_div(keys_[1] * kvh, 8 * cus)), 64) * scale[1];
+        per[1] = round_up(std::max<size_t>(KV_MIN_ROWS_KEYS, ceil_div(keys_[1] * kvh, KV_ROWS_SHARE * cus)), 64) * scale[1];
         per[0] = round_up(std::max<size_t>(KV_MIN_TILE_KEYS, ceil_div(keys_[0] * kvh, cus * 3 / 2)), 64) * scale[0];
         // Where there are records for it, no tile's piece is so long that it needs additions of its own (a quarter
         // more than `per` is one piece).  A multiple of 64 like any other: pieces begin at blocks, and the last of many shall have keys left.
-        if (scale[0] == 1) per[0] = std::min(per[0], KV_LONG_ITEM * 4 / 5 / 64 * 64);
+        if (scale[0] == 1) per[0] = std::min(per[0], KV_LONG_PIECE);
         std::vector<int> shared(toks_.size(), 0), own(toks_.size(), 0), pieces(tiles_.size());
         size_t extra[2] = {0, 0}, more[2] = {0, 0};  // items and records that splitting takes
         for (size_t i = 0; i < tiles_.size(); i++) {
@@ -1045,6 +1047,10 @@ int th_kv_batch_create(th_kv_cache* c, size_t max_seqs, size_t max_rows, size_t 
     // is split (a plan that would need more splits less), 1 GiB of them at most.
     const size_t G = n_heads / c->n_kv_heads;
     b->max_recs = std::max<size_t>(64, std::min<size_t>(8192, ((size_t)1 << 30) / (n_heads * c->hd * 4)));
+    // ... and no more than max_rows tokens can have: a piece of each of a token's two ranges of keys at most by length, and by the chip's share
+    const size_t by_len = c->max_len / std::min(KV_MIN_ROWS_KEYS, KV_MIN_TILE_KEYS) + 2;
+    const size_t by_share = 2 * (KV_ROWS_SHARE * (size_t)c->dev->num_cus / c->n_kv_heads + 2) + c->max_len / KV_LONG_PIECE + 2;
+    b->max_recs = std::min(b->max_recs, std::max<size_t>(4, std::min(by_len, by_share)) * max_rows);
     b->max_items = 2 * (max_seqs + ceil_div(max_rows, std::max<size_t>(1, KV_TILE / G))) + 4096;
     try {
         TH_HIP(hipMalloc((void**)&b->block, 16 + max_rows * sizeof(KvRow)));

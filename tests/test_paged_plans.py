@@ -160,3 +160,34 @@ def test_documents_behind_a_short_common_start(lib, page):
     assert keys == 2 * 1280 + 8
     c.call("th_kv_batch_destroy", b)
     c.close()
+
+
+@pytest.mark.parametrize("rows,max_len,most", [(1, 4096, 1 << 20), (1, 131072, 10 << 20), (64, 1024, 10 << 20), (8192, 131072, 300 << 20)])
+def test_memory_of_a_batch(lib, rows, max_len, most):
+    """Records for what its rows can have, not for what any batch could."""
+    c = Cache(lib, kh=8, hd=128, pages=8, seqs=4, max_len=max_len)
+    before = lib.host_bytes()
+    b = c.batch(4, rows, 32)
+    assert lib.host_bytes() - before <= most
+    c.call("th_kv_batch_destroy", b)
+    c.close()
+
+
+@pytest.mark.parametrize("news", [[1], [1, 1, 1, 1], [30], [3, 1]])
+@pytest.mark.parametrize("n,window", [(256 * 40 + 1, 0), (3000, 0), (10000, 5000), (300, 0)])
+def test_small_batches_are_cut_as_large_ones(lib, news, n, window):
+    """A batch with room for just these rows has the plan of one with room for thousands."""
+    c = Cache(lib, pages=4000, seqs=9, max_len=256 * 42)
+    plans = []
+    for most in (sum(news), 4000):
+        b = c.batch(len(news), most, 2)
+        a = c.create()
+        c.resize(a, n)
+        seqs = c.fork(a, len(news), n - n % 16)
+        c.begin(b, seqs, news)
+        c.attend(b, sum(news), 2, window, 4)
+        plans.append(c.plan(sum(news)))
+        c.free(seqs + [a])
+        c.call("th_kv_batch_destroy", b)
+    assert all(np.array_equal(x, y) for x, y in zip(*plans))
+    c.close()

@@ -677,9 +677,10 @@ static void require_x(const th_kv_cache* c, const th_buffer* b, size_t n, const 
     if (b->dev != c->dev) throw Error(TH_ERR_INVALID, std::string("buffer ") + what + " is on another device handle");
 }
 
-// Tables, pairs and positions of a rotary call, checked.
+// Tables, pairs and positions of a rotary call, checked.  out: what it writes, which other threads' tables must not be.
 static void rope_args(KvRopeArgs& a, const th_device* dev, const th_buffer* cos_t, const th_buffer* sin_t, const th_buffer* positions,
-                      size_t rows, size_t hd, size_t rot, int layout, size_t top) {
+                      size_t rows, size_t hd, size_t rot, int layout, size_t top, const th_buffer* out) {
+    TH_REQUIRE(!out || (out != cos_t && out != sin_t), "the result must not be a table");
     TH_REQUIRE(rot % 2 == 0 && rot <= hd, "rot_dim must be even and at most head_dim");
     TH_REQUIRE(layout == TH_ROPE_INTERLEAVED || layout == TH_ROPE_HALF, "unknown pair layout");
     a.rot = (int)rot;
@@ -1195,7 +1196,7 @@ int th_kv_append(th_kv_batch* b, size_t layer, const th_buffer* q, const th_buff
         require_x(c, q_out, qn, "q_out");
         TH_REQUIRE(q_out != k && q_out != v, "q_out must not be k or v");
     }
-    rope_args(a, c->dev, cos_t, sin_t, positions, rows, c->hd, rot_dim, layout, b->step.top);
+    rope_args(a, c->dev, cos_t, sin_t, positions, rows, c->hd, rot_dim, layout, b->step.top, q_out);
     a.q = q ? q->ptr : nullptr;
     a.k = k->ptr;
     a.v = v->ptr;
@@ -1340,7 +1341,7 @@ int th_rope_rows(th_device* dev, const th_buffer* in, const th_buffer* cos_t, co
     require_len_any(out, n_rows * n_heads * head_dim, "out");
     TH_REQUIRE(in != out || in->dtype == out->dtype, "out in place of the input needs its type");
     KvRopeArgs a = {};
-    rope_args(a, dev, cos_t, sin_t, positions, n_rows, head_dim, rot_dim, layout, start_pos + n_rows);
+    rope_args(a, dev, cos_t, sin_t, positions, n_rows, head_dim, rot_dim, layout, start_pos + n_rows, out);
     a.q = in->ptr;
     a.q_out = out->ptr;
     a.xdt = in->dtype;

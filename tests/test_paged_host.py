@@ -156,3 +156,20 @@ def test_rows_of_rotary_positions_that_pass_32_bits(lib):
         c.call("th_rope_rows", c.dev, x, t, t, None, 0, 1, (1 << 18) - 1, 1 << 16, 2, 0, x)
     c.call("th_rope_rows", c.dev, x, t, t, None, 0, 1, 1, 64, 2, 0, x)
     c.close()
+
+
+def test_rotated_rows_over_the_tables_they_read(lib):
+    """A result in the place of a table that other rows still read."""
+    c = Cache(lib, pages=4, seqs=1)
+    b, s = c.batch(1, 4, 2), c.create()
+    c.begin(b, [s], [4])
+    x, kv, t, u = (c.buffer(256, capi.F32) for _ in range(4))
+    for cos, sin, out in ((t, u, t), (t, u, u), (t, t, t)):
+        for name, args in (("th_rope_rows", (c.dev, x, cos, sin, None, 0, 4, 2, 8, 8, 0, out)),
+                           ("th_kv_append", (b, 0, x, kv, kv, cos, sin, None, 8, 0, out))):
+            with pytest.raises(Refused, match="table") as e:
+                c.call(name, *args)
+            assert e.value.code == capi.TH_ERR_INVALID
+    c.call("th_rope_rows", c.dev, x, t, u, None, 0, 4, 2, 8, 8, 0, x)
+    c.call("th_kv_batch_destroy", b)
+    c.close()

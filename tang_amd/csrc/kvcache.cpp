@@ -1215,7 +1215,8 @@ int th_kv_batch_attention(th_kv_batch* b, size_t layer, const th_buffer* q, size
     th_kv_cache* c = b->cache;
     TH_REQUIRE(q && out, "null argument");
     TH_REQUIRE(q != out, "out must not be q");
-    TH_REQUIRE(std::isfinite(scale) && scale >= 0.0f, "scale must be finite and not negative");
+    // (finite times log2(e) too, which the kernels take)
+    TH_REQUIRE(std::isfinite(scale * 1.44269504f) && scale >= 0.0f, "scale must be finite and not negative");
     DeviceScope scope(c->dev);
     const bool capturing = c->dev->capturing;
     const size_t n = (capturing ? b->max_rows : b->step.rows) * b->n_heads * c->hd;

@@ -173,3 +173,17 @@ def test_rotated_rows_over_the_tables_they_read(lib):
     c.call("th_rope_rows", c.dev, x, t, u, None, 0, 4, 2, 8, 8, 0, x)
     c.call("th_kv_batch_destroy", b)
     c.close()
+
+
+def test_scales_that_overflow(lib):
+    """3e38 is finite, 3e38 log2(e) is not: every row would be NaN."""
+    c = Cache(lib, pages=4, seqs=1)
+    b, s = c.batch(1, 4), c.create()
+    c.begin(b, [s], [4])
+    q, o = c.buffer(256), c.buffer(256)
+    for scale in (3e38, float("inf"), float("nan"), -1.0):
+        with pytest.raises(Refused, match="scale"):
+            c.call("th_kv_batch_attention", b, 0, q, 0, 0, scale, o)
+    c.call("th_kv_batch_attention", b, 0, q, 0, 0, 2e38, o)
+    c.call("th_kv_batch_destroy", b)
+    c.close()

@@ -25,7 +25,7 @@ __global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void kv_attn_rows_kernel(KvA
 // records w, w + 4, ... with lane l on dims DE l ..; the waves meet in LDS.  One round of loads covers
 // 64 records: latency is what it costs.
 template <int DE>
-__global__ __launch_bounds__(256) void kv_attn_join_few_kernel(KvAttnArgs a, const KvTok* __restrict__ list) {
+__device__ __forceinline__ void kv_join_few(const KvAttnArgs& a, const KvTok* __restrict__ list, int room) {
     constexpr int U = DE == 4 ? 8 : 16;
     typedef float vec __attribute__((ext_vector_type(DE == 1 ? 2 : DE)));
     __shared__ float sA[4][64 * DE], sM[4], sL[4];
@@ -33,7 +33,7 @@ __global__ __launch_bounds__(256) void kv_attn_join_few_kernel(KvAttnArgs a, con
     const int total = a.head->n_joins * a.n_heads;
     const size_t step = (size_t)a.n_heads * hd;
     int x = blockIdx.x;
-    KvTok t = list[x / a.n_heads];  // (read with the count: the list has room for it)
+    KvTok t = list[min(x / a.n_heads, room - 1)];  // (read with the count, before it is known to be there)
     for (; x < total; x += gridDim.x, t = list[min(x, total - 1) / a.n_heads]) {
         const int hq = x % a.n_heads;
         const int n = t.own_n >> 16, mine = (n - wave + 3) / 4;  // this wave's records
@@ -100,12 +100,12 @@ __global__ __launch_bounds__(256) void kv_attn_join_few_kernel(KvAttnArgs a, con
 
 // Many rows of few records: LPR lanes for each, eight dims a lane, two records in flight.
 template <int LPR>
-__global__ __launch_bounds__(256) void kv_attn_join_many_kernel(KvAttnArgs a, const KvTok* __restrict__ list) {
+__device__ __forceinline__ void kv_join_many(const KvAttnArgs& a, const KvTok* __restrict__ list, int room) {
     const int hd = a.pages.hd, part = threadIdx.x % LPR, d0 = part * 8;
     const int total = a.head->n_joins * a.n_heads;
     const size_t step = (size_t)a.n_heads * hd;
     int x = blockIdx.x * (256 / LPR) + threadIdx.x / LPR;
-    KvTok t = list[x / a.n_heads];
+    KvTok t = list[min(x / a.n_heads, room - 1)];
     for (; x < total; x += gridDim.x * (256 / LPR), t = list[min(x, total - 1) / a.n_heads]) {
         const int hq = x % a.n_heads;
         const int n = t.own_n >> 16;
@@ -144,14 +144,33 @@ __global__ __launch_bounds__(256) void kv_attn_join_many_kernel(KvAttnArgs a, co
     }
 }
 
-void launch_kv_attn_join(const KvAttnArgs& a, const KvTok* list, size_t n, size_t n_recs, hipStream_t s) {
+template <int DE>
+__global__ __launch_bounds__(256) void kv_attn_join_few_kernel(KvAttnArgs a, const KvTok* __restrict__ list, int room) {
+    kv_join_few<DE>(a, list, room);
+}
+template <int DE>
+__global__ __launch_bounds__(256) void kv_attn_join_many_kernel(KvAttnArgs a, const KvTok* __restrict__ list, int room) {
+    kv_join_many<8 * DE>(a, list, room);
+}
+// As the plan says (captured calls).
+template <int DE>
+__global__ __launch_bounds__(256) void kv_attn_join_kernel(KvAttnArgs a, const KvTok* __restrict__ list, int room) {
+    if (a.head->flags & KV_PLAN_MANY) kv_join_many<8 * DE>(a, list, room);
+    else kv_join_few<DE>(a, list, room);
+}
+
+// 33 records a row: few 9.4 us, many 12.1; about 3 records for each of 3000 rows: many 11, one wave a row 19
+bool kv_join_many(size_t n, size_t n_recs, size_t n_heads) { return n * n_heads > 1024 && n_recs < 8 * n; }
+
+void launch_kv_attn_join(const KvAttnArgs& a, const KvTok* list, size_t n, size_t room, int flags, hipStream_t s) {
     if (n == 0) return;
     const size_t rows = n * a.n_heads;
     auto with = [&](auto de) {
         constexpr int DE = decltype(de)::value, LPR = 8 * DE;
-        // 33 records a row: few 9.4 us, many 12.1; about 3 records for each of 3000 rows: many 11, one wave a row 19
-        if (rows <= 1024 || n_recs >= 8 * n) TH_LAUNCH((kv_attn_join_few_kernel<DE>), dim3((unsigned)std::min(rows, KV_MAX_BLOCKS)), dim3(256), 0, s, a, list);
-        else TH_LAUNCH((kv_attn_join_many_kernel<LPR>), dim3((unsigned)std::min(ceil_div(rows, (size_t)(256 / LPR)), KV_MAX_BLOCKS)), dim3(256), 0, s, a, list);
+        const dim3 few((unsigned)std::min(rows, KV_MAX_BLOCKS)), many((unsigned)std::min(ceil_div(rows, (size_t)(256 / LPR)), KV_MAX_BLOCKS));
+        if (flags == KV_BY_PLAN) TH_LAUNCH((kv_attn_join_kernel<DE>), few, dim3(256), 0, s, a, list, (int)room);
+        else if (flags & KV_PLAN_MANY) TH_LAUNCH((kv_attn_join_many_kernel<DE>), many, dim3(256), 0, s, a, list, (int)room);
+        else TH_LAUNCH((kv_attn_join_few_kernel<DE>), few, dim3(256), 0, s, a, list, (int)room);
     };
     if (a.pages.hd <= 64) with(std::integral_constant<int, 1>{});
     else if (a.pages.hd <= 128) with(std::integral_constant<int, 2>{});

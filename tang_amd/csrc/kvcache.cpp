@@ -360,8 +360,8 @@ class PlanMaker {
     }
 
     std::vector<uint32_t> words;  // head, tokens, rows items, tile items, joined tokens
-    bool far = false;                              // an item of tiles has more than KV_LONG_ITEM keys
-    size_t n_toks = 0, n_items[2] = {0, 0}, n_joins = 0, n_recs = 0;  // items: [0] tiles, [1] rows
+    int flags = 0;                // KvPlanHead::flags
+    size_t n_toks = 0, n_items[2] = {0, 0}, n_joins = 0;  // items: [0] tiles, [1] rows
 
    private:
     const int* table(int s) const { return c_->mirror.data() + (size_t)s * c_->pages_per_seq; }
@@ -468,7 +468,7 @@ class PlanMaker {
         // that uneven lengths level out.  Tiles are longer, since each of their pieces leaves 128 rows of
         // records: 1.5 pieces a CU (six ragged prompt chunks behind a window 49 us, 64 rows on a prefix
         // of 8192 99 us, 512 tokens beside 32 decode steps 146 us, 128 rows on a prefix of 16000 115 us; with 4 a CU 59 and
-        // 112, with 2 54 and 109, with 1 59, 95, 138 and 126).
+        // 112, with 2 54 and 109, with 1 59, 95, 138 and 126; the last two workloads on pages of zeros: 166 and 125 us on random values).
         size_t per[2];
         per[1] = round_up(std::max<size_t>(KV_MIN_ROWS_KEYS, ceil_div(keys_[1] * kvh, KV_ROWS_SHARE * cus)), 64) * scale[1];
         per[0] = round_up(std::max<size_t>(KV_MIN_TILE_KEYS, ceil_div(keys_[0] * kvh, cus * 3 / 2)), 64) * scale[0];
@@ -547,13 +547,14 @@ class PlanMaker {
         // the longest first: the last workgroups to start are short
         for (auto& v : items)
             std::stable_sort(v.begin(), v.end(), [](const KvItem& x, const KvItem& y) { return x.j1 - x.j0 > y.j1 - y.j0; });
-        far = !items[0].empty() && (size_t)(items[0][0].j1 - items[0][0].j0) > KV_LONG_ITEM;
+        if (!items[0].empty() && (size_t)(items[0][0].j1 - items[0][0].j0) > KV_LONG_ITEM) flags |= KV_PLAN_FAR;
+        if (kv_join_many(joins.size(), rec, b_->n_heads)) flags |= KV_PLAN_MANY;
         n_toks = toks_.size();
         n_items[0] = items[0].size();
         n_items[1] = items[1].size();
         n_joins = joins.size();
-        n_recs = rec;
         KvPlanHead head = {};
+        head.flags = flags;
         head.n_joins = (int)n_joins;
         head.n_rows_items = (int)n_items[1];
         head.n_tile_items = (int)n_items[0];
@@ -584,8 +585,7 @@ static size_t plan_toks(const th_kv_batch*) { return KV_HEAD_WORDS; }
 static size_t plan_rows(const th_kv_batch* b) { return plan_toks(b) + b->max_rows * sizeof(KvTok) / 4; }
 static size_t plan_tiles(const th_kv_batch* b) { return plan_rows(b) + b->max_items * sizeof(KvItem) / 4; }
 static size_t plan_joins(const th_kv_batch* b) { return plan_tiles(b) + b->max_items * sizeof(KvItem) / 4; }
-// (the join kernels read an entry before they know whether it is there: up to 32 rows behind the last)
-static size_t plan_words(const th_kv_batch* b) { return plan_joins(b) + (b->max_rows + 32) * sizeof(KvTok) / 4; }
+static size_t plan_words(const th_kv_batch* b) { return plan_joins(b) + b->max_rows * sizeof(KvTok) / 4; }
 
 static KvRuns plan_runs(const th_kv_batch* b, const PlanMaker& m) {
     KvRuns runs;
@@ -607,8 +607,7 @@ static void send_plan(th_kv_batch* b, const PlanMaker& m, const KvRuns& runs, th
     p.n_tile_items = m.n_items[0];
     p.n_rows_items = m.n_items[1];
     p.n_joins = m.n_joins;
-    p.n_recs = m.n_recs;
-    p.far = m.far;
+    p.flags = m.flags;
     p.built = true;
 }
 
@@ -1250,17 +1249,18 @@ int th_kv_batch_attention(th_kv_batch* b, size_t layer, const th_buffer* q, size
     a.head = (const KvPlanHead*)p.block;
     a.rows_items = (const KvItem*)(p.block + plan_rows(b));
     a.tile_items = (const KvItem*)(p.block + plan_tiles(b));
+    const KvTok* joins = (const KvTok*)(p.block + plan_joins(b));
     const size_t items = p.n_tile_items + p.n_rows_items;
     if (capturing) {
         // whatever plan the batch has at replay: every kernel, on grids that walk their lists
         launch_kv_attn_both(a, c->dtype, std::max(items, ceil_div(4 * (size_t)c->dev->num_cus, c->n_kv_heads)),
-                            c->max_len > KV_LONG_ITEM, c->dev->stream);
-        launch_kv_attn_join(a, (const KvTok*)(p.block + plan_joins(b)), std::min<size_t>(b->max_rows, 1024), p.n_recs, c->dev->stream);
+                            c->max_len > KV_LONG_ITEM ? KV_BY_PLAN : 0, c->dev->stream);
+        launch_kv_attn_join(a, joins, std::min<size_t>(b->max_rows, 1024), b->max_rows, KV_BY_PLAN, c->dev->stream);
     } else {
-        if (p.n_tile_items && p.n_rows_items) launch_kv_attn_both(a, c->dtype, items, p.far, c->dev->stream);
-        else if (p.n_tile_items) launch_kv_attn_tiles(a, c->dtype, items, p.far, c->dev->stream);
+        if (p.n_tile_items && p.n_rows_items) launch_kv_attn_both(a, c->dtype, items, p.flags, c->dev->stream);
+        else if (p.n_tile_items) launch_kv_attn_tiles(a, c->dtype, items, p.flags, c->dev->stream);
         else launch_kv_attn_rows(a, c->dtype, items, c->dev->stream);
-        launch_kv_attn_join(a, (const KvTok*)(p.block + plan_joins(b)), p.n_joins, p.n_recs, c->dev->stream);
+        launch_kv_attn_join(a, joins, p.n_joins, b->max_rows, p.flags, c->dev->stream);
     }
     TH_API_END
 }

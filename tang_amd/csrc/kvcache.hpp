@@ -40,7 +40,10 @@ constexpr int KV_REC_OWN = 1 << 30;
 
 // An attention plan in device memory: counts, tokens, the two kernels'
 // items and the tokens whose records are joined, each part at a place of its own that does not change with the step.
-struct KvPlanHead { int n_rows_items, n_tile_items, n_joins, pad; };
+struct KvPlanHead { int n_rows_items, n_tile_items, n_joins, flags; };
+// flags: an item of tiles has more than KV_LONG_ITEM keys; the join is that of many rows.  What they choose adds up in another order, so a captured
+// call, which runs on whatever plan there is, goes by them as an eager one does.
+constexpr int KV_PLAN_FAR = 1, KV_PLAN_MANY = 2;
 constexpr int KV_HEAD_WORDS = sizeof(KvPlanHead) / 4;
 
 struct KvAttnArgs {
@@ -109,14 +112,16 @@ void launch_kv_append(const KvRopeArgs& a, const KvPages& p, th_dtype cache, con
 void launch_rope_rows(const KvRopeArgs& a, size_t n_rows, hipStream_t s);
 
 // grid: how many items the launch covers at a time (the kernels walk the rest; a launch has below 2^32 threads).
-// far: a tile item may have more than KV_LONG_ITEM keys.
+// flags: of the plan, or KV_BY_PLAN for a call that is captured.
 constexpr size_t KV_LONG_ITEM = 16384;
 constexpr size_t KV_MAX_BLOCKS = (size_t)1 << 23;
+constexpr int KV_BY_PLAN = -1;
 void launch_kv_attn_rows(const KvAttnArgs& a, th_dtype cache, size_t grid, hipStream_t s);
-void launch_kv_attn_tiles(const KvAttnArgs& a, th_dtype cache, size_t grid, bool far, hipStream_t s);
-void launch_kv_attn_both(const KvAttnArgs& a, th_dtype cache, size_t grid, bool far, hipStream_t s);
-// n: tokens to join, n_recs: their records (by which the kernel is chosen).
-void launch_kv_attn_join(const KvAttnArgs& a, const KvTok* list, size_t n, size_t n_recs, hipStream_t s);
+void launch_kv_attn_tiles(const KvAttnArgs& a, th_dtype cache, size_t grid, int flags, hipStream_t s);
+void launch_kv_attn_both(const KvAttnArgs& a, th_dtype cache, size_t grid, int flags, hipStream_t s);
+// n: tokens to join (captured: how many the launch covers at a time), room: entries that the list has memory for.
+bool kv_join_many(size_t n, size_t n_recs, size_t n_heads);
+void launch_kv_attn_join(const KvAttnArgs& a, const KvTok* list, size_t n, size_t room, int flags, hipStream_t s);
 
 // Rows (tokens x query heads of a kv head) that one item has at most.
 constexpr int KV_ROWS = 16, KV_TILE = 128;
@@ -196,8 +201,8 @@ struct th_kv_batch {
     int* block = nullptr;      // device: the number of rows (16 bytes), then KvRow[max_rows]
     struct Plan {
         int* block = nullptr;  // device
-        size_t n_rows_items = 0, n_tile_items = 0, n_joins = 0, n_recs = 0;
-        bool far = false;      // an item of tiles has more than KV_LONG_ITEM keys
+        size_t n_rows_items = 0, n_tile_items = 0, n_joins = 0;
+        int flags = 0;         // KvPlanHead::flags
         bool built = false;    // for the batch as it is begun
         std::vector<uint64_t> graphs;  // th_graph::id of those that may read it (and of some that are gone)
     };

@@ -178,9 +178,10 @@ static KvAttnArgs g_plan;
 static const KvTok* g_joins;
 static void keep(const KvAttnArgs& a) { g_plan = a; }
 void launch_kv_attn_rows(const KvAttnArgs& a, th_dtype, size_t, hipStream_t) { keep(a); }
-void launch_kv_attn_tiles(const KvAttnArgs& a, th_dtype, size_t, bool, hipStream_t) { keep(a); }
-void launch_kv_attn_both(const KvAttnArgs& a, th_dtype, size_t, bool, hipStream_t) { keep(a); }
-void launch_kv_attn_join(const KvAttnArgs&, const KvTok* list, size_t, size_t, hipStream_t) { g_joins = list; }
+void launch_kv_attn_tiles(const KvAttnArgs& a, th_dtype, size_t, int, hipStream_t) { keep(a); }
+void launch_kv_attn_both(const KvAttnArgs& a, th_dtype, size_t, int, hipStream_t) { keep(a); }
+bool kv_join_many(size_t, size_t, size_t) { return false; }
+void launch_kv_attn_join(const KvAttnArgs&, const KvTok* list, size_t, size_t, int, hipStream_t) { g_joins = list; }
 
 }  // namespace th
 

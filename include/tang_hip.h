@@ -459,8 +459,9 @@ int th_rope_rows(th_device* dev, const th_buffer* in, const th_buffer* cos_buf, 
  * cpu.rs:257).  A cache has n_pages pages of page_size positions for every
  * layer; a sequence is a list of pages that grows with it, lowest vacant page first.  Forks share
  * pages, and a page that is shared is copied when one of its sequences writes
- * to it.  Bookkeeping is the host's: calls that change sequences cost no
- * synchronisation, and are made between replays of captured graphs, not recorded.  One that finds no memory changes nothing.
+ * to it.  Bookkeeping is the host's: calls that change sequences do not synchronise (they may wait for earlier work where
+ * large uploads follow one another, and where staging memory or the handle's workspace has to grow), and
+ * are made between replays of captured graphs, not recorded.  One that finds no memory changes nothing.
  * All calls on a cache are its device handle's: one host thread, one stream. */
 typedef struct th_kv_cache th_kv_cache;
 typedef struct th_kv_batch th_kv_batch;
@@ -515,7 +516,8 @@ int th_kv_batch_trim(th_kv_batch* b, const uint32_t* n_keep, size_t n);
  * any of them (it may be q, with q's type).  A row's position is its place in its sequence, or positions[row] where
  * that is given (as in th_rope_rows).  rot_dim 0 rotates nothing (tables may be NULL);
  * q and q_out may be NULL together.  Captured: buffers for max_rows rows, and a
- * replay runs on the batch as it last began (rows behind the tables' end get NaN pairs then). */
+ * replay runs on the batch as it last began (rows behind the tables' end get NaN pairs then).  Replays belong between
+ * th_kv_batch_begin and the next call that changes one of its sequences: one that comes later writes to pages that may be another's by then. */
 int th_kv_append(th_kv_batch* b, size_t layer, const th_buffer* q, const th_buffer* k, const th_buffer* v,
                  const th_buffer* cos_buf, const th_buffer* sin_buf, const th_buffer* positions, size_t rot_dim,
                  int layout, th_buffer* q_out);
@@ -526,8 +528,8 @@ int th_kv_append(th_kv_batch* b, size_t layer, const th_buffer* q, const th_buff
  * the cache's type, more than 16 rows (new positions x query heads of a kv head) taken together, as in prompts and on shared
  * prefixes, have probabilities rounded to it, in the dividend and the divisor alike; all else keeps f32's precision or, for such types, 2^-18.  Sequences
  * of the batch that share (by th_kv_seq_fork) the pages of their first 128 positions at least are a group: the pages that all of a group have in
- * common from the start on are read once for it (a member that left early shortens them for the others; some thousand new
- * positions on shared pages at most).
+ * common from the start on are read once for it (a member that left early shortens them for the others; up to 3072 new
+ * positions of a batch, fewer where one's results take more than 128 KiB in f32; those beyond read their pages by themselves).
  * Captured (after the same call has been made once): buffers for max_rows rows, and
  * a replay runs on the batch as it last began. */
 int th_kv_batch_attention(th_kv_batch* b, size_t layer, const th_buffer* q, size_t window, size_t n_sinks, float scale,

@@ -704,7 +704,8 @@ class HipComputeDevice:
 
     def capture(self, fn):
         """Record the library calls fn() makes on this device's stream into a
-        Graph (th_capture_begin / th_capture_end)."""
+        Graph (th_capture_begin / th_capture_end). Python's cyclic collector is off,
+        for the whole process, until fn has returned."""
         collecting = gc.isenabled()
         gc.disable()  # a buffer that the collector frees in the middle would end the capture
         try:

@@ -528,7 +528,7 @@ int th_kv_append(th_kv_batch* b, size_t layer, const th_buffer* q, const th_buff
  * the cache's type, more than 16 rows (new positions x query heads of a kv head) taken together, as in prompts and on shared
  * prefixes, have probabilities rounded to it, in the dividend and the divisor alike; all else keeps f32's precision or, for such types, 2^-18.  Sequences
  * of the batch that share (by th_kv_seq_fork) the pages of their first 128 positions at least are a group: the pages that all of a group have in
- * common from the start on are read once for it (a member that left early shortens them for the others; up to 3072 new
+ * common from the start on are read once for it (a member that left early shortens them for the others; up to some 3000 new
  * positions of a batch, fewer where one's results take more than 128 KiB in f32; those beyond read their pages by themselves).
  * Captured (after the same call has been made once): buffers for max_rows rows, and
  * a replay runs on the batch as it last began. */

@@ -1,4 +1,5 @@
 """The paged cache's bookkeeping without a GPU: calls that find no memory leave everything as it was."""
+import ctypes
 import os
 
 import numpy as np
@@ -185,5 +186,41 @@ def test_scales_that_overflow(lib):
         with pytest.raises(Refused, match="scale"):
             c.call("th_kv_batch_attention", b, 0, q, 0, 0, scale, o)
     c.call("th_kv_batch_attention", b, 0, q, 0, 0, 2e38, o)
+    c.call("th_kv_batch_destroy", b)
+    c.close()
+
+
+def _fails_in_turn(lib, call, undo=lambda x: None):
+    """call() with each of its allocations failing in turn, until none does; how many there were."""
+    for fail in range(50):
+        lib.host_fail(fail)
+        try:
+            x = call()
+        except Refused as e:
+            assert e.code == capi.TH_ERR_OOM
+            continue
+        finally:
+            lib.host_fail(-1)
+        undo(x)
+        return fail
+    raise AssertionError("refused for good")
+
+
+def test_handles_plans_and_reads_that_find_no_memory(lib):
+    """The calls that change no sequence: refused, and the next one works."""
+    rng = np.random.default_rng(2)
+    c = Cache(lib, pages=4000, seqs=4, max_len=30000)
+    cfg = capi.KvCacheConfig(capi.F16, 1, 1, 8, 16, 10, 2, 100)
+    assert _fails_in_turn(lib, lambda: c.new("th_kv_cache_create", c.dev, ctypes.byref(cfg)), lambda h: c.call("th_kv_cache_destroy", h)) >= 10
+    assert _fails_in_turn(lib, lambda: c.batch(2, 100), lambda h: c.call("th_kv_batch_destroy", h)) == 3
+    b, s = c.batch(2, 20000), c.create()
+    c.grow(rng, b, [s], [20000])
+    assert _fails_in_turn(lib, lambda: c.attend(b, 20000)) >= 2  # the plan's block, its upload
+    assert _fails_in_turn(lib, lambda: c.attend(b, 20000, window=50)) >= 1
+    kid = c.fork(s, 1, 20000)[0]
+    c.select(s, np.arange(20000))  # (the child's table row goes up as entries now)
+    c.check()
+    c.fork(kid, 1, 20000)
+    c.check()
     c.call("th_kv_batch_destroy", b)
     c.close()

@@ -10,7 +10,7 @@
 // keys 4h .. 4h + 3 and 8 + 4h ..), so probabilities never leave their lane.
 //
 // Bound by the SIMDs' issue: the MFMAs' time and the softmax's vector instructions (four for a score, six with two parts) add up.
-// A prompt of 8192 (bf16, 32 heads of 128 on 8): 605 to 620 us by box, 890 to 910 TFLOP/s of what rows see, where a large matrix product
+// A prompt of 8192 (bf16, 32 heads of 128 on 8): 600 to 620 us by box, 890 to 915 TFLOP/s of what rows see, where a large matrix product
 // reaches 1231.  Eight waves in two phases, wave priorities, two chains of MFMAs and blocks of 32 keys
 // with three workgroups a CU gave nothing more.  f32 queries on an f16 cache take twice the MFMAs.
 #pragma once

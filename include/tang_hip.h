@@ -452,6 +452,18 @@ int th_rope_tables_scaled(size_t rot_dim, size_t max_seq, double base, const th_
 int th_rope_rows(th_device* dev, const th_buffer* in, const th_buffer* cos_buf, const th_buffer* sin_buf,
                  const th_buffer* positions, size_t start_pos, size_t n_rows, size_t n_heads, size_t head_dim,
                  size_t rot_dim, int layout, th_buffer* out);
+/* Norms of query and key heads, and their rotation, in one pass: each head h becomes
+ * h / sqrt(mean(h^2) + eps) * weight, then its pairs turn as th_rope_rows's (rot_dim 0: none do; tables
+ * may be NULL).  q [n_rows][n_heads][head_dim], k [n_rows][n_kv_heads][head_dim], of one type, f32, f16
+ * or bf16, computed in f32 (squares that leave f32's range in f64) and rounded once; weights [head_dim]
+ * f32 or bf16, NULL: ones.  q_stride, k_stride: elements from row to row, 0: none between them.
+ * k NULL: the keys follow the queries in q's rows (what follows the keys, as the values of
+ * a packed product, is left alone).  k_out NULL: they follow them in q_out's.  Each result may be its input (q_out q,
+ * k_out k), in place then; otherwise its rows have nothing between them. */
+int th_qk_norm_rope(th_device* dev, const th_buffer* q, size_t q_stride, const th_buffer* k, size_t k_stride,
+                    const th_buffer* q_weight, const th_buffer* k_weight, float eps, const th_buffer* cos_buf,
+                    const th_buffer* sin_buf, const th_buffer* positions, size_t start_pos, size_t n_rows, size_t n_heads,
+                    size_t n_kv_heads, size_t head_dim, size_t rot_dim, int layout, th_buffer* q_out, th_buffer* k_out);
 
 /* ---- paged key/value cache -----------------------------------------------------
  * For programs that serve several sequences at a time; no counterpart in the
@@ -521,6 +533,11 @@ int th_kv_batch_trim(th_kv_batch* b, const uint32_t* n_keep, size_t n);
 int th_kv_append(th_kv_batch* b, size_t layer, const th_buffer* q, const th_buffer* k, const th_buffer* v,
                  const th_buffer* cos_buf, const th_buffer* sin_buf, const th_buffer* positions, size_t rot_dim,
                  int layout, th_buffer* q_out);
+/* th_kv_append with the heads of q and k brought to their norm first, as in th_qk_norm_rope (v as it is).
+ * k and v NULL: q's rows hold all three, [rows][n_heads + 2 n_kv_heads][head_dim], and q_out is another buffer. */
+int th_kv_append_norm(th_kv_batch* b, size_t layer, const th_buffer* q, const th_buffer* k, const th_buffer* v,
+                      const th_buffer* q_weight, const th_buffer* k_weight, float eps, const th_buffer* cos_buf,
+                      const th_buffer* sin_buf, const th_buffer* positions, size_t rot_dim, int layout, th_buffer* q_out);
 /* Attention of the step's rows over the pages: the row at place p of its sequence
  * sees keys j <= p with window == 0, j > p - window or j < n_sinks.  q and out
  * [rows][n_heads][head_dim], each f32, f16 or bf16, query head h reads kv head

@@ -151,6 +151,8 @@ SIGNATURES = {
     "th_kv_batch_begin": ([_P, _P, _P, _S], _I),
     "th_kv_batch_trim": ([_P, _P, _S], _I),
     "th_kv_append": ([_P, _S, _P, _P, _P, _P, _P, _P, _S, _I, _P], _I),
+    "th_qk_norm_rope": ([_P, _P, _S, _P, _S, _P, _P, _F, _P, _P, _P, _S, _S, _S, _S, _S, _S, _I, _P, _P], _I),
+    "th_kv_append_norm": ([_P, _S, _P, _P, _P, _P, _P, _F, _P, _P, _P, _S, _I, _P], _I),
     "th_kv_batch_attention": ([_P, _S, _P, _S, _S, _F, _P], _I),
     "th_synth_seed": ([_U64, _U64, _U64], _U64),
     "th_synth_q4": ([_U64, _S, _S, _F, _F, _P, _P], _I),
@@ -615,6 +617,7 @@ class KvBatch:
         # a step is many short calls
         self._begin, self._trim, self._append, self._attention = (L.th_kv_batch_begin, L.th_kv_batch_trim, L.th_kv_append,
                                                                   L.th_kv_batch_attention)
+        self._append_norm = L.th_kv_append_norm
 
     def begin(self, seqs, n_new):
         s, n = array.array("i", seqs), array.array("I", n_new)
@@ -633,6 +636,14 @@ class KvBatch:
     def append(self, layer, q, k, v, q_out, cos_buf=None, sin_buf=None, rot_dim=0, layout=ROPE_INTERLEAVED, positions=None):
         rc = self._append(self.handle, layer, _handle(q), k.handle, v.handle, _handle(cos_buf), _handle(sin_buf), _handle(positions),
                           rot_dim, layout, _handle(q_out))
+        if rc:
+            check(rc)
+
+    def append_norm(self, layer, q, k, v, q_out, q_weight, k_weight, eps, cos_buf=None, sin_buf=None, rot_dim=0, layout=ROPE_INTERLEAVED,
+                    positions=None):
+        """append() of heads brought to their norm first; k and v None: q holds packed rows of all three (th_kv_append_norm)."""
+        rc = self._append_norm(self.handle, layer, _handle(q), _handle(k), _handle(v), _handle(q_weight), _handle(k_weight), eps, _handle(cos_buf),
+                               _handle(sin_buf), _handle(positions), rot_dim, layout, _handle(q_out))
         if rc:
             check(rc)
 
@@ -798,6 +809,19 @@ class HipComputeDevice:
         h = [b.handle if b is not None else None for b in (x, cos_buf, sin_buf, positions)]
         check(lib().th_rope_rows(self.handle, *h, start_pos, n_rows, n_heads, head_dim, rot_dim, layout, out.handle))
         return out
+
+    def qk_norm_rope(self, q, k, q_weight, k_weight, eps, cos_buf, sin_buf, n_rows, n_heads, n_kv_heads, head_dim, rot_dim,
+                     layout=ROPE_INTERLEAVED, start_pos=0, positions=None, q_stride=0, k_stride=0, q_out=None, k_out=None):
+        """Norms of query and key heads with their rotation (th_qk_norm_rope). k None: the keys follow the queries in q's rows.
+        Without q_out, both results are new buffers; with q_out and without k_out, the keys follow the queries in q_out's rows."""
+        if q_out is None:
+            q_out = self.alloc(n_rows * n_heads * head_dim, q.dtype)
+            if k_out is None and n_kv_heads:
+                k_out = self.alloc(n_rows * n_kv_heads * head_dim, q.dtype)
+        check(lib().th_qk_norm_rope(self.handle, q.handle, q_stride, _handle(k), k_stride, _handle(q_weight), _handle(k_weight), eps,
+                                    _handle(cos_buf), _handle(sin_buf), _handle(positions), start_pos, n_rows, n_heads, n_kv_heads, head_dim,
+                                    rot_dim, layout, q_out.handle, _handle(k_out)))
+        return q_out, k_out
 
     def kv_cache(self, n_layers, n_kv_heads, head_dim, page_size, n_pages, max_seqs, max_len, dtype=F16):
         return KvCache(self, n_layers, n_kv_heads, head_dim, page_size, n_pages, max_seqs, max_len, dtype)

@@ -704,6 +704,28 @@ static void rope_args(KvRopeArgs& a, const th_device* dev, const th_buffer* cos_
     TH_REQUIRE(a.table_rows > 0 || rows == 0, "empty tables");
 }
 
+// Weights of the heads' norms, checked (null: ones).  hd: dims of a head.
+static void norm_args(KvRopeArgs& a, const th_device* dev, const th_buffer* qw, const th_buffer* kw, float eps, size_t hd) {
+    TH_REQUIRE(std::isfinite(eps) && eps >= 0.0f, "eps must be finite and not negative");
+    for (const th_buffer* w : {qw, kw}) {
+        if (!w) continue;
+        require_len_any(w, hd, "weight");
+        TH_REQUIRE(w->dtype == TH_F32 || w->dtype == TH_BF16, "weights must be f32 or bf16");
+        TH_REQUIRE(w->dev == dev, "a weight is on another device handle");
+    }
+    a.norm = true;
+    a.eps = eps;
+    a.qw = qw ? qw->ptr : nullptr;
+    a.kw = kw ? kw->ptr : nullptr;
+    a.qw_bf16 = qw && qw->dtype == TH_BF16;
+    a.kw_bf16 = kw && kw->dtype == TH_BF16;
+}
+// What a launch writes must not be what its other threads read.
+static void require_apart(const th_buffer* out, std::initializer_list<const th_buffer*> in, const char* what) {
+    for (const th_buffer* b : in)
+        if (b && b == out) throw Error(TH_ERR_INVALID, std::string("buffer ") + what + " is also an input that others read");
+}
+
 }  // namespace th
 
 using namespace th;
@@ -1208,6 +1230,54 @@ int th_kv_append(th_kv_batch* b, size_t layer, const th_buffer* q, const th_buff
     TH_API_END
 }
 
+int th_kv_append_norm(th_kv_batch* b, size_t layer, const th_buffer* q, const th_buffer* k, const th_buffer* v,
+                      const th_buffer* q_weight, const th_buffer* k_weight, float eps, const th_buffer* cos_t,
+                      const th_buffer* sin_t, const th_buffer* positions, size_t rot_dim, int layout, th_buffer* q_out) {
+    TH_API_BEGIN
+    require_begun(b, layer, __func__);
+    th_kv_cache* c = b->cache;
+    TH_REQUIRE((k == nullptr) == (v == nullptr), "k and v go together");
+    TH_REQUIRE((q == nullptr) == (q_out == nullptr), "q and q_out go together");
+    TH_REQUIRE(q || k, "null argument");
+    DeviceScope scope(c->dev);
+    // a captured call runs on whatever the batch begins with later
+    const size_t rows = c->dev->capturing ? b->max_rows : b->step.rows;
+    const size_t kv = c->n_kv_heads * c->hd, qn = b->n_heads * c->hd;
+    KvRopeArgs a = {};
+    if (k) {
+        require_x(c, k, rows * kv, "k");
+        require_x(c, v, rows * kv, "v");
+        TH_REQUIRE(k->dtype == v->dtype && (!q || q->dtype == k->dtype), "q, k and v must be of one type");
+        a.q = q ? q->ptr : nullptr;
+        a.k = k->ptr;
+        a.v = v->ptr;
+        a.q_row = qn;
+        a.k_row = a.v_row = kv;
+        a.xdt = k->dtype;
+    } else {  // one row holds all three
+        a.q = q->ptr;
+        a.k = (const char*)q->ptr + qn * dtype_size(q->dtype);
+        a.v = (const char*)a.k + kv * dtype_size(q->dtype);
+        a.q_row = a.k_row = a.v_row = qn + 2 * kv;
+        a.xdt = q->dtype;
+    }
+    if (q) {
+        require_x(c, q, rows * a.q_row, "q");
+        require_x(c, q_out, rows * qn, "q_out");
+        TH_REQUIRE(k || q_out != q, "q_out must not be the packed rows");
+        require_apart(q_out, {k, v, q_weight, k_weight, positions}, "q_out");
+    }
+    rope_args(a, c->dev, cos_t, sin_t, positions, rows, c->hd, rot_dim, layout, b->step.top, q_out);
+    norm_args(a, c->dev, q_weight, k_weight, eps, c->hd);
+    a.q_out = q_out ? q_out->ptr : nullptr;
+    a.qdt = q_out ? q_out->dtype : TH_F32;
+    a.qo_row = qn;
+    a.n_heads = q ? (int)b->n_heads : 0;
+    a.hd = (int)c->hd;
+    launch_kv_append(a, layer_pages(c, layer), c->dtype, b->block, (const KvRow*)(b->block + 4), rows, c->dev->stream);
+    TH_API_END
+}
+
 int th_kv_batch_attention(th_kv_batch* b, size_t layer, const th_buffer* q, size_t window, size_t n_sinks, float scale, th_buffer* out) {
     TH_API_BEGIN
     require_begun(b, layer, __func__);
@@ -1349,6 +1419,60 @@ int th_rope_rows(th_device* dev, const th_buffer* in, const th_buffer* cos_t, co
     a.qdt = out->dtype;
     a.start = start_pos;
     a.n_heads = (int)n_heads;
+    a.hd = (int)head_dim;
+    DeviceScope scope(dev);
+    launch_rope_rows(a, n_rows, dev->stream);
+    TH_API_END
+}
+
+int th_qk_norm_rope(th_device* dev, const th_buffer* q, size_t q_stride, const th_buffer* k, size_t k_stride, const th_buffer* q_weight,
+                    const th_buffer* k_weight, float eps, const th_buffer* cos_t, const th_buffer* sin_t, const th_buffer* positions,
+                    size_t start_pos, size_t n_rows, size_t n_heads, size_t n_kv_heads, size_t head_dim, size_t rot_dim, int layout,
+                    th_buffer* q_out, th_buffer* k_out) {
+    TH_API_BEGIN
+    TH_REQUIRE(dev && q && q_out, "null argument");
+    TH_REQUIRE(!dev->closed, "the device was destroyed");
+    auto ok = [&](const th_buffer* b) { return !b || ((b->dtype == TH_F32 || b->dtype == TH_F16 || b->dtype == TH_BF16) && b->dev == dev); };
+    TH_REQUIRE(ok(q) && ok(k) && ok(q_out) && ok(k_out), "buffers must be f32, f16 or bf16, of this device handle");
+    TH_REQUIRE(!k || k->dtype == q->dtype, "q and k must be of one type");
+    TH_REQUIRE(n_kv_heads > 0 || (!k && !k_out), "keys without key heads");
+    TH_REQUIRE(n_heads > 0 && head_dim > 0, "no queries");
+    constexpr size_t HEADS = (size_t)1 << 16, WIDE = (size_t)1 << 32;
+    TH_REQUIRE(n_heads <= HEADS && n_kv_heads <= HEADS && head_dim <= HEADS && n_rows < (size_t)1 << 31, "sizes out of range");
+    TH_REQUIRE(q_stride < WIDE && k_stride < WIDE, "strides out of range");
+    TH_REQUIRE(n_rows == 0 || start_pos <= SIZE_MAX - n_rows, "sizes out of range");
+    const size_t qn = n_heads * head_dim, kn = n_kv_heads * head_dim;
+    const size_t q_in = k ? qn : qn + kn, q_to = k_out ? qn : qn + kn;  // keys behind the queries in a row
+    // the last row ends with its heads
+    auto reach = [&](size_t row, size_t width) { return n_rows ? (n_rows - 1) * row + width : 0; };
+    KvRopeArgs a = {};
+    a.q_row = q_stride ? q_stride : q_in;
+    a.k_row = k ? (k_stride ? k_stride : kn) : a.q_row;
+    TH_REQUIRE(a.q_row >= q_in && a.k_row >= kn, "a stride shorter than its row");
+    TH_REQUIRE(k || k_stride == 0, "a stride of no keys");
+    a.qo_row = q_out == q ? a.q_row : q_to;
+    a.ko_row = !k_out ? a.qo_row : k_out == k ? a.k_row : kn;
+    TH_REQUIRE(a.qo_row >= q_to, "no room for the keys behind the queries");
+    require_len_any(q, reach(a.q_row, q_in), "q");
+    require_len_any(q_out, reach(a.qo_row, q_to), "q_out");
+    if (k) require_len_any(k, reach(a.k_row, kn), "k");
+    if (k_out) require_len_any(k_out, reach(a.ko_row, kn), "k_out");
+    TH_REQUIRE(k != q && q_out != k_out, "queries and keys must be buffers of their own");
+    require_apart(q_out, {k, q_weight, k_weight, positions}, "q_out");
+    if (k_out) require_apart(k_out, {q, q_weight, k_weight, positions}, "k_out");
+    rope_args(a, dev, cos_t, sin_t, positions, n_rows, head_dim, rot_dim, layout, start_pos + n_rows, q_out);
+    TH_REQUIRE(!k_out || (k_out != cos_t && k_out != sin_t), "the result must not be a table");
+    norm_args(a, dev, q_weight, k_weight, eps, head_dim);
+    a.q = q->ptr;
+    a.k = k ? k->ptr : (const char*)q->ptr + qn * dtype_size(q->dtype);
+    a.q_out = q_out->ptr;
+    a.k_out = k_out ? k_out->ptr : (char*)q_out->ptr + qn * dtype_size(q_out->dtype);
+    a.xdt = q->dtype;
+    a.qdt = q_out->dtype;
+    a.kdt = k_out ? k_out->dtype : q_out->dtype;
+    a.start = start_pos;
+    a.n_heads = (int)n_heads;
+    a.n_kv = (int)n_kv_heads;
     a.hd = (int)head_dim;
     DeviceScope scope(dev);
     launch_rope_rows(a, n_rows, dev->stream);

@@ -105,11 +105,24 @@ struct KvRopeArgs {
     const uint32_t* positions;   // of each row, or null: the row's place in its sequence (or start + row)
     size_t table_rows, start;
     int n_heads, hd, rot, half;  // half: pairs (i, i + rot/2), else (2i, 2i+1)
+    // Norms of the heads before they turn (kvnorm.hip); without `norm` none of the rest is read.
+    bool norm;
+    float eps;
+    const void *qw, *kw;         // [hd], null: ones
+    int qw_bf16, kw_bf16;        // else f32
+    int n_kv;                    // key heads of rows that go to k_out
+    void* k_out;
+    th_dtype kdt;
+    size_t q_row, k_row, v_row, qo_row, ko_row;  // elements from row to row
 };
-// q_out = turned q.  n_rows_dev (device) bounds the rows of a batch, n_rows the grid.
+// q_out = turned q.  n_rows_dev (device) bounds the rows of a batch, n_rows the grid.  Both go to
+// kvnorm.hip where norms are asked for.
 void launch_kv_append(const KvRopeArgs& a, const KvPages& p, th_dtype cache, const int* n_rows_dev, const KvRow* rows,
                       size_t n_rows, hipStream_t s);
 void launch_rope_rows(const KvRopeArgs& a, size_t n_rows, hipStream_t s);
+void launch_norm_append(const KvRopeArgs& a, const KvPages& p, th_dtype cache, const int* n_rows_dev, const KvRow* rows,
+                        size_t n_rows, hipStream_t s);
+void launch_norm_rows(const KvRopeArgs& a, size_t n_rows, hipStream_t s);
 
 // grid: how many items the launch covers at a time (the kernels walk the rest; a launch has below 2^32 threads).
 // flags: of the plan, or KV_BY_PLAN for a call that is captured.

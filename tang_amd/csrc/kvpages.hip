@@ -3,6 +3,7 @@
 #include <algorithm>
 
 #include "kvcache.hpp"
+#include "kvrows.hpp"
 #include "ops.hpp"
 
 namespace th {
@@ -176,49 +177,6 @@ void launch_kv_read(const KvPages& p, int seq, size_t from, size_t n, size_t row
 // memory: q, k and v are read once and written once, in one launch; the tables'
 // rows are shared by a token's heads and stay in the caches.  16000 f32 tokens of 32 + 8 + 8 heads of 128
 // into an f16 cache: 167 us, 4.4 TB/s.  One token: a launch.
-struct kv_f8 { float v[8]; };
-
-template <typename X>
-__device__ __forceinline__ kv_f8 kv_load8(const X* p) {
-    kv_f8 r;
-    if constexpr (sizeof(X) == 4) {
-        const float4 a = ((const float4*)p)[0], b = ((const float4*)p)[1];
-        r = kv_f8{{a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w}};
-    } else {
-        typedef X x8 __attribute__((ext_vector_type(8)));
-        const x8 a = *(const x8*)p;
-#pragma unroll
-        for (int i = 0; i < 8; i++) r.v[i] = (float)a[i];
-    }
-    return r;
-}
-
-template <typename Y>
-__device__ __forceinline__ void kv_put8(Y* p, const kv_f8& r) {
-    if constexpr (sizeof(Y) == 4) {
-        ((float4*)p)[0] = make_float4(r.v[0], r.v[1], r.v[2], r.v[3]);
-        ((float4*)p)[1] = make_float4(r.v[4], r.v[5], r.v[6], r.v[7]);
-    } else {
-        typedef Y y8 __attribute__((ext_vector_type(8)));
-        y8 a;
-#pragma unroll
-        for (int i = 0; i < 8; i++) a[i] = (Y)r.v[i];
-        *(y8*)p = a;
-    }
-}
-
-__device__ __forceinline__ void kv_store8(void* base, th_dtype dt, size_t at, const kv_f8& r) {
-    if (dt == TH_F32) kv_put8((float*)base + at, r);
-    else if (dt == TH_F16) kv_put8((_Float16*)base + at, r);
-    else kv_put8((__bf16*)base + at, r);
-}
-
-__device__ __forceinline__ void kv_store1(void* base, th_dtype dt, size_t at, float v) {
-    if (dt == TH_F32) ((float*)base)[at] = v;
-    else if (dt == TH_F16) ((_Float16*)base)[at] = (_Float16)v;
-    else ((__bf16*)base)[at] = (__bf16)v;
-}
-
 // One head of one row: thread c of `lanes` takes its chunks.  VEC: rot is a
 // multiple of 16, so that chunks of eight never straddle halves or the rest.
 template <typename X, bool VEC>
@@ -326,6 +284,7 @@ static void rope_types(const KvRopeArgs& a, F&& f) {
 void launch_kv_append(const KvRopeArgs& a, const KvPages& p, th_dtype cache, const int* n_rows_dev, const KvRow* rows,
                       size_t n_rows, hipStream_t s) {
     if (n_rows == 0) return;
+    if (a.norm) return launch_norm_append(a, p, cache, n_rows_dev, rows, n_rows, s);
     const unsigned grid = rope_grid(n_rows * (a.n_heads + 2 * p.n_kv_heads) * (a.hd / 8));
     rope_types(a, [&](auto x, auto vec) {
         TH_LAUNCH((kv_append_kernel<decltype(x), decltype(vec)::value>), dim3(grid), dim3(256), 0, s, a, p, cache, n_rows_dev, rows);
@@ -334,6 +293,7 @@ void launch_kv_append(const KvRopeArgs& a, const KvPages& p, th_dtype cache, con
 }
 
 void launch_rope_rows(const KvRopeArgs& a, size_t n_rows, hipStream_t s) {
+    if (a.norm) return launch_norm_rows(a, n_rows, s);
     const size_t threads = n_rows * a.n_heads * ((a.hd + 7) / 8);
     if (threads == 0) return;
     rope_types(a, [&](auto x, auto vec) {

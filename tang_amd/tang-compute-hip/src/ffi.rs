@@ -271,6 +271,7 @@ extern "C" {
     pub fn th_buffer_ptr(buf: *const th_buffer, ptr: *mut *mut c_void) -> c_int;
     pub fn th_rope_tables_scaled(rot_dim: usize, max_seq: usize, base: f64, s: *const th_rope_scaling, cos_table: *mut f32, sin_table: *mut f32) -> c_int;
     pub fn th_rope_rows(dev: *mut th_device, in_: *const th_buffer, cos_buf: *const th_buffer, sin_buf: *const th_buffer, positions: *const th_buffer, start_pos: usize, n_rows: usize, n_heads: usize, head_dim: usize, rot_dim: usize, layout: c_int, out: *mut th_buffer) -> c_int;
+    pub fn th_qk_norm_rope(dev: *mut th_device, q: *const th_buffer, q_stride: usize, k: *const th_buffer, k_stride: usize, q_weight: *const th_buffer, k_weight: *const th_buffer, eps: f32, cos_buf: *const th_buffer, sin_buf: *const th_buffer, positions: *const th_buffer, start_pos: usize, n_rows: usize, n_heads: usize, n_kv_heads: usize, head_dim: usize, rot_dim: usize, layout: c_int, q_out: *mut th_buffer, k_out: *mut th_buffer) -> c_int;
     pub fn th_kv_cache_create(dev: *mut th_device, cfg: *const th_kv_cache_config, out: *mut *mut th_kv_cache) -> c_int;
     pub fn th_kv_cache_destroy(c: *mut th_kv_cache) -> c_int;
     pub fn th_kv_cache_info(c: *const th_kv_cache, pages_vacant: *mut usize, seqs_vacant: *mut usize) -> c_int;
@@ -288,6 +289,7 @@ extern "C" {
     pub fn th_kv_batch_begin(b: *mut th_kv_batch, seqs: *const i32, n_new: *const u32, n: usize) -> c_int;
     pub fn th_kv_batch_trim(b: *mut th_kv_batch, n_keep: *const u32, n: usize) -> c_int;
     pub fn th_kv_append(b: *mut th_kv_batch, layer: usize, q: *const th_buffer, k: *const th_buffer, v: *const th_buffer, cos_buf: *const th_buffer, sin_buf: *const th_buffer, positions: *const th_buffer, rot_dim: usize, layout: c_int, q_out: *mut th_buffer) -> c_int;
+    pub fn th_kv_append_norm(b: *mut th_kv_batch, layer: usize, q: *const th_buffer, k: *const th_buffer, v: *const th_buffer, q_weight: *const th_buffer, k_weight: *const th_buffer, eps: f32, cos_buf: *const th_buffer, sin_buf: *const th_buffer, positions: *const th_buffer, rot_dim: usize, layout: c_int, q_out: *mut th_buffer) -> c_int;
     pub fn th_kv_batch_attention(b: *mut th_kv_batch, layer: usize, q: *const th_buffer, window: usize, n_sinks: usize, scale: f32, out: *mut th_buffer) -> c_int;
     pub fn th_synth_seed(base: u64, layer: u64, tensor: u64) -> u64;
     pub fn th_synth_q4(seed: u64, rows: usize, cols: usize, smin: f32, smax: f32, nib: *mut u8, scales_f16: *mut u16) -> c_int;

@@ -174,6 +174,24 @@ int th_st_upload_q8(th_device* dev, const th_st_file* f, const char* name, th_qw
 int th_gemm_q4(th_device* dev, const th_buffer* x, size_t m, const th_qweight* w, th_buffer* y);
 int th_gemv_q8(th_device* dev, const th_buffer* x, size_t m, const th_qweight* w, th_buffer* y);
 
+/* The same product in 8-bit integers (no counterpart in the reference): activations are brought to
+ * int8 with a scale for each row, and multiplied with q8 weights that have one scale a row
+ * (th_q8_upload_rowwise, th_q8_pack_rows) on the i8 MFMA, at twice bf16's rate.
+ *
+ * x [m][k], f32, f16 or bf16 -> q int8 [m][kp], kp = k rounded up to 64 (zeros behind k), and scale [m]:
+ * scale_i = f32(max |x_i| / 127), q = x / scale to the nearest integer, ties to even, at most 127 in size.  A
+ * row of zeros has scale 0; one with an infinity or NaN has scale NaN and zeros (its products are NaN).  k below 2^17. */
+int th_quantize_rows(th_device* dev, const th_buffer* x, size_t m, size_t k, th_buffer* q, th_buffer* scale);
+/* A q8 weight with one scale a row from rows on the device: q int8 [rows][kp] and scale [rows] as
+ * th_quantize_rows gives them (there of a weight matrix [rows][cols]). */
+int th_q8_pack_rows(th_device* dev, const th_buffer* q, const th_buffer* scale, size_t rows, size_t cols, th_qweight** out);
+/* y[m][n] = (sum_k q[m][k] w[n][k]) x_scale[m] w_scale[n] + bias[n].  xq int8 [m][kp] (what
+ * lies behind k is not looked at), bias f32 [n] or NULL; y f32, f16 or bf16.  Sums are exact (int32), the
+ * products with the scales and the bias in f64, rounded to f32 and then to y's type.  Weights of
+ * fewer than 2^17 columns; those with a scale for each group of 32 are TH_ERR_UNSUPPORTED. */
+int th_gemm_i8(th_device* dev, const th_buffer* xq, const th_buffer* x_scale, size_t m, const th_qweight* w,
+               const th_buffer* bias, th_buffer* y);
+
 /* Allocation-free form of th_gemm_q4 (no counterpart in the reference): for
  * callers that cannot allocate device memory (code under HIP graph capture,
  * tight serving loops, harnesses that forbid hipMalloc).  Same arguments,

@@ -78,6 +78,9 @@ SIGNATURES = {
     "th_gemm_q4": ([_P, _P, _S, _P, _P], _I),
     "th_gemv_q8": ([_P, _P, _S, _P, _P], _I),
     "th_gemm_q4_noalloc": ([_P, _P, _S, _P, _P], _I),
+    "th_quantize_rows": ([_P, _P, _S, _S, _P, _P], _I),
+    "th_q8_pack_rows": ([_P, _P, _P, _S, _S, _P], _I),
+    "th_gemm_i8": ([_P, _P, _P, _S, _P, _P, _P], _I),
     "th_bench_linear": ([_P, _P, _S, _P, _S, _P, _S, _I, _P], _I),
     "th_rms_norm": ([_P, _P, _P, _S, _S, _F, _P], _I),
     "th_rms_norm_residual": ([_P, _P, _P, _P, _S, _S, _F, _P, _P], _I),
@@ -771,6 +774,25 @@ class HipComputeDevice:
     def gemv_q8(self, x, m, w, y=None):
         y = y or self.alloc(m * w.rows)
         check(lib().th_gemv_q8(self.handle, x.handle, m, w.handle, y.handle))
+        return y
+
+    def quantize_rows(self, x, m, k, q=None, scale=None):
+        """Rows to int8 with a scale each (th_quantize_rows): q [m][k rounded up to 64] and scale [m]."""
+        q = q or self.alloc(m * (-(-k // 64) * 64), I8)
+        scale = scale or self.alloc(m)
+        check(lib().th_quantize_rows(self.handle, x.handle, m, k, q.handle, scale.handle))
+        return q, scale
+
+    def q8_pack_rows(self, q, scale, rows, cols):
+        """A weight from quantize_rows' results of its matrix [rows][cols]."""
+        h = ctypes.c_void_p()
+        check(lib().th_q8_pack_rows(self.handle, q.handle, scale.handle, rows, cols, ctypes.byref(h)))
+        return QWeight(h, rows, cols, 8)
+
+    def gemm_i8(self, q, scale, m, w, y=None, bias=None):
+        """Product of quantized rows with a q8 weight that has one scale a row (th_gemm_i8)."""
+        y = y or self.alloc(m * w.rows)
+        check(lib().th_gemm_i8(self.handle, q.handle, scale.handle, m, w.handle, _handle(bias), y.handle))
         return y
 
     def bench_linear(self, x, m, weights, y, iters, use_graph=False):

@@ -1,0 +1,89 @@
+// The 8-bit products' entry points: checks of arguments (i8gemm.hpp).
+#include "capi_util.hpp"
+#include "i8gemm.hpp"
+#include "kvcache.hpp"
+
+using namespace th;
+
+extern "C" {
+
+int th_quantize_rows(th_device* dev, const th_buffer* x, size_t m, size_t k, th_buffer* q, th_buffer* scale) {
+    TH_API_BEGIN
+    TH_REQUIRE(dev && x && q && scale, "null argument");
+    TH_REQUIRE(!dev->closed, "the device was destroyed");
+    TH_REQUIRE(x->dev == dev && q->dev == dev && scale->dev == dev, "a buffer is on another device handle");
+    TH_REQUIRE(x->dtype == TH_F32 || x->dtype == TH_F16 || x->dtype == TH_BF16, "x must be f32, f16 or bf16");
+    TH_REQUIRE(k > 0 && k <= I8_MAX_K, "k must be from 1 to 2^17 - 1");
+    TH_REQUIRE(m < (size_t)1 << 31, "too many rows");
+    const size_t kp = round_up(k, 64);
+    require_len_any(x, m * k, "x");
+    require_len(q, TH_I8, m * kp, "q");
+    require_len(scale, TH_F32, m, "scale");
+    TH_REQUIRE(scale != x, "scale must not be x");
+    DeviceScope scope(dev);
+    launch_quantize_rows(x->ptr, x->dtype, m, k, (int8_t*)q->ptr, (float*)scale->ptr, dev->stream);
+    TH_API_END
+}
+
+int th_q8_pack_rows(th_device* dev, const th_buffer* q, const th_buffer* scale, size_t rows, size_t cols, th_qweight** out) {
+    TH_API_BEGIN
+    TH_REQUIRE(dev && q && scale && out, "null argument");
+    TH_REQUIRE(!dev->closed, "the device was destroyed");
+    TH_REQUIRE(q->dev == dev && scale->dev == dev, "a buffer is on another device handle");
+    TH_REQUIRE(rows > 0 && cols > 0, "empty matrix");
+    TH_REQUIRE(rows < (size_t)1 << 27 && cols <= I8_MAX_K, "sizes out of range");
+    TH_REQUIRE(!dev->capturing, "packs a new weight: not while a graph is captured");
+    const size_t Np = round_up(rows, 16), Kp = round_up(cols, 64);
+    require_len(q, TH_I8, rows * Kp, "q");
+    require_len(scale, TH_F32, rows, "scale");
+    DeviceScope scope(dev);
+    th_qweight* w = new th_qweight();
+    w->dev = dev;
+    w->bits = 8;
+    w->rows = rows;
+    w->cols = cols;
+    w->Np = Np;
+    w->Kp = Kp;
+    w->scale_dtype = TH_F32;
+    w->per_row = true;
+    w->data_bytes = Np * Kp;
+    w->scale_bytes = Np * 4;
+    try {
+        TH_HIP(hipMalloc(&w->data, w->data_bytes));
+        TH_HIP(hipMalloc(&w->scales, w->scale_bytes));
+        launch_q8_pack((const int8_t*)q->ptr, (const float*)scale->ptr, w, dev->stream);
+    } catch (...) {
+        (void)hipStreamSynchronize(dev->stream);
+        if (w->data) (void)hipFree(w->data);
+        if (w->scales) (void)hipFree(w->scales);
+        delete w;
+        throw;
+    }
+    device_retain(dev);
+    *out = w;
+    TH_API_END
+}
+
+int th_gemm_i8(th_device* dev, const th_buffer* xq, const th_buffer* x_scale, size_t m, const th_qweight* w, const th_buffer* bias, th_buffer* y) {
+    TH_API_BEGIN
+    TH_REQUIRE(dev && xq && x_scale && w && y, "null argument");
+    TH_REQUIRE(!dev->closed, "the device was destroyed");
+    TH_REQUIRE(xq->dev == dev && x_scale->dev == dev && w->dev == dev && y->dev == dev && (!bias || bias->dev == dev),
+               "a buffer or the weight is on another device handle");
+    TH_REQUIRE(w->bits == 8, "weight is not q8");
+    if (!w->per_row) throw Error(TH_ERR_UNSUPPORTED, "th_gemm_i8: the weight has a scale for each group of 32 (th_gemv_q8 takes those): needs one a row");
+    TH_REQUIRE(w->cols <= I8_MAX_K, "sums of 2^17 products and more leave 32 bits");
+    TH_REQUIRE(y->dtype == TH_F32 || y->dtype == TH_F16 || y->dtype == TH_BF16, "y must be f32, f16 or bf16");
+    TH_REQUIRE(m < (size_t)1 << 31 && w->rows < (size_t)1 << 31, "sizes out of range");
+    require_len(xq, TH_I8, m * w->Kp, "xq");
+    require_len(x_scale, TH_F32, m, "x_scale");
+    if (bias) require_len(bias, TH_F32, w->rows, "bias");
+    require_len_any(y, m * w->rows, "y");
+    TH_REQUIRE(y != x_scale && y != bias, "y must not be an input");
+    DeviceScope scope(dev);
+    const I8Out out{y->ptr, (const float*)x_scale->ptr, (const float*)w->scales, bias ? (const float*)bias->ptr : nullptr, y->dtype, (int)w->rows};
+    launch_i8_linear(dev, w, (const int8_t*)xq->ptr, out, m);
+    TH_API_END
+}
+
+}  // extern "C"

@@ -1,0 +1,31 @@
+// Products of 8-bit integers with a scale for each token and each channel.
+//
+//   s_i = f32(max_k |x_ik| / 127), q_ik = x_ik / s_i to the nearest integer (ties to even)
+//   y_ij = (sum_k q_ik w_jk) s_i t_j + b_j
+//
+// Rows of q are Kp = K rounded up to 64 bytes long; w are the q8 weights with one
+// scale a row (th_qweight in common.hpp), whose tiles of 16 rows x 64 k are, lane
+// by lane, an operand of the 16x16x64 i8 MFMA.  What lies behind K meets zero weights.
+#pragma once
+
+#include "common.hpp"
+
+namespace th {
+
+// Sums of K products of two int8 (at most 2^14 each) stay in 32 bits below this.
+constexpr size_t I8_MAX_K = ((size_t)1 << 17) - 1;
+
+// Where results go: (sum s_i) t_j + b_j in f64, so that no order of the scales
+// leaves f32's range on the way, rounded to f32 and then to the output's type.
+struct I8Out {
+    void* y;
+    const float *xs, *ws, *bias;  // [M], [N], [N] or null
+    th_dtype dt;                  // of y
+    int N;
+};
+
+void launch_quantize_rows(const void* x, th_dtype xdt, size_t m, size_t K, int8_t* q, float* scale, hipStream_t s);
+void launch_q8_pack(const int8_t* q, const float* scale, const th_qweight* w, hipStream_t s);
+void launch_i8_linear(th_device* dev, const th_qweight* w, const int8_t* xq, const I8Out& out, size_t m);
+
+}  // namespace th

@@ -223,6 +223,9 @@ extern "C" {
     pub fn th_st_upload_q8(dev: *mut th_device, f: *const th_st_file, name: *const c_char, out: *mut *mut th_qweight) -> c_int;
     pub fn th_gemm_q4(dev: *mut th_device, x: *const th_buffer, m: usize, w: *const th_qweight, y: *mut th_buffer) -> c_int;
     pub fn th_gemv_q8(dev: *mut th_device, x: *const th_buffer, m: usize, w: *const th_qweight, y: *mut th_buffer) -> c_int;
+    pub fn th_quantize_rows(dev: *mut th_device, x: *const th_buffer, m: usize, k: usize, q: *mut th_buffer, scale: *mut th_buffer) -> c_int;
+    pub fn th_q8_pack_rows(dev: *mut th_device, q: *const th_buffer, scale: *const th_buffer, rows: usize, cols: usize, out: *mut *mut th_qweight) -> c_int;
+    pub fn th_gemm_i8(dev: *mut th_device, xq: *const th_buffer, x_scale: *const th_buffer, m: usize, w: *const th_qweight, bias: *const th_buffer, y: *mut th_buffer) -> c_int;
     pub fn th_gemm_q4_noalloc(dev: *mut th_device, x: *const th_buffer, m: usize, w: *const th_qweight, y: *mut th_buffer) -> c_int;
     pub fn th_bench_linear(dev: *mut th_device, x: *const th_buffer, m: usize, ws: *const *mut th_qweight, n_w: usize, y: *mut th_buffer, iters: usize, use_graph: c_int, ms: *mut f32) -> c_int;
     pub fn th_matmul_ex(dev: *mut th_device, a: *const th_buffer, b: *const th_buffer, m: usize, k: usize, n: usize, trans_a: c_int, trans_b: c_int, accumulate: c_int, c: *mut th_buffer) -> c_int;

@@ -1,0 +1,92 @@
+"""What the 8-bit products' calls refuse, on the host (no GPU)."""
+import ctypes
+import os
+
+import pytest
+
+from host_operators import CLANG, Cache, Refusals, Refused, build
+from tang_amd import capi
+
+pytestmark = pytest.mark.skipif(not os.path.exists(CLANG), reason="needs ROCm's clang++")
+
+F32, F16, I8, U8 = capi.F32, capi.F16, capi.I8, capi.U8
+
+
+@pytest.fixture(scope="module")
+def lib(tmp_path_factory):
+    return build(tmp_path_factory.mktemp("host"))
+
+
+def test_quantize_rows(lib):
+    c, other = Cache(lib), Cache(lib)
+    f = Refusals(c, "th_quantize_rows", dev=c.dev, x=c.buffer(3 * 65, F32), m=3, k=65, q=c.buffer(3 * 128, I8), scale=c.buffer(3, F32))
+    f.call()
+    f.call(m=0)
+    f.call(x=c.buffer(3 * 65, F16))
+    for name in ("dev", "x", "q", "scale"):
+        f.refused("null", **{name: None})
+    f.refused("f32, f16 or bf16", x=c.buffer(3 * 65, I8))
+    f.refused("k must", k=0)
+    f.refused("k must", k=1 << 17)
+    f.refused("too many rows", m=1 << 31)
+    f.refused("buffer x .*too small", x=c.buffer(3 * 65 - 1, F32))
+    f.refused("buffer q .*too small", q=c.buffer(3 * 128 - 1, I8))
+    f.refused("dtype", q=c.buffer(3 * 128, U8))
+    f.refused("dtype", scale=c.buffer(3, F16))
+    f.refused("buffer scale .*too small", scale=c.buffer(2, F32))
+    for name, n, dt in (("x", 195, F32), ("q", 384, I8), ("scale", 3, F32)):
+        f.refused("another device", **{name: other.buffer(n, dt)})
+    x = c.buffer(195, F32)
+    f.refused("must not be x", x=x, scale=x)
+
+
+def test_pack_and_product(lib):
+    c, other = Cache(lib), Cache(lib)
+    q, s = c.buffer(20 * 128, I8), c.buffer(20, F32)
+    out = ctypes.c_void_p()
+    f = Refusals(c, "th_q8_pack_rows", dev=c.dev, q=q, scale=s, rows=20, cols=70, out=ctypes.byref(out))
+    f.call()
+    w = ctypes.c_void_p(out.value)
+    for name in ("dev", "q", "scale", "out"):
+        f.refused("null", **{name: None})
+    f.refused("empty", rows=0)
+    f.refused("empty", cols=0)
+    f.refused("out of range", cols=1 << 17)
+    f.refused("out of range", rows=1 << 27)
+    f.refused("another device", q=other.buffer(20 * 128, I8))
+    f.refused("buffer q .*too small", q=c.buffer(20 * 128 - 1, I8))
+    f.refused("buffer scale .*too small", scale=c.buffer(19, F32))
+    # a failed allocation leaves nothing behind
+    for n in range(2):
+        lib.host_fail(n)
+        f.refused("hipMalloc", code=capi.TH_ERR_OOM)
+    lib.host_fail(-1)
+
+    y = c.buffer(3 * 20, F32)
+    g = Refusals(c, "th_gemm_i8", dev=c.dev, xq=c.buffer(3 * 128, I8), xs=c.buffer(3, F32), m=3, w=w, bias=None, y=y)
+    g.call()
+    g.call(m=0)
+    g.call(bias=c.buffer(20, F32), y=c.buffer(60, F16))
+    for name in ("dev", "xq", "xs", "w", "y"):
+        g.refused("null", **{name: None})
+    g.refused("buffer xq .*too small", xq=c.buffer(3 * 128 - 1, I8))
+    g.refused("dtype", xq=c.buffer(3 * 128, U8))
+    g.refused("buffer x_scale .*too small", xs=c.buffer(2, F32))
+    g.refused("buffer bias .*too small", bias=c.buffer(19, F32))
+    g.refused("dtype", bias=c.buffer(20, F16))
+    g.refused("buffer y .*too small", y=c.buffer(59, F32))
+    g.refused("f32, f16 or bf16", y=c.buffer(60, I8))
+    g.refused("out of range", m=1 << 31)
+    g.refused("must not be an input", xs=y)
+    g.refused("must not be an input", bias=y)
+    g.refused("another device", y=other.buffer(60, F32))
+    lib.host_grouped(w, 8, 0)
+    g.refused("each group", code=capi.TH_ERR_UNSUPPORTED)
+    lib.host_grouped(w, 4, 1)
+    g.refused("not q8")
+    lib.host_grouped(w, 8, 1)
+    g.call()
+    c.call("th_qweight_free", w)
+    with pytest.raises(Refused, match="capture"):
+        c.call("th_capture_begin", c.dev)
+        f.call()

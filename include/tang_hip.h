@@ -409,6 +409,20 @@ int th_sampler_destroy(th_sampler* s);
  * tokens seen so far (for the repetition penalty). */
 int th_sampler_sample(th_sampler* s, const float* logits, size_t vocab, const int32_t* past, size_t n_past,
                       int32_t* token);
+/* The sampler on the device, a token for each row of logits [n_rows][vocab] (f32, f16 or bf16; vocab up to 2^20)
+ * from given random numbers u [n_rows], f32 in [0, 1).  Settings of each row, NULL: off.
+ *  temperature  f32; not above 0: the first of the largest logits (as th_argmax)
+ *  top_k        u32; keeps the logits from the k-th largest on (equal ones too, as th_sampler_sample); 0 or from vocab on: off
+ *  top_p        f32; of those, the shortest run in descending order (equal ones: lower index first) whose weights
+ *               exp(logit / temperature) reach top_p of their sum; from 1 on: off, down to 0: one token
+ *  min_p        f32; of those, weights from min_p times the largest on; 0: off
+ * The token is the first, by index, at which the running sum of kept weights exceeds u times their sum; tokens u32
+ * [n_rows], prob f32 [n_rows] (may be NULL): its share of that sum.  Weights and borders are right to 2^-42 of the
+ * largest weight.  A NaN logit counts as -inf; infinite ones share all weight; a row that has nothing above -inf gives
+ * token 0 with prob 0. */
+int th_sample_rows(th_device* dev, const th_buffer* logits, size_t n_rows, size_t vocab, const th_buffer* u,
+                   const th_buffer* temperature, const th_buffer* top_k, const th_buffer* top_p, const th_buffer* min_p,
+                   th_buffer* tokens, th_buffer* prob);
 /* generate() (sampling.rs:229-256) on the decode engine: prompt_last is fed
  * at position pos (positions < pos already in the KV cache); each step runs on
  * the device, the logits come to the host and the sampler picks the next

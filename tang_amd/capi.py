@@ -109,6 +109,7 @@ SIGNATURES = {
     "th_sampler_create": ([_P, _U64, _P], _I),
     "th_sampler_destroy": ([_P], _I),
     "th_sampler_sample": ([_P, _P, _S, _P, _S, _P], _I),
+    "th_sample_rows": ([_P, _P, _S, _S, _P, _P, _P, _P, _P, _P, _P], _I),
     "th_llama_generate_sampled": ([_P, _P, _P, _S, _S, _P, _P], _I),
     "th_llama_prefill": ([_P, _P, _S, _S, _P, _P], _I),
     "th_llama_time_prefill": ([_P, _P, _S, _S, _P], _I),
@@ -878,6 +879,13 @@ class HipComputeDevice:
         out = self.alloc(n_rows, U32)
         check(lib().th_argmax(self.handle, data.handle, n_rows, n, out.handle))
         return out
+
+    def sample_rows(self, logits, n_rows, vocab, u, temperature=None, top_k=None, top_p=None, min_p=None, tokens=None, prob=None):
+        """A token for each row from given random numbers, with each row's own settings (th_sample_rows)."""
+        tokens = tokens or self.alloc(n_rows, U32)
+        check(lib().th_sample_rows(self.handle, logits.handle, n_rows, vocab, u.handle, _handle(temperature), _handle(top_k), _handle(top_p),
+                                   _handle(min_p), tokens.handle, _handle(prob)))
+        return tokens
 
     def mla_decode(self, q_nope, q_rope, cache, B, H, L, dn, dr, r, dv, w_uk, w_uv, sm_scale, out=None):
         """Absorbed MLA decode: q_nope/q_rope f32, cache bf16 [B][L][r+dr],

@@ -265,6 +265,7 @@ extern "C" {
     pub fn th_sampler_create(cfg: *const th_sampling_config, seed: u64, out: *mut *mut th_sampler) -> c_int;
     pub fn th_sampler_destroy(s: *mut th_sampler) -> c_int;
     pub fn th_sampler_sample(s: *mut th_sampler, logits: *const f32, vocab: usize, past: *const i32, n_past: usize, token: *mut i32) -> c_int;
+    pub fn th_sample_rows(dev: *mut th_device, logits: *const th_buffer, n_rows: usize, vocab: usize, u: *const th_buffer, temperature: *const th_buffer, top_k: *const th_buffer, top_p: *const th_buffer, min_p: *const th_buffer, tokens: *mut th_buffer, prob: *mut th_buffer) -> c_int;
     pub fn th_llama_generate_sampled(m: *mut th_llama, s: *mut th_sampler, prompt: *const i32, n_prompt: usize, pos: usize, tokens_out: *mut i32, n_out: *mut usize) -> c_int;
     pub fn th_moe_create(dev: *mut th_device, d_model: usize, d_ff: usize, n_experts: usize, n_shared: usize, top_k: usize, out: *mut *mut th_moe) -> c_int;
     pub fn th_moe_destroy(moe: *mut th_moe) -> c_int;

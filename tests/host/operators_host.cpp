@@ -1,8 +1,9 @@
-// The host side of the operators around the paged cache (i8gemm.cpp), over the runtime of kvcache_host.cpp and
+// The host side of the operators around the paged cache (i8gemm.cpp, samplerows.cpp), over the runtime of kvcache_host.cpp and
 // launchers that only check what they are handed.
 #include "kvcache_host.cpp"
 
 #include "../../tang_amd/csrc/i8gemm.cpp"
+#include "../../tang_amd/csrc/samplerows.cpp"
 
 namespace th {
 
@@ -19,6 +20,12 @@ void launch_i8_linear(th_device*, const th_qweight* w, const int8_t* xq, const I
     CHECK(xq && out.y && out.xs && out.ws == w->scales && out.N == (int)w->rows);
     g_m = m;
     g_k = w->cols;
+}
+
+void launch_sample_rows(const SampleArgs& a, hipStream_t) {
+    CHECK(a.x && a.u && a.token);
+    g_m = a.rows;
+    g_k = a.vocab;
 }
 
 }  // namespace th

@@ -175,10 +175,30 @@ static void i8_rows_launch(const th_qweight* w, const int8_t* xq, const I8Out& o
     TH_LAUNCH_CHECK();
 }
 
+template <int TM, int TN, int WPE>
+static void i8_tile_launch(th_device* dev, const th_qweight* w, const int8_t* xq, const I8Out& out, size_t m, size_t ks) {
+    constexpr size_t smem = (size_t)3 * 4 * (TM + TN) * 1024 + 64 * (TM + 2 * TN) * 4;
+    auto k = i8_tile_kernel<TM, TN, WPE>;
+    (void)hipFuncSetAttribute((const void*)k, hipFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+    const size_t NCH = w->Kp / 64, cps = ceil_div(NCH, ks);
+    ks = ceil_div(NCH, cps);
+    int* part = ks > 1 ? (int*)device_scratch(dev, ks * m * w->rows * 4) : nullptr;
+    const dim3 grid((unsigned)ceil_div(w->rows, (size_t)(64 * TN)), (unsigned)ceil_div(m, (size_t)(64 * TM)), (unsigned)ks);
+    TH_LAUNCH(k, grid, dim3(256), smem, dev->stream, (const uint4*)w->data, xq, out, (int)m, (int)w->Kp, (int)cps, part);
+    TH_LAUNCH_CHECK();
+    if (part) {
+        TH_LAUNCH(i8_join_kernel, dim3((unsigned)std::min<size_t>(ceil_div(m * w->rows, 256), 8192)), dim3(256), 0, dev->stream, part, out, (int)m,
+                  (int)ks);
+        TH_LAUNCH_CHECK();
+    }
+}
+
 static void i8_linear(th_device* dev, const th_qweight* w, const int8_t* xq, const I8Out& out, size_t m) {
     const hipStream_t s = dev->stream;
     if (m <= 16) i8_rows_launch<1, 1, 8>(w, xq, out, m, s);
-    else i8_rows_launch<2, 4, 2>(w, xq, out, m, s);
+    else if (m <= 64) i8_rows_launch<2, 4, 2>(w, xq, out, m, s);
+    else if (m <= 1024) i8_tile_launch<2, 2, 2>(dev, w, xq, out, m, 1);
+    else i8_tile_launch<4, 4, 1>(dev, w, xq, out, m, 1);
 }
 
 void launch_i8_linear(th_device* dev, const th_qweight* w, const int8_t* xq, const I8Out& out, size_t m) {

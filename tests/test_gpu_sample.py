@@ -131,6 +131,32 @@ def test_equal_logits(dev, V):
     assert list(got) == [0] + [int(np.float32(v) * V) for v in (0.3, 0.6, 0.999)]
 
 
+def test_min_p_that_leaves_fewer_than_k(dev):
+    """A k far beyond what min-p keeps, with and without top-p; a k in the middle of them."""
+    rng = np.random.default_rng(13)
+    n, V = 9, 40000
+    x = _logits(rng, n, V, 1.0)
+    for k in (3, 50, 5000, 39000):
+        for low in (1.0, 0.5, 1e-3):
+            for p in (None, np.full(n, 0.95)):
+                _check(dev, x, F32, rng.random(n, np.float32), k=np.full(n, k, np.uint32), low=np.full(n, low), p=p)
+
+
+@pytest.mark.parametrize("V", [5000, 33000, 70000])
+def test_lists_that_are_full(dev, V):
+    """Candidates about as many as a list holds (4096), one fewer, one more: by k, by p over equal ones, by min-p."""
+    rng = np.random.default_rng(V)
+    for m in (4095, 4096, 4097):
+        x = np.full((3, V), -30.0, np.float32)
+        for r in x:
+            r[rng.permutation(V)[:m]] = rng.uniform(0, 0.001, m)
+        u = rng.random(3, np.float32)
+        _check(dev, x, F32, u, k=np.full(3, m, np.uint32))
+        _check(dev, x, F32, u, k=np.full(3, 4000, np.uint32), p=np.full(3, 0.7))
+        _check(dev, x, F32, u, p=np.full(3, 0.99))
+        _check(dev, x, F32, u, low=np.full(3, 0.9))
+
+
 def test_masked_and_infinite(dev):
     rng = np.random.default_rng(9)
     V = 9001

@@ -10,10 +10,12 @@ namespace th {
 typedef int i32x4_t __attribute__((ext_vector_type(4)));
 typedef int i32x16_t __attribute__((ext_vector_type(16)));
 
-__device__ __forceinline__ float i8_value(const I8Out& o, int sum, double s, double t, int n) {
-    double v = (double)sum * s * t;
-    if (o.bias) v += (double)o.bias[n];
-    return (float)v;
+// (sum s) t + b.  For f32 results in f64, rounded once (no order of the scales leaves
+// its range); for 16-bit ones in f32 from the scales' mantissas and the sum of their exponents: off
+// by 3 2^-24 of the product, far below their own rounding, at a third of the time.
+__device__ __forceinline__ float i8_wide(int sum, float s, float t, float b) { return (float)((double)sum * (double)s * (double)t + (double)b); }
+__device__ __forceinline__ float i8_narrow(int sum, float s, float t, int exponent, float b) {
+    return __builtin_amdgcn_ldexpf((float)sum * (s * t), exponent) + b;
 }
 __device__ __forceinline__ void i8_store(const I8Out& o, size_t m, int n, float v) {
     const size_t at = m * o.N + n;
@@ -22,34 +24,36 @@ __device__ __forceinline__ void i8_store(const I8Out& o, size_t m, int n, float 
     else ((__bf16*)o.y)[at] = (__bf16)v;
 }
 
-__device__ __forceinline__ void i8_store4(const I8Out& o, size_t m, int n, float a, float b, float c, float d) {
-    const size_t at = m * o.N + n;
-    typedef _Float16 h4_t __attribute__((ext_vector_type(4)));
-    typedef __bf16 b4_t __attribute__((ext_vector_type(4)));
-    if (o.dt == TH_F32) *(float4*)((float*)o.y + at) = make_float4(a, b, c, d);
-    else if (o.dt == TH_F16) *(h4_t*)((_Float16*)o.y + at) = (h4_t){(_Float16)a, (_Float16)b, (_Float16)c, (_Float16)d};
-    else *(b4_t*)((__bf16*)o.y + at) = (b4_t){(__bf16)a, (__bf16)b, (__bf16)c, (__bf16)d};
+// Four channels from n on, those of them that there are (rows may start at any element).
+template <typename Y>
+__device__ __forceinline__ void i8_store4(Y* to, size_t m, int n, int N, const float (&y)[4]) {
+    typedef Y y4_t __attribute__((ext_vector_type(4), aligned(sizeof(Y))));
+    to += m * N + n;
+    if (n + 4 <= N) {
+        *(y4_t*)to = (y4_t){(Y)y[0], (Y)y[1], (Y)y[2], (Y)y[3]};
+    } else {
+#pragma unroll
+        for (int i = 0; i < 3; i++)
+            if (n + i < N) to[i] = (Y)y[i];
+    }
 }
 
 // A few rows, bound by the stream of the weights: a workgroup has RT tiles of 16
-// channels and CB of 16 rows, its NW waves take chunks of 64 k in turn (eight
+// channels and all rows, CB tiles of 16, its NW waves take chunks of 64 k in turn (eight
 // waves read 8 KiB of a tile row at a time), operands come from global memory
 // straight into registers, and the waves' sums meet in LDS.  Integer sums: any split gives the same bits.
 template <int RT, int CB, int U, int NW>
-__global__ __launch_bounds__(64 * NW) void i8_rows_kernel(const uint4* __restrict__ wt, const int8_t* __restrict__ xq, I8Out out, int M, int Kp,
-                                                          int nbx) {
+__global__ __launch_bounds__(64 * NW) void i8_rows_kernel(const uint4* __restrict__ wt, const int8_t* __restrict__ xq, I8Out out, int M, int Kp) {
     extern __shared__ i32x4_t red[];  // [NW][RT * CB][64]
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int q = lane >> 4, r = lane & 15;
-    const int bx = blockIdx.x % nbx, by = blockIdx.x / nbx;
-    const int NCH = Kp >> 6, NT = (out.N + 15) >> 4;
-    const int m0 = by * CB * 16;
+    const int bx = blockIdx.x, NCH = Kp >> 6, NT = (out.N + 15) >> 4;
     const i32x4_t* w[RT];
     const i32x4_t* x[CB];
 #pragma unroll
     for (int a = 0; a < RT; a++) w[a] = (const i32x4_t*)wt + (size_t)min(bx * RT + a, NT - 1) * NCH * 64 + lane;
 #pragma unroll
-    for (int b = 0; b < CB; b++) x[b] = (const i32x4_t*)(xq + (size_t)min(m0 + b * 16 + r, M - 1) * Kp) + q;
+    for (int b = 0; b < CB; b++) x[b] = (const i32x4_t*)(xq + (size_t)min(b * 16 + r, M - 1) * Kp) + q;
     i32x4_t acc[RT][CB];
 #pragma unroll
     for (int a = 0; a < RT; a++)
@@ -90,12 +94,12 @@ __global__ __launch_bounds__(64 * NW) void i8_rows_kernel(const uint4* __restric
 #pragma unroll
         for (int v = 1; v < NW; v++) s += red[v * RT * CB * 64 + i];
         const int t = i >> 6, a = t / CB, b = t % CB, ln = i & 63;
-        const int n = (bx * RT + a) * 16 + (ln & 15), m = m0 + b * 16 + (ln >> 4) * 4;
+        const int n = (bx * RT + a) * 16 + (ln & 15), m = b * 16 + (ln >> 4) * 4;
         if (n >= out.N) continue;
-        const double wsc = (double)out.ws[n];
+        const float wsc = out.ws[n], bias = out.bias ? out.bias[n] : 0.0f;
 #pragma unroll
         for (int e = 0; e < 4; e++)
-            if (m + e < M) i8_store(out, m + e, n, i8_value(out, s[e], (double)out.xs[m + e], wsc, n));
+            if (m + e < M) i8_store(out, m + e, n, i8_wide(s[e], out.xs[m + e], wsc, bias));
     }
 }
 
@@ -103,20 +107,31 @@ __global__ __launch_bounds__(64 * NW) void i8_rows_kernel(const uint4* __restric
 // waves) on the 32x32x32 MFMA, 64 k a step.  LDS holds three steps: one is read,
 // the next is there (its first operands are read ahead), the one after is
 // written, so one barrier a step orders all and no wave waits for LDS behind
-// it.  Rows come through registers, two steps ahead of their place in LDS.  Both operands lie
+// it.  Rows come through registers, ST steps ahead of their place in LDS.  Both operands lie
 // in LDS as they are read: 1 KiB blocks of 16 rows x 64 k, lane by lane.
-// part: the sums of a K split instead of results, [split][M][N].
-template <int TM, int TN, int WPE>
-__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(WPE, WPE))) void i8_tile_kernel(
-    const uint4* __restrict__ wt, const int8_t* __restrict__ xq, I8Out out, int M, int Kp, int chunks_per_split, int* __restrict__ part) {
+// KW: groups of four waves, each with every KW-th step of k and LDS of its own, whose
+// sums meet at the end, for tiles that are alone on their CU.
+// Measured: 8192 x 8192 x 8192 2205 TOP/s (the library's product there: 2456), 8192 x 4096 x 11008 1845 (2186), where
+// the matrix operations take 59 % of the cycles at the 1.75 GHz that the chip then runs at; 2048 x 4096 x 4096 1650 (1677),
+// 512 x 4096 x 4096 940 (837).  Tried: weights from memory straight into registers (each wave its own, 1846 and 1639:
+// they are loaded twice), more steps ahead (the same).
+// LDS in bytes: the stages, or the strips that results leave through; then the tile's scales and bias.
+template <int TM, int TN, int KW>
+struct I8TileLds {
+    static constexpr int STAGES = 3 * KW * 4 * (TM + TN) * 1024, STRIPS = KW * 4 * 32 * (32 * TN + 4) * 4;
+    static constexpr int SCALES = STAGES > STRIPS ? STAGES : STRIPS, BYTES = SCALES + 64 * (2 * TM + 3 * TN) * 4;
+};
+template <int TM, int TN, int KW, int ST, int WPE>
+__global__ __launch_bounds__(256 * KW) __attribute__((amdgpu_waves_per_eu(WPE, WPE))) void i8_tile_kernel(
+    const uint4* __restrict__ wt, const int8_t* __restrict__ xq, I8Out out, int M, int Kp) {
     constexpr int NA = 4 * TM, NB = 4 * TN, SZ = (NA + NB) * 64;
-    extern __shared__ i32x4_t tile[];  // [3][NA + NB][64], then the scales and the bias of the tile
-    float* const scales = (float*)(tile + 3 * SZ);
-    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    int bx = blockIdx.x, by = blockIdx.y, split = blockIdx.z;
-    gemm_xcd_tile(bx, by, split);
+    extern __shared__ i32x4_t tile[];  // [3][KW][NA + NB][64], then the scales and the bias of the tile
+    float* const scales = (float*)((char*)tile + I8TileLds<TM, TN, KW>::SCALES);
+    const int tid = threadIdx.x, lane = tid & 63, wave8 = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int wave = wave8 & 3, group = wave8 >> 2;
+    int bx = blockIdx.x, by = blockIdx.y, bz = 0;
+    gemm_xcd_tile(bx, by, bz);
     const int NCH = Kp >> 6, NT = (out.N + 15) >> 4;
-    const int c0 = split * chunks_per_split, steps = min(NCH - c0, chunks_per_split);
     const int m0 = by * 64 * TM, n0 = bx * 64 * TN;
     // this wave's blocks: rows past the end re-read the last one
     uint32_t xo[TM], wo[TN];
@@ -125,22 +140,17 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(WPE, WPE)))
     for (int i = 0; i < TM; i++) xo[i] = (uint32_t)min((wave * TM + i) * 16 + (lane & 15), mlast) * (uint32_t)Kp + (lane >> 4) * 16;
 #pragma unroll
     for (int i = 0; i < TN; i++) wo[i] = (uint32_t)min(wave * TN + i, tlast) * (uint32_t)NCH * 1024u + lane * 16;
-    const __amdgpu_buffer_rsrc_t xb = buffer_rsrc(xq + (size_t)m0 * Kp + (size_t)c0 * 64, (uint32_t)(min(M - m0, 64 * TM) * Kp - c0 * 64));
-    const __amdgpu_buffer_rsrc_t wb =
-        buffer_rsrc(wt + ((size_t)(n0 / 16) * NCH + c0) * 64, (uint32_t)((min(NT - n0 / 16, 4 * TN) * NCH - c0) * 1024));
-    for (int i = tid; i < 64 * TM; i += 256) scales[i] = out.xs[min(m0 + i, M - 1)];
-    for (int i = tid; i < 64 * TN; i += 256) {
-        const int n = min(n0 + i, out.N - 1);
-        scales[64 * TM + i] = out.ws[n];
-        scales[64 * (TM + TN) + i] = out.bias ? out.bias[n] : 0.0f;
-    }
-    i32x4_t g[2][TM + TN];
+    const __amdgpu_buffer_rsrc_t xb = buffer_rsrc(xq + (size_t)m0 * Kp, (uint32_t)(min(M - m0, 64 * TM) * Kp));
+    const __amdgpu_buffer_rsrc_t wb = buffer_rsrc(wt + (size_t)(n0 / 16) * NCH * 64, (uint32_t)(min(NT - n0 / 16, 4 * TN) * NCH * 1024));
+    // Steps come in turns of ST by KW: chunks before the first of k fill them up, as zeros.
+    const int steps = (NCH + KW * ST - 1) / (KW * ST) * ST, lead = steps * KW - NCH;
+    i32x4_t g[ST][TM + TN];
+    auto chunk = [&](int s) { return max(0, min(s * KW + group - lead, NCH - 1)); };
     auto gload = [&](int set, int c, int i) {
         const auto v = i < TM ? __builtin_amdgcn_raw_buffer_load_b128(xb, (int)xo[i < TM ? i : 0], c * 64, 0)
                               : __builtin_amdgcn_raw_buffer_load_b128(wb, (int)wo[i < TM ? 0 : i - TM], c * 1024, 0);
         g[set][i] = __builtin_bit_cast(i32x4_t, v);
     };
-    auto chunk = [&](int s) { return max(0, min(s, steps - 1)); };
     auto lwrite = [&](int set, i32x4_t* to, int i) { to[(i < TM ? wave * TM + i : NA + wave * TN + i - TM) * 64 + lane] = g[set][i]; };
     auto load_all = [&](int set, int s) {
 #pragma unroll
@@ -149,6 +159,11 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(WPE, WPE)))
     auto write_all = [&](int set, i32x4_t* to) {
 #pragma unroll
         for (int i = 0; i < TM + TN; i++) lwrite(set, to, i);
+    };
+    auto zeros_before = [&](int set, int s) {
+        if (s * KW + group < lead)
+#pragma unroll
+            for (int i = 0; i < TM; i++) g[set][i] = (i32x4_t){0, 0, 0, 0};
     };
     // operand of 32 rows and 32 k: lanes 0..31 have its first 16 k
     const int wm = wave >> 1, wn = wave & 1;
@@ -164,24 +179,33 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(WPE, WPE)))
         for (int j = 0; j < TN; j++)
 #pragma unroll
             for (int e = 0; e < 16; e++) acc[i][j][e] = 0;
-    // steps come in pairs: the first of an odd number of them has zeros before it
-    const int first = -(steps & 1);
-    load_all(0, first);
-    load_all(1, first + 1);
-    if (first < 0)
+    i32x4_t *now = tile + group * SZ, *next = now + KW * SZ, *after = next + KW * SZ;
 #pragma unroll
-        for (int i = 0; i < TM; i++) g[0][i] = (i32x4_t){0, 0, 0, 0};
-    write_all(0, tile);
-    load_all(0, first + 2);
-    write_all(1, tile + SZ);
-    load_all(1, first + 3);
+    for (int i = 0; i < ST; i++) load_all(i, i);
+    float *const rs = scales, *const cs = rs + 64 * TM, *const cb = cs + 64 * TN;
+    int *const re = (int*)(cb + 64 * TN), *const ce = re + 64 * TM;
+    const bool wide = out.dt == TH_F32;
+    for (int i = tid; i < 64 * (TM + TN); i += 256 * KW) {
+        const int n = min(n0 + i - 64 * TM, out.N - 1);
+        const float v = i < 64 * TM ? out.xs[min(m0 + i, M - 1)] : out.ws[n];
+        int e = 0;
+        const float f = __builtin_frexpf(v, &e);
+        rs[i] = wide ? v : f;  // (rows, then columns)
+        if (i >= 64 * TM) cb[i - 64 * TM] = out.bias ? out.bias[n] : 0.0f;
+        re[i] = e;
+    }
+#pragma unroll
+    for (int i = 0; i < 2; i++) {
+        zeros_before(i, i);
+        write_all(i, i ? next : now);
+        load_all(i, ST + i);
+    }
     lds_barrier();
 #pragma unroll
-    for (int i = 0; i < TM + TN; i++) lread(tile, 0, i);
-    i32x4_t *now = tile, *next = tile + SZ, *after = tile + 2 * SZ;
+    for (int i = 0; i < TM + TN; i++) lread(now, 0, i);
     // The order is the source's: a step's LDS accesses lie evenly between its
     // matrix operations (four waves' reads or writes behind every one of them are
-    // more than LDS takes: 2011 against N TOP/s at 8192 x 8192 x 8192), operands
+    // more than LDS takes: 2011 against 2167 TOP/s at 8192 x 8192 x 8192), operands
     // are read in the order of their use, half a step ahead.
     constexpr int NM = TM * TN, NR = TM + TN;
     auto operand = [&](int r) { return r == 0 ? 0 : r <= TN ? TM + r - 1 : r - TN; };
@@ -193,14 +217,16 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(WPE, WPE)))
 #pragma unroll
             for (int r = 0; r < NR; r++) {
                 if (r * NM / NR == q) lread(half ? next : now, 1 - half, operand(r));
-                if (r * 2 * NM / NR + NM / NR / 2 == half * NM + q) lwrite(set, after, r);
-                if (r * 2 * NM / NR + NM / NR + NM / NR / 2 == half * NM + q) gload(set, c, r);
+                const int write = (4 * r + 1) * NM / (2 * NR), load = (4 * r + 3) * NM / (2 * NR);  // of the step's 2 NM places
+                if (write == half * NM + q) lwrite(set, after, r);
+                if (load == half * NM + q) gload(set, c, r);
             }
             __builtin_amdgcn_sched_barrier(0);
         }
     };
-    auto step = [&](int set, int s) {
-        const int c = chunk(s + 4);
+    auto step = [&](int set, int s) {  // writes step s + 2, which `set` holds, and loads step s + 2 + ST into it
+        const int c = chunk(s + 2 + ST);
+        if (ST * KW > 2) zeros_before(set, s + 2);
         half_step(0, set, c);
         half_step(1, set, c);
         lds_barrier();
@@ -209,65 +235,66 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(WPE, WPE)))
         next = after;
         after = t;
     };
-    for (int s = first; s < steps; s += 2) {
-        step(0, s);
-        step(1, s + 1);
+    for (int s = 0; s < steps; s += ST) {
+#pragma unroll
+        for (int i = 0; i < ST; i++) step((2 + i) % ST, s + i);
     }
-    // Strips of 32 rows go through LDS (each wave's own part) and leave as whole
-    // rows: four channels a lane, or one where rows do not start on four.
-    asm volatile("s_nop 15\n\ts_nop 3");  // (the last MFMA's 16 passes, see mfma_settle)
-    constexpr int W = 32 * TN, LW = W + 4;
+    // Strips of 32 rows go through LDS (each wave's own part), where the groups'
+    // sums meet, and leave as whole rows, four channels a lane and four rows at a
+    // time, in code of their type's own (K = 64, 256 x 256 tiles: with a branch
+    // for each value 25.9 us a launch).
+    asm volatile("s_nop 15\n\ts_nop 3");  // (the last MFMA's passes, see mfma_settle)
+    constexpr int W = 32 * TN, LW = W + 4, LPR = W / 4, RPI = 64 / LPR;  // lanes of a row, rows a wave reads at once
+    constexpr int ITS = 32 / RPI / KW, AT_ONCE = ITS < 4 ? ITS : 4;
     int* const strip = (int*)tile + wave * 32 * LW;
-    const int nw = n0 + wn * W;
+    const int c = lane % LPR * 4, n = n0 + wn * W + c;
+    const float4 ws = *(const float4*)&cs[wn * W + c], bs = *(const float4*)&cb[wn * W + c];
+    const int4 we = *(const int4*)&ce[wn * W + c];
+    const float t[4] = {ws.x, ws.y, ws.z, ws.w}, b[4] = {bs.x, bs.y, bs.z, bs.w};
+    const int te[4] = {we.x, we.y, we.z, we.w};
+    auto leave = [&](auto as) {
+        using Y = decltype(as);
 #pragma unroll
-    for (int i = 0; i < TM; i++) {
+        for (int i = 0; i < TM; i++) {
+            int* const to = strip + group * 4 * 32 * LW + (lane >> 5) * 4 * LW + (lane & 31);
 #pragma unroll
-        for (int j = 0; j < TN; j++)
+            for (int j = 0; j < TN; j++)
 #pragma unroll
-            for (int e = 0; e < 16; e++) strip[((e >> 2) * 8 + (lane >> 5) * 4 + (e & 3)) * LW + j * 32 + (lane & 31)] = acc[i][j][e];
-        wave_lds_fence();
-        const int ml = (wm * TM + i) * 32;
-        if (part) {
-            for (int x = lane; x < 32 * W; x += 64) {
-                const int r = x / W, c = x % W, m = m0 + ml + r, n = nw + c;
-                if (m < M && n < out.N) part[((size_t)split * M + m) * out.N + n] = strip[r * LW + c];
-            }
-        } else if ((out.N & 3) == 0) {
-            constexpr int LPR = W / 4;  // lanes of a row
-            const int c = lane % LPR * 4, n = nw + c;
-            const float4 ws = *(const float4*)&scales[64 * TM + wn * W + c], bs = *(const float4*)&scales[64 * (TM + TN) + wn * W + c];
-            if (n < out.N)
-#pragma unroll 4
-                for (int r = lane / LPR; r < 32; r += 64 / LPR) {
-                    const int m = m0 + ml + r;
-                    if (m >= M) break;
-                    const i32x4_t v = *(const i32x4_t*)&strip[r * LW + c];
-                    const double s = (double)scales[ml + r];
-                    i8_store4(out, m, n, (float)((double)v[0] * s * (double)ws.x + (double)bs.x), (float)((double)v[1] * s * (double)ws.y + (double)bs.y),
-                              (float)((double)v[2] * s * (double)ws.z + (double)bs.z), (float)((double)v[3] * s * (double)ws.w + (double)bs.w));
+                for (int e = 0; e < 16; e++) to[((e >> 2) * 8 + (e & 3)) * LW + j * 32] = acc[i][j][e];
+            if constexpr (KW > 1) __syncthreads();
+            else wave_lds_fence();
+            const int ml = (wm * TM + i) * 32;
+#pragma unroll 1
+            for (int it = 0; it < ITS; it += AT_ONCE) {
+                i32x4_t v[AT_ONCE];
+                float s[AT_ONCE];
+                int se[AT_ONCE];
+#pragma unroll
+                for (int x = 0; x < AT_ONCE; x++) {
+                    const int r = ((it + x) * KW + group) * RPI + lane / LPR;
+                    v[x] = *(const i32x4_t*)&strip[r * LW + c];
+#pragma unroll
+                    for (int k = 1; k < KW; k++) v[x] += *(const i32x4_t*)&strip[k * 4 * 32 * LW + r * LW + c];
+                    s[x] = rs[ml + r];
+                    se[x] = re[ml + r];
                 }
-        } else {
-            for (int x = lane; x < 32 * W; x += 64) {
-                const int r = x / W, c = x % W, m = m0 + ml + r, n = nw + c;
-                if (m < M && n < out.N)
-                    i8_store(out, m, n, (float)((double)strip[r * LW + c] * (double)scales[ml + r] * (double)scales[64 * TM + wn * W + c] +
-                                                (double)scales[64 * (TM + TN) + wn * W + c]));
+#pragma unroll
+                for (int x = 0; x < AT_ONCE; x++) {
+                    float y[4];
+#pragma unroll
+                    for (int e = 0; e < 4; e++)
+                        y[e] = sizeof(Y) == 4 ? i8_wide(v[x][e], s[x], t[e], b[e]) : i8_narrow(v[x][e], s[x], t[e], se[x] + te[e], b[e]);
+                    const int m = m0 + ml + ((it + x) * KW + group) * RPI + lane / LPR;
+                    if (m < M && n < out.N) i8_store4((Y*)out.y, m, n, out.N, y);
+                }
             }
+            if constexpr (KW > 1) __syncthreads();
+            else wave_lds_fence();
         }
-        wave_lds_fence();
-    }
-}
-
-// The splits' sums, and what is done to them.
-__global__ __launch_bounds__(256) void i8_join_kernel(const int* __restrict__ part, I8Out out, int M, int splits) {
-    const size_t total = (size_t)M * out.N;
-    for (size_t i = blockIdx.x * (size_t)256 + threadIdx.x; i < total; i += (size_t)gridDim.x * 256) {
-        int v = 0;
-        for (int s = 0; s < splits; s++) v += part[(size_t)s * total + i];
-        const size_t m = i / out.N;
-        const int n = (int)(i - m * out.N);
-        i8_store(out, m, n, i8_value(out, v, (double)out.xs[m], (double)out.ws[n], n));
-    }
+    };
+    if (out.dt == TH_F32) leave(float{});
+    else if (out.dt == TH_F16) leave((_Float16)0);
+    else leave((__bf16)0.0f);
 }
 
 }  // namespace th

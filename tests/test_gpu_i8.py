@@ -1,9 +1,9 @@
 """Rows to 8-bit integers and their products, against the formulas in 64 bits:
-every integer, and every result to the bit."""
+every integer, every f32 result to the bit, 16-bit ones to their rounding."""
 import numpy as np
 import pytest
 
-from paged_ref import from_bits, rounded, to_bits
+from paged_ref import EPS, LEAST, from_bits, rounded, to_bits
 from tang_amd import capi
 
 pytestmark = pytest.mark.gpu
@@ -100,10 +100,23 @@ def _run(dev, rng, m, k, n, dt=F32, bias=False, w=None):
     dev.gemm_i8(dev.upload(rows, I8), dev.upload(s), m, w, y, None if b is None else dev.upload(b))
     got = y.to_numpy()
     assert np.all(got[m * n:] == (9.0 if dt == F32 else 0x1234))
-    want = to_bits(_product(q, s, wq, t, b), dt)
     got = got[:m * n].reshape(m, n)
-    bad = np.argwhere(got != want)
-    assert not len(bad), (len(bad), bad[0], got[tuple(bad[0])], want[tuple(bad[0])])
+    if dt == F32:
+        want = _product(q, s, wq, t, b)
+        bad = np.argwhere(got != want)
+        assert not len(bad), (len(bad), bad[0], got[tuple(bad[0])], want[tuple(bad[0])])
+        return
+    # In f32: the sum's, the scales' and their product's rounding (3 half steps of it), the bias' addition (one of the result), then the result's own.
+    p = (q.astype(np.int64) @ wq.astype(np.int64).T) * s.astype(np.float64)[:, None] * t.astype(np.float64)
+    y = p if b is None else p + b
+    tol = (3 * 2.0 ** -24 * np.abs(p) + 2.0 ** -24 * np.abs(y)) * (1 + 2.0 ** -8) + np.maximum(EPS[dt] * np.abs(y), LEAST[dt])
+    top = {F16: 65520.0, BF16: 3.39e38}[dt]  # what rounds to infinity
+    got = from_bits(got, dt)
+    fine = np.abs(y) < top * (1 - 2.0 ** -10)
+    bad = np.argwhere(fine & ~(np.abs(got - y) <= tol))
+    assert not len(bad), (len(bad), bad[0], got[tuple(bad[0])], y[tuple(bad[0])])
+    over = np.abs(y) > top * (1 + 2.0 ** -10)
+    assert np.array_equal(got[over], np.sign(y[over]) * np.inf)
 
 
 SIZES = [(1, 1, 1), (1, 64, 16), (1, 4096, 250), (3, 65, 17), (2, 11008, 40), (16, 130, 33), (17, 2047, 100), (31, 320, 64), (33, 64, 15), (61, 4096, 300),
@@ -132,6 +145,12 @@ def test_product_of_the_largest(dev):
         got = y.to_numpy().reshape(m, 5)
         assert np.array_equal(got, want[np.arange(m) % 2])
         assert np.isinf(got[1, 4]) and got[0, 4] != 0 and got[1, 3] == 0
+        y16 = dev.alloc(m * 5, BF16)
+        dev.gemm_i8(dev.upload(rows, I8), dev.upload(s), m, dev.q8_upload_rowwise(w, t, 5, k), y16)
+        got16 = from_bits(y16.to_numpy(), BF16).reshape(m, 5)
+        fine = np.isfinite(got)
+        assert np.array_equal(np.isfinite(got16), fine)
+        assert np.all(np.abs(got16[fine].astype(np.float64) - got[fine]) <= (EPS[BF16] + 2.0 ** -22) * np.abs(got[fine]) + LEAST[BF16])
 
 
 def test_rows_without_a_scale(dev):

@@ -178,15 +178,19 @@ int th_gemv_q8(th_device* dev, const th_buffer* x, size_t m, const th_qweight* w
  * int8 with a scale for each row, and multiplied with q8 weights that have one scale a row
  * (th_q8_upload_rowwise, th_q8_pack_rows) on the i8 MFMA, at twice bf16's rate.
  *
- * x [m][k], f32, f16 or bf16 -> q int8 [m][kp], kp = k rounded up to 64 (zeros behind k), and scale [m]:
+ * x [m][k], f32, f16 or bf16 -> q, m * kp int8 (kp = k rounded up to 64; zeros behind k), and scale [m]:
  * scale_i = f32(max |x_i| / 127), q = x / scale to the nearest integer, ties to even, at most 127 in size.  A
- * row of zeros has scale 0; one with an infinity or NaN has scale NaN and zeros (its products are NaN).  k below 2^17. */
+ * row of zeros has scale 0; one with an infinity or NaN has scale NaN and zeros (its products are NaN).  k below 2^17.
+ * q lies in blocks of h = 16 rows (fewer in the last): value (i, k) is at
+ * (i - i % 16) * kp + (k - k % 16) * h + i % 16 * 16 + k % 16. */
 int th_quantize_rows(th_device* dev, const th_buffer* x, size_t m, size_t k, th_buffer* q, th_buffer* scale);
-/* A q8 weight with one scale a row from rows on the device: q int8 [rows][kp] and scale [rows] as
- * th_quantize_rows gives them (there of a weight matrix [rows][cols]). */
+/* q8 weights with one scale a row from what is on the device: from a matrix [rows][cols], f32, f16 or bf16, by the
+ * same rule; or from int8 [rows][kp], row by row (kp = cols rounded up to 64, what lies behind cols does not
+ * count), and scale [rows]. */
+int th_q8_quantize(th_device* dev, const th_buffer* x, size_t rows, size_t cols, th_qweight** out);
 int th_q8_pack_rows(th_device* dev, const th_buffer* q, const th_buffer* scale, size_t rows, size_t cols, th_qweight** out);
-/* y[m][n] = (sum_k q[m][k] w[n][k]) x_scale[m] w_scale[n] + bias[n].  xq int8 [m][kp] (what
- * lies behind k is not looked at), bias f32 [n] or NULL; y f32, f16 or bf16.  Sums are exact (int32); the
+/* y[m][n] = (sum_k q[m][k] w[n][k]) x_scale[m] w_scale[n] + bias[n].  xq as th_quantize_rows gives it (what
+ * lies behind k does not count), bias f32 [n] or NULL; y f32, f16 or bf16.  Sums are exact (int32); the
  * rest is in f64, rounded once, for f32 results, and in f32 (off by 3 2^-24 of the product) for 16-bit ones.  Weights of
  * fewer than 2^17 columns; those with a scale for each group of 32 are TH_ERR_UNSUPPORTED. */
 int th_gemm_i8(th_device* dev, const th_buffer* xq, const th_buffer* x_scale, size_t m, const th_qweight* w,

@@ -79,6 +79,7 @@ SIGNATURES = {
     "th_gemv_q8": ([_P, _P, _S, _P, _P], _I),
     "th_gemm_q4_noalloc": ([_P, _P, _S, _P, _P], _I),
     "th_quantize_rows": ([_P, _P, _S, _S, _P, _P], _I),
+    "th_q8_quantize": ([_P, _P, _S, _S, _P], _I),
     "th_q8_pack_rows": ([_P, _P, _P, _S, _S, _P], _I),
     "th_gemm_i8": ([_P, _P, _P, _S, _P, _P, _P], _I),
     "th_bench_linear": ([_P, _P, _S, _P, _S, _P, _S, _I, _P], _I),
@@ -778,14 +779,20 @@ class HipComputeDevice:
         return y
 
     def quantize_rows(self, x, m, k, q=None, scale=None):
-        """Rows to int8 with a scale each (th_quantize_rows): q [m][k rounded up to 64] and scale [m]."""
+        """Rows to int8 with a scale each (th_quantize_rows): q (m times k rounded up to 64, in blocks) and scale [m]."""
         q = q or self.alloc(m * (-(-k // 64) * 64), I8)
         scale = scale or self.alloc(m)
         check(lib().th_quantize_rows(self.handle, x.handle, m, k, q.handle, scale.handle))
         return q, scale
 
+    def q8_quantize(self, x, rows, cols):
+        """A q8 weight with one scale a row from a matrix on the device (th_q8_quantize)."""
+        h = ctypes.c_void_p()
+        check(lib().th_q8_quantize(self.handle, x.handle, rows, cols, ctypes.byref(h)))
+        return QWeight(h, rows, cols, 8)
+
     def q8_pack_rows(self, q, scale, rows, cols):
-        """A weight from quantize_rows' results of its matrix [rows][cols]."""
+        """A q8 weight from int8 rows [rows][cols rounded up to 64] and their scales on the device."""
         h = ctypes.c_void_p()
         check(lib().th_q8_pack_rows(self.handle, q.handle, scale.handle, rows, cols, ctypes.byref(h)))
         return QWeight(h, rows, cols, 8)

@@ -3,6 +3,47 @@
 #include "i8gemm.hpp"
 #include "kvcache.hpp"
 
+namespace th {
+
+static void require_weight(const th_device* dev, size_t rows, size_t cols) {
+    TH_REQUIRE(!dev->closed, "the device was destroyed");
+    TH_REQUIRE(rows > 0 && cols > 0, "empty matrix");
+    TH_REQUIRE(rows < (size_t)1 << 27 && cols <= I8_MAX_K, "sizes out of range");
+    TH_REQUIRE(!dev->capturing, "makes a new weight: not while a graph is captured");
+}
+
+// A q8 weight with one scale a row, whose memory `fill` enqueues the contents of.
+template <typename F>
+static th_qweight* new_weight(th_device* dev, size_t rows, size_t cols, F&& fill) {
+    DeviceScope scope(dev);
+    th_qweight* w = new th_qweight();
+    w->dev = dev;
+    w->bits = 8;
+    w->rows = rows;
+    w->cols = cols;
+    w->Np = round_up(rows, 16);
+    w->Kp = round_up(cols, 64);
+    w->scale_dtype = TH_F32;
+    w->per_row = true;
+    w->data_bytes = w->Np * w->Kp;
+    w->scale_bytes = w->Np * 4;
+    try {
+        TH_HIP(hipMalloc(&w->data, w->data_bytes));
+        TH_HIP(hipMalloc(&w->scales, w->scale_bytes));
+        fill(w);
+    } catch (...) {
+        (void)hipStreamSynchronize(dev->stream);
+        if (w->data) (void)hipFree(w->data);
+        if (w->scales) (void)hipFree(w->scales);
+        delete w;
+        throw;
+    }
+    device_retain(dev);
+    return w;
+}
+
+}  // namespace th
+
 using namespace th;
 
 extern "C" {
@@ -21,46 +62,31 @@ int th_quantize_rows(th_device* dev, const th_buffer* x, size_t m, size_t k, th_
     require_len(scale, TH_F32, m, "scale");
     TH_REQUIRE(scale != x, "scale must not be x");
     DeviceScope scope(dev);
-    launch_quantize_rows(x->ptr, x->dtype, m, k, (int8_t*)q->ptr, (float*)scale->ptr, dev->stream);
+    launch_quantize_rows(x->ptr, x->dtype, m, k, (int8_t*)q->ptr, (float*)scale->ptr, false, dev->stream);
     TH_API_END
 }
 
 int th_q8_pack_rows(th_device* dev, const th_buffer* q, const th_buffer* scale, size_t rows, size_t cols, th_qweight** out) {
     TH_API_BEGIN
     TH_REQUIRE(dev && q && scale && out, "null argument");
-    TH_REQUIRE(!dev->closed, "the device was destroyed");
     TH_REQUIRE(q->dev == dev && scale->dev == dev, "a buffer is on another device handle");
-    TH_REQUIRE(rows > 0 && cols > 0, "empty matrix");
-    TH_REQUIRE(rows < (size_t)1 << 27 && cols <= I8_MAX_K, "sizes out of range");
-    TH_REQUIRE(!dev->capturing, "packs a new weight: not while a graph is captured");
-    const size_t Np = round_up(rows, 16), Kp = round_up(cols, 64);
-    require_len(q, TH_I8, rows * Kp, "q");
+    require_weight(dev, rows, cols);
+    require_len(q, TH_I8, rows * round_up(cols, 64), "q");
     require_len(scale, TH_F32, rows, "scale");
-    DeviceScope scope(dev);
-    th_qweight* w = new th_qweight();
-    w->dev = dev;
-    w->bits = 8;
-    w->rows = rows;
-    w->cols = cols;
-    w->Np = Np;
-    w->Kp = Kp;
-    w->scale_dtype = TH_F32;
-    w->per_row = true;
-    w->data_bytes = Np * Kp;
-    w->scale_bytes = Np * 4;
-    try {
-        TH_HIP(hipMalloc(&w->data, w->data_bytes));
-        TH_HIP(hipMalloc(&w->scales, w->scale_bytes));
-        launch_q8_pack((const int8_t*)q->ptr, (const float*)scale->ptr, w, dev->stream);
-    } catch (...) {
-        (void)hipStreamSynchronize(dev->stream);
-        if (w->data) (void)hipFree(w->data);
-        if (w->scales) (void)hipFree(w->scales);
-        delete w;
-        throw;
-    }
-    device_retain(dev);
-    *out = w;
+    *out = new_weight(dev, rows, cols, [&](const th_qweight* w) { launch_q8_pack((const int8_t*)q->ptr, (const float*)scale->ptr, w, dev->stream); });
+    TH_API_END
+}
+
+int th_q8_quantize(th_device* dev, const th_buffer* x, size_t rows, size_t cols, th_qweight** out) {
+    TH_API_BEGIN
+    TH_REQUIRE(dev && x && out, "null argument");
+    TH_REQUIRE(x->dev == dev, "a buffer is on another device handle");
+    TH_REQUIRE(x->dtype == TH_F32 || x->dtype == TH_F16 || x->dtype == TH_BF16, "x must be f32, f16 or bf16");
+    require_weight(dev, rows, cols);
+    require_len_any(x, rows * cols, "x");
+    *out = new_weight(dev, rows, cols, [&](const th_qweight* w) {
+        launch_quantize_rows(x->ptr, x->dtype, rows, cols, (int8_t*)w->data, (float*)w->scales, true, dev->stream);
+    });
     TH_API_END
 }
 

@@ -10,15 +10,6 @@ namespace th {
 // Rows to integers
 // ---------------------------------------------------------------------------
 
-// Eight consecutive elements at any element's alignment, as f32.
-template <typename X>
-__device__ __forceinline__ void load8_any(const X* p, float (&v)[8]) {
-    typedef X x8 __attribute__((ext_vector_type(8), aligned(sizeof(X))));
-    const x8 t = *(const x8*)p;
-#pragma unroll
-    for (int i = 0; i < 8; i++) v[i] = (float)t[i];
-}
-
 // x / s to the nearest integer, ties to even, exactly: the rounded product with
 // the reciprocal is off by one at most, and the rest x - q s has no rounding
 // (it is a multiple of the smaller operand's last bit and not above s).
@@ -49,83 +40,101 @@ struct RowScale {
     }
 };
 
-// One workgroup a row; C chunks of eight elements stay in a thread's registers
-// between the search for the largest and the rounding, so x is read once (0: any
-// length, read twice).
-template <typename X, int C>
-__global__ __launch_bounds__(256) void quantize_rows_kernel(const X* __restrict__ x, size_t m, int K, int Kp, int8_t* __restrict__ q,
-                                                            float* __restrict__ scale) {
-    __shared__ uint32_t red[4];
-    const int tid = threadIdx.x;
-    for (size_t row = blockIdx.x; row < m; row += gridDim.x) {
-        const X* xr = x + row * K;
-        uint2* qr = (uint2*)(q + row * Kp);
-        auto load = [&](int c, float (&v)[8]) {
-            const int k = c * 8;
-            if (k + 8 <= K) {
-                load8_any(xr + k, v);
-            } else {
+// WPR waves a row, ROWS rows a workgroup; a lane has 16 consecutive elements, one
+// piece of a block, and up to IT pieces stay in its registers between the search
+// for the largest and the rounding (0: any length, read twice).  Few rows: four
+// waves each, for the latency of one.  Many: sixteen rows a workgroup, which fill
+// their blocks' lines together.
+template <typename X, int WPR, int ROWS, int IT>
+__global__ __launch_bounds__(64 * WPR * ROWS) void quantize_rows_kernel(const X* __restrict__ x, int m, int K, int Kp, int8_t* __restrict__ q,
+                                                                        float* __restrict__ scale, int whole) {
+    typedef X x16_t __attribute__((ext_vector_type(16), aligned(sizeof(X))));
+    typedef X r16_t __attribute__((ext_vector_type(16)));
+    __shared__ uint32_t red[WPR * ROWS];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, t = (wave % WPR) * 64 + lane;
+    const int row = blockIdx.x * ROWS + wave / WPR;
+    const bool there = row < m;
+    const X* xr = x + (size_t)(there ? row : 0) * K;
+    auto load = [&](int c) -> r16_t {
+        const int k = c * 16;
+        if (there && k + 16 <= K) return *(const x16_t*)(xr + k);
+        r16_t r;
 #pragma unroll
-                for (int i = 0; i < 8; i++) v[i] = k + i < K ? (float)xr[k + i] : 0.0f;
-            }
-        };
-        float v[C ? C : 1][8];
-        uint32_t top = 0;
-        auto look = [&](const float (&t)[8]) {
+        for (int i = 0; i < 16; i++) r[i] = there && k + i < K ? xr[k + i] : (X)0.0f;
+        return r;
+    };
+    uint32_t top = 0;
+    auto look = [&](const r16_t& r) {
 #pragma unroll
-            for (int i = 0; i < 8; i++) top = max(top, __float_as_uint(t[i]) & 0x7FFFFFFFu);
-        };
-        if constexpr (C > 0) {
+        for (int i = 0; i < 16; i++) top = max(top, __float_as_uint((float)r[i]) & 0x7FFFFFFFu);
+    };
+    r16_t held[IT ? IT : 1];
+    if constexpr (IT > 0) {
 #pragma unroll
-            for (int c = 0; c < C; c++) load(c * 256 + tid, v[c]);
+        for (int i = 0; i < IT; i++) held[i] = load(i * 64 * WPR + t);
 #pragma unroll
-            for (int c = 0; c < C; c++) look(v[c]);
-        } else {
-            for (int c = tid; c * 8 < K; c += 256) {
-                load(c, v[0]);
-                look(v[0]);
-            }
-        }
+        for (int i = 0; i < IT; i++) look(held[i]);
+    } else {
+        for (int c = t; c * 16 < K; c += 64 * WPR) look(load(c));
+    }
 #pragma unroll
-        for (int o = 32; o > 0; o >>= 1) top = max(top, (uint32_t)__shfl_xor((int)top, o, 64));
-        if ((tid & 63) == 0) red[tid >> 6] = top;
+    for (int o = 32; o > 0; o >>= 1) top = max(top, (uint32_t)__shfl_xor((int)top, o, 64));
+    if constexpr (WPR > 1) {
+        if (lane == 0) red[wave] = top;
         __syncthreads();
-        const RowScale rs(max(max(red[0], red[1]), max(red[2], red[3])));
-        __syncthreads();
-        if (tid == 0) scale[row] = rs.s;
-        if constexpr (C > 0) {
 #pragma unroll
-            for (int c = 0; c < C; c++)
-                if ((c * 256 + tid) * 8 < Kp) qr[c * 256 + tid] = make_uint2(rs.four(v[c]), rs.four(v[c] + 4));
-        } else {
-            for (int c = tid; c * 8 < Kp; c += 256) {
-                load(c, v[0]);
-                qr[c] = make_uint2(rs.four(v[0]), rs.four(v[0] + 4));
-            }
-        }
+        for (int i = 0; i < WPR; i++) top = max(top, red[wave / WPR * WPR + i]);
+    }
+    const int first = row & ~15, h = whole ? 16 : min(16, m - first);
+    if (!there && !(whole && first < m)) return;
+    const RowScale rs(top);
+    if (t == 0) scale[row] = rs.s;
+    uint4* const to = (uint4*)(q + (size_t)first * Kp) + (row & 15);
+    auto put = [&](int c, const r16_t& r) {
+        if (c * 16 >= Kp) return;
+        float v[16];
+#pragma unroll
+        for (int i = 0; i < 16; i++) v[i] = (float)r[i];
+        to[(size_t)c * h] = make_uint4(rs.four(v), rs.four(v + 4), rs.four(v + 8), rs.four(v + 12));
+    };
+    if constexpr (IT > 0) {
+#pragma unroll
+        for (int i = 0; i < IT; i++) put(i * 64 * WPR + t, held[i]);
+    } else {
+        for (int c = t; c * 16 < Kp; c += 64 * WPR) put(c, load(c));
     }
 }
 
 template <typename X>
-static void quantize_types(const void* x, size_t m, size_t K, size_t Kp, int8_t* q, float* scale, hipStream_t s) {
-    const dim3 grid((unsigned)std::min<size_t>(m, (size_t)1 << 20));
-    auto go = [&](auto c) {
-        TH_LAUNCH((quantize_rows_kernel<X, decltype(c)::value>), grid, dim3(256), 0, s, (const X*)x, m, (int)K, (int)Kp, q, scale);
+static void quantize_types(const void* x, size_t m, size_t K, size_t Kp, int8_t* q, float* scale, bool whole, hipStream_t s) {
+    auto go = [&](auto wpr, auto rows, auto it) {
+        constexpr int W = decltype(wpr)::value, R = decltype(rows)::value;
+        const size_t n = whole ? round_up(m, 16) : m;
+        TH_LAUNCH((quantize_rows_kernel<X, W, R, decltype(it)::value>), dim3((unsigned)ceil_div(n, (size_t)R)), dim3(64 * W * R), 0, s, (const X*)x,
+                  (int)m, (int)K, (int)Kp, q, scale, (int)whole);
     };
-    if (Kp <= 2048) go(std::integral_constant<int, 1>{});
-    else if (Kp <= 4096) go(std::integral_constant<int, 2>{});
-    else if (Kp <= 8192) go(std::integral_constant<int, 4>{});
-    else if (Kp <= 16384) go(std::integral_constant<int, 8>{});
-    else go(std::integral_constant<int, 0>{});
+    using std::integral_constant;
+    const integral_constant<int, 1> one;
+    const integral_constant<int, 4> four;
+    if (m >= 1024 && Kp <= 4096) go(one, integral_constant<int, 16>{}, four);
+    else if (m >= 1024 && Kp <= 16384) go(four, four, four);
+    else if (Kp <= 4096) go(four, one, one);
+    else if (Kp <= 16384) go(four, one, four);
+    else go(four, one, integral_constant<int, 0>{});
     TH_LAUNCH_CHECK();
 }
 
-void launch_quantize_rows(const void* x, th_dtype xdt, size_t m, size_t K, int8_t* q, float* scale, hipStream_t s) {
-    if (m == 0) return;
+void launch_quantize_rows(const void* x, th_dtype xdt, size_t m, size_t K, int8_t* q, float* scale, bool whole, hipStream_t s) {
+    constexpr size_t ROWS = (size_t)1 << 22;  // a launch has below 2^32 threads
     const size_t Kp = round_up(K, 64);
-    if (xdt == TH_F32) quantize_types<float>(x, m, K, Kp, q, scale, s);
-    else if (xdt == TH_F16) quantize_types<_Float16>(x, m, K, Kp, q, scale, s);
-    else quantize_types<__bf16>(x, m, K, Kp, q, scale, s);
+    for (size_t m0 = 0; m0 < m; m0 += ROWS) {
+        const void* xo = (const char*)x + m0 * K * dtype_size(xdt);
+        const size_t n = std::min(ROWS, m - m0);
+        int8_t* qo = q + m0 * Kp;
+        if (xdt == TH_F32) quantize_types<float>(xo, n, K, Kp, qo, scale + m0, whole, s);
+        else if (xdt == TH_F16) quantize_types<_Float16>(xo, n, K, Kp, qo, scale + m0, whole, s);
+        else quantize_types<__bf16>(xo, n, K, Kp, qo, scale + m0, whole, s);
+    }
 }
 
 // Rows of int8 into the tiles of th_qweight, and their scales: zeros behind K and the last row.

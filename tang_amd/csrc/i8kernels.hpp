@@ -50,10 +50,15 @@ __global__ __launch_bounds__(64 * NW) void i8_rows_kernel(const uint4* __restric
     const int bx = blockIdx.x, NCH = Kp >> 6, NT = (out.N + 15) >> 4;
     const i32x4_t* w[RT];
     const i32x4_t* x[CB];
+    int xstep[CB];
 #pragma unroll
     for (int a = 0; a < RT; a++) w[a] = (const i32x4_t*)wt + (size_t)min(bx * RT + a, NT - 1) * NCH * 64 + lane;
 #pragma unroll
-    for (int b = 0; b < CB; b++) x[b] = (const i32x4_t*)(xq + (size_t)min(b * 16 + r, M - 1) * Kp) + q;
+    for (int b = 0; b < CB; b++) {  // rows past the end re-read the last one
+        const int first = min(b, (M - 1) >> 4) * 16, h = min(16, M - first);
+        x[b] = (const i32x4_t*)(xq + (size_t)first * Kp) + q * h + min(r, h - 1);
+        xstep[b] = 4 * h;
+    }
     i32x4_t acc[RT][CB];
 #pragma unroll
     for (int a = 0; a < RT; a++)
@@ -68,7 +73,7 @@ __global__ __launch_bounds__(64 * NW) void i8_rows_kernel(const uint4* __restric
 #pragma unroll
                 for (int a = 0; a < RT; a++) wv[u][a] = __builtin_nontemporal_load(w[a] + (size_t)c * 64);
 #pragma unroll
-                for (int b = 0; b < CB; b++) xv[u][b] = x[b][(size_t)c * 4];
+                for (int b = 0; b < CB; b++) xv[u][b] = x[b][(size_t)c * xstep[b]];
             } else {
 #pragma unroll
                 for (int a = 0; a < RT; a++) wv[u][a] = (i32x4_t){0, 0, 0, 0};
@@ -133,11 +138,16 @@ __global__ __launch_bounds__(256 * KW) __attribute__((amdgpu_waves_per_eu(WPE, W
     gemm_xcd_tile(bx, by, bz);
     const int NCH = Kp >> 6, NT = (out.N + 15) >> 4;
     const int m0 = by * 64 * TM, n0 = bx * 64 * TN;
-    // this wave's blocks: rows past the end re-read the last one
+    // this wave's blocks: those past the end re-read the last one
     uint32_t xo[TM], wo[TN];
-    const int mlast = M - 1 - m0, tlast = NT - 1 - n0 / 16;
+    int xstep[TM];
+    const int mlast = (M - 1 - m0) >> 4, tlast = NT - 1 - n0 / 16;
 #pragma unroll
-    for (int i = 0; i < TM; i++) xo[i] = (uint32_t)min((wave * TM + i) * 16 + (lane & 15), mlast) * (uint32_t)Kp + (lane >> 4) * 16;
+    for (int i = 0; i < TM; i++) {
+        const int blk = min(wave * TM + i, mlast), h = min(16, M - m0 - blk * 16);
+        xo[i] = (uint32_t)blk * 16u * (uint32_t)Kp + ((lane >> 4) * h + min(lane & 15, h - 1)) * 16;
+        xstep[i] = 64 * h;
+    }
 #pragma unroll
     for (int i = 0; i < TN; i++) wo[i] = (uint32_t)min(wave * TN + i, tlast) * (uint32_t)NCH * 1024u + lane * 16;
     const __amdgpu_buffer_rsrc_t xb = buffer_rsrc(xq + (size_t)m0 * Kp, (uint32_t)(min(M - m0, 64 * TM) * Kp));
@@ -147,7 +157,7 @@ __global__ __launch_bounds__(256 * KW) __attribute__((amdgpu_waves_per_eu(WPE, W
     i32x4_t g[ST][TM + TN];
     auto chunk = [&](int s) { return max(0, min(s * KW + group - lead, NCH - 1)); };
     auto gload = [&](int set, int c, int i) {
-        const auto v = i < TM ? __builtin_amdgcn_raw_buffer_load_b128(xb, (int)xo[i < TM ? i : 0], c * 64, 0)
+        const auto v = i < TM ? __builtin_amdgcn_raw_buffer_load_b128(xb, (int)xo[i < TM ? i : 0], c * xstep[i < TM ? i : 0], 0)
                               : __builtin_amdgcn_raw_buffer_load_b128(wb, (int)wo[i < TM ? 0 : i - TM], c * 1024, 0);
         g[set][i] = __builtin_bit_cast(i32x4_t, v);
     };

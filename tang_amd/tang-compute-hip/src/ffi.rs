@@ -224,6 +224,7 @@ extern "C" {
     pub fn th_gemm_q4(dev: *mut th_device, x: *const th_buffer, m: usize, w: *const th_qweight, y: *mut th_buffer) -> c_int;
     pub fn th_gemv_q8(dev: *mut th_device, x: *const th_buffer, m: usize, w: *const th_qweight, y: *mut th_buffer) -> c_int;
     pub fn th_quantize_rows(dev: *mut th_device, x: *const th_buffer, m: usize, k: usize, q: *mut th_buffer, scale: *mut th_buffer) -> c_int;
+    pub fn th_q8_quantize(dev: *mut th_device, x: *const th_buffer, rows: usize, cols: usize, out: *mut *mut th_qweight) -> c_int;
     pub fn th_q8_pack_rows(dev: *mut th_device, q: *const th_buffer, scale: *const th_buffer, rows: usize, cols: usize, out: *mut *mut th_qweight) -> c_int;
     pub fn th_gemm_i8(dev: *mut th_device, xq: *const th_buffer, x_scale: *const th_buffer, m: usize, w: *const th_qweight, bias: *const th_buffer, y: *mut th_buffer) -> c_int;
     pub fn th_gemm_q4_noalloc(dev: *mut th_device, x: *const th_buffer, m: usize, w: *const th_qweight, y: *mut th_buffer) -> c_int;

@@ -8,7 +8,7 @@
 namespace th {
 
 static size_t g_m, g_k;  // of the last launch
-void launch_quantize_rows(const void* x, th_dtype, size_t m, size_t K, int8_t* q, float* scale, hipStream_t) {
+void launch_quantize_rows(const void* x, th_dtype, size_t m, size_t K, int8_t* q, float* scale, bool, hipStream_t) {
     CHECK(x && q && scale);
     g_m = m;
     g_k = K;

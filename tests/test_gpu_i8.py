@@ -15,6 +15,13 @@ def _kp(k):
     return -(-k // 64) * 64
 
 
+def _places(m, k):
+    """Where value (i, k) lies in quantized rows."""
+    i, kk = np.arange(m)[:, None], np.arange(k)[None]
+    first = i - i % 16
+    return first * _kp(k) + (kk - kk % 16) * np.minimum(16, m - first) + i % 16 * 16 + kk % 16
+
+
 def _quantized(x):
     """(q, scale) of f32 rows. In 64 bits x / s is off by 2^-46 at most, and x / s that is not on a half is at least 2^-26 from it."""
     top = np.abs(x).max(1)
@@ -33,14 +40,14 @@ def _quantize(dev, x, dt):
     dev.quantize_rows(dev.upload(to_bits(x, dt), dt), m, k, q, s)
     gq, gs = q.to_numpy(), s.to_numpy()
     assert np.all(gq[m * _kp(k):] == 99) and gs[m] == 99
-    gq = gq[:m * _kp(k)].reshape(m, _kp(k))
+    gq = gq[_places(m, _kp(k))]
     assert not gq[:, k:].any()
     return gq[:, :k], gs[:m]
 
 
 @pytest.mark.parametrize("dt", [F32, F16, BF16])
 @pytest.mark.parametrize("m,k", [(1, 1), (3, 2), (5, 63), (2, 64), (7, 65), (4, 2047), (3, 2048), (2, 4095), (3, 4097), (2, 8192), (2, 11008), (3, 16385),
-                                 (2, 131071), (300, 130)])
+                                 (2, 131071), (300, 130), (16, 640), (17, 4097), (1024, 33), (1030, 4096), (1040, 5000), (1025, 16400)])
 def test_quantize(dev, dt, m, k):
     rng = np.random.default_rng(m * 100 + k)
     x = rng.standard_normal((m, k)) * np.exp(rng.uniform(-8, 8, (m, 1)))
@@ -93,8 +100,8 @@ def _run(dev, rng, m, k, n, dt=F32, bias=False, w=None):
     q, wq = (rng.integers(-128, 128, (r, k)).astype(np.int8) for r in (m, n))
     s, t = (np.exp(rng.uniform(-9, 3, r)).astype(np.float32) for r in (m, n))
     b = rng.standard_normal(n).astype(np.float32) if bias else None
-    rows = rng.integers(-128, 128, (m, _kp(k))).astype(np.int8)
-    rows[:, :k] = q
+    rows = rng.integers(-128, 128, m * _kp(k)).astype(np.int8)
+    rows[_places(m, _kp(k))[:, :k]] = q
     w = dev.q8_upload_rowwise(wq, t, n, k)
     y = dev.upload(np.full(m * n + 7, 9.0, np.float32) if dt == F32 else np.full(m * n + 7, 0x1234, np.uint16), dt)
     dev.gemm_i8(dev.upload(rows, I8), dev.upload(s), m, w, y, None if b is None else dev.upload(b))
@@ -135,8 +142,8 @@ def test_product_of_the_largest(dev):
     k = 131071
     for m in (2, 40, 300):
         q, w = np.full((m, k), -128, np.int8), np.full((5, k), -128, np.int8)
-        rows = np.zeros((m, _kp(k)), np.int8)
-        rows[:, :k] = q
+        rows = np.zeros(m * _kp(k), np.int8)
+        rows[_places(m, _kp(k))[:, :k]] = q
         s = np.where(np.arange(m) % 2 == 0, 1e-30, 2e36).astype(np.float32)
         t = np.array([1e-30, 1e-10, 1.0, 0.0, 1e30], np.float32)
         y = dev.gemm_i8(dev.upload(rows, I8), dev.upload(s), m, dev.q8_upload_rowwise(w, t, 5, k))
@@ -177,7 +184,9 @@ def test_packed_weights(dev, rows, cols):
     a, b = dev.q8_upload_rowwise(wq, t, rows, cols), dev.q8_pack_rows(dev.upload(noisy, I8), dev.upload(t), rows, cols)
     x = dev.upload(rng.standard_normal((5, cols)).astype(np.float32))
     q, s = dev.quantize_rows(x, 5, cols)
-    q.upload(np.where(np.arange(q.n) % _kp(cols) < cols, q.to_numpy(), 77))
+    behind = q.to_numpy()
+    behind[_places(5, _kp(cols))[:, cols:]] = 77
+    q.upload(behind)
     assert np.array_equal(dev.gemv_q8(x, 5, a).to_numpy(), dev.gemv_q8(x, 5, b).to_numpy())
     assert np.array_equal(dev.gemm_i8(q, s, 5, a).to_numpy(), dev.gemm_i8(q, s, 5, b).to_numpy())
 
@@ -189,13 +198,29 @@ def test_weights_quantized_on_the_device(dev):
     rng = np.random.default_rng(4)
     m, k, n = 70, 900, 130
     x, w = rng.standard_normal((m, k)).astype(np.float32), rng.standard_normal((n, k)).astype(np.float32)
-    qw, tw = dev.quantize_rows(dev.upload(w), n, k)
     qx, sx = dev.quantize_rows(dev.upload(x), m, k)
-    y = dev.gemm_i8(qx, sx, m, dev.q8_pack_rows(qw, tw, n, k)).to_numpy().reshape(m, n)
-    s, t = sx.to_numpy().astype(np.float64)[:, None], tw.to_numpy().astype(np.float64)
+    y = dev.gemm_i8(qx, sx, m, dev.q8_quantize(dev.upload(w), n, k)).to_numpy().reshape(m, n)
+    qw, tw = _quantized(w)
+    assert np.array_equal(y, _product(_quantized(x)[0], _quantized(x)[1], qw, tw, None))
+    s, t = sx.to_numpy().astype(np.float64)[:, None], tw.astype(np.float64)
     bound = np.abs(x).sum(1, dtype=np.float64)[:, None] * t / 2 + np.abs(w).sum(1, dtype=np.float64) * s / 2 + k * s * t / 4
     want = x.astype(np.float64) @ w.astype(np.float64).T
     assert np.all(np.abs(y - want) <= bound * (1 + 2.0 ** -20))
+
+
+@pytest.mark.parametrize("dt", [F32, BF16, F16])
+@pytest.mark.parametrize("rows,cols", [(1, 1), (15, 64), (16, 100), (33, 4097), (1100, 130), (1030, 4200), (2, 20000)])
+def test_weight_of_a_matrix(dev, dt, rows, cols):
+    """th_q8_quantize's weight is the one that the quantized rows make: rows behind the last in its tiles are zeros."""
+    rng = np.random.default_rng(rows + cols)
+    w = rounded(rng.standard_normal((rows, cols)).astype(np.float32), dt)
+    q, s = _quantized(w)
+    x = dev.upload(rng.standard_normal((3, cols)).astype(np.float32))
+    qx, sx = dev.quantize_rows(x, 3, cols)
+    a, b = dev.q8_quantize(dev.upload(to_bits(w, dt), dt), rows, cols), dev.q8_upload_rowwise(q, s, rows, cols)
+    assert np.array_equal(dev.gemm_i8(qx, sx, 3, a).to_numpy(), dev.gemm_i8(qx, sx, 3, b).to_numpy())
+    if cols < 5000:
+        assert np.array_equal(dev.gemv_q8(x, 3, a).to_numpy(), dev.gemv_q8(x, 3, b).to_numpy())
 
 
 def test_captured(dev):

@@ -62,6 +62,18 @@ def test_pack_and_product(lib):
         f.refused("hipMalloc", code=capi.TH_ERR_OOM)
     lib.host_fail(-1)
 
+    x = c.buffer(20 * 70, F32)
+    z = Refusals(c, "th_q8_quantize", dev=c.dev, x=x, rows=20, cols=70, out=ctypes.byref(out))
+    z.call()
+    c.call("th_qweight_free", ctypes.c_void_p(out.value))
+    z.refused("null", x=None)
+    z.refused("null", out=None)
+    z.refused("empty", rows=0)
+    z.refused("out of range", cols=1 << 17)
+    z.refused("another device", x=other.buffer(20 * 70, F32))
+    z.refused("buffer x .*too small", x=c.buffer(20 * 70 - 1, F32))
+    z.refused("f32, f16 or bf16", x=c.buffer(20 * 70, I8))
+
     y = c.buffer(3 * 20, F32)
     g = Refusals(c, "th_gemm_i8", dev=c.dev, xq=c.buffer(3 * 128, I8), xs=c.buffer(3, F32), m=3, w=w, bias=None, y=y)
     g.call()
@@ -87,6 +99,6 @@ def test_pack_and_product(lib):
     lib.host_grouped(w, 8, 1)
     g.call()
     c.call("th_qweight_free", w)
-    with pytest.raises(Refused, match="capture"):
-        c.call("th_capture_begin", c.dev)
-        f.call()
+    c.call("th_capture_begin", c.dev)
+    f.refused("capture")
+    z.refused("capture")

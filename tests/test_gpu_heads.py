@@ -159,6 +159,36 @@ def test_no_rows_and_many(dev):
 
 
 @pytest.mark.parametrize("half", [0, 1])
+def test_many_heads_a_group(dev, half):
+    """So many rows that lanes take several heads of a row, whose number is no multiple of theirs; in place too, and into pages."""
+    rng = np.random.default_rng(7 + half)
+    n, H, K, hd = 30000, 7, 2, 64
+    cos, sin, dc, ds = _tables(dev, 48, n)
+    w, dw = _weights(dev, rng, hd, F32)
+    x = rounded(2 * _normal(rng, n, H + K, hd), BF16)
+    dx = dev.upload(to_bits(x, BF16), BF16)
+    args = (dx, None, *dw, 1e-6, dc, ds, n, H, K, hd, 48, half)
+    q, k = dev.qk_norm_rope(*args)
+    want = [_formula(t, v, 1e-6, cos, sin, np.arange(n), 48, half) for t, v in ((x[:, :H], w[0]), (x[:, H:], w[1]))]
+    _check(from_bits(q.to_numpy(), BF16).reshape(n, H, hd), want[0], BF16)
+    _check(from_bits(k.to_numpy(), BF16).reshape(n, K, hd), want[1], BF16)
+    dev.qk_norm_rope(*args, q_out=dx)
+    got = dx.to_numpy().reshape(n, H + K, hd)
+    assert np.array_equal(got[:, :H].reshape(-1), q.to_numpy()) and np.array_equal(got[:, H:].reshape(-1), k.to_numpy())
+    # 30000 rows of 6 + 2 + 2 heads into pages
+    cache = dev.kv_cache(1, K, hd, 64, 480, 1, n, F16)
+    batch, seqs = cache.batch(1, n, 6), cache.seq_create(1)
+    batch.begin(seqs, [n])
+    x = rounded(2 * _normal(rng, n, 6 + 2 * K, hd), F16)
+    out = dev.alloc(n * 6 * hd, F16)
+    batch.append_norm(0, dev.upload(to_bits(x, F16), F16), None, None, out, *dw, 1e-6, dc, ds, 48, half)
+    _check(from_bits(out.to_numpy(), F16).reshape(n, 6, hd), _formula(x[:, :6], w[0], 1e-6, cos, sin, np.arange(n), 48, half), F16)
+    gk, gv = (from_bits(b.to_numpy(), F16).reshape(n, K, hd) for b in cache.seq_read(seqs[0], 0))
+    _check(gk, _formula(x[:, 6:8], w[1], 1e-6, cos, sin, np.arange(n), 48, half), F16)
+    assert np.array_equal(gv, x[:, 8:])
+
+
+@pytest.mark.parametrize("half", [0, 1])
 @pytest.mark.parametrize("hd,rot,heads", [(64, 64, 4), (128, 128, 6), (80, 48, 2), (96, 20, 2), (256, 96, 8)])
 @pytest.mark.parametrize("xdt,cdt,odt", [(F32, F16, F32), (BF16, BF16, BF16), (F16, BF16, F32)])
 @pytest.mark.parametrize("packed", [False, True])

@@ -18,16 +18,17 @@
 
 namespace th {
 
-constexpr int SNT = 1024, SBINS = 2048, SLIST = 64, SCAP = 4096;
+constexpr int SNT = 1024, SBINS = 2048, SLIST = 64, SCAP = 4096, SBITS = 5, STABLE = 1 << SBITS;
+typedef uint32_t u32x2_t __attribute__((ext_vector_type(2)));
 typedef unsigned long long u64_t;
 
 struct SampleLds {
     u64_t sum[SBINS];
     uint32_t count[SBINS];
-    double table[64];  // 2^(i / 64)
+    double table[STABLE];  // 2^(S + i / STABLE), its high word less i << 10
     u64_t list_w[SLIST];
     uint32_t list_key[SLIST];
-    u64_t wave[SNT / 64], wave2[SNT / 64];
+    u64_t wave[SNT / 64], wave2[SNT / 64], part[SNT / 64];
     u64_t above, eq, end;
     uint32_t bin, key, n, lo, hi, found;
     u64_t list[SCAP];  // order_entry's of candidates
@@ -38,6 +39,12 @@ static __shared__ SampleLds s;
 
 __device__ __forceinline__ u64_t shfl_up64(u64_t v, int d) {
     const uint32_t lo = (uint32_t)__shfl_up((int)(uint32_t)v, d, 64), hi = (uint32_t)__shfl_up((int)(v >> 32), d, 64);
+    return (u64_t)hi << 32 | lo;
+}
+__device__ __forceinline__ uint32_t uniform(uint32_t v) { return (uint32_t)__builtin_amdgcn_readfirstlane((int)v); }
+__device__ __forceinline__ float uniform(float v) { return __uint_as_float(uniform(__float_as_uint(v))); }
+__device__ __forceinline__ u64_t shfl_64(u64_t v, int from) {
+    const uint32_t lo = (uint32_t)__shfl((int)(uint32_t)v, from, 64), hi = (uint32_t)__shfl((int)(v >> 32), from, 64);
     return (u64_t)hi << 32 | lo;
 }
 __device__ __forceinline__ u64_t wave_scan(u64_t v, int lane) {  // inclusive
@@ -55,93 +62,112 @@ __device__ __forceinline__ u64_t wave_total(u64_t v) {
     return v;
 }
 
-// Order of f32 values as unsigned integers (a -0 is made +0 before).
+// Order of f32 values as unsigned integers.
 __device__ __forceinline__ uint32_t order_key(float v) {
-    const uint32_t b = __float_as_uint(v);
+    const uint32_t b = __float_as_uint(v + 0.0f);  // (-0 as +0)
     return b & 0x80000000u ? ~b : b | 0x80000000u;
 }
 
-// A row's logits: thread t has elements (j 1024 + t) 8 + e of block j.  A pass
-// streams them, two blocks at a time and two ahead (later passes from the
-// caches).  Rows held in registers were slower: every pass is unrolled then, and 32 logits
-// a thread no longer fit the instruction cache (32000 logits, no filter: 28 against 18.5 us).
+// A row's logits.  A wave has a sixteenth of them, as they lie, and of its block j
+// a lane has eight, so that sums by wave are sums of runs of indexes.  A pass
+// streams them, two blocks ahead (later passes from the caches).  Rows held in
+// registers were slower by half: every pass is unrolled then, and 32 logits a thread no longer fit the instruction cache.
 template <typename X>
 struct SampleRow {
     typedef X x8_t __attribute__((ext_vector_type(8), aligned(sizeof(X))));
     typedef X r8_t __attribute__((ext_vector_type(8)));
     const X* x;
-    int V, blocks;
+    int V, blocks, start;  // start: of the wave
+    bool infinite;  // the largest is +inf: such logits count as 0 and all others as -inf
 
-    __device__ __forceinline__ r8_t read(int j) const {
-        const int i = (j * SNT + (int)threadIdx.x) * 8;
-        if (i + 8 <= V) return *(const x8_t*)(x + i);
+    __device__ __forceinline__ SampleRow(const X* at, int n, bool inf)
+        : x(at), V(n), blocks((n + SNT * 8 - 1) / (SNT * 8)), start((int)uniform(threadIdx.x >> 6) * blocks * 512), infinite(inf) {}
+    // Eight a lane from index `at` of the wave on, -inf from `end` on (at most V).  All branches are the whole wave's:
+    // where lanes took ways of their own at the end of a row and registers were short, the compiler copied
+    // some before all lanes were back, and the others lost what was in them.
+    __device__ __forceinline__ r8_t read_at(int at, int end) const {
+        const int i = at + ((int)threadIdx.x & 63) * 8;
         r8_t r;
+        if (at + 512 <= end) {
+            r = *(const x8_t*)(x + i);
+        } else if (at < end) {
 #pragma unroll
-        for (int e = 0; e < 8; e++) r[e] = i + e < V ? x[i + e] : (X)-INFINITY;
+            for (int e = 0; e < 8; e++) r[e] = x[min(i + e, V - 1)];
+#pragma unroll
+            for (int e = 0; e < 8; e++) r[e] = i + e < end ? r[e] : (X)-INFINITY;
+        } else {
+#pragma unroll
+            for (int e = 0; e < 8; e++) r[e] = (X)-INFINITY;
+        }
         return r;
     }
-    __device__ __forceinline__ SampleRow(const X* at, int n) : x(at), V(n), blocks((n + SNT * 8 - 1) / (SNT * 8)) {}
-    // NaN as -inf, -0 as +0
-    static __device__ __forceinline__ void values(const r8_t& r, float (&v)[8]) {
+    __device__ __forceinline__ float value(float l) const { return !infinite ? l : l == INFINITY ? 0.0f : -INFINITY; }
+    __device__ __forceinline__ void values(const r8_t& r, float (&v)[8]) const {
 #pragma unroll
-        for (int e = 0; e < 8; e++) {
-            v[e] = (float)r[e] + 0.0f;
-            v[e] = v[e] == v[e] ? v[e] : -INFINITY;
+        for (int e = 0; e < 8; e++) v[e] = (float)r[e];
+        if (infinite) {
+#pragma unroll
+            for (int e = 0; e < 8; e++) v[e] = value(v[e]);
         }
     }
-    // f(block, the eight values); blocks behind the last hold -inf
+    // f(index of the first, the eight values); what lies behind the row holds -inf
     template <typename F>
     __device__ __forceinline__ void blocks_of(F&& f) const {
-        auto one = [&](int j, const r8_t& r) {
-            float v[8];
-            values(r, v);
-            f(j, v);
-        };
+        auto read = [&](int j) { return read_at(start + j * 512, j < blocks ? V : 0); };
         r8_t a = read(0), b = read(1);
 #pragma unroll 1
-        for (int j = 0; j < blocks; j += 2) {
-            const r8_t a0 = a, b0 = b;
-            a = read(j + 2);
-            b = read(j + 3);
-            one(j, a0);
-            one(j + 1, b0);
+        for (int j = 0; j < blocks; j++) {
+            const r8_t now = a;
+            a = b;
+            b = read(j + 2);
+            float v[8];
+            values(now, v);
+            f(start + j * 512 + ((int)threadIdx.x & 63) * 8, v);
         }
     }
+    __device__ __forceinline__ int passed() const { return blocks * 8; }  // logits of a lane in a pass, with those behind the end
     template <typename F>
     __device__ __forceinline__ void each(F&& f) const {
-        blocks_of([&](int j, const float (&v)[8]) {
+        blocks_of([&](int i, const float (&v)[8]) {
 #pragma unroll
-            for (int e = 0; e < 8; e++) f((j * SNT + (int)threadIdx.x) * 8 + e, v[e]);
+            for (int e = 0; e < 8; e++) f(i + e, v[e]);
         });
     }
 };
 
 // Weights of a row.
 struct SampleWeights {
-    float M, cf, limit;
-    double c, Mc;  // log2(e) / T; times M
+    float M, cb;  // cb: bins a unit of a logit
+    double Md, c, least;  // c: log2(e) / T in steps of the table
     int S;
     const double* table;
 
-    // Bits that a logit is below the largest, in f32: monotone in l, and what decides whether it has a weight at all.
-    __device__ __forceinline__ float below(float l) const { return l == M ? 0.0f : (M - l) * cf; }
-    __device__ __forceinline__ bool alive(float l) const { return below(l) < limit; }
-    // of a logit that is alive: 2^x = 2^n 2^(i/64) 2^r, the last by its series in r ln 2 to the fifth power (r up to 1/128: off by 2^-54)
-    __device__ __forceinline__ u64_t weight(float l) const {
-        if (l == M) return (u64_t)1 << S;
-        const double x = __builtin_fma((double)l, c, -Mc);
-        const double big = 0x1.8p52, y = __builtin_fma(x, 64.0, big);
-        const int k = (int)(uint32_t)(u64_t)__double_as_longlong(y);
-        const double r = __builtin_fma(y - big, -1.0 / 64, x);
-        double p = __builtin_fma(r, 1.3333558146428443e-3, 9.618129107628477e-3);  // ln(2)^n / n!
-        p = __builtin_fma(p, r, 5.550410866482158e-2);
-        p = __builtin_fma(p, r, 2.402265069591007e-1);
-        p = __builtin_fma(p, r, 6.931471805599453e-1);
+    // Bins that a logit is below the largest, in f32: monotone in l.  Bins have equal widths in the logarithm
+    // of the weight; behind the last (NaN, too) a weight is below 2^-(S+1).
+    __device__ __forceinline__ float below(float l) const { return (M - l) * cb; }
+    __device__ __forceinline__ bool alive(float l) const { return below(l) < (float)SBINS; }
+    __device__ __forceinline__ int bin_of(float l) const { return (int)min(below(l), (float)(SBINS - 1)); }
+    // w 2^S to the nearest, as the bits of 2^52 + w 2^S.  With x = n + i/32 + r the table has 2^(i/32), and
+    // 2^r is its series to the fifth power (r up to 2^-6: off by 2^-48).  All rows' elements pass through here,
+    // and as instructions are what the passes are bound by, there is no branch: a logit that has no weight, NaN
+    // too, is lifted to 2^-(S+2), which rounds to none (256 rows of 131072 without a filter: 44 us,
+    // 61 with such branches and 64 entries; 1024 entries and two terms less: 52, as lanes then meet in the banks).
+    __device__ __forceinline__ u64_t bits(float l) const {
+        const double big = 0x1.8p52, x = fmax(((double)l - Md) * c, least), y = x + big;
+        const uint32_t k = (uint32_t)(u64_t)__double_as_longlong(y);
+        const double r = x - (y - big);
+        constexpr double h = 1.0 / STABLE;
+        double p = __builtin_fma(r, 1.3333558146428443e-3 * h * h * h * h * h, 9.618129107628477e-3 * h * h * h * h);  // ln(2)^n / n!
+        p = __builtin_fma(p, r, 5.550410866482158e-2 * h * h * h);
+        p = __builtin_fma(p, r, 2.402265069591007e-1 * h * h);
+        p = __builtin_fma(p, r, 6.931471805599453e-1 * h);
         p = __builtin_fma(p, r, 1.0);
-        const double m = table[k & 63] * p;  // from 0.99 to 2
-        const double w = __longlong_as_double(__double_as_longlong(m) + ((long long)((k >> 6) + S) << 52));
-        return (u64_t)__double_as_longlong(w + 0x1p52) & (((u64_t)1 << 52) - 1);
+        u32x2_t m = __builtin_bit_cast(u32x2_t, table[k & (STABLE - 1)]);
+        m.y += k << (20 - SBITS);  // (the table's index is in both: it cancels)
+        return __builtin_bit_cast(u64_t, __builtin_fma(__builtin_bit_cast(double, m), p, 0x1p52));
     }
+    static constexpr u64_t NONE = (u64_t)0x43300000 << 32;  // the bits of 2^52
+    __device__ __forceinline__ u64_t weight(float l) const { return bits(l) - NONE; }
 };
 
 // The first of SBINS bins at which the running sum reaches target (1 to the sum of all): in s.bin, what lies
@@ -269,59 +295,73 @@ __device__ __forceinline__ void select_key(const Row& row, const SampleWeights& 
     __syncthreads();
 }
 
-// Of the part s.bin of a row (a wave's share of a block), the index at which the running sum of f(index, logit) reaches rest: in s.found.
-template <typename Row, typename F>
-__device__ __forceinline__ void pick_in(const Row& row, u64_t rest, F&& f) {
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, bin = (int)s.bin;
-    if ((bin & (SNT / 64 - 1)) != wave) return;
-    const int j = bin / (SNT / 64);
-    float v[8];
-    row.values(row.read(j), v);
-    u64_t mine = 0;
+// Sums of what the waves have in v: the sum of all, and what lies before each wave's.
+__device__ __forceinline__ u64_t over_waves(u64_t v, u64_t* room, u64_t& before) {
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    if (lane == 0) room[wave] = v;
+    __syncthreads();
+    u64_t all = 0;
 #pragma unroll
-    for (int e = 0; e < 8; e++) mine += f((j * SNT + tid) * 8 + e, v[e]);
-    u64_t upto = wave_scan(mine, lane) - mine;
-    if (!(upto < rest && rest <= upto + mine)) return;
-    bool done = false;
-#pragma unroll
-    for (int e = 0; e < 8; e++) {
-        upto += f((j * SNT + tid) * 8 + e, v[e]);
-        if (!done && upto >= rest) {
-            s.found = (uint32_t)((j * SNT + tid) * 8 + e);
-            done = true;
-        }
+    for (int w = 0; w < SNT / 64; w++) {
+        if (w == wave) before = all;
+        all += room[w];
     }
+    return all;
+}
+
+// The index at which the running sum, by index, of f(logits from an index on) reaches target, where s.part has the waves' sums: in s.found.
+template <typename Row, typename F>
+__device__ __forceinline__ void pick(const Row& row, u64_t target, F&& f) {
+    const int tid = threadIdx.x, lane = tid & 63;
+    int w = 0;
+    u64_t before = 0;
+    while (w < SNT / 64 - 1 && before + s.part[w] < target) before += s.part[w++];
+    u64_t rest = target - before;
+    // the wave's logits, by the whole block
+    const int first = (int)uniform((uint32_t)w) * row.blocks * 512, end = min(row.V, first + row.blocks * 512), wave = (int)uniform((uint32_t)tid >> 6);
+    for (int at = first; at < end; at += SNT * 8) {
+        const int i = at + tid * 8;
+        float v[8];
+        row.values(row.read_at(at + wave * 512, end), v);
+        u64_t mine = 0;
+#pragma unroll
+        for (int e = 0; e < 8; e++) mine += f(i + e, v[e]);
+        const u64_t incl = wave_scan(mine, lane);
+        u64_t upto;
+        __syncthreads();  // (the last round has read s.wave)
+        const u64_t all = over_waves(shfl_64(incl, 63), s.wave, upto);
+        upto += incl - mine;
+        if (upto < rest && rest <= upto + mine) {
+            bool done = false;
+#pragma unroll
+            for (int e = 0; e < 8; e++) {
+                upto += f(i + e, v[e]);
+                if (!done && upto >= rest) {
+                    s.found = (uint32_t)(i + e);
+                    done = true;
+                }
+            }
+        }
+        if (rest <= all) break;
+        rest -= all;
+    }
+    __syncthreads();
 }
 
 // The index at which the running sum, by index, of f(index, logit) reaches target(sum of all): in s.found, or not at all
-// if the sum is 0.  Returns the sum.
+// if the sum is 0.  Returns the sum.  f's sums are over a wave's logits, `extra` for each that passes (see NONE).
 template <typename Row, typename F, typename T>
-__device__ __forceinline__ u64_t find_index(const Row& row, F&& f, T&& target_of) {
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-    clear_bins(true, false);
+__device__ __forceinline__ u64_t find_index(const Row& row, u64_t extra, F&& f, T&& target_of) {
+    u64_t t = 0, before;
+    row.each([&](int i, float l) { t += f(i, l); });
+    t -= extra * (u64_t)row.passed();
     __syncthreads();
-    auto of_block = [&](int j, const float (&v)[8]) {
-        u64_t t = 0;
-#pragma unroll
-        for (int e = 0; e < 8; e++) t += f((j * SNT + tid) * 8 + e, v[e]);
-        return t;
-    };
-    row.blocks_of([&](int j, const float (&v)[8]) {
-        const u64_t t = wave_total(of_block(j, v));
-        if (lane == 0 && t) s.sum[j * (SNT / 64) + wave] = t;
-    });
-    __syncthreads();
-    u64_t mine, before;
-    const u64_t all = total_of(s.sum, mine, before);
+    const u64_t all = over_waves(wave_total(t), s.part, before);
     if (all == 0) {
         __syncthreads();
         return 0;
     }
-    const u64_t target = target_of(all);
-    find_bin(s.sum, mine, before, target);
-    const u64_t rest = target - s.above;
-    pick_in(row, rest, f);
-    __syncthreads();
+    pick(row, target_of(all), [&](int i, float l) { return f(i, l) - extra; });
     return all;
 }
 
@@ -329,39 +369,66 @@ __device__ __forceinline__ u64_t find_index(const Row& row, F&& f, T&& target_of
 __device__ __forceinline__ u64_t order_entry(uint32_t key, uint32_t index) { return (u64_t)~key << 32 | index; }
 __device__ __forceinline__ float key_value(uint32_t key) { return __uint_as_float(key & 0x80000000u ? key & 0x7FFFFFFFu : ~key); }
 
-// s.list[0, n), n a power of two from 2 on, in ascending order (all different, but for ones behind the end).  Short lists
-// by counting: the lanes of an entry count those below it.
+__device__ __forceinline__ u64_t shfl_xor64(u64_t v, int d) {
+    return (u64_t)(uint32_t)__shfl_xor((int)(v >> 32), d, 64) << 32 | (uint32_t)__shfl_xor((int)(uint32_t)v, d, 64);
+}
+
+// s.list[0, n), n a power of two from 2 on, in ascending order (all different, but for ones behind the end).  Up to 128
+// by counting: the lanes of an entry count those below it.  More pass a bitonic network, up to 1024 with an
+// entry a thread, where only what passes between waves goes through shared memory (1024 entries: 9 us, 13 us with every step there).
 __device__ __forceinline__ void sort_list(int n) {
     const int tid = threadIdx.x;
-    if (n <= 256) {
-        __syncthreads();
-        const int g = min(64, SNT / n), e = tid / g, part = tid % g, len = (n + g - 1) / g;  // (2 entries: 128 threads are enough)
-        const bool mine = e < n;
-        const u64_t v = mine ? s.list[e] : 0;
-        int below = 0;
-        if (mine)
-            for (int i = 0; i < len; i++) {
-                const int at = part * len + i;
-                if (at < n) below += s.list[at] < v || (s.list[at] == v && at < e);
+    if (n > SNT) {
+        for (int size = 2; size <= n; size *= 2)
+            for (int d = size / 2; d > 0; d /= 2) {
+                __syncthreads();
+                for (int i = tid; i < n / 2; i += SNT) {
+                    const int lo = 2 * i - (i & (d - 1)), hi = lo + d;
+                    const u64_t a = s.list[lo], b = s.list[hi];
+                    if ((a > b) == ((lo & size) == 0)) {
+                        s.list[lo] = b;
+                        s.list[hi] = a;
+                    }
+                }
             }
-        for (int o = 1; o < g; o *= 2) below += __shfl_xor(below, o, 64);
-        __syncthreads();
-        if (mine && part == 0) s.list[below] = v;
         __syncthreads();
         return;
     }
-    for (int size = 2; size <= n; size *= 2)
-        for (int d = size / 2; d > 0; d /= 2) {
-            __syncthreads();
-            for (int i = tid; i < n / 2; i += SNT) {
-                const int lo = 2 * i - (i & (d - 1)), hi = lo + d;
-                const u64_t a = s.list[lo], b = s.list[hi];
-                if ((a > b) == ((lo & size) == 0)) {
-                    s.list[lo] = b;
-                    s.list[hi] = a;
+    if (n > 128) {
+        __syncthreads();
+        u64_t v = tid < n ? s.list[tid] : ~(u64_t)0;
+        int at = SNT;  // two places in turn
+        for (int size = 2; size <= n; size *= 2)
+            for (int d = size / 2; d > 0; d /= 2) {
+                u64_t o;
+                if (d >= 64) {
+                    s.list[at + tid] = v;
+                    __syncthreads();
+                    o = s.list[at + (tid ^ d)];
+                    at = 3 * SNT - at;
+                } else {
+                    o = shfl_xor64(v, d);
                 }
+                const bool least = ((tid & d) == 0) == ((tid & size) == 0);
+                v = (o < v) == least ? o : v;
             }
+        s.list[tid] = v;
+        __syncthreads();
+        return;
+    }
+    __syncthreads();
+    const int g = min(64, SNT / n), e = tid / g, part = tid % g, len = (n + g - 1) / g;  // (2 entries: 128 threads are enough)
+    const bool mine = e < n;
+    const u64_t v = mine ? s.list[e] : 0;
+    int below = 0;
+    if (mine)
+        for (int i = 0; i < len; i++) {
+            const int at = part * len + i;
+            if (at < n) below += s.list[at] < v || (s.list[at] == v && at < e);
         }
+    for (int o = 1; o < g; o *= 2) below += __shfl_xor(below, o, 64);
+    __syncthreads();
+    if (mine && part == 0) s.list[below] = v;
     __syncthreads();
 }
 
@@ -401,18 +468,18 @@ __device__ __forceinline__ u64_t run_of(float p, u64_t all) {  // that top-p's r
 // A row with more candidates than a list holds: thresholds by refined histograms, then the sum over the row.  The
 // token goes to s.found, the sum to s.above.
 template <typename X>
-__device__ __noinline__ void sample_many(const X* x, int V, SampleWeights sw, uint32_t k, bool by_k, float p, bool by_p, u64_t least_w, float u) {
+__device__ __noinline__ void sample_many(const X* x, int V, bool infinite, SampleWeights sw, uint32_t k, bool by_k, float p, bool by_p, u64_t least_w, float u) {
     const int tid = threadIdx.x, lane = tid & 63;
-    const float per_bit = (float)SBINS / sw.limit;
-    auto bin_of = [&](float l) { return (int)min(sw.below(l) * per_bit, (float)(SBINS - 1)); };
-    const SampleRow<X> row(x, V);
+    // scalars come to a function in vector registers
+    const u64_t at = (u64_t)x;
+    const SampleRow<X> row((const X*)((u64_t)uniform((uint32_t)(at >> 32)) << 32 | uniform((uint32_t)at)), (int)uniform((uint32_t)V), uniform((uint32_t)infinite));
     uint32_t key = 0, last = 0xFFFFFFFFu;  // kept: keys above `key`, and that one up to index `last`
     if (by_k || by_p) {
         clear_bins(by_p, by_k);
         __syncthreads();
         row.each([&](int, float l) {
             if (!sw.alive(l)) return;
-            const int b = bin_of(l);
+            const int b = sw.bin_of(l);
             if (by_k) atomicAdd(&s.count[b], 1u);
             if (by_p) atomicAdd(&s.sum[b], sw.weight(l));
         });
@@ -428,14 +495,14 @@ __device__ __noinline__ void sample_many(const X* x, int V, SampleWeights sw, ui
                 __syncthreads();
                 // the sums are needed again: they move to registers while keys are sorted
                 const u64_t s0 = s.sum[2 * tid], s1 = s.sum[2 * tid + 1];
-                select_key<false>(row, sw, rest, [&](float l, uint32_t) { return sw.alive(l) && bin_of(l) == (int)kbin; });
+                select_key<false>(row, sw, rest, [&](float l, uint32_t) { return sw.alive(l) && sw.bin_of(l) == (int)kbin; });
                 key = s.key;
                 if (by_p) {
                     s.sum[2 * tid] = s0;
                     s.sum[2 * tid + 1] = s1;
                     u64_t part = 0;
                     row.each([&](int, float l) {
-                        if (sw.alive(l) && bin_of(l) == (int)kbin && order_key(l) >= key) part += sw.weight(l);
+                        if (sw.alive(l) && sw.bin_of(l) == (int)kbin && order_key(l) >= key) part += sw.weight(l);
                     });
                     part = wave_total(part);
                     __syncthreads();
@@ -458,20 +525,20 @@ __device__ __noinline__ void sample_many(const X* x, int V, SampleWeights sw, ui
             const u64_t rest = want - s.above;
             __syncthreads();
             const uint32_t least = key;
-            select_key<true>(row, sw, rest, [&](float l, uint32_t kk) { return sw.alive(l) && bin_of(l) == pbin && kk >= least; });
+            select_key<true>(row, sw, rest, [&](float l, uint32_t kk) { return sw.alive(l) && sw.bin_of(l) == pbin && kk >= least; });
             key = s.key;
             const u64_t w = sw.weight(key_value(key)), ties = (rest - s.above + w - 1) / w;  // so many of the equal ones are kept
             const bool some = s.eq != ties * w;
             __syncthreads();
             if (some) {
-                find_index(row, [&](int, float l) { return (u64_t)(order_key(l) == key); }, [&](u64_t) { return ties; });
+                find_index(row, 0, [&](int, float l) { return (u64_t)(order_key(l) == key); }, [&](u64_t) { return ties; });
                 last = s.found;
                 __syncthreads();
             }
         }
     }
     const u64_t all = find_index(
-        row,
+        row, 0,
         [&](int i, float l) -> u64_t {
             const uint32_t kk = order_key(l);
             if (kk < key || (kk == key && (uint32_t)i > last) || !sw.alive(l)) return 0;
@@ -483,29 +550,140 @@ __device__ __noinline__ void sample_many(const X* x, int V, SampleWeights sw, ui
     __syncthreads();
 }
 
+// Top-p without top-k.  The token goes to s.found, the sum to s.above; false: too many to list.  (Inlined: as a
+// function it saves 48 registers a lane, and 256 rows of 32000 take 46 us, not 34.)
+template <typename X>
+__device__ __forceinline__ bool sample_run(const SampleRow<X>& row, const SampleWeights& sw, float p, u64_t least, float u) {
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    // Runs of any length: f32 sums of the weights find the bin where the run
+    // ends, and one pass with the weights themselves sums up what lies
+    // before it (for the whole row, and for the draw by wave) and lists that bin.
+    clear_bins(true, false);
+    __syncthreads();
+    const float per_bin = -(float)(sw.S + 1) / SBINS;
+    row.each([&](int, float l) {
+        const float b = sw.below(l);
+        if (b < (float)SBINS) atomicAdd(&s.sum[(int)b], (u64_t)(uint32_t)(__builtin_amdgcn_exp2f(__builtin_fmaf(b, per_bin, 31.0f))));
+    });
+    __syncthreads();
+    u64_t mine, before;
+    // The f32 weights are off by 2^-16 of themselves at most (b per_bin, up to 52, by four roundings) and by less than 1
+    // that is cut off, and so are the sum of all and any sum up to a bin: the run ends between these two.
+    const u64_t about = total_of(s.sum, mine, before), want_about = run_of(p, about), off = (about >> 15) + 2 * (u64_t)row.V;
+    find_bin(s.sum, mine, before, want_about > off ? want_about - off : 1);
+    const float first = (float)uniform(s.bin);
+    __syncthreads();
+    find_bin(s.sum, mine, before, min(want_about + off, about));
+    const float past = (float)(uniform(s.bin) + 1);
+    __syncthreads();
+    if (tid == 0) s.n = 0;
+    __syncthreads();
+    u64_t all = 0, sure = 0, part = 0;
+    auto pass = [&](auto by_least) {
+        row.blocks_of([&](int i, const float (&v)[8]) {
+            bool in[8], any = false;
+#pragma unroll
+            for (int e = 0; e < 8; e++) {
+                const u64_t w = sw.bits(v[e]);
+                const float b = sw.below(v[e]);
+                all += w;
+                const u64_t before_it = b < first ? w : SampleWeights::NONE;
+                sure += before_it;
+                if (by_least) part += before_it >= least + SampleWeights::NONE ? before_it : SampleWeights::NONE;
+                in[e] = b >= first && b < past;
+                any |= in[e];
+            }
+            if (any) {
+#pragma unroll
+                for (int e = 0; e < 8; e++)
+                    if (in[e]) {
+                        const uint32_t at = atomicAdd(&s.n, 1u);
+                        if (at < SCAP) s.list[at] = order_entry(order_key(v[e]), (uint32_t)(i + e));
+                    }
+            }
+        });
+    };
+    if (uniform((uint32_t)(least > 1))) pass(std::true_type{});
+    else pass(std::false_type{});
+    const u64_t none = SampleWeights::NONE * (u64_t)row.passed();
+    all -= none;
+    sure -= none;
+    part = least > 1 ? part - none : sure;
+    part = wave_total(part);
+    if (lane == 0) s.part[wave] = part;
+    all = over_waves(wave_total(all), s.wave, before);
+    sure = over_waves(wave_total(sure), s.wave2, before);
+    const int n = (int)uniform(s.n);
+    const u64_t want = run_of(p, all);
+    __syncthreads();
+    if (n <= SCAP && sure < want) {
+        int room = 2;
+        while (room < n) room *= 2;
+        for (int i = n + tid; i < room; i += SNT) s.list[i] = ~(u64_t)0;
+        sort_list(room);
+        u64_t w[4];
+        const u64_t listed = scan_list(n, w, before, [&](int i) { return sw.weight(key_value(~(uint32_t)(s.list[i] >> 32))); });
+        if (want <= sure + listed) {
+            u64_t run = sure + before;
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+                if (w[e] && run < want) {
+                    const u64_t v = s.list[4 * tid + e];
+                    if (w[e] >= least) atomicAdd(&s.part[((uint32_t)v >> 9) / (uint32_t)row.blocks], w[e]);
+                    if (run + w[e] >= want) s.end = v;
+                }
+                run += w[e];
+            }
+            __syncthreads();
+            const u64_t end = s.end;
+            u64_t sum = 0;
+#pragma unroll
+            for (int v = 0; v < SNT / 64; v++) sum += s.part[v];
+            pick(row, drawn(u, sum), [&](int i, float l) -> u64_t {
+                const float b = sw.below(l);
+                if (!(b < past) || (b >= first && order_entry(order_key(l), (uint32_t)i) > end)) return 0;
+                const u64_t w = sw.weight(l);
+                return w >= least ? w : 0;
+            });
+            if (tid == 0) s.above = sum;
+            __syncthreads();
+            return true;
+        }
+    }
+    return false;
+}
+
 template <typename X>
 __global__ __launch_bounds__(SNT) void sample_rows_kernel(SampleArgs a, int S) {
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-    if (tid < 64) s.table[tid] = exp2(tid / 64.0);
     const int r = blockIdx.x;
-    const SampleRow<X> row((const X*)a.x + (size_t)r * a.vocab, a.vocab);
-    // the largest
+    const X* const x = (const X*)a.x + (size_t)r * a.vocab;
+    const float T = uniform(a.temp ? a.temp[r] : 1.0f);
+    // the largest (NaN is none); greedy: and where it is first
     float M = -INFINITY;
-    row.each([&](int, float l) { M = fmaxf(M, l); });
+    uint32_t first_of = 0;
+    const bool greedy = !(T > 0.0f);
+    {
+        const SampleRow<X> raw(x, a.vocab, false);
+        if (greedy) raw.each([&](int i, float l) {
+            first_of = l > M ? (uint32_t)i : first_of;
+            M = l > M ? l : M;
+        });
+        else raw.each([&](int, float l) { M = fmaxf(M, l); });
+    }
+    const float mine_M = M;
     M = wave_max(M);
     if (lane == 0) s.wave[wave] = __float_as_uint(M);
-    if (tid == 0) s.found = s.bin = 0;  // (always places in the row and in the bins)
+    if (tid == 0) {
+        s.found = greedy ? 0xFFFFFFFFu : 0;  // (otherwise always places in the row and in the bins)
+        s.bin = 0;
+    }
     __syncthreads();
 #pragma unroll
     for (int w = 0; w < SNT / 64; w++) M = fmaxf(M, __uint_as_float((uint32_t)s.wave[w]));
-    __syncthreads();
-    const float T = a.temp ? a.temp[r] : 1.0f;
-    if (!(T > 0.0f) || M == -INFINITY) {  // greedy, or no logit at all: token 0
-        if (tid == 0) s.found = 0xFFFFFFFFu;
-        __syncthreads();
-        uint32_t first = 0xFFFFFFFFu;
-        row.each([&](int i, float l) { first = l == M ? min(first, (uint32_t)i) : first; });
-        if (first != 0xFFFFFFFFu) atomicMin(&s.found, first);
+    M = uniform(M);
+    if (greedy || M == -INFINITY) {  // (no logit at all: token 0)
+        if (M != -INFINITY && mine_M == M) atomicMin(&s.found, first_of);
         __syncthreads();
         if (tid == 0) {
             a.token[r] = M == -INFINITY ? 0 : s.found;
@@ -513,149 +691,62 @@ __global__ __launch_bounds__(SNT) void sample_rows_kernel(SampleArgs a, int S) {
         }
         return;
     }
+    if (tid < STABLE) s.table[tid] = __longlong_as_double(__double_as_longlong(exp2(tid / (double)STABLE)) + ((long long)S << 52) - ((long long)tid << (52 - SBITS)));
+    __syncthreads();
+    const bool infinite = M == INFINITY;
+    const SampleRow<X> row(x, a.vocab, infinite);
     SampleWeights sw;
-    sw.M = M;
-    sw.c = 1.44269504088896340736 / (double)T;
-    sw.Mc = (double)M * sw.c;
-    sw.cf = (float)sw.c;
+    const double c = 1.44269504088896340736 / (double)T;
+    sw.M = infinite ? 0.0f : M;
+    sw.Md = sw.M;
+    sw.c = c * STABLE;
+    sw.least = -(double)(S + 2) * STABLE;
+    const float per_bit = (float)SBINS / (float)(S + 1);
+    sw.cb = (float)min(c * per_bit, 0x1p127);  // (finite: 0 times it has to be 0)
     sw.S = S;
-    sw.limit = (float)(S + 1);
     sw.table = s.table;
-    const uint32_t k = a.top_k ? a.top_k[r] : 0;
-    const float p = a.top_p ? a.top_p[r] : 1.0f, low = a.min_p ? a.min_p[r] : 0.0f;
+    const uint32_t k = uniform(a.top_k ? a.top_k[r] : 0u);
+    const float p = uniform(a.top_p ? a.top_p[r] : 1.0f), low = uniform(a.min_p ? a.min_p[r] : 0.0f);
     const bool by_k = k > 0 && k < (uint32_t)a.vocab, by_p = p < 1.0f;
     const float u = a.u[r];
     const u64_t least = low > 0.0f ? (u64_t)ceil((double)min(low, 1.0f) * (double)((u64_t)1 << S)) : 1;
     auto answer = [&](uint32_t index, float l, u64_t all) {
         a.token[r] = index;
-        if (a.prob)
-            a.prob[r] = (float)((l == M ? 1.0 : exp2(((double)l - (double)M) * sw.c)) * (double)((u64_t)1 << S) / (double)all);
+        if (a.prob) a.prob[r] = (float)(exp2(l == sw.M ? 0.0 : ((double)l - sw.Md) * c) * (double)((u64_t)1 << S) / (double)all);
     };
-    // bins of equal width in the logarithm of the weight, from the largest down
-    const float per_bit = (float)SBINS / sw.limit;
-    auto bin_of = [&](float l) { return (int)min(sw.below(l) * per_bit, (float)(SBINS - 1)); };
     bool many = true;
     if (by_p && !by_k) {
-        // Runs of any length: f32 sums of the weights find the bin where the run
-        // ends, and one pass with the weights themselves sums up what lies
-        // before it (for the whole row, and for the draw in parts of a wave's
-        // share of a block) and lists that bin and its neighbours.
-        clear_bins(true, false);
-        __syncthreads();
-        row.each([&](int, float l) {
-            if (sw.alive(l)) atomicAdd(&s.sum[bin_of(l)], (u64_t)(uint32_t)(__builtin_amdgcn_exp2f(-sw.below(l)) * 0x1p31f));
-        });
-        __syncthreads();
-        u64_t mine, before;
-        const u64_t about = total_of(s.sum, mine, before);
-        find_bin(s.sum, mine, before, run_of(p, about));
-        const int first = max((int)s.bin - 1, 0), final = (int)s.bin + 1;
-        __syncthreads();
-        clear_bins(true, false);
-        if (tid == 0) s.n = 0;
-        __syncthreads();
-        u64_t all = 0, sure = 0;
-        row.blocks_of([&](int j, const float (&v)[8]) {
-            u64_t part = 0;
-#pragma unroll
-            for (int e = 0; e < 8; e++) {
-                const float l = v[e];
-                if (!sw.alive(l)) continue;
-                const u64_t w = sw.weight(l);
-                const int b = bin_of(l);
-                all += w;
-                if (b < first) {
-                    sure += w;
-                    part += w >= least ? w : 0;
-                } else if (b <= final) {
-                    const uint32_t at = atomicAdd(&s.n, 1u);
-                    if (at < SCAP) s.list[at] = order_entry(order_key(l), (uint32_t)((j * SNT + tid) * 8 + e));
-                }
-            }
-            part = wave_total(part);
-            if (lane == 0 && part) s.sum[j * (SNT / 64) + wave] = part;
-        });
-        all = wave_total(all);
-        sure = wave_total(sure);
-        if (lane == 0) {
-            s.wave[wave] = all;
-            s.wave2[wave] = sure;
-        }
-        __syncthreads();
-        all = sure = 0;
-#pragma unroll
-        for (int w = 0; w < SNT / 64; w++) {
-            all += s.wave[w];
-            sure += s.wave2[w];
-        }
-        const int n = (int)s.n;
-        const u64_t want = run_of(p, all);
-        __syncthreads();
-        if (n <= SCAP && sure < want) {
-            int room = 2;
-            while (room < n) room *= 2;
-            for (int i = n + tid; i < room; i += SNT) s.list[i] = ~(u64_t)0;
-            sort_list(room);
-            u64_t w[4];
-            const u64_t listed = scan_list(n, w, before, [&](int i) { return sw.weight(key_value(~(uint32_t)(s.list[i] >> 32))); });
-            if (want <= sure + listed) {
-                many = false;
-                u64_t run = sure + before;
-#pragma unroll
-                for (int e = 0; e < 4; e++) {
-                    if (w[e] && run < want) {
-                        const u64_t v = s.list[4 * tid + e];
-                        if (w[e] >= least) atomicAdd(&s.sum[(uint32_t)v >> 9], w[e]);  // (an index's part: 512 lie in one)
-                        if (run + w[e] >= want) s.end = v;
-                    }
-                    run += w[e];
-                }
-                __syncthreads();
-                const u64_t end = s.end, sum = total_of(s.sum, mine, before);
-                const u64_t target = drawn(u, sum);
-                find_bin(s.sum, mine, before, target);
-                const u64_t rest = target - s.above;
-                pick_in(row, rest, [&](int i, float l) -> u64_t {
-                    if (!sw.alive(l)) return 0;
-                    const int b = bin_of(l);
-                    if (b > final || (b >= first && order_entry(order_key(l), (uint32_t)i) > end)) return 0;
-                    const u64_t w = sw.weight(l);
-                    return w >= least ? w : 0;
-                });
-                __syncthreads();  // (the others have read s.above)
-                if (tid == 0) s.above = sum;
-                __syncthreads();
-            }
-        }
+        many = !sample_run(row, sw, p, least, u);
     } else if (by_k || low > 0.0f) {
         // Few candidates are the usual case: they are listed and sorted.
-        int edge = SBINS - 1;  // the last bin that can hold a kept one
+        float edge = (float)SBINS;  // behind the last bin that can hold a kept one
         u64_t want = 0;
         bool cut = false;  // by k
         if (by_k) {
             clear_bins(false, true);
             __syncthreads();
             row.each([&](int, float l) {
-                if (sw.alive(l)) atomicAdd(&s.count[bin_of(l)], 1u);
+                const float b = sw.below(l);
+                if (b < (float)SBINS) atomicAdd(&s.count[(int)b], 1u);
             });
             __syncthreads();
             u64_t mine, before;
             cut = total_of(s.count, mine, before) > k;  // (otherwise all that have a weight are kept)
             if (cut) {
                 find_bin(s.count, mine, before, k);
-                edge = (int)s.bin;
+                edge = (float)(uniform(s.bin) + 1);
             }
         }
-        if (low > 0.0f && !by_p) edge = min(edge, (int)min(per_bit * (0.01f - log2f(min(low, 1.0f))), (float)(SBINS - 1)));
+        if (low > 0.0f && !by_p) edge = min(edge, per_bit * (0.01f - log2f(min(low, 1.0f))) + 1.0f);
         if (tid == 0) s.n = 0;
         __syncthreads();
         row.each([&](int i, float l) {
-            if (!sw.alive(l) || bin_of(l) > edge) return;
+            if (!(sw.below(l) < edge)) return;
             const uint32_t at = atomicAdd(&s.n, 1u);
             if (at < SCAP) s.list[at] = order_entry(order_key(l), (uint32_t)i);
         });
         __syncthreads();
-        const int n = (int)s.n;
+        const int n = (int)uniform(s.n);
         if (n <= SCAP) {
             int room = 2;
             while (room < n) room *= 2;
@@ -705,13 +796,13 @@ __global__ __launch_bounds__(SNT) void sample_rows_kernel(SampleArgs a, int S) {
         }
     }
     if ((by_p && !by_k) ? many : (by_k || low > 0.0f)) {
-        sample_many<X>((const X*)a.x + (size_t)r * a.vocab, a.vocab, sw, k, by_k, p, by_p, least, u);
+        sample_many<X>(x, a.vocab, infinite, sw, k, by_k, p, by_p, least, u);
     } else if (!(by_p && !by_k)) {
-        const u64_t all = find_index(row, [&](int, float l) -> u64_t { return sw.alive(l) ? sw.weight(l) : 0; }, [&](u64_t sum) { return drawn(u, sum); });
+        const u64_t all = find_index(row, SampleWeights::NONE, [&](int, float l) { return sw.bits(l); }, [&](u64_t sum) { return drawn(u, sum); });
         if (tid == 0) s.above = all;
         __syncthreads();
     }
-    if (tid == 0) answer(s.found, (float)((const X*)a.x)[(size_t)r * a.vocab + s.found], s.above);
+    if (tid == 0) answer(s.found, row.value((float)x[s.found]), s.above);
 }
 
 void launch_sample_rows(const SampleArgs& all, hipStream_t s) {

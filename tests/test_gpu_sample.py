@@ -100,6 +100,16 @@ def test_one_setting(dev, V, which):
     _check(dev, _logits(rng, n, V), F32, rng.random(n, np.float32), **over)
 
 
+@pytest.mark.parametrize("dt", [F32, BF16])
+@pytest.mark.parametrize("V", [511, 513, 8191, 16385, 32000])
+def test_runs(dev, V, dt):
+    """Top-p alone and with min-p, from runs of one to runs of nearly all: their ends and shares over every wave's part of a row."""
+    rng = np.random.default_rng(V)
+    n = 40
+    u, temp, p = rng.random(n, dtype=np.float32), rng.uniform(0.3, 2.5, n), rng.uniform(0.3, 1, n)
+    _check(dev, _logits(rng, n, V), dt, u, temp, None, p, np.where(rng.random(n) < 0.5, 0, rng.uniform(0, 0.05, n)))
+
+
 @pytest.mark.parametrize("spread", [0.0, 1e-6, 1e-3, 0.05])
 def test_rows_that_are_nearly_flat(dev, spread):
     """All weights in one bin: values a few steps of f32 apart, at a large and a small base."""

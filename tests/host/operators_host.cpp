@@ -43,6 +43,7 @@ void host_grouped(th_qweight* w, int bits, int per_row) {
     w->bits = bits;
     w->per_row = per_row != 0;
 }
+void host_rows(th_qweight* w, size_t rows) { w->rows = rows; }
 void host_last(size_t* v) {
     v[0] = g_m;
     v[1] = g_k;

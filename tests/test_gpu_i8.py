@@ -244,3 +244,20 @@ def test_captured(dev):
             graph.launch()
             assert np.array_equal(y.to_numpy(), want)
         graph.free()
+
+
+def test_results_beyond_32_bits_of_places(dev):
+    """More than 2^31 results, and rows of quantized values that begin beyond 2^31 bytes of the results."""
+    m, k, n = 67200, 64, 32000
+    rng = np.random.default_rng(6)
+    x = rng.integers(-128, 128, m * k).astype(np.int8)
+    w, s, t = rng.integers(-128, 128, (n, k)).astype(np.int8), rng.uniform(1, 2, m).astype(np.float32), rng.uniform(1, 2, n).astype(np.float32)
+    y = dev.alloc(m * n, BF16)
+    dev.gemm_i8(dev.upload(x, I8), dev.upload(s), m, dev.q8_upload_rowwise(w, t, n, k), y)
+    got = y.to_numpy().reshape(m, n)
+    y.free()
+    for rows in (range(0, 20), range(67100, 67121), range(67184, 67200)):
+        q = x[_places(m, k)[list(rows)]]
+        p = (q.astype(np.int64) @ w.astype(np.int64).T) * s[list(rows)].astype(np.float64)[:, None] * t.astype(np.float64)
+        tol = 3 * 2.0 ** -24 * np.abs(p) * (1 + 2.0 ** -8) + np.maximum(EPS[BF16] * np.abs(p), LEAST[BF16])
+        assert np.all(np.abs(from_bits(got[list(rows)], BF16) - p) <= tol)

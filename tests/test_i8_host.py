@@ -92,6 +92,9 @@ def test_pack_and_product(lib):
     g.refused("must not be an input", xs=y)
     g.refused("must not be an input", bias=y)
     g.refused("another device", y=other.buffer(60, F32))
+    lib.host_rows(w, ctypes.c_size_t(1 << 27))
+    g.refused("out of range")
+    lib.host_rows(w, ctypes.c_size_t(20))
     lib.host_grouped(w, 8, 0)
     g.refused("each group", code=capi.TH_ERR_UNSUPPORTED)
     lib.host_grouped(w, 4, 1)

@@ -567,9 +567,10 @@ __device__ __forceinline__ bool sample_run(const SampleRow<X>& row, const Sample
     });
     __syncthreads();
     u64_t mine, before;
-    // The f32 weights are off by 2^-16 of themselves at most (b per_bin, up to 52, by four roundings) and by less than 1
-    // that is cut off, and so are the sum of all and any sum up to a bin: the run ends between these two.
-    const u64_t about = total_of(s.sum, mine, before), want_about = run_of(p, about), off = (about >> 15) + 2 * (u64_t)row.V;
+    // Up to a bin, the f32 sums are off by 2^-18 of the sum of all (roundings of b shift the weights by up to 2^-22 of the bits that they
+    // are below the largest, which is less than log2(vocab) on average, and most of that is the same for all), and by less than 1 a
+    // weight that is cut off.  Were it more, the exact sums below would tell, and the row go to sample_many.
+    const u64_t about = total_of(s.sum, mine, before), want_about = run_of(p, about), off = (about >> 18) + 2 * (u64_t)row.V;
     find_bin(s.sum, mine, before, want_about > off ? want_about - off : 1);
     const float first = (float)uniform(s.bin);
     __syncthreads();

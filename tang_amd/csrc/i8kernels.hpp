@@ -116,9 +116,10 @@ __global__ __launch_bounds__(64 * NW) void i8_rows_kernel(const uint4* __restric
 // in LDS as they are read: 1 KiB blocks of 16 rows x 64 k, lane by lane.
 // KW: groups of four waves, each with every KW-th step of k and LDS of its own, whose
 // sums meet at the end, for tiles that are alone on their CU.
-// Measured: 8192 x 8192 x 8192 2205 TOP/s (the library's product there: 2456), 8192 x 4096 x 11008 1845 (2186), where
-// the matrix operations take 59 % of the cycles at the 1.75 GHz that the chip then runs at; 2048 x 4096 x 4096 1650 (1677),
-// 512 x 4096 x 4096 940 (837).  Tried: weights from memory straight into registers (each wave its own, 1846 and 1639:
+// Measured: 8192 x 8192 x 8192 2308 TOP/s (the library's product there: 2456), 8192 x 4096 x 11008 1914 (2186), where
+// the matrix operations take half of the cycles at the 1.75 GHz that the chip then runs at (5.4 rounds of tiles take six, and no other
+// tile of its CU works while one fills its pipe or leaves); 512 x 4096 x 4096 1000 (837), 128 x 4096 x 11008 648 (488).
+// Tried: weights from memory straight into registers (each wave its own, 1846 and 1639:
 // they are loaded twice), more steps ahead (the same).
 // LDS in bytes: the stages, or the strips that results leave through; then the tile's scales and bias.
 template <int TM, int TN, int KW>

@@ -369,6 +369,16 @@ __device__ __forceinline__ u64_t find_index(const Row& row, u64_t extra, F&& f, 
 __device__ __forceinline__ u64_t order_entry(uint32_t key, uint32_t index) { return (u64_t)~key << 32 | index; }
 __device__ __forceinline__ float key_value(uint32_t key) { return __uint_as_float(key & 0x80000000u ? key & 0x7FFFFFFFu : ~key); }
 
+// Of eight logits from index i on, those that are `in`, to the list.  (Asked for eight at a time: few blocks have any.)
+__device__ __forceinline__ void list_some(int i, const float (&v)[8], const bool (&in)[8]) {
+#pragma unroll
+    for (int e = 0; e < 8; e++)
+        if (in[e]) {
+            const uint32_t at = atomicAdd(&s.n, 1u);
+            if (at < SCAP) s.list[at] = order_entry(order_key(v[e]), (uint32_t)(i + e));
+        }
+}
+
 __device__ __forceinline__ u64_t shfl_xor64(u64_t v, int d) {
     return (u64_t)(uint32_t)__shfl_xor((int)(v >> 32), d, 64) << 32 | (uint32_t)__shfl_xor((int)(uint32_t)v, d, 64);
 }
@@ -594,14 +604,7 @@ __device__ __forceinline__ bool sample_run(const SampleRow<X>& row, const Sample
                 in[e] = b >= first && b < past;
                 any |= in[e];
             }
-            if (any) {
-#pragma unroll
-                for (int e = 0; e < 8; e++)
-                    if (in[e]) {
-                        const uint32_t at = atomicAdd(&s.n, 1u);
-                        if (at < SCAP) s.list[at] = order_entry(order_key(v[e]), (uint32_t)(i + e));
-                    }
-            }
+            if (any) list_some(i, v, in);
         });
     };
     if (uniform((uint32_t)(least > 1))) pass(std::true_type{});
@@ -664,6 +667,10 @@ __global__ __launch_bounds__(SNT) void sample_rows_kernel(SampleArgs a, int S) {
     float M = -INFINITY;
     uint32_t first_of = 0;
     const bool greedy = !(T > 0.0f);
+    if (!greedy && tid >= SNT - STABLE) {  // (the last wave has the least of a row)
+        const int i = tid - (SNT - STABLE);
+        s.table[i] = __longlong_as_double(__double_as_longlong(exp2(i / (double)STABLE)) + ((long long)S << 52) - ((long long)i << (52 - SBITS)));
+    }
     {
         const SampleRow<X> raw(x, a.vocab, false);
         if (greedy) raw.each([&](int i, float l) {
@@ -692,7 +699,6 @@ __global__ __launch_bounds__(SNT) void sample_rows_kernel(SampleArgs a, int S) {
         }
         return;
     }
-    if (tid < STABLE) s.table[tid] = __longlong_as_double(__double_as_longlong(exp2(tid / (double)STABLE)) + ((long long)S << 52) - ((long long)tid << (52 - SBITS)));
     __syncthreads();
     const bool infinite = M == INFINITY;
     const SampleRow<X> row(x, a.vocab, infinite);
@@ -741,10 +747,14 @@ __global__ __launch_bounds__(SNT) void sample_rows_kernel(SampleArgs a, int S) {
         if (low > 0.0f && !by_p) edge = min(edge, per_bit * (0.01f - log2f(min(low, 1.0f))) + 1.0f);
         if (tid == 0) s.n = 0;
         __syncthreads();
-        row.each([&](int i, float l) {
-            if (!(sw.below(l) < edge)) return;
-            const uint32_t at = atomicAdd(&s.n, 1u);
-            if (at < SCAP) s.list[at] = order_entry(order_key(l), (uint32_t)i);
+        row.blocks_of([&](int i, const float (&v)[8]) {
+            bool in[8], any = false;
+#pragma unroll
+            for (int e = 0; e < 8; e++) {
+                in[e] = sw.below(v[e]) < edge;
+                any |= in[e];
+            }
+            if (any) list_some(i, v, in);
         });
         __syncthreads();
         const int n = (int)uniform(s.n);

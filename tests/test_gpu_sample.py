@@ -218,6 +218,18 @@ def test_settings_at_their_ends(dev):
             assert np.array_equal(got, [kept(r, 1.0, k, 1.0, 1e-12)[0][at] for r in x]), (k, v)
 
 
+@pytest.mark.parametrize("V", [700, 9001])
+def test_temperatures_below_the_normal_range(dev, V):
+    """Logits and temperatures that are subnormal: bins are all one then, and the weights alone decide."""
+    rng = np.random.default_rng(V)
+    n = 20
+    x, u = rng.standard_normal((n, V)).astype(np.float32) * np.float32(3e-42), rng.random(n, dtype=np.float32)
+    temp = rng.uniform(1e-42, 3e-42, n)
+    for settings in (dict(), dict(k=rng.integers(1, 300, n).astype(np.uint32)), dict(p=rng.uniform(0.3, 1, n)), dict(low=rng.uniform(0.01, 0.3, n)),
+                     dict(k=rng.integers(1, 300, n).astype(np.uint32), p=rng.uniform(0.3, 1, n), low=rng.uniform(0, 0.1, n))):
+        _check(dev, x, F32, u, temp=temp, **settings)
+
+
 def test_no_rows(dev):
     tokens = dev.upload(np.array([9], np.uint32), capi.U32)
     dev.sample_rows(dev.alloc(1), 0, 5, dev.alloc(1), tokens=tokens)

@@ -39,7 +39,7 @@ struct RowScale {
     }
     // Sixteen of a row: the integer is what an addition of 1.5 2^23 leaves in the low byte. x rs is off by 2^-17, so
     // only where one lies as near to a half, for one in 25000, the sixteen are rounded as above (8192 rows of 4096 in bf16:
-    // 32 us, 41 with all of them so, bound by instructions).
+    // 26 us; with all of them so it took 41, bound by instructions).
     __device__ __forceinline__ uint4 sixteen(const float (&x)[16]) const {
         if (!(s > 0.0f)) return make_uint4(0, 0, 0, 0);  // (zero or NaN)
         uint32_t y[16], w[4];
@@ -86,8 +86,9 @@ struct RowTop {
 // WPR waves a row, ROWS rows a workgroup; a lane has 16 consecutive elements, one
 // piece of a block, and up to IT pieces stay in its registers between the search
 // for the largest and the rounding (0: any length, read twice).  Few rows: four
-// waves each, for the latency of one.  Many: sixteen rows a workgroup, which fill
-// their blocks' lines together.
+// waves each, for the latency of one.  Many: four rows a workgroup, which leave their
+// blocks together, of two waves or four (8192 x 4096 in bf16, waves by rows: 2 x 4 26 us, 2 x 8 27, 2 x 2 28, 4 x 4 31,
+// 1 x 16, which the chip holds all at once, so that reading and writing take turns, 32).
 template <typename X, int WPR, int ROWS, int IT>
 __global__ __launch_bounds__(64 * WPR * ROWS) void quantize_rows_kernel(const X* __restrict__ x, int m, int K, int Kp, int8_t* __restrict__ q,
                                                                         float* __restrict__ scale, int whole) {
@@ -155,8 +156,9 @@ static void quantize_types(const void* x, size_t m, size_t K, size_t Kp, int8_t*
     };
     using std::integral_constant;
     const integral_constant<int, 1> one;
+    const integral_constant<int, 2> two;
     const integral_constant<int, 4> four;
-    if (m >= 1024 && Kp <= 4096) go(one, integral_constant<int, 16>{}, four);
+    if (m >= 1024 && Kp <= 4096) go(two, four, two);
     else if (m >= 1024 && Kp <= 16384) go(four, four, four);
     else if (Kp <= 4096) go(four, one, one);
     else if (Kp <= 16384) go(four, one, four);

@@ -137,7 +137,7 @@ struct SampleRow {
 
 // Weights of a row.
 struct SampleWeights {
-    float M, cb;  // cb: bins a unit of a logit
+    float M, cb, bins;  // cb: bins a unit of a logit; how many there are
     double Md, c, least;  // c: log2(e) / T in steps of the table
     int S;
     const double* table;
@@ -145,7 +145,7 @@ struct SampleWeights {
     // Bins that a logit is below the largest, in f32: monotone in l.  Bins have equal widths in the logarithm
     // of the weight; behind the last (NaN, too) a weight is below 2^-(S+1).
     __device__ __forceinline__ float below(float l) const { return (M - l) * cb; }
-    __device__ __forceinline__ bool alive(float l) const { return below(l) < (float)SBINS; }
+    __device__ __forceinline__ bool alive(float l) const { return below(l) < bins; }
     __device__ __forceinline__ int bin_of(float l) const { return (int)min(below(l), (float)(SBINS - 1)); }
     // w 2^S to the nearest, as the bits of 2^52 + w 2^S.  With x = n + i/32 + r the table has 2^(i/32), and
     // 2^r is its series to the fifth power (r up to 2^-6: off by 2^-48).  All rows' elements pass through here,
@@ -570,17 +570,21 @@ __device__ __forceinline__ bool sample_run(const SampleRow<X>& row, const Sample
     // before it (for the whole row, and for the draw by wave) and lists that bin.
     clear_bins(true, false);
     __syncthreads();
-    const float per_bin = -(float)(sw.S + 1) / SBINS;
-    row.each([&](int, float l) {
+    const int per_bit = SBINS / (sw.S + 1);
+    const float a_bin = 1.0f / (float)per_bit;
+    row.each([&](int, float l) {  // each bin in units of its own, 2^-31 of the power of two above its weights
         const float b = sw.below(l);
-        if (b < (float)SBINS) atomicAdd(&s.sum[(int)b], (u64_t)(uint32_t)(__builtin_amdgcn_exp2f(__builtin_fmaf(b, per_bin, 31.0f))));
+        if (b < sw.bins) atomicAdd(&s.sum[(int)b], (u64_t)(uint32_t)__builtin_amdgcn_exp2f(31.0f - __builtin_amdgcn_fractf(b * a_bin)));
     });
     __syncthreads();
+#pragma unroll
+    for (int i = 0; i < 2; i++) s.sum[2 * tid + i] = s.sum[2 * tid + i] << 11 >> (2 * tid + i) / per_bit;  // in 2^-42 of the largest weight
+    __syncthreads();
     u64_t mine, before;
-    // Up to a bin, the f32 sums are off by 2^-18 of the sum of all (roundings of b shift the weights by up to 2^-22 of the bits that they
+    // Up to a bin, these sums are off by 2^-18 of the sum of all (roundings of b shift the weights by up to 2^-22 of the bits that they
     // are below the largest, which is less than log2(vocab) on average, and most of that is the same for all), and by less than 1 a
-    // weight that is cut off.  Were it more, the exact sums below would tell, and the row go to sample_many.
-    const u64_t about = total_of(s.sum, mine, before), want_about = run_of(p, about), off = (about >> 18) + 2 * (u64_t)row.V;
+    // bin that is cut off.  Were it more, the exact sums below would tell, and the row go to sample_many.
+    const u64_t about = total_of(s.sum, mine, before), want_about = run_of(p, about), off = (about >> 18) + 2 * SBINS;
     find_bin(s.sum, mine, before, want_about > off ? want_about - off : 1);
     const float first = (float)uniform(s.bin);
     __syncthreads();
@@ -708,7 +712,8 @@ __global__ __launch_bounds__(SNT) void sample_rows_kernel(SampleArgs a, int S) {
     sw.Md = sw.M;
     sw.c = c * STABLE;
     sw.least = -(double)(S + 2) * STABLE;
-    const float per_bit = (float)SBINS / (float)(S + 1);
+    const float per_bit = (float)(SBINS / (S + 1));  // (whole: a bin's weights are between two powers of two)
+    sw.bins = per_bit * (float)(S + 1);
     sw.cb = (float)min(c * per_bit, 0x1p127);  // (finite: 0 times it has to be 0)
     sw.S = S;
     sw.table = s.table;
@@ -726,7 +731,7 @@ __global__ __launch_bounds__(SNT) void sample_rows_kernel(SampleArgs a, int S) {
         many = !sample_run(row, sw, p, least, u);
     } else if (by_k || low > 0.0f) {
         // Few candidates are the usual case: they are listed and sorted.
-        float edge = (float)SBINS;  // behind the last bin that can hold a kept one
+        float edge = sw.bins;  // behind the last bin that can hold a kept one
         u64_t want = 0;
         bool cut = false;  // by k
         if (by_k) {
@@ -734,7 +739,7 @@ __global__ __launch_bounds__(SNT) void sample_rows_kernel(SampleArgs a, int S) {
             __syncthreads();
             row.each([&](int, float l) {
                 const float b = sw.below(l);
-                if (b < (float)SBINS) atomicAdd(&s.count[(int)b], 1u);
+                if (b < sw.bins) atomicAdd(&s.count[(int)b], 1u);
             });
             __syncthreads();
             u64_t mine, before;

@@ -8,7 +8,7 @@ namespace th {
 static void require_weight(const th_device* dev, size_t rows, size_t cols) {
     TH_REQUIRE(!dev->closed, "the device was destroyed");
     TH_REQUIRE(rows > 0 && cols > 0, "empty matrix");
-    TH_REQUIRE(rows < (size_t)1 << 27 && cols <= I8_MAX_K, "sizes out of range");
+    TH_REQUIRE(rows <= I8_MAX_ROWS && cols <= I8_MAX_K, "sizes out of range");
     TH_REQUIRE(!dev->capturing, "makes a new weight: not while a graph is captured");
 }
 
@@ -100,7 +100,7 @@ int th_gemm_i8(th_device* dev, const th_buffer* xq, const th_buffer* x_scale, si
     if (!w->per_row) throw Error(TH_ERR_UNSUPPORTED, "th_gemm_i8: the weight has a scale for each group of 32 (th_gemv_q8 takes those): needs one a row");
     TH_REQUIRE(w->cols <= I8_MAX_K, "sums of 2^17 products and more leave 32 bits");
     TH_REQUIRE(y->dtype == TH_F32 || y->dtype == TH_F16 || y->dtype == TH_BF16, "y must be f32, f16 or bf16");
-    TH_REQUIRE(m < (size_t)1 << 31 && w->rows < (size_t)1 << 27, "sizes out of range");  // (a launch has below 2^32 threads)
+    TH_REQUIRE(m < (size_t)1 << 31 && w->rows <= I8_MAX_ROWS, "sizes out of range");
     require_len(xq, TH_I8, m * w->Kp, "xq");
     require_len(x_scale, TH_F32, m, "x_scale");
     if (bias) require_len(bias, TH_F32, w->rows, "bias");

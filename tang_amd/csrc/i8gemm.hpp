@@ -18,6 +18,8 @@ namespace th {
 
 // Sums of K products of two int8 (at most 2^14 each) stay in 32 bits below this.
 constexpr size_t I8_MAX_K = ((size_t)1 << 17) - 1;
+// Rows of a weight: 2^23 tiles of 16 by 512 threads would be the 2^32 that a launch stays below.
+constexpr size_t I8_MAX_ROWS = ((size_t)1 << 27) - 16;
 
 // Where results go: (sum s_i) t_j + b_j in f64, so that no order of the scales
 // leaves f32's range on the way, rounded to f32 and then to the output's type.

@@ -105,3 +105,28 @@ def test_pack_and_product(lib):
     c.call("th_capture_begin", c.dev)
     f.refused("capture")
     z.refused("capture")
+
+
+def test_as_many_rows_as_a_launch_takes(lib):
+    """A launch has 32 threads for each weight row at most (512 for 16 of them), and below 2^32 of them in all: weights of up to 2^27 - 16 rows,
+    as more are 2^27 in whole tiles of 16."""
+    c = Cache(lib)
+    out = ctypes.c_void_p()
+    q, s, x = c.buffer(64, I8), c.buffer(1, F32), c.buffer(1, F32)
+    pack = Refusals(c, "th_q8_pack_rows", dev=c.dev, q=q, scale=s, rows=1, cols=1, out=ctypes.byref(out))
+    make = Refusals(c, "th_q8_quantize", dev=c.dev, x=x, rows=1, cols=1, out=ctypes.byref(out))
+    pack.call()
+    w = ctypes.c_void_p(out.value)
+    g = Refusals(c, "th_gemm_i8", dev=c.dev, xq=q, xs=s, m=0, w=w, bias=None, y=x)
+    for rows in ((1 << 27) - 15, (1 << 27) - 1):
+        pack.refused("out of range", rows=rows)
+        make.refused("out of range", rows=rows)
+        lib.host_rows(w, ctypes.c_size_t(rows))
+        g.refused("out of range")
+    # one tile fewer is taken (the buffers are too small for such weights)
+    pack.refused("too small", rows=(1 << 27) - 16)
+    make.refused("too small", rows=(1 << 27) - 16)
+    lib.host_rows(w, ctypes.c_size_t((1 << 27) - 16))
+    g.call()
+    lib.host_rows(w, ctypes.c_size_t(1))
+    c.call("th_qweight_free", w)

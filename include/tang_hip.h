@@ -191,8 +191,8 @@ int th_q8_quantize(th_device* dev, const th_buffer* x, size_t rows, size_t cols,
 int th_q8_pack_rows(th_device* dev, const th_buffer* q, const th_buffer* scale, size_t rows, size_t cols, th_qweight** out);
 /* y[m][n] = (sum_k q[m][k] w[n][k]) x_scale[m] w_scale[n] + bias[n].  xq as th_quantize_rows gives it (what
  * lies behind k does not count), bias f32 [n] or NULL; y f32, f16 or bf16.  Sums are exact (int32); the
- * rest is in f64, rounded once, for f32 results, and in f32 (off by 3 2^-24 of the product) for 16-bit ones.  Weights of
- * fewer than 2^17 columns and up to 2^27 - 16 rows; those with a scale for each group of 32 are TH_ERR_UNSUPPORTED. */
+ * rest is in f64, rounded once, for f32 results, and in f32 (off by 3 2^-24 of the product, which is infinite
+ * beyond f32's range) for 16-bit ones.  A row's results are the same bits in any batch.  Weights of fewer than 2^17 columns and up to 2^27 - 16 rows; those with a scale for each group of 32 are TH_ERR_UNSUPPORTED. */
 int th_gemm_i8(th_device* dev, const th_buffer* xq, const th_buffer* x_scale, size_t m, const th_qweight* w,
                const th_buffer* bias, th_buffer* y);
 

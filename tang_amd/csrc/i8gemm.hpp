@@ -21,8 +21,8 @@ constexpr size_t I8_MAX_K = ((size_t)1 << 17) - 1;
 // Rows of a weight: 2^23 tiles of 16 by 512 threads would be the 2^32 that a launch stays below.
 constexpr size_t I8_MAX_ROWS = ((size_t)1 << 27) - 16;
 
-// Where results go: (sum s_i) t_j + b_j in f64, so that no order of the scales
-// leaves f32's range on the way, rounded to f32 and then to the output's type.
+// Where results go: (sum s_i) t_j + b_j, so formed that no order of the scales
+// leaves f32's range on the way (i8kernels.hpp), and rounded to the output's type.
 struct I8Out {
     void* y;
     const float *xs, *ws, *bias;  // [M], [N], [N] or null

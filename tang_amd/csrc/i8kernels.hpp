@@ -12,7 +12,8 @@ typedef int i32x16_t __attribute__((ext_vector_type(16)));
 
 // (sum s) t + b.  For f32 results in f64, rounded once (no order of the scales leaves
 // its range); for 16-bit ones in f32 from the scales' mantissas and the sum of their exponents: off
-// by 3 2^-24 of the product, far below their own rounding, at a third of the time.
+// by 3 2^-24 of the product, far below their own rounding, at a third of the time.  Both
+// kernels do the same, so that a row has the same bits in any batch.
 __device__ __forceinline__ float i8_wide(int sum, float s, float t, float b) { return (float)((double)sum * (double)s * (double)t + (double)b); }
 __device__ __forceinline__ float i8_narrow(int sum, float s, float t, int exponent, float b) {
     return __builtin_amdgcn_ldexpf((float)sum * (s * t), exponent) + b;
@@ -102,9 +103,16 @@ __global__ __launch_bounds__(64 * NW) void i8_rows_kernel(const uint4* __restric
         const int n = (bx * RT + a) * 16 + (ln & 15), m = b * 16 + (ln >> 4) * 4;
         if (n >= out.N) continue;
         const float wsc = out.ws[n], bias = out.bias ? out.bias[n] : 0.0f;
+        int we = 0;
+        const float wf = __builtin_frexpf(wsc, &we);
 #pragma unroll
-        for (int e = 0; e < 4; e++)
-            if (m + e < M) i8_store(out, m + e, n, i8_wide(s[e], out.xs[m + e], wsc, bias));
+        for (int e = 0; e < 4; e++) {
+            if (m + e >= M) continue;
+            const float xsc = out.xs[m + e];
+            int xe = 0;
+            const float xf = __builtin_frexpf(xsc, &xe);
+            i8_store(out, m + e, n, out.dt == TH_F32 ? i8_wide(s[e], xsc, wsc, bias) : i8_narrow(s[e], xf, wf, xe + we, bias));
+        }
     }
 }
 

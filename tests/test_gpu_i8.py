@@ -261,3 +261,24 @@ def test_results_beyond_32_bits_of_places(dev):
         p = (q.astype(np.int64) @ w.astype(np.int64).T) * s[list(rows)].astype(np.float64)[:, None] * t.astype(np.float64)
         tol = 3 * 2.0 ** -24 * np.abs(p) * (1 + 2.0 ** -8) + np.maximum(EPS[BF16] * np.abs(p), LEAST[BF16])
         assert np.all(np.abs(from_bits(got[list(rows)], BF16) - p) <= tol)
+
+
+@pytest.mark.parametrize("dt", [F32, F16, BF16])
+@pytest.mark.parametrize("bias", [False, True])
+def test_rows_have_their_bits_in_any_batch(dev, dt, bias):
+    """A row's results are the same bits alone, among few rows and among many."""
+    rng = np.random.default_rng(21)
+    m, k, n = 300, 1000, 2000
+    x = rng.standard_normal((m, k)).astype(np.float32) * np.exp(rng.uniform(-3, 3, (m, 1))).astype(np.float32)
+    w = dev.q8_quantize(dev.upload(rng.standard_normal((n, k)).astype(np.float32)), n, k)
+    b = dev.upload(rng.standard_normal(n).astype(np.float32)) if bias else None
+
+    def rows(first, count):
+        q, s = dev.quantize_rows(dev.upload(x[first:first + count]), count, k)
+        return dev.gemm_i8(q, s, count, w, dev.alloc(count * n, dt), b).to_numpy().reshape(count, n)
+    want = rows(0, m)
+    assert len(set(want.reshape(-1).tolist())) > 1000
+    for first, count in ((0, 1), (7, 16), (20, 31), (100, 64), (40, 65), (3, 200)):
+        got = rows(first, count)
+        bad = np.argwhere(got != want[first:first + count])
+        assert not len(bad), (count, len(bad), bad[0])

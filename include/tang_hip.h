@@ -421,8 +421,9 @@ int th_sampler_sample(th_sampler* s, const float* logits, size_t vocab, const in
  *               exp(logit / temperature) reach top_p of their sum; from 1 on: off, down to 0: one token
  *  min_p        f32; of those, weights from min_p times the largest on; 0: off
  * The token is the first, by index, at which the running sum of kept weights exceeds u times their sum; tokens u32
- * [n_rows], prob f32 [n_rows] (may be NULL): its share of that sum.  Weights and borders are right to 2^-42 of the
- * largest weight.  A NaN logit counts as -inf; infinite ones share all weight; a row that has nothing above -inf gives
+ * [n_rows], prob f32 [n_rows] (may be NULL): its share of that sum.  Weights are right to 2^-45 of themselves, and rounded to 2^-S of the largest one
+ * (below half of that: none), S = 62 less the bits of vocab - 1 and at most 51.  So sums, and the borders that they are,
+ * are off by up to vocab 2^-(S+1) of the largest weight: 2^-42 at 1024, 2^-33 at 32000, 2^-29 at 131072, 2^-23 at 2^20.  A NaN logit counts as -inf; infinite ones share all weight; a row that has nothing above -inf gives
  * token 0 with prob 0. */
 int th_sample_rows(th_device* dev, const th_buffer* logits, size_t n_rows, size_t vocab, const th_buffer* u,
                    const th_buffer* temperature, const th_buffer* top_k, const th_buffer* top_p, const th_buffer* min_p,

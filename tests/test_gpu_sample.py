@@ -280,3 +280,33 @@ def test_captured(dev):
         seen.append(tuple(want[0]))
     assert len(set(seen)) == 4
     graph.free()
+
+
+@pytest.mark.parametrize("V", [1000, 32000, 131072, 1 << 20])
+@pytest.mark.parametrize("part", [1.2, 0.8, 0.0])
+def test_small_weights_that_all_round_alike(dev, V, part):
+    """One large weight and V - 1 of which each is 2^-part of the last place that weights are held to: all become none (1.2), twice
+    as much as they nearly are (0.8), or what they are (0).  Running sums are off by half a last place for each weight, and by 2^-45 of
+    themselves (a weight's exponent has three roundings of up to 53 bits, 2^-46.2 of the weight; its series 2^-48; the table and the products 2^-50).
+    So each token's part of the sum, from border to border, reaches to u times the sum within twice that; its share is off by as much of the
+    sum and its rounding."""
+    last = 62 - (V - 1).bit_length() if V > 2048 else 51
+    off = V * 2.0 ** -(last + 1)
+    rng = np.random.default_rng(V)
+    u = np.concatenate((1 - 2.0 ** -np.arange(1, 25), rng.random(8))).astype(np.float32)
+    n = len(u)
+    small = np.float32(-(last + part) * np.log(2))
+    x = np.full((n, V), small, np.float32)
+    at = rng.integers(0, V, n)
+    x[np.arange(n), at] = 0
+    w = np.exp(float(small))
+    total = 1 + (V - 1) * w
+    off += total * 2.0 ** -45
+    for settings in (dict(), dict(k=np.full(n, V - 1, np.uint32)), dict(low=np.full(n, 1e-30))):
+        got, prob = _run(dev, x, F32, u, **settings)
+        for r in range(n):
+            before = got[r] * w + (1 - w if got[r] > at[r] else 0)
+            mine = 1.0 if got[r] == at[r] else w
+            target = float(u[r]) * total
+            assert before - 2 * off <= target <= before + mine + 2 * off, (r, got[r], at[r])
+            assert abs(prob[r] - mine / total) <= mine / total * (off + 2.0 ** -24)

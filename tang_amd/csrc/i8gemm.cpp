@@ -1,4 +1,6 @@
 // The 8-bit products' entry points: checks of arguments (i8gemm.hpp).
+#include <algorithm>
+
 #include "capi_util.hpp"
 #include "i8gemm.hpp"
 #include "kvcache.hpp"
@@ -40,6 +42,50 @@ static th_qweight* new_weight(th_device* dev, size_t rows, size_t cols, F&& fill
     }
     device_retain(dev);
     return w;
+}
+
+// Up to 64 rows the weights' stream bounds a product, and each workgroup takes all
+// rows and one to three tiles of 16 channels, so many that there is one a CU up to 768 tiles (12288 channels; beyond, three: the
+// last round of workgroups may be short):
+// 61 rows, 4096 x 11008: one tile 29.2 us, two 23.2, three 16.8.  (Up to 16 rows one tile is best: 12.3 against 12.4 us with
+// two, 4096 x 4096 at one row 4.7 against 5.4.)
+static I8Form i8_few_rows(size_t m, size_t n, size_t cus) {
+    const size_t tiles = ceil_div(ceil_div(n, (size_t)16), cus);
+    if (m <= 16) return I8Form::ROWS_1X1;
+    if (m <= 32) return tiles == 1 ? I8Form::ROWS_1X2 : I8Form::ROWS_2X2;
+    return tiles == 1 ? I8Form::ROWS_1X4 : tiles == 2 ? I8Form::ROWS_2X4 : I8Form::ROWS_3X4;
+}
+
+// Beyond: the tile whose rounds over the chip take least, by what one costs a CU (us, measured at K = 64 and 4096; workgroups that
+// share a CU take as long as one after the other).  512 x 4096 x 4096: 64 x 64 tiles 26.3 us, 64 x 128 18.3 to 19.6, 128 x 128 25.9;
+// 2048 x 4096 x 4096: 128 x 128 52.8, 128 x 256 41.6, 256 x 256 63.9; 8192 x 8192 x 8192: 128 x 256 547, 256 x 256 499.
+// A 64 x 128 tile alone on its CU has two groups of waves (100 x 4096 x 11008: 18.9 against 24.4 us; 509 x 2047 x 5631, where
+// two share a CU: 20.7 against 17.9).  A round counts as one however few CUs work in it: k is not split over workgroups.
+I8Form i8_form(size_t m, size_t n, size_t k, size_t cus) {
+    if (m <= 64) return i8_few_rows(m, n, cus);
+    const double steps = (double)ceil_div(k, (size_t)64);
+    struct Tile { size_t rows, cols; double fixed, step; I8Form form; };
+    const Tile tiles[] = {{64, 64, 1.0, 0.175, I8Form::TILE_64X64}, {64, 128, 2.2, 0.23, I8Form::TILE_64X128},
+                          {128, 128, 4.0, 0.304, I8Form::TILE_128X128}, {128, 256, 7.0, 0.47, I8Form::TILE_128X256},
+                          {256, 256, 14.5, 0.8, I8Form::TILE_256X256}};
+    const Tile* best = nullptr;
+    double least = 0.0;
+    size_t count = 0;
+    for (const Tile& tile : tiles) {
+        const size_t c = ceil_div(m, tile.rows) * ceil_div(n, tile.cols);
+        const double t = (double)ceil_div(c, cus) * (tile.fixed + tile.step * steps);
+        if (!best || t < least) {
+            best = &tile;
+            least = t;
+            count = c;
+        }
+    }
+    return best->form == I8Form::TILE_64X128 && count <= cus ? I8Form::TILE_64X128_TWO : best->form;
+}
+
+// A launch has below 2^32 threads (at most 8 for each 16 x 16 results) and 2^16 blocks of rows; whole blocks of quantized rows.
+size_t i8_rows_at_once(size_t n) {
+    return std::min<size_t>((size_t)1 << 21, std::max<size_t>(16, ((size_t)1 << 28) / ceil_div(n, (size_t)16) / 16 * 16));
 }
 
 }  // namespace th

@@ -235,62 +235,31 @@ static void i8_tile_launch(const th_qweight* w, const int8_t* xq, const I8Out& o
     TH_LAUNCH_CHECK();
 }
 
-// Up to 64 rows the weights' stream bounds a product, and each workgroup takes all
-// rows and one to three tiles of 16 channels, so many that there is one a CU:
-// 61 rows, 4096 x 11008: one tile 29.2 us, two 23.2, three 16.8.  (Up to 16 rows one tile is best: 12.3 against 12.4 us with
-// two, 4096 x 4096 at one row 4.7 against 5.4.)
-static void i8_few_rows(const th_qweight* w, const int8_t* xq, const I8Out& out, size_t m, size_t cus, hipStream_t s) {
-    const size_t tiles = ceil_div(w->Np / 16, cus);
-    if (m <= 16) i8_rows_launch<1, 1, 8>(w, xq, out, m, s);
-    else if (m <= 32 && tiles == 1) i8_rows_launch<1, 2, 4>(w, xq, out, m, s);
-    else if (m <= 32) i8_rows_launch<2, 2, 4>(w, xq, out, m, s);
-    else if (tiles == 1) i8_rows_launch<1, 4, 2>(w, xq, out, m, s);
-    else if (tiles == 2) i8_rows_launch<2, 4, 2>(w, xq, out, m, s);
-    else i8_rows_launch<3, 4, 2>(w, xq, out, m, s);
-}
-
-// Beyond: the tile whose rounds over the chip take least, by what one costs a CU (us, measured at K = 64 and 4096; workgroups that
-// share a CU take as long as one after the other).  512 x 4096 x 4096: 64 x 64 tiles 26.3 us, 64 x 128 18.3 to 19.6, 128 x 128 25.9;
-// 2048 x 4096 x 4096: 128 x 128 52.8, 128 x 256 41.6, 256 x 256 63.9; 8192 x 8192 x 8192: 128 x 256 547, 256 x 256 499.
-// A 64 x 128 tile alone on its CU has two groups of waves (100 x 4096 x 11008: 18.9 against 24.4 us; 509 x 2047 x 5631, where
-// two share a CU: 20.7 against 17.9).
-static void i8_many_rows(const th_qweight* w, const int8_t* xq, const I8Out& out, size_t m, size_t cus, hipStream_t s) {
-    const double steps = (double)(w->Kp / 64);
-    struct Tile { size_t rows, cols; double fixed, step; };
-    const Tile tiles[] = {{64, 64, 1.0, 0.175}, {64, 128, 2.2, 0.23}, {128, 128, 4.0, 0.304}, {128, 256, 7.0, 0.47}, {256, 256, 14.5, 0.8}};
-    int best = 0;
-    double least = 0.0;
-    size_t count = 0;
-    for (int i = 0; i < 5; i++) {
-        const size_t n = ceil_div(m, tiles[i].rows) * ceil_div(w->rows, tiles[i].cols);
-        const double t = (double)ceil_div(n, cus) * (tiles[i].fixed + tiles[i].step * steps);
-        if (i == 0 || t < least) {
-            best = i;
-            least = t;
-            count = n;
-        }
-    }
-    switch (best) {
-        case 0: return i8_tile_launch<1, 1, 1, 4, 4>(w, xq, out, m, s);
-        case 1:
-            if (count <= cus) return i8_tile_launch<1, 2, 2, 2, 2>(w, xq, out, m, s);
-            return i8_tile_launch<1, 2, 1, 4, 3>(w, xq, out, m, s);
-        case 2: return i8_tile_launch<2, 2, 1, 2, 2>(w, xq, out, m, s);
-        case 3: return i8_tile_launch<2, 4, 1, 2, 2>(w, xq, out, m, s);
-        default: return i8_tile_launch<4, 4, 1, 2, 1>(w, xq, out, m, s);
+static void i8_launch(I8Form form, const th_qweight* w, const int8_t* xq, const I8Out& out, size_t m, hipStream_t s) {
+    switch (form) {
+        case I8Form::ROWS_1X1: return i8_rows_launch<1, 1, 8>(w, xq, out, m, s);
+        case I8Form::ROWS_1X2: return i8_rows_launch<1, 2, 4>(w, xq, out, m, s);
+        case I8Form::ROWS_2X2: return i8_rows_launch<2, 2, 4>(w, xq, out, m, s);
+        case I8Form::ROWS_1X4: return i8_rows_launch<1, 4, 2>(w, xq, out, m, s);
+        case I8Form::ROWS_2X4: return i8_rows_launch<2, 4, 2>(w, xq, out, m, s);
+        case I8Form::ROWS_3X4: return i8_rows_launch<3, 4, 2>(w, xq, out, m, s);
+        case I8Form::TILE_64X64: return i8_tile_launch<1, 1, 1, 4, 4>(w, xq, out, m, s);
+        case I8Form::TILE_64X128_TWO: return i8_tile_launch<1, 2, 2, 2, 2>(w, xq, out, m, s);
+        case I8Form::TILE_64X128: return i8_tile_launch<1, 2, 1, 4, 3>(w, xq, out, m, s);
+        case I8Form::TILE_128X128: return i8_tile_launch<2, 2, 1, 2, 2>(w, xq, out, m, s);
+        case I8Form::TILE_128X256: return i8_tile_launch<2, 4, 1, 2, 2>(w, xq, out, m, s);
+        case I8Form::TILE_256X256: return i8_tile_launch<4, 4, 1, 2, 1>(w, xq, out, m, s);
     }
 }
 
 void launch_i8_linear(th_device* dev, const th_qweight* w, const int8_t* xq, const I8Out& out, size_t m) {
-    // a launch has below 2^32 threads (at most 8 for each 16 x 16 results) and 2^16 blocks of rows
-    const size_t rows = std::min<size_t>((size_t)1 << 21, std::max<size_t>(16, ((size_t)1 << 28) / (w->Np / 16) / 16 * 16));
+    const size_t rows = i8_rows_at_once(w->rows);
     for (size_t m0 = 0; m0 < m; m0 += rows) {
         I8Out o = out;
         o.y = (char*)out.y + m0 * w->rows * dtype_size(out.dt);
         o.xs = out.xs + m0;
         const size_t n = std::min(rows, m - m0);
-        if (n <= 64) i8_few_rows(w, xq + m0 * w->Kp, o, n, (size_t)dev->num_cus, dev->stream);
-        else i8_many_rows(w, xq + m0 * w->Kp, o, n, (size_t)dev->num_cus, dev->stream);
+        i8_launch(i8_form(n, w->rows, w->cols, (size_t)dev->num_cus), w, xq + m0 * w->Kp, o, n, dev->stream);
     }
 }
 

@@ -30,6 +30,12 @@ struct I8Out {
     int N;
 };
 
+// The kernel of a product (i8gemm.hip): of up to 64 rows, by tiles of 16 channels and of 16 rows that a workgroup has; of more, by
+// the tile's rows and channels.  At most i8_rows_at_once(n) rows go to a launch.
+enum class I8Form { ROWS_1X1, ROWS_1X2, ROWS_2X2, ROWS_1X4, ROWS_2X4, ROWS_3X4, TILE_64X64, TILE_64X128_TWO, TILE_64X128, TILE_128X128, TILE_128X256, TILE_256X256 };
+I8Form i8_form(size_t m, size_t n, size_t k, size_t cus);
+size_t i8_rows_at_once(size_t n);
+
 // whole: the last block too has 16 rows, zeros (and scales of zero) behind the m.
 void launch_quantize_rows(const void* x, th_dtype xdt, size_t m, size_t K, int8_t* q, float* scale, bool whole, hipStream_t s);
 void launch_q8_pack(const int8_t* q, const float* scale, const th_qweight* w, hipStream_t s);

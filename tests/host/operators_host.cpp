@@ -43,6 +43,8 @@ void host_grouped(th_qweight* w, int bits, int per_row) {
     w->bits = bits;
     w->per_row = per_row != 0;
 }
+int host_i8_form(size_t m, size_t n, size_t k, size_t cus) { return (int)i8_form(m, n, k, cus); }
+size_t host_i8_rows(size_t n) { return i8_rows_at_once(n); }
 void host_rows(th_qweight* w, size_t rows) { w->rows = rows; }
 void host_last(size_t* v) {
     v[0] = g_m;

@@ -4,6 +4,7 @@ import os
 
 import pytest
 
+import i8_sizes
 from host_operators import CLANG, Cache, Refusals, Refused, build
 from tang_amd import capi
 
@@ -130,3 +131,34 @@ def test_as_many_rows_as_a_launch_takes(lib):
     g.call()
     lib.host_rows(w, ctypes.c_size_t(1))
     c.call("th_qweight_free", w)
+
+
+def test_every_form_of_a_product_is_run(lib):
+    """The sizes that the GPU tests run take, by the rule on a card of 256 CUs, the forms that stand beside them: each of them, with rows and channels
+    that are no whole tiles and a k of no whole chunks."""
+    lib.host_i8_form.argtypes = [ctypes.c_size_t] * 4
+    names = [i8_sizes.FORMS[lib.host_i8_form(m, n, k, 256)] for _, m, k, n in i8_sizes.SIZES]
+    assert names == [s[0] for s in i8_sizes.SIZES]
+    for f in i8_sizes.FORMS:
+        mine = [s for s in i8_sizes.SIZES if s[0] == f]
+        assert any(m % 16 and n % 16 for _, m, k, n in mine) and any(k % 64 for _, m, k, n in mine) and any(-(-k // 64) % 4 > 0 for _, m, k, n in mine), f
+
+
+def test_launches_of_a_product(lib):
+    """Slices of rows are whole blocks of 16; a launch has below 2^32 threads and 2^16 tiles of rows."""
+    lib.host_i8_rows.argtypes, lib.host_i8_rows.restype = [ctypes.c_size_t], ctypes.c_size_t
+    lib.host_i8_form.argtypes = [ctypes.c_size_t] * 4
+    threads = {"tile 64x64": 256, "tile 64x128, two groups": 512, "tile 64x128": 256, "tile 128x128": 256, "tile 128x256": 256, "tile 256x256": 256}
+    for n in (1, 16, 17, 4096, 32000, (1 << 20) + 5, 1 << 24, (1 << 27) - 16):
+        rows = lib.host_i8_rows(n)
+        assert rows % 16 == 0 and 16 <= rows <= 1 << 21
+        for m in (1, 17, 33, 65, 129, rows):
+            if m > rows:
+                continue
+            form = i8_sizes.FORMS[lib.host_i8_form(m, n, 64, 256)]
+            kind, size = form.split(",")[0].split()
+            a, b = (int(v) for v in size.split("x"))
+            if kind == "rows":
+                assert -(-n // 16 // a) * 512 < 1 << 32 and -(-m // 16) <= b
+            else:
+                assert -(-m // a) * -(-n // b) * threads[form] < 1 << 32 and -(-m // a) < 1 << 16

@@ -310,3 +310,30 @@ def test_small_weights_that_all_round_alike(dev, V, part):
             target = float(u[r]) * total
             assert before - 2 * off <= target <= before + mine + 2 * off, (r, got[r], at[r])
             assert abs(prob[r] - mine / total) <= mine / total * (off + 2.0 ** -24)
+
+
+def test_rows_in_slices(dev):
+    """2^21 rows and three more, which a launch of its own takes, each with its settings: of two logits (all rows checked), and of one."""
+    rng = np.random.default_rng(31)
+    n = (1 << 21) + 3
+    x = rng.standard_normal((n, 2)).astype(np.float32)
+    u, temp = rng.random(n, np.float32), np.where(rng.random(n) < 0.1, 0.0, rng.uniform(0.3, 2, n)).astype(np.float32)
+    k = rng.integers(0, 4, n).astype(np.uint32)
+    p, low = (np.where(rng.random(n) < 0.5, off, rng.random(n)).astype(np.float32) for off in (1.0, 0.0))
+    with np.errstate(divide="ignore"):
+        w = np.exp(-np.abs(x[:, 0].astype(np.float64) - x[:, 1]) / temp)  # of the smaller one
+    first = (x[:, 1] > x[:, 0]).astype(np.int64)
+    share = np.where(first == 0, 1 / (1 + w), w / (1 + w))  # of the logit at 0
+    u[np.abs(u - share) < 1e-5] = 0  # (none on a border)
+    p[np.abs(1 - p * (1 + w)) < 1e-5] = 1
+    low[np.abs(w - low) < 1e-5] = 0
+    both = (temp > 0) & (k != 1) & ((p >= 1) | (p * (1 + w) > 1)) & ((low <= 0) | (w >= low))
+    want = np.where(both, (u >= share).astype(np.int64), first)
+    part = np.where(both, np.where(want == 0, share, 1 - share), 1.0)
+    got, prob = _run(dev, x, F32, u, temp, k, p, low)
+    bad = np.flatnonzero(got != want)
+    assert not len(bad), (len(bad), bad[0], u[bad[0]], share[bad[0]])
+    assert np.all(np.abs(prob - part) <= part * 2.0 ** -22)
+    x[::7] = -np.inf
+    got, prob = _run(dev, x[:, :1], BF16, u, temp, k, p, low)
+    assert not got.any() and np.array_equal(prob, np.isfinite(x[:, 0]).astype(np.float32))

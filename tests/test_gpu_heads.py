@@ -271,3 +271,57 @@ def test_replays_give_the_eager_bits(dev):
         assert all(np.array_equal(a, b) for a, b in zip(*got))
         assert np.all(got[0][0][n * H * hd:] == 0x4321) and not np.any(got[0][0][:n * H * hd] == 0x4321)
     graph.free()
+
+
+@pytest.mark.parametrize("hd,rot", [(64, 64), (96, 20), (6, 2)])
+@pytest.mark.parametrize("xdt,qdt,kdt", [(F32, BF16, F16), (BF16, F32, F16), (F16, BF16, F32), (BF16, BF16, F32), (F16, F32, F16)])
+def test_results_of_two_types(dev, hd, rot, xdt, qdt, kdt):
+    """Queries and keys that leave in types of their own, from rows of their own and from packed ones."""
+    rng = np.random.default_rng(hd + rot + xdt)
+    n, H, K = 9, 3, 2
+    cos, sin, dc, ds = _tables(dev, rot, 20)
+    w, dw = _weights(dev, rng, hd, F32)
+    x = rounded(2 * _normal(rng, n, H + K, hd), xdt)
+    want = [_formula(t, v, 1e-6, cos, sin, np.arange(n) + 4, rot, 1) for t, v in ((x[:, :H], w[0]), (x[:, H:], w[1]))]
+    for packed in (False, True):
+        q, k = dev.alloc(n * H * hd, qdt), dev.alloc(n * K * hd, kdt)
+        up = lambda t: dev.upload(to_bits(np.ascontiguousarray(t), xdt), xdt)  # noqa: E731
+        ins = (up(x), None) if packed else (up(x[:, :H]), up(x[:, H:]))
+        dev.qk_norm_rope(*ins, *dw, 1e-6, dc, ds, n, H, K, hd, rot, 1, start_pos=4, q_out=q, k_out=k)
+        _check(from_bits(q.to_numpy(), qdt).reshape(n, H, hd), want[0], qdt)
+        _check(from_bits(k.to_numpy(), kdt).reshape(n, K, hd), want[1], kdt)
+
+
+def test_replays_of_a_long_batch_on_few_rows(dev):
+    """A step captured for so many rows that lanes take several heads each, replayed on one row, a few and all: the eager bits, and
+    what lies behind the rows stays."""
+    rng = np.random.default_rng(17)
+    K, H, hd, top = 2, 6, 64, 30000
+    cache = dev.kv_cache(1, K, hd, 64, 480, 2, top, F16)
+    batch, seqs = cache.batch(2, top, H), cache.seq_create(2)
+    cos, sin, dc, ds = _tables(dev, 48, top)
+    w, dw = _weights(dev, rng, hd, F32)
+    x, out = dev.alloc(top * (H + 2 * K) * hd, F16), dev.alloc(top * H * hd, F16)
+    call = lambda: batch.append_norm(0, x, None, None, out, *dw, 1e-6, dc, ds, 48, 1)  # noqa: E731
+    batch.begin(seqs, [1, 0])
+    graph = dev.capture(call)
+    batch.trim([0, 0])
+    had = np.zeros(2, int)
+    for news in ([1, 0], [30, 31], [1, 1], [0, 61], [25000, 4875]):
+        n = sum(news)
+        rows = rounded(2 * _normal(rng, n, H + 2 * K, hd), F16)
+        full = np.zeros(top * (H + 2 * K) * hd, np.uint16)
+        full[:rows.size] = to_bits(rows, F16).reshape(-1)
+        x.upload(full)
+        batch.begin(seqs, news)
+        got = []
+        for go in (call, graph.launch):
+            out.upload(np.full(top * H * hd, 0x4321, np.uint16))
+            go()
+            got.append([out.to_numpy()] + [b.to_numpy() for i, s in enumerate(seqs) if had[i] + news[i] for b in cache.seq_read(s, 0)])
+        assert all(np.array_equal(a, b) for a, b in zip(*got, strict=True))
+        assert np.all(got[0][0][n * H * hd:] == 0x4321)
+        pos = np.concatenate([np.arange(had[i], had[i] + news[i]) for i in range(2)])
+        _check(from_bits(got[0][0][:n * H * hd], F16).reshape(n, H, hd), _formula(rows[:, :H], w[0], 1e-6, cos, sin, pos, 48, 1), F16)
+        had += news
+    graph.free()

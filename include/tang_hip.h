@@ -180,7 +180,8 @@ int th_gemv_q8(th_device* dev, const th_buffer* x, size_t m, const th_qweight* w
  *
  * x [m][k], f32, f16 or bf16 -> q, m * kp int8 (kp = k rounded up to 64; zeros behind k), and scale [m]:
  * scale_i = f32(max |x_i| / 127), q = x / scale to the nearest integer, ties to even, at most 127 in size.  A
- * row of zeros has scale 0; one with an infinity or NaN has scale NaN and zeros (its products are NaN).  k below 2^17.
+ * row of zeros has scale 0, as has one with nothing above 63 2^-149, whose q are zeros too; one with an infinity or NaN has
+ * scale NaN and zeros (its products are NaN).  k below 2^17.
  * q lies in blocks of h = 16 rows (fewer in the last): value (i, k) is at
  * (i - i % 16) * kp + (k - k % 16) * h + i % 16 * 16 + k % 16. */
 int th_quantize_rows(th_device* dev, const th_buffer* x, size_t m, size_t k, th_buffer* q, th_buffer* scale);
@@ -192,7 +193,8 @@ int th_q8_pack_rows(th_device* dev, const th_buffer* q, const th_buffer* scale, 
 /* y[m][n] = (sum_k q[m][k] w[n][k]) x_scale[m] w_scale[n] + bias[n].  xq as th_quantize_rows gives it (what
  * lies behind k does not count), bias f32 [n] or NULL; y f32, f16 or bf16.  Sums are exact (int32); the
  * rest is in f64, rounded once, for f32 results, and in f32 (off by 3 2^-24 of the product, which is infinite
- * beyond f32's range) for 16-bit ones.  A row's results are the same bits in any batch.  Weights of fewer than 2^17 columns and up to 2^27 - 16 rows; those with a scale for each group of 32 are TH_ERR_UNSUPPORTED. */
+ * beyond f32's range) for 16-bit ones.  A row's results are the same bits in any batch.  Weights of fewer than
+ * 2^17 columns and up to 2^27 - 16 rows; those with a scale for each group of 32 are TH_ERR_UNSUPPORTED. */
 int th_gemm_i8(th_device* dev, const th_buffer* xq, const th_buffer* x_scale, size_t m, const th_qweight* w,
                const th_buffer* bias, th_buffer* y);
 
@@ -421,10 +423,11 @@ int th_sampler_sample(th_sampler* s, const float* logits, size_t vocab, const in
  *               exp(logit / temperature) reach top_p of their sum; from 1 on: off, down to 0: one token
  *  min_p        f32; of those, weights from min_p times the largest on; 0: off
  * The token is the first, by index, at which the running sum of kept weights exceeds u times their sum; tokens u32
- * [n_rows], prob f32 [n_rows] (may be NULL): its share of that sum.  Weights are right to 2^-45 of themselves, and rounded to 2^-S of the largest one
- * (below half of that: none), S = 62 less the bits of vocab - 1 and at most 51.  So sums, and the borders that they are,
- * are off by up to vocab 2^-(S+1) of the largest weight: 2^-42 at 1024, 2^-33 at 32000, 2^-29 at 131072, 2^-23 at 2^20.  A NaN logit counts as -inf; infinite ones share all weight; a row that has nothing above -inf gives
- * token 0 with prob 0. */
+ * [n_rows], prob f32 [n_rows] (may be NULL): its share of that sum.  Weights are right to 2^-45 of themselves, and
+ * rounded to 2^-S of the largest one (below half of that: none), S = 62 less the bits of vocab - 1 and at most 51.  So
+ * sums, and with them borders, are off by up to vocab 2^-(S+1) of the largest weight: 2^-42 at 1024, 2^-33 at 32000,
+ * 2^-29 at 131072, 2^-23 at 2^20.  A NaN logit counts as -inf; infinite ones share all weight; a row that has nothing
+ * above -inf gives token 0 with prob 0. */
 int th_sample_rows(th_device* dev, const th_buffer* logits, size_t n_rows, size_t vocab, const th_buffer* u,
                    const th_buffer* temperature, const th_buffer* top_k, const th_buffer* top_p, const th_buffer* min_p,
                    th_buffer* tokens, th_buffer* prob);

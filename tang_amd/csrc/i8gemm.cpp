@@ -45,10 +45,11 @@ static th_qweight* new_weight(th_device* dev, size_t rows, size_t cols, F&& fill
 }
 
 // Up to 64 rows the weights' stream bounds a product, and each workgroup takes all
-// rows and one to three tiles of 16 channels, so many that there is one a CU up to 768 tiles (12288 channels; beyond, three: the
-// last round of workgroups may be short):
+// rows and one to three tiles of 16 channels, so many that there is one workgroup a CU:
 // 61 rows, 4096 x 11008: one tile 29.2 us, two 23.2, three 16.8.  (Up to 16 rows one tile is best: 12.3 against 12.4 us with
-// two, 4096 x 4096 at one row 4.7 against 5.4.)
+// two, 4096 x 4096 at one row 4.7 against 5.4.)  Beyond 768 tiles, 12288 channels on 256 CUs, there are more workgroups than
+// CUs, and of those with three tiles (96 KiB) a CU holds one, so that a last round may be nearly empty: 61 rows of 4096, 12288 channels 12.9 us, 12304
+// 20.4, 14336 23.0, 24576 26.3.
 static I8Form i8_few_rows(size_t m, size_t n, size_t cus) {
     const size_t tiles = ceil_div(ceil_div(n, (size_t)16), cus);
     if (m <= 16) return I8Form::ROWS_1X1;

@@ -477,7 +477,8 @@ __device__ __forceinline__ u64_t run_of(float p, u64_t all) {  // that top-p's r
 }
 
 // A row with more candidates than a list holds: thresholds by refined histograms, then the sum over the row.  The
-// token goes to s.found, the sum to s.above.
+// token goes to s.found, the sum to s.above.  Up to some ten passes, each bound by one CU's vector instructions (48 rows of 50001 normal
+// logits: top-k 8000 74 us, and top-p 0.9 of those 122; all logits in one bin 184 and 293, top-p alone 227, where lists take 40).
 template <typename X>
 __device__ __noinline__ void sample_many(const X* x, int V, bool infinite, SampleWeights sw, uint32_t k, bool by_k, float p, bool by_p, u64_t least_w, float u) {
     const int tid = threadIdx.x, lane = tid & 63;

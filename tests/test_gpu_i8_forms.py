@@ -74,3 +74,31 @@ def test_rows_quantized_in_slices(dev):
     one, unit = dev.upload(np.concatenate((np.array([3], np.int8), np.zeros(63, np.int8))), I8), dev.upload(np.array([0.5], np.float32))
     y = dev.gemm_i8(one, unit, 1, dev.q8_quantize(dx, m, 1)).to_numpy()
     assert np.array_equal(y, (3.0 * q[:, 0].astype(np.float64) * 0.5 * s.astype(np.float64)).astype(np.float32))
+
+
+@pytest.mark.parametrize("dt", [F32, F16, BF16])
+@pytest.mark.parametrize("m", [3, 40, 90])
+def test_scales_at_the_ends_of_f32(dev, m, dt):
+    """Subnormal scales beside large ones, zeros, infinities and NaN, whose products are ordinary numbers, none, infinite or NaN."""
+    rng = np.random.default_rng(m)
+    k, n = 70, 36
+    q, wq = (rng.integers(-128, 128, (r, k)).astype(np.int8) for r in (m, n))
+    wq[:, 0] = 0
+    q[:, 1:][0] = 0  # sums of zero
+    rows = np.zeros(m * _kp(k), np.int8)
+    rows[_places(m, _kp(k))[:, :k]] = q
+    ends = np.array([1e-45, 3e-42, 1e-39, 1.2e-38, 1e-30, 1.0, 1e30, 3e38, 0.0, np.inf, np.nan], np.float32)
+    s, t = ends[np.arange(m) % len(ends)], ends[rng.permutation(np.arange(n) % len(ends))]
+    y = dev.alloc(m * n, dt)
+    dev.gemm_i8(dev.upload(rows, I8), dev.upload(s), m, dev.q8_upload_rowwise(wq, t, n, k), y)
+    got = y.to_numpy().reshape(m, n)
+    with np.errstate(all="ignore"):
+        p = (q.astype(np.float64) @ wq.T.astype(np.float64)) * s.astype(np.float64)[:, None] * t.astype(np.float64)
+        if dt == F32:
+            return np.testing.assert_array_equal(got, p.astype(np.float32))
+        got = from_bits(got, dt).astype(np.float64)
+        assert np.array_equal(np.isnan(got), np.isnan(p))
+        top = {F16: 65520.0, BF16: 3.39e38}[dt]
+        over, fine = np.abs(p) > top * (1 + 2.0 ** -7), np.abs(p) < top * (1 - 2.0 ** -7)
+        assert np.array_equal(got[over], np.sign(p[over]) * np.inf)
+        assert np.all(np.abs(got - p)[fine] <= _tolerance(p, p, dt)[fine] + 2.0 ** -150)

@@ -84,7 +84,8 @@ I8Form i8_form(size_t m, size_t n, size_t k, size_t cus) {
     return best->form == I8Form::TILE_64X128 && count <= cus ? I8Form::TILE_64X128_TWO : best->form;
 }
 
-// A launch has below 2^32 threads (at most 8 for each 16 x 16 results) and 2^16 blocks of rows; whole blocks of quantized rows.
+// A launch has below 2^32 threads (16 for each 16 x 16 results of a tile; of few rows see I8_MAX_ROWS) and 2^16 tiles of rows; whole
+// blocks of quantized rows.
 size_t i8_rows_at_once(size_t n) {
     return std::min<size_t>((size_t)1 << 21, std::max<size_t>(16, ((size_t)1 << 28) / ceil_div(n, (size_t)16) / 16 * 16));
 }
